@@ -51,7 +51,8 @@ const char* mi_cuda_last_error(void);
 int mi_cuda_init(int device);
 
 /* Reads and clears the device error word that bounded waits set when they
- * give up (0 = none, else MI_CUDA_ERR_TIMEOUT). Synchronizes the device. */
+ * give up (0 = none, else MI_CUDA_ERR_TIMEOUT; MI_CUDA_ERR_ARG after a cache slot
+ * outside its cache). Synchronizes the device. */
 int mi_cuda_device_error(int device, int32_t* code_out);
 
 /* ---------------------------------------------------------------------------
@@ -202,6 +203,103 @@ int mi_cuda_expf(const float* d_x, int64_t n, float* d_y, mi_cuda_stream s);
 /* Compares the device expf with this host's libm expf on every float whose
  * bit pattern is in [first, first + count); returns the mismatch count. */
 int mi_cuda_expf_verify(uint64_t first, uint64_t count, uint64_t* n_mismatch);
+
+/* ---------------------------------------------------------------------------
+ * A step of drafted tokens (no counterpart in the reference, whose decode takes
+ * one token per step over an F32 cache)
+ *
+ * Per layer: mi_cuda_qk_norm_rope on the drafted tokens' queries and keys,
+ * mi_cuda_kv_append_q8_0 into the cache's next rows, mi_cuda_attention_tree_q8_0;
+ * after the LM head mi_cuda_logits_process on the drafted tokens' rows. The
+ * accepted tokens' keys and values are then written again, at the rows where
+ * they stay (slots; the rejected ones' are negative).
+ *
+ * Sums, norms and softmax statistics are held in 32 bits, in an order of the
+ * library's own: results agree with the formulas to float rounding and are the
+ * same from call to call. Pointers are of the calling thread's current device;
+ * nothing is allocated, so every call can be captured into a CUDA graph once
+ * mi_cuda_init has run.
+ * ------------------------------------------------------------------------- */
+
+/* Norms of queries and keys per head with the rotation (NEOX pairing, as
+ * mi_cuda_rope_neox) in one pass. d_q: n_tokens rows q_stride floats apart, each
+ * [n_head][head_dim]; d_k likewise with n_head_kv heads (both may be parts of
+ * stacked q|k|v rows). A head is divided by its root mean square (+ eps) and
+ * multiplied by d_q_norm / d_k_norm [head_dim]; NULL leaves it as it is. Then
+ * its first n_dims elements are rotated by the token's position: d_pos[t], or
+ * n_past + t where d_pos is NULL (drafted tokens of one depth share a position).
+ * The angles pos * freq_base^(-2p / n_dims) are formed in 64 bits, the
+ * reference's and mi_cuda_rope_neox's in 32 (2^-24 of the angle off: 0.004 rad at
+ * position 65536), so rows of one cache should come from one of the two.
+ * head_dim at most 256. Results are dense; d_q_dst == d_q (or d_k_dst == d_k) is
+ * allowed where the rows are dense. */
+int mi_cuda_qk_norm_rope(const float* d_q, int64_t q_stride, const float* d_k, int64_t k_stride,
+                         const float* d_q_norm, const float* d_k_norm, float eps, int64_t head_dim,
+                         int64_t n_head, int64_t n_head_kv, int64_t n_tokens, const int32_t* d_pos,
+                         int32_t n_past, int32_t n_dims, float freq_base, float* d_q_dst,
+                         float* d_k_dst, mi_cuda_stream s);
+
+/* A Q8_0 key (or value) cache of one layer, 34/32 bytes per value: int8 quants
+ * [n_head_kv][n_ctx][head_dim], then fp16 scales [n_head_kv][n_ctx][head_dim / 32].
+ * head_dim a multiple of 32, at most 256; 0 for a bad shape. */
+size_t mi_cuda_kv_q8_0_bytes(int64_t n_ctx, int64_t n_head_kv, int64_t head_dim);
+
+/* Quantises n_tokens rows of keys and values ([n_head_kv][head_dim], k_stride /
+ * v_stride floats apart) into cache rows n_past + t, or d_slots[t] where d_slots is
+ * given (n_past is then not used): a negative slot skips the token, of two tokens
+ * with one slot the later is kept, and a slot >= n_ctx is skipped and sets the
+ * device error word to MI_CUDA_ERR_ARG (mi_cuda_device_error). Other rows stay as
+ * they are. Per 32 values d = fp16(max|x| / 127), at most 65504, and
+ * q = rint(x / d) in [-127, 127] (0 where d is 0); a block with an infinity or a
+ * NaN is stored as d = NaN. Caches 16-byte aligned. */
+int mi_cuda_kv_append_q8_0(const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride,
+                           int64_t head_dim, int64_t n_head_kv, int64_t n_tokens, int64_t n_ctx,
+                           int64_t n_past, const int32_t* d_slots, void* d_cache_k, void* d_cache_v,
+                           mi_cuda_stream s);
+
+/* Cache rows [first, first + n_rows) as F32 rows [n_rows][n_head_kv][head_dim], the
+ * layout of the F32 caches above. Pointers 16-byte aligned. */
+int mi_cuda_kv_read_q8_0(const void* d_cache_k, const void* d_cache_v, int64_t head_dim, int64_t n_head_kv,
+                         int64_t n_ctx, int64_t first, int64_t n_rows, float* d_k, float* d_v, mi_cuda_stream s);
+
+/* Attention of n_tokens (0 to 1024) drafted tokens over a cache whose rows
+ * n_past + j hold their own keys and values. d_q: rows q_stride floats apart, each
+ * [n_head][head_dim], rotated. Token i attends to rows [0, n_past) and to row
+ * n_past + j where bit j (bit j % 32 of word j / 32) of its mask row is set; d_mask
+ * is [n_tokens][ceil(n_tokens / 32)] words, NULL for causal (j <= i). A token that
+ * attends to nothing gives zeros; what masked rows and rows from n_past + n_tokens
+ * on hold is never used. n_tokens = 1 is the single-token form. head_dim 32, 64, 96
+ * or 128. d_scratch holds mi_cuda_attention_tree_scratch_bytes() bytes (of
+ * n_kv = n_past + n_tokens or more) and belongs to this call until it has run;
+ * caches and scratch 16-byte aligned. dst [n_tokens][n_head][head_dim].
+ * mi_cuda_attention_tree reads F32 caches [n_ctx][n_head_kv][head_dim],
+ * mi_cuda_attention_tree_q8_0 caches of mi_cuda_kv_append_q8_0. */
+size_t mi_cuda_attention_tree_scratch_bytes(int64_t n_head, int64_t n_head_kv, int64_t n_kv, int64_t n_tokens,
+                                            int64_t head_dim);
+int mi_cuda_attention_tree(const float* d_q, int64_t q_stride, const float* d_cache_k, const float* d_cache_v,
+                           int64_t head_dim, int64_t n_head, int64_t n_head_kv, int64_t n_ctx, int64_t n_past,
+                           int64_t n_tokens, const uint32_t* d_mask, float scale, void* d_scratch, float* d_dst,
+                           mi_cuda_stream s);
+int mi_cuda_attention_tree_q8_0(const float* d_q, int64_t q_stride, const void* d_cache_k, const void* d_cache_v,
+                                int64_t head_dim, int64_t n_head, int64_t n_head_kv, int64_t n_ctx, int64_t n_past,
+                                int64_t n_tokens, const uint32_t* d_mask, float scale, void* d_scratch, float* d_dst,
+                                mi_cuda_stream s);
+
+/* Penalties, biases and a grammar's mask on n_rows rows of logits (`stride` floats
+ * apart), and the greedy token of what is left. With c = how often token j is in
+ * the row's history (n_hist ids, rows hist_stride apart, 0: one history for all;
+ * ids outside [0, n_vocab) are padding):
+ *   x = l;  c > 0: x = (l > 0 ? l / repeat : l * repeat) - (c * frequency + presence)
+ *   x += the biases of j (d_bias[i] for d_bias_ids[i] == j, summed in order)
+ *   x = -infinity where bit j of the row's d_allowed words is 0 (rows
+ *   allowed_stride words apart, 0: one mask for all; NULL: all allowed)
+ * d_dst gets dense rows (d_dst == d_logits is allowed for dense rows), d_tokens
+ * (may be NULL) each row's lowest index of the maximum, -1 where nothing is above
+ * -infinity (NaN never wins). */
+int mi_cuda_logits_process(const float* d_logits, int64_t stride, int64_t n_vocab, int64_t n_rows, const int32_t* d_hist,
+                           int64_t n_hist, int64_t hist_stride, float repeat, float frequency, float presence,
+                           const int32_t* d_bias_ids, const float* d_bias, int64_t n_bias, const uint32_t* d_allowed,
+                           int64_t allowed_stride, float* d_dst, int32_t* d_tokens, mi_cuda_stream s);
 
 /* ---------------------------------------------------------------------------
  * Qwen2 decode executor (ref src/model_qwen2.h:83-189)

@@ -410,6 +410,81 @@ cudaError_t launch_advance(int32_t* pos, cudaStream_t s, bool pdl, uint32_t* epo
 cudaError_t launch_set_pos(int32_t* pos, int32_t value, cudaStream_t s);
 
 // ---------------------------------------------------------------------------
+// A step of drafted tokens: head norms with rotation, the Q8_0 cache, tree
+// attention, logits processing
+// ---------------------------------------------------------------------------
+constexpr int kRopeMaxDim = 256;
+struct QkRopeParams {
+  const float* q;  // [n_tokens] rows q_stride floats apart, [H][D]
+  const float* k;  // ... k_stride ..., [HKV][D]
+  int64_t q_stride, k_stride;
+  const float* wq;  // [D], nullptr: no norm
+  const float* wk;
+  float eps;
+  int32_t D, H, HKV, n_dims, n_past;
+  int64_t n_tokens;
+  const int32_t* pos;  // nullptr: n_past + t
+  float* q_out;        // dense
+  float* k_out;
+  double freq[kRopeMaxDim / 2];  // set by the launcher: radians per position of each pair
+};
+cudaError_t launch_qk_norm_rope(QkRopeParams& p, float freq_base, cudaStream_t s);
+
+struct KvAppendParams {
+  const float* k;
+  const float* v;
+  int64_t k_stride, v_stride, n_tokens;
+  int32_t D, HKV, n_ctx, n_past;
+  const int32_t* slots;  // nullptr: n_past + t
+  uint8_t* cache_k;
+  uint8_t* cache_v;
+  int32_t* err;
+};
+cudaError_t launch_kv_append_q8(const KvAppendParams& p, cudaStream_t s);
+struct KvReadParams {
+  const uint8_t* cache_k;
+  const uint8_t* cache_v;
+  int32_t D, HKV, n_ctx;
+  int64_t first, n_rows;
+  float* k;  // [n_rows][HKV][D]
+  float* v;
+};
+cudaError_t launch_kv_read_q8(const KvReadParams& p, cudaStream_t s);
+
+constexpr int64_t kTreeMaxTokens = 1024;
+struct TreeAttnParams {
+  const float* q;  // [T] rows q_stride floats apart, [H][D]
+  int64_t q_stride;
+  const void* cache_k;  // F32 [n_ctx][HKV][D], or q8: the Q8_0 cache
+  const void* cache_v;
+  int32_t D, H, HKV, n_ctx, n_past, T;
+  bool q8;
+  const uint32_t* mask;  // [T][ceil(T / 32)], nullptr: causal
+  float scale;
+  void* scratch;
+  float* out;  // [T][H][D]
+};
+bool attn_tree_fits(int64_t D, int64_t H, int64_t HKV, int64_t T);
+size_t attn_tree_scratch_bytes(int64_t H, int64_t HKV, int64_t n_kv, int64_t T, int64_t D);
+cudaError_t launch_attn_tree(const TreeAttnParams& p, cudaStream_t s);
+
+struct LogitsParams {
+  const float* logits;  // rows `stride` floats apart
+  int64_t stride, n_vocab;
+  const int32_t* hist;
+  int64_t n_hist, hist_stride;
+  float repeat, frequency, presence;
+  const int32_t* bias_ids;
+  const float* bias;
+  int64_t n_bias;
+  const uint32_t* allowed;
+  int64_t allowed_stride;
+  float* out;       // dense rows
+  int32_t* tokens;  // optional
+};
+cudaError_t launch_logits_process(const LogitsParams& p, int64_t n_rows, cudaStream_t s);
+
+// ---------------------------------------------------------------------------
 // Library state (ops_capi.cu)
 // ---------------------------------------------------------------------------
 struct DeviceCtx {

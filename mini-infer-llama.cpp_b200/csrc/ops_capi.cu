@@ -445,6 +445,207 @@ int mi_cuda_attention_decode_split(const float* d_q, const float* d_cache_k, con
                      "attention_decode_split");
 }
 
+// Whether [a, a + na) and [b, b + nb) share a byte.
+static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+// Bytes of n rows of `row` floats that lie `stride` floats apart.
+static int64_t span_bytes(int64_t n, int64_t row, int64_t stride) { return n > 0 ? ((n - 1) * stride + row) * 4 : 0; }
+
+int mi_cuda_qk_norm_rope(const float* d_q, int64_t q_stride, const float* d_k, int64_t k_stride,
+                         const float* d_q_norm, const float* d_k_norm, float eps, int64_t head_dim,
+                         int64_t n_head, int64_t n_head_kv, int64_t n_tokens, const int32_t* d_pos,
+                         int32_t n_past, int32_t n_dims, float freq_base, float* d_q_dst,
+                         float* d_k_dst, mi_cuda_stream s) {
+  MI_REQUIRE(d_q && d_k && d_q_dst && d_k_dst && head_dim > 0 && head_dim <= kRopeMaxDim && n_head > 0 &&
+                 n_head <= 65535 && n_head_kv > 0 && n_head_kv <= 65535 && n_tokens >= 0 && n_tokens <= (1ll << 28) &&
+                 n_past >= 0 && q_stride >= n_head * head_dim && k_stride >= n_head_kv * head_dim &&
+                 q_stride < (1ll << 31) && k_stride < (1ll << 31),
+             "mi_cuda_qk_norm_rope: bad arguments");
+  MI_REQUIRE(n_dims > 0 && n_dims <= head_dim && n_dims % 2 == 0, "mi_cuda_qk_norm_rope: n_dims is even, at most head_dim");
+  MI_REQUIRE(freq_base > 0.0f && freq_base <= 3.402823466e38f && eps >= 0.0f,
+             "mi_cuda_qk_norm_rope: freq_base is finite and above 0, eps not below 0");
+  MI_REQUIRE(d_pos || n_past + n_tokens <= (1ll << 31), "mi_cuda_qk_norm_rope: positions pass 32 bits");
+  // a row may be written over only where it was read
+  const int64_t E = n_head * head_dim, F = n_head_kv * head_dim;
+  const int64_t qi = span_bytes(n_tokens, E, q_stride), ki = span_bytes(n_tokens, F, k_stride);
+  const int64_t qo = n_tokens * E * 4, ko = n_tokens * F * 4;
+  MI_REQUIRE(!overlap(d_q_dst, qo, d_k, ki) && !overlap(d_k_dst, ko, d_q, qi) && !overlap(d_q_dst, qo, d_k_dst, ko) &&
+                 (!overlap(d_q_dst, qo, d_q, qi) || (d_q_dst == d_q && (q_stride == E || n_tokens == 1))) &&
+                 (!overlap(d_k_dst, ko, d_k, ki) || (d_k_dst == d_k && (k_stride == F || n_tokens == 1))),
+             "mi_cuda_qk_norm_rope: outputs overlap the inputs (only dense rows can be rotated in place)");
+  MI_CTX(c);
+  QkRopeParams p{};
+  p.q = d_q;
+  p.k = d_k;
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.wq = d_q_norm;
+  p.wk = d_k_norm;
+  p.eps = eps;
+  p.D = (int32_t)head_dim;
+  p.H = (int32_t)n_head;
+  p.HKV = (int32_t)n_head_kv;
+  p.n_dims = n_dims;
+  p.n_past = n_past;
+  p.n_tokens = n_tokens;
+  p.pos = d_pos;
+  p.q_out = d_q_dst;
+  p.k_out = d_k_dst;
+  return cuda_status(launch_qk_norm_rope(p, freq_base, S(s)), "qk_norm_rope");
+}
+
+size_t mi_cuda_kv_q8_0_bytes(int64_t n_ctx, int64_t n_head_kv, int64_t head_dim) {
+  if (n_ctx <= 0 || n_ctx >= (1ll << 31) || n_head_kv <= 0 || n_head_kv > 65535 || head_dim <= 0 || head_dim > 256 ||
+      head_dim % 32 != 0)
+    return 0;
+  return (size_t)(n_ctx * n_head_kv * head_dim / 32 * 34);
+}
+
+int mi_cuda_kv_append_q8_0(const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride,
+                           int64_t head_dim, int64_t n_head_kv, int64_t n_tokens, int64_t n_ctx,
+                           int64_t n_past, const int32_t* d_slots, void* d_cache_k, void* d_cache_v,
+                           mi_cuda_stream s) {
+  const int64_t row = n_head_kv * head_dim;
+  MI_REQUIRE(d_k && d_v && d_cache_k && d_cache_v && mi_cuda_kv_q8_0_bytes(n_ctx, n_head_kv, head_dim) > 0 &&
+                 n_tokens >= 0 && n_tokens < (1ll << 31) && n_past >= 0 && k_stride >= row && v_stride >= row &&
+                 (uintptr_t)d_cache_k % 16 == 0 && (uintptr_t)d_cache_v % 16 == 0,
+             "mi_cuda_kv_append_q8_0: bad arguments (head_dim a multiple of 32, at most 256; 16-byte aligned caches)");
+  MI_REQUIRE(d_slots || n_past <= n_ctx - n_tokens, "mi_cuda_kv_append_q8_0: rows behind the cache's last");
+  MI_CTX(c);
+  KvAppendParams p{};
+  p.k = d_k;
+  p.v = d_v;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.n_tokens = n_tokens;
+  p.D = (int32_t)head_dim;
+  p.HKV = (int32_t)n_head_kv;
+  p.n_ctx = (int32_t)n_ctx;
+  p.n_past = d_slots ? 0 : (int32_t)n_past;
+  p.slots = d_slots;
+  p.cache_k = (uint8_t*)d_cache_k;
+  p.cache_v = (uint8_t*)d_cache_v;
+  p.err = c->err;
+  return cuda_status(launch_kv_append_q8(p, S(s)), "kv_append_q8_0");
+}
+
+int mi_cuda_kv_read_q8_0(const void* d_cache_k, const void* d_cache_v, int64_t head_dim, int64_t n_head_kv,
+                         int64_t n_ctx, int64_t first, int64_t n_rows, float* d_k, float* d_v, mi_cuda_stream s) {
+  MI_REQUIRE(d_cache_k && d_cache_v && d_k && d_v && mi_cuda_kv_q8_0_bytes(n_ctx, n_head_kv, head_dim) > 0 &&
+                 (uintptr_t)d_cache_k % 16 == 0 && (uintptr_t)d_cache_v % 16 == 0 && (uintptr_t)d_k % 16 == 0 &&
+                 (uintptr_t)d_v % 16 == 0,
+             "mi_cuda_kv_read_q8_0: bad arguments (head_dim a multiple of 32, at most 256; 16-byte aligned pointers)");
+  MI_REQUIRE(first >= 0 && n_rows >= 0 && first <= n_ctx && n_rows <= n_ctx - first,
+             "mi_cuda_kv_read_q8_0: rows outside the cache");
+  MI_CTX(c);
+  KvReadParams p{};
+  p.cache_k = (const uint8_t*)d_cache_k;
+  p.cache_v = (const uint8_t*)d_cache_v;
+  p.D = (int32_t)head_dim;
+  p.HKV = (int32_t)n_head_kv;
+  p.n_ctx = (int32_t)n_ctx;
+  p.first = first;
+  p.n_rows = n_rows;
+  p.k = d_k;
+  p.v = d_v;
+  return cuda_status(launch_kv_read_q8(p, S(s)), "kv_read_q8_0");
+}
+
+size_t mi_cuda_attention_tree_scratch_bytes(int64_t n_head, int64_t n_head_kv, int64_t n_kv, int64_t n_tokens,
+                                            int64_t head_dim) {
+  if (!attn_tree_fits(head_dim, n_head, n_head_kv, n_tokens) || n_kv < n_tokens || n_kv >= (1ll << 31)) return 0;
+  return attn_tree_scratch_bytes(n_head, n_head_kv, n_kv, n_tokens, head_dim);
+}
+
+static int attention_tree_common(const char* name, const float* d_q, int64_t q_stride, const void* d_cache_k,
+                                 const void* d_cache_v, bool q8, int64_t head_dim, int64_t n_head, int64_t n_head_kv,
+                                 int64_t n_ctx, int64_t n_past, int64_t n_tokens, const uint32_t* d_mask, float scale,
+                                 void* d_scratch, float* d_dst, mi_cuda_stream s) {
+  MI_REQUIRE(d_q && d_cache_k && d_cache_v && d_scratch && d_dst && n_past >= 0 && n_ctx > 0 && n_ctx < (1ll << 31) &&
+                 (uintptr_t)d_cache_k % 16 == 0 && (uintptr_t)d_cache_v % 16 == 0 && (uintptr_t)d_scratch % 16 == 0,
+             std::string(name) + ": bad arguments (16-byte aligned caches and scratch)");
+  MI_REQUIRE(attn_tree_fits(head_dim, n_head, n_head_kv, n_tokens),
+             std::string(name) + ": head_dim 32, 64, 96 or 128, n_head a multiple of n_head_kv, at most 1024 tokens");
+  MI_REQUIRE(q_stride >= n_head * head_dim, std::string(name) + ": q_stride below a row");
+  MI_REQUIRE(n_past <= n_ctx - n_tokens, std::string(name) + ": rows behind the cache's last");
+  MI_CTX(c);
+  TreeAttnParams p{};
+  p.q = d_q;
+  p.q_stride = q_stride;
+  p.cache_k = d_cache_k;
+  p.cache_v = d_cache_v;
+  p.D = (int32_t)head_dim;
+  p.H = (int32_t)n_head;
+  p.HKV = (int32_t)n_head_kv;
+  p.n_ctx = (int32_t)n_ctx;
+  p.n_past = (int32_t)n_past;
+  p.T = (int32_t)n_tokens;
+  p.q8 = q8;
+  p.mask = d_mask;
+  p.scale = scale;
+  p.scratch = d_scratch;
+  p.out = d_dst;
+  return cuda_status(launch_attn_tree(p, S(s)), name);
+}
+
+int mi_cuda_attention_tree(const float* d_q, int64_t q_stride, const float* d_cache_k, const float* d_cache_v,
+                           int64_t head_dim, int64_t n_head, int64_t n_head_kv, int64_t n_ctx, int64_t n_past,
+                           int64_t n_tokens, const uint32_t* d_mask, float scale, void* d_scratch, float* d_dst,
+                           mi_cuda_stream s) {
+  return attention_tree_common("mi_cuda_attention_tree", d_q, q_stride, d_cache_k, d_cache_v, false, head_dim, n_head,
+                               n_head_kv, n_ctx, n_past, n_tokens, d_mask, scale, d_scratch, d_dst, s);
+}
+
+int mi_cuda_attention_tree_q8_0(const float* d_q, int64_t q_stride, const void* d_cache_k, const void* d_cache_v,
+                                int64_t head_dim, int64_t n_head, int64_t n_head_kv, int64_t n_ctx, int64_t n_past,
+                                int64_t n_tokens, const uint32_t* d_mask, float scale, void* d_scratch, float* d_dst,
+                                mi_cuda_stream s) {
+  return attention_tree_common("mi_cuda_attention_tree_q8_0", d_q, q_stride, d_cache_k, d_cache_v, true, head_dim,
+                               n_head, n_head_kv, n_ctx, n_past, n_tokens, d_mask, scale, d_scratch, d_dst, s);
+}
+
+int mi_cuda_logits_process(const float* d_logits, int64_t stride, int64_t n_vocab, int64_t n_rows, const int32_t* d_hist,
+                           int64_t n_hist, int64_t hist_stride, float repeat, float frequency, float presence,
+                           const int32_t* d_bias_ids, const float* d_bias, int64_t n_bias, const uint32_t* d_allowed,
+                           int64_t allowed_stride, float* d_dst, int32_t* d_tokens, mi_cuda_stream s) {
+  MI_REQUIRE(d_logits && d_dst && n_vocab > 0 && n_vocab < (1ll << 31) - 65536 && n_rows >= 0 && n_rows <= 65535 &&
+                 stride >= n_vocab && stride < (1ll << 40),
+             "mi_cuda_logits_process: bad arguments");
+  MI_REQUIRE(n_hist >= 0 && n_hist < (1ll << 31) && (n_hist == 0 || d_hist) && (hist_stride == 0 || hist_stride >= n_hist),
+             "mi_cuda_logits_process: a history of n_hist tokens, rows hist_stride apart (0: one for all)");
+  MI_REQUIRE(n_bias >= 0 && n_bias < (1ll << 31) && (n_bias == 0 || (d_bias_ids && d_bias)),
+             "mi_cuda_logits_process: n_bias without biases");
+  MI_REQUIRE(!d_allowed || allowed_stride == 0 || allowed_stride >= (n_vocab + 31) / 32,
+             "mi_cuda_logits_process: allowed_stride below a row of words");
+  MI_REQUIRE(repeat > 0.0f && repeat <= 3.402823466e38f && frequency - frequency == 0.0f && presence - presence == 0.0f,
+             "mi_cuda_logits_process: penalties are finite, repeat is above 0");
+  MI_REQUIRE(!overlap(d_dst, n_rows * n_vocab * 4, d_logits, span_bytes(n_rows, n_vocab, stride)) ||
+                 (d_dst == d_logits && (stride == n_vocab || n_rows == 1)),
+             "mi_cuda_logits_process: d_dst overlaps the logits (only dense rows can be processed in place)");
+  MI_CTX(c);
+  LogitsParams p{};
+  p.logits = d_logits;
+  p.stride = stride;
+  p.n_vocab = n_vocab;
+  p.hist = d_hist;
+  p.n_hist = n_hist;
+  p.hist_stride = hist_stride;
+  p.repeat = repeat;
+  p.frequency = frequency;
+  p.presence = presence;
+  p.bias_ids = d_bias_ids;
+  p.bias = d_bias;
+  p.n_bias = n_bias;
+  p.allowed = d_allowed;
+  p.allowed_stride = allowed_stride;
+  p.out = d_dst;
+  p.tokens = d_tokens;
+  return cuda_status(launch_logits_process(p, n_rows, S(s)), "logits_process");
+}
+
 int mi_cuda_argmax(const float* d_x, int64_t n, int32_t* d_out, mi_cuda_stream s) {
   MI_CTX(c);
   MI_REQUIRE(d_x && d_out && n > 0 && n < (1ll << 31), "mi_cuda_argmax: bad arguments");

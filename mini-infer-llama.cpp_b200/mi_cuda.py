@@ -71,6 +71,14 @@ _SIGS = {
     "mi_cuda_attention_decode_split_scratch_bytes": (SZ, [I64, I64, I64, I64]),
     "mi_cuda_attention_decode_split": (I32, [P, P, P, I64, I64, I64, I64, F32, P, P, P]),
     "mi_cuda_argmax": (I32, [P, I64, P, P]),
+    "mi_cuda_qk_norm_rope": (I32, [P, I64, P, I64, P, P, F32, I64, I64, I64, I64, P, I32, I32, F32, P, P, P]),
+    "mi_cuda_kv_q8_0_bytes": (SZ, [I64, I64, I64]),
+    "mi_cuda_kv_append_q8_0": (I32, [P, I64, P, I64, I64, I64, I64, I64, I64, P, P, P, P]),
+    "mi_cuda_kv_read_q8_0": (I32, [P, P, I64, I64, I64, I64, I64, P, P, P]),
+    "mi_cuda_attention_tree_scratch_bytes": (SZ, [I64, I64, I64, I64, I64]),
+    "mi_cuda_attention_tree": (I32, [P, I64, P, P, I64, I64, I64, I64, I64, I64, P, F32, P, P, P]),
+    "mi_cuda_attention_tree_q8_0": (I32, [P, I64, P, P, I64, I64, I64, I64, I64, I64, P, F32, P, P, P]),
+    "mi_cuda_logits_process": (I32, [P, I64, I64, I64, P, I64, I64, F32, F32, F32, P, P, I64, P, I64, P, P, P]),
     "mi_cuda_expf": (I32, [P, I64, P, P]),
     "mi_cuda_expf_verify": (I32, [U64, U64, P]),
     "mi_cuda_qwen2_model_load": (I32, [C.c_char_p, I32, P]),
@@ -318,6 +326,227 @@ def argmax(x):
     out = torch.empty(1, dtype=torch.int32, device=x.device)
     check(lib().mi_cuda_argmax(_p(x), x.numel(), _p(out), _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# A step of drafted tokens: head norms with rotation, the Q8_0 cache, attention
+# of a tree over a cache, logits processing
+# ---------------------------------------------------------------------------
+
+def _arg(t, name: str, dtypes, shape=None, dense_from: int = 0):
+    """Checks a tensor argument: on a GPU, one of `dtypes`, `shape` (None: any
+    size of that dimension), dense from dimension `dense_from` on."""
+    if not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor is needed")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: {t.dtype} where {' or '.join(map(str, dtypes))} is needed")
+    if shape is not None:
+        if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+            raise ValueError(f"{name}: shape {tuple(t.shape)} where {shape} is needed")
+    if not t.is_contiguous():
+        want = 1
+        for n, st in zip(reversed(t.shape[dense_from:]), reversed(t.stride()[dense_from:])):
+            if n != 1 and st != want:
+                raise ValueError(f"{name}: strides {t.stride()} (dense from dimension {dense_from} on is needed)")
+            want *= n
+    return t
+
+
+def _row_stride(t) -> int:
+    """Elements between the rows of dimension 0 (of a single row: the row itself)."""
+    return t.stride(0) if t.shape[0] > 1 else t.numel()
+
+
+class _on:
+    """Makes the tensors' device the current one for a call and gives its current
+    stream; refuses tensors of several devices."""
+
+    __slots__ = ("dev", "back")
+
+    def __init__(self, *tensors):
+        dev = tensors[0].get_device()
+        for t in tensors:
+            if t is not None and t.get_device() != dev:
+                raise ValueError("the tensors are on several devices")
+        self.dev = dev
+
+    def __enter__(self):
+        cuda = _torch().cuda
+        now = cuda.current_device()
+        self.back = now if now != self.dev else -1
+        if self.back >= 0:
+            cuda.set_device(self.dev)
+        return cuda.current_stream(self.dev).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.back >= 0:
+            _torch().cuda.set_device(self.back)
+
+
+def qk_norm_rope(q, k, q_norm, k_norm, eps: float, n_past: int, n_dims: int, freq_base: float, pos=None,
+                 q_out=None, k_out=None):
+    """q [T, H, D] and k [T, HKV, D] (views of stacked rows may be given) normed per
+    head (q_norm / k_norm [D], or None) and rotated to position pos[t] (or n_past + t)."""
+    torch = _torch()
+    f32 = (torch.float32,)
+    T, H, D = _arg(q, "q", f32, (None, None, None), 1).shape
+    HKV = _arg(k, "k", f32, (T, None, D), 1).shape[1]
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if t is not None:
+            _arg(t, name, f32, (D,))
+    if pos is not None:
+        _arg(pos, "pos", (torch.int32,), (T,))
+    q_out = torch.empty((T, H, D), dtype=torch.float32, device=q.device) if q_out is None else _arg(q_out, "q_out", f32, (T, H, D))
+    k_out = torch.empty((T, HKV, D), dtype=torch.float32, device=q.device) if k_out is None else _arg(k_out, "k_out", f32, (T, HKV, D))
+    if T == 0:
+        return q_out, k_out
+    with _on(q, k, q_norm, k_norm, pos, q_out, k_out) as s:
+        check(lib().mi_cuda_qk_norm_rope(_p(q), _row_stride(q), _p(k), _row_stride(k), _p(q_norm), _p(k_norm), eps, D, H, HKV,
+                                         T, _p(pos), n_past, n_dims, freq_base, _p(q_out), _p(k_out), s))
+    return q_out, k_out
+
+
+def kv_q8_0_cache(n_ctx: int, n_head_kv: int, head_dim: int, device="cuda"):
+    """A zeroed Q8_0 cache (keys or values) of one layer, as a uint8 tensor."""
+    nb = lib().mi_cuda_kv_q8_0_bytes(n_ctx, n_head_kv, head_dim)
+    if nb == 0:
+        raise ValueError(f"no Q8_0 cache of {n_ctx} rows of {n_head_kv} heads of {head_dim}")
+    return _torch().zeros(nb, dtype=_torch().uint8, device=device)
+
+
+def _kv_q8_0_arg(t, name: str, n_ctx: int, n_head_kv: int, head_dim: int):
+    nb = lib().mi_cuda_kv_q8_0_bytes(n_ctx, n_head_kv, head_dim)
+    if nb == 0:
+        raise ValueError(f"{name}: no Q8_0 cache of {n_ctx} rows of {n_head_kv} heads of {head_dim}")
+    if _arg(t, name, (_torch().uint8,)).numel() != nb:
+        raise ValueError(f"{name}: {t.numel()} bytes where the cache has {nb}")
+
+
+def kv_append_q8_0(k, v, cache_k, cache_v, n_ctx: int, n_past: int = 0, slots=None):
+    """Quantises k and v [T, HKV, D] into cache rows n_past + t, or slots[t] (int32; negative: skipped)."""
+    torch = _torch()
+    T, HKV, D = _arg(k, "k", (torch.float32,), (None, None, None), 1).shape
+    _arg(v, "v", (torch.float32,), (T, HKV, D), 1)
+    _kv_q8_0_arg(cache_k, "cache_k", n_ctx, HKV, D)
+    _kv_q8_0_arg(cache_v, "cache_v", n_ctx, HKV, D)
+    if slots is not None:
+        _arg(slots, "slots", (torch.int32,), (T,))
+    if T == 0:
+        return
+    with _on(k, v, cache_k, cache_v, slots) as s:
+        check(lib().mi_cuda_kv_append_q8_0(_p(k), _row_stride(k), _p(v), _row_stride(v), D, HKV, T, n_ctx, n_past, _p(slots),
+                                           _p(cache_k), _p(cache_v), s))
+
+
+def kv_read_q8_0(cache_k, cache_v, n_head_kv: int, head_dim: int, n_ctx: int, first: int, n_rows: int):
+    """Cache rows [first, first + n_rows) as F32 tensors (k, v) of [n_rows, n_head_kv, head_dim]."""
+    torch = _torch()
+    _kv_q8_0_arg(cache_k, "cache_k", n_ctx, n_head_kv, head_dim)
+    _kv_q8_0_arg(cache_v, "cache_v", n_ctx, n_head_kv, head_dim)
+    if first < 0 or n_rows < 0 or first + n_rows > n_ctx:
+        raise ValueError(f"rows [{first}, {first + n_rows}) of a cache of {n_ctx}")
+    k = torch.empty((n_rows, n_head_kv, head_dim), dtype=torch.float32, device=cache_k.device)
+    v = torch.empty((n_rows, n_head_kv, head_dim), dtype=torch.float32, device=cache_k.device)
+    if n_rows:
+        with _on(cache_k, cache_v) as s:
+            check(lib().mi_cuda_kv_read_q8_0(_p(cache_k), _p(cache_v), head_dim, n_head_kv, n_ctx, first, n_rows, _p(k), _p(v), s))
+    return k, v
+
+
+def tree_mask(parents) -> np.ndarray:
+    """The mask of a draft tree, int32 [n, ceil(n / 32)] on the host: bit j of row i
+    is set where token j is token i or one of its ancestors. parents[i] is the index
+    of token i's parent (before i), or negative for one that follows the cached text."""
+    n = len(parents)
+    bits = np.zeros((n, (n + 31) // 32 * 32), dtype=np.uint32)
+    for i, p in enumerate(parents):
+        if p >= i:
+            raise ValueError(f"token {i} comes before its parent {p}")
+        if p >= 0:
+            bits[i] = bits[p]
+        bits[i, i] = 1
+    return (bits.reshape(n, (n + 31) // 32, 32) << np.arange(32, dtype=np.uint32)).sum(-1, dtype=np.uint32).view(np.int32)
+
+
+def attention_tree_scratch(n_head: int, n_head_kv: int, n_kv: int, n_tokens: int, head_dim: int, device="cuda"):
+    """The workspace of attention_tree / attention_tree_q8_0 for up to n_kv = n_past + n_tokens rows."""
+    torch = _torch()
+    nb = lib().mi_cuda_attention_tree_scratch_bytes(n_head, n_head_kv, n_kv, n_tokens, head_dim)
+    if nb == 0:
+        raise ValueError(f"no tree attention of {n_tokens} tokens, {n_head} / {n_head_kv} heads of {head_dim}, {n_kv} rows")
+    return torch.empty(nb, dtype=torch.uint8, device=device)
+
+
+def _attention_tree(fn, q, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch):
+    torch = _torch()
+    T, H, D = q.shape
+    if mask is not None:
+        _arg(mask, "mask", (torch.int32, torch.uint32), (T, (T + 31) // 32))
+    out = torch.empty((T, H, D), dtype=torch.float32, device=q.device)
+    if T == 0:
+        return out
+    if scratch is None:
+        scratch = attention_tree_scratch(H, n_head_kv, n_past + T, T, D, q.device)
+    elif _arg(scratch, "scratch", (torch.uint8,)).numel() < lib().mi_cuda_attention_tree_scratch_bytes(H, n_head_kv, n_past + T, T, D):
+        raise ValueError("scratch: too small (attention_tree_scratch)")
+    with _on(q, cache_k, cache_v, mask, scratch) as s:
+        check(fn(_p(q), _row_stride(q), _p(cache_k), _p(cache_v), D, H, n_head_kv, n_ctx, n_past, T, _p(mask), scale_,
+                 _p(scratch), _p(out), s))
+    return out
+
+
+def attention_tree(q, cache_k, cache_v, n_head_kv: int, n_past: int, scale_: float, mask=None, scratch=None):
+    """Attention of drafted tokens q [T, H, D] over F32 caches [n_ctx, HKV, D] whose rows
+    n_past + j hold the drafted tokens' own; mask as tree_mask gives it (None: causal)."""
+    torch = _torch()
+    f32 = (torch.float32,)
+    D = _arg(q, "q", f32, (None, None, None), 1).shape[2]
+    n_ctx = _arg(cache_k, "cache_k", f32, (None, n_head_kv, D)).shape[0]
+    _arg(cache_v, "cache_v", f32, (n_ctx, n_head_kv, D))
+    return _attention_tree(lib().mi_cuda_attention_tree, q, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch)
+
+
+def attention_tree_q8_0(q, cache_k, cache_v, n_head_kv: int, n_ctx: int, n_past: int, scale_: float, mask=None, scratch=None):
+    """attention_tree over Q8_0 caches (kv_q8_0_cache, kv_append_q8_0)."""
+    D = _arg(q, "q", (_torch().float32,), (None, None, None), 1).shape[2]
+    _kv_q8_0_arg(cache_k, "cache_k", n_ctx, n_head_kv, D)
+    _kv_q8_0_arg(cache_v, "cache_v", n_ctx, n_head_kv, D)
+    return _attention_tree(lib().mi_cuda_attention_tree_q8_0, q, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch)
+
+
+def logits_process(logits, hist=None, repeat: float = 1.0, frequency: float = 0.0, presence: float = 0.0, bias_ids=None,
+                   bias=None, allowed=None, out=None):
+    """Penalties for the tokens of `hist` (int32 [n] or [rows, n], ids outside the vocabulary
+    are padding), biases (int32 ids and F32 values) and a mask of allowed tokens (bits of
+    int32 [words] or [rows, words]) on logits [rows, V]: (processed logits, greedy tokens
+    int32 [rows], -1 where nothing is left). out may be the logits themselves."""
+    torch = _torch()
+    n, V = _arg(logits, "logits", (torch.float32,), (None, None), 1).shape
+    i32 = (torch.int32,)
+
+    def rows_of(t, name, dtypes, least):
+        if t.dim() == 2 and t.shape[0] != n or t.dim() not in (1, 2) or t.shape[-1] < least:
+            raise ValueError(f"{name}: shape {tuple(t.shape)} for {n} rows of {V} tokens")
+        _arg(t, name, dtypes, None, t.dim() - 1)
+        return 0 if t.dim() == 1 else _row_stride(t)
+
+    hs = rows_of(hist, "hist", i32, 0) if hist is not None else 0
+    nh = hist.shape[-1] if hist is not None else 0
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias go together")
+    nb = 0
+    if bias is not None:
+        nb = _arg(bias, "bias", (torch.float32,), (None,)).shape[0]
+        _arg(bias_ids, "bias_ids", i32, (nb,))
+    als = rows_of(allowed, "allowed", (torch.int32, torch.uint32), (V + 31) // 32) if allowed is not None else 0
+    out = torch.empty((n, V), dtype=torch.float32, device=logits.device) if out is None else _arg(out, "out", (torch.float32,), (n, V))
+    tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
+    if n:
+        with _on(logits, hist, bias_ids, bias, allowed, out) as s:
+            check(lib().mi_cuda_logits_process(_p(logits), _row_stride(logits), V, n, _p(hist) if nh else None, nh, hs if nh else 0,
+                                               repeat, frequency, presence, _p(bias_ids) if nb else None, _p(bias) if nb else None, nb,
+                                               _p(allowed), als, _p(out), _p(tokens), s))
+    return out, tokens
 
 
 # ---------------------------------------------------------------------------
