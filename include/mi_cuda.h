@@ -269,8 +269,8 @@ int mi_cuda_kv_read_q8_0(const void* d_cache_k, const void* d_cache_v, int64_t h
  * is [n_tokens][ceil(n_tokens / 32)] words, NULL for causal (j <= i). A token that
  * attends to nothing gives zeros; what masked rows and rows from n_past + n_tokens
  * on hold is never used. n_tokens = 1 is the single-token form. head_dim 32, 64, 96
- * or 128. d_scratch holds mi_cuda_attention_tree_scratch_bytes() bytes (of
- * n_kv = n_past + n_tokens or more) and belongs to this call until it has run;
+ * or 128, n_head a multiple of n_head_kv, at most 4096. d_scratch holds mi_cuda_attention_tree_scratch_bytes() bytes
+ * (those for a larger n_kv = n_past + n_tokens or n_tokens are enough too) and belongs to this call until it has run;
  * caches and scratch 16-byte aligned. dst [n_tokens][n_head][head_dim].
  * mi_cuda_attention_tree reads F32 caches [n_ctx][n_head_kv][head_dim],
  * mi_cuda_attention_tree_q8_0 caches of mi_cuda_kv_append_q8_0. */

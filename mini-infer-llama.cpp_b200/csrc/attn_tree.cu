@@ -4,88 +4,753 @@
 //
 // Token i of T attends to cache rows [0, n_past) and to row n_past + j (drafted
 // token j's) where bit j of its mask is set; without a mask to j <= i.
-//   s = scale q.k,  p = exp(s - max s),  out = sum p v / sum p
+//   s = scale q.k,  p = e^(s - max s),  out = sum p v / sum p
 // over the attended rows, and zeros where there is none. The cache is F32
 // ([n_ctx][n_head_kv][D]) or Q8_0 (kv_q8.cu).
+//
+// The n_rep query heads of a KV head times T tokens are the rows of two matrix
+// products over the KV head's positions, S = Q K^T and O = P V, and run on the
+// tensor cores (tcgen05) at float precision:
+//
+//   * every operand is split into two fp16 planes, x = hi + lo, after its row was
+//     scaled by a power of two (so that neither half leaves fp16's range): hi + lo
+//     is x to 22 bits, and for a Q8_0 value exactly (11 bits of scale times 7 of
+//     quant: hi = fl(d q) and lo = fma(d, q, -hi) is the whole rest). A product
+//     takes three MMAs (hi hi, hi lo, lo hi); what is left out is 2^-22 of it.
+//   * the rows' powers of two leave the products as factors: a position's key
+//     exponent multiplies its column of S, its value exponent e is added to the
+//     score that makes P (P = 2^(s + e - M)), and the sum of the weights takes it
+//     out again.
+//
+// One CTA: up to 256 rows (two tiles of 128, one TMEM lane each) over one range of
+// positions, 64 at a time. Warps 0-7 softmax (a thread per row), 8-11 convert keys
+// and 12-15 values into the MMAs' layout, 16 issues the MMAs. S (64 columns), P's
+// planes (32 + 32) and O (D) of both tiles fill TMEM at D = 128; the two tiles let
+// one's MMAs run under the other's exponentials. The running maximum M moves only
+// when a score passes it by 2^8 (fp16 holds 2^15), so O is rarely rescaled.
+//
+// The positions are split over CTAs to fill the GPU; a second kernel joins the
+// splits' (M, sum, O) records.
+#include <cuda_fp16.h>
+
 #include <algorithm>
 
-#include "mi_device.cuh"
+#include "mi_tc.cuh"
 
 namespace mi {
 
 namespace {
 
-constexpr int kTrNT = 128;
+constexpr int kTrTile = 64;      // positions per step
+constexpr int kTrRows = 128;     // rows per tile (MMA M)
+constexpr int kTrWarpK = 8, kTrWarpV = 12, kTrWarpMma = 16;
+constexpr int kTrThreads = 17 * 32;
+constexpr int kTrSlots = 4;      // steps whose column factors are kept
+constexpr uint32_t kTrCols = 512;
+// TMEM columns of a row tile
+constexpr uint32_t kColS = 0, kColPhi = 64, kColPlo = 96, kColO = 128, kColTile = 256;
 
-__device__ __forceinline__ bool attends(const TreeAttnParams& p, int t, int64_t pos) {
-  if (pos < p.n_past) return true;
-  const int j = (int)(pos - p.n_past);
-  if (!p.mask) return j <= t;
-  return (p.mask[(int64_t)t * ((p.T + 31) / 32) + (j >> 5)] >> (j & 31)) & 1u;
+template <int D>
+struct TrSmem {
+  static constexpr int plane_q = kTrRows * D * 2, plane_kv = kTrTile * D * 2;
+  static constexpr int q = 0;                      // [2 tiles][hi, lo]
+  static constexpr int k = q + 4 * plane_q;        // [hi, lo]
+  static constexpr int v = k + 2 * plane_kv;
+  static constexpr int col = v + 2 * plane_kv;     // float [kTrSlots][3][64]: key factor, value exponent, what takes it out of the sum
+  static constexpr int rowf = col + kTrSlots * 3 * kTrTile * 4;  // float [256]: scale * log2(e) * the row's factor
+  static constexpr int bars = rowf + 2 * kTrRows * 4;
+  static constexpr int n_bars = 4 + kTrSlots + 8 + 1;
+  static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
+  static constexpr int used = misc + 16;
+  // above half of an SM's shared memory: two CTAs must not share its TMEM
+  static constexpr int total = used > 120 * 1024 ? used : 120 * 1024;
+};
+static_assert(TrSmem<128>::total <= 227 * 1024, "shared memory of one CTA");
+
+struct TreeSplit {
+  int32_t R, RG, S, per;  // rows of a KV head, groups of 256, splits, steps of 64 positions per split
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <bool Q8>
-__device__ __forceinline__ float cached(const TreeAttnParams& p, const void* c, int kvh, int64_t pos, int e) {
-  if (!Q8) return ((const float*)c)[(pos * p.HKV + kvh) * p.D + e];
-  const int64_t at = (int64_t)kvh * p.n_ctx + pos, plane = (int64_t)p.HKV * p.n_ctx * p.D;
-  return __fmul_rn((float)((const int8_t*)c)[at * p.D + e],
-                   __half2float(((const __half*)((const uint8_t*)c + plane))[at * (p.D / 32) + (e >> 5)]));
+// D (+)= A B, f32 += f16 x f16; A from shared memory or (TS) from TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+      : "memory");
 }
 
-// One CTA per (head, token), 128 positions at a time.
-template <bool Q8>
-__global__ void __launch_bounds__(kTrNT) attn_tree_kernel(const TreeAttnParams p) {
-  __shared__ float q[128], e_s[kTrNT], red[kTrNT / 32];
-  const int h = blockIdx.x, t = blockIdx.y, tid = threadIdx.x, kvh = h / (p.H / p.HKV);
-  const int64_t n_kv = p.n_past + p.T;
-  if (tid < p.D) q[tid] = p.q[t * p.q_stride + (int64_t)h * p.D + tid];
-  float m = -INFINITY, l = 0.0f, acc = 0.0f;
-  for (int64_t t0 = 0; t0 < n_kv; t0 += kTrNT) {
-    __syncthreads();
-    const int64_t pos = t0 + tid;
-    float s = -INFINITY;
-    if (pos < n_kv && attends(p, t, pos)) {
-      s = 0.0f;
-      for (int e = 0; e < p.D; e++) s = __fmaf_rn(q[e], cached<Q8>(p, p.cache_k, kvh, pos, e), s);
-      s = __fmul_rn(s, p.scale);
-      if (s != s) s = INFINITY;  // (the maximum passes a NaN over; e^(inf - inf) brings it back)
-    }
-    const float wm = warp_max(s);
-    if ((tid & 31) == 0) red[tid >> 5] = wm;
-    __syncthreads();
-    float mn = m;
-    for (int w = 0; w < kTrNT / 32; w++) mn = fmaxf(mn, red[w]);
-    if (mn == -INFINITY) continue;
-    e_s[tid] = expf(s - mn);
-    __syncthreads();
-    const float f = expf(m - mn);
-    l = __fmul_rn(l, f);
-    acc = __fmul_rn(acc, f);
-    m = mn;
-    const int n = (int)min((int64_t)kTrNT, n_kv - t0);
-    for (int i = 0; i < n; i++) {
-      l = __fadd_rn(l, e_s[i]);
-      if (tid < p.D && e_s[i] != 0.0f) acc = __fmaf_rn(e_s[i], cached<Q8>(p, p.cache_v, kvh, t0 + i, tid), acc);
+#define MI_R8(a, i) a[i], a[i + 1], a[i + 2], a[i + 3], a[i + 4], a[i + 5], a[i + 6], a[i + 7]
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+      "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(addr));
+}
+// tcgen05.wait::ld with the loaded registers threaded through it, so that none
+// of their uses is scheduled before it.
+__device__ __forceinline__ void tmem_wait_ld(float* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                 "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]),
+                 "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]),
+                 "+f"(r[30]), "+f"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Eight floats (scaled) as the two fp16 planes' 16-byte pieces.
+__device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float a = __fmul_rn(x[2 * i], f), b = __fmul_rn(x[2 * i + 1], f);
+    const __half2 hh = __floats2half2_rn(a, b);
+    const float2 back = __half22float2(hh);
+    h[i] = h2_bits(hh);
+    l[i] = h2_bits(__floats2half2_rn(__fsub_rn(a, back.x), __fsub_rn(b, back.y)));
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// A row of floats held by four lanes (lane bits 3 and 4), N values each: the
+// exponent e that brings its largest magnitude to [2^14, 2^15) as 2^(14 - e), or
+// false where the row holds an infinity or a NaN. Rows below 2^-100 keep e = -100:
+// their halves lose bits below 2^-138, nothing that a float sum of products shows.
+template <int N>
+__device__ __forceinline__ bool row_exponent(const float* x, int& e) {
+  float m = 0.0f;
+  bool fine = true;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    m = fmaxf(m, fabsf(x[i]));
+    fine &= fabsf(x[i]) <= 3.402823466e38f;
+  }
+  if (!fine) m = INFINITY;
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+  e = max((int)(__float_as_uint(m) >> 23) - 127, -100);
+  return m <= 3.402823466e38f;
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
+
+// 64 positions of one cache (keys or values) of one KV head, by four warps: a
+// warp takes rows of eight positions, lane = position % 8 + 8 * g, and of each 32
+// dims the eight g * 8... -- a block of 32 dims in four lanes, 16-byte pieces of
+// the two planes in core matrices of 8 positions x 8 dims.
+template <int D, bool Q8>
+struct KvTile {
+  static constexpr int NC = D / 32;
+  // what a lane holds of its two rows
+  uint2 q[Q8 ? 2 : 1][Q8 ? NC : 1];
+  uint16_t d[Q8 ? 2 : 1][Q8 ? NC : 1];
+  float x[Q8 ? 1 : 2][Q8 ? 1 : NC * 8];
+
+  __device__ __forceinline__ void load(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv,
+                                       int w, int lane) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int64_t pos = pos0 + (w + 4 * k) * 8 + (lane & 7);
+      const int g = lane >> 3;
+      const bool in = pos < n_kv;
+      if (Q8) {
+        const int64_t at = (int64_t)kvh * p.n_ctx + (in ? pos : 0);
+        const uint8_t* qs = (const uint8_t*)cache + at * D + 8 * g;
+        const uint16_t* ds = (const uint16_t*)((const uint8_t*)cache + (int64_t)p.HKV * p.n_ctx * D) + at * NC;
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+          q[k][i] = in ? *(const uint2*)(qs + 32 * i) : make_uint2(0u, 0u);
+          d[k][i] = in ? ds[i] : (uint16_t)0;
+        }
+      } else {
+        const float* src = (const float*)cache + ((in ? pos : 0) * p.HKV + kvh) * D + 8 * g;
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+          const float4 a = in ? *(const float4*)(src + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 b = in ? *(const float4*)(src + 32 * i + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+          float* o = &x[k][8 * i];
+          o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
+        }
+      }
     }
   }
-  if (tid < p.D) p.out[((int64_t)t * p.H + h) * p.D + tid] = l == 0.0f ? 0.0f : __fdiv_rn(acc, l);
+
+  // The exponent by which row k's planes are scaled down (the row is planes *
+  // 2^e), or false for a row with a NaN scale, an infinity or a NaN.
+  __device__ __forceinline__ bool exponent(int k, int& e) const {
+    if (Q8) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < NC; i++) m = max(m, (uint32_t)d[k][i] & 0x7fffu);
+      e = max((int)(m >> 10), 1) - 15;  // the largest scale becomes 1..2 (below it for subnormal ones)
+      return m < 0x7c00u;
+    }
+    const bool fine = row_exponent<NC * 8>(x[k], e);
+    e -= 14;
+    return fine;
+  }
+
+  __device__ __forceinline__ void store(uint8_t* planes, int w, int lane, const int (&e)[2], const bool (&fine)[2]) const {
+    constexpr int plane = kTrTile * D * 2;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      uint8_t* dst = planes + (w + 4 * k) * (16 * D) + (lane >> 3) * 128 + (lane & 7) * 16;
+#pragma unroll
+      for (int i = 0; i < NC; i++) {
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+        if (fine[k]) {
+          if (Q8) {
+            const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+            // 2^-e: fp16 holds 2^14 down to 2^-15
+            const __half2 f = __half2half2(__hmul_rn(__ushort_as_half(d[k][i]), __float2half_rn(pow2f(-e[k]))));
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const uint32_t b = j < 2 ? q[k][i].x : q[k][i].y;
+              // two signed bytes as fp16: 1024 + (byte + 128) - 1152
+              const uint32_t t = __byte_perm(b, 0x64646464u, j & 1 ? 0x7362 : 0x5140) ^ 0x00800080u;
+              const __half2 n = __hsub2_rn(*reinterpret_cast<const __half2*>(&t), off);
+              const __half2 hh = __hmul2_rn(n, f);
+              h[j] = h2_bits(hh);
+              l[j] = h2_bits(__hfma2(n, f, __hneg2(hh)));
+            }
+            hi = make_uint4(h[0], h[1], h[2], h[3]);
+            lo = make_uint4(l[0], l[1], l[2], l[3]);
+          } else {
+            split8(&x[k][8 * i], pow2f(-e[k]), hi, lo);
+          }
+        }
+        *(uint4*)(dst + i * 512) = hi;
+        *(uint4*)(dst + plane + i * 512) = lo;
+      }
+    }
+  }
+};
+
+// Bit c: whether token t attends to position pos0 + c (c < 64).
+__device__ __forceinline__ uint64_t attended64(const TreeAttnParams& p, int t, int64_t pos0, int64_t n_kv) {
+  uint64_t m = 0;
+  const int64_t j0 = pos0 - p.n_past;  // drafted index of bit 0 (negative: cached text)
+  if (p.mask) {
+    const int words = (p.T + 31) >> 5;
+    const uint32_t* row = p.mask + (int64_t)t * words;
+    // words that hold drafted tokens j0 .. j0 + 63
+    for (int w = max(0, (int)max(j0, (int64_t)0) >> 5); w < words && (int64_t)w * 32 < j0 + 64; w++) {
+      const int64_t sh = (int64_t)w * 32 - j0;
+      const uint64_t v = row[w];
+      m |= sh >= 0 ? v << sh : v >> -sh;
+    }
+  } else {
+    const int64_t n = (int64_t)t - j0 + 1;  // drafted tokens 0..t
+    m = n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+  }
+  if (j0 < 0) m |= j0 <= -64 ? ~0ull : (1ull << -j0) - 1;
+  const int64_t left = n_kv - pos0;
+  if (left < 64) m &= left <= 0 ? 0ull : (1ull << left) - 1;
+  return m;
+}
+
+template <int D, bool Q8>
+__global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_constant__ TreeAttnParams p,
+                                                                  const TreeSplit sp, const int vec_q) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  using L = TrSmem<D>;
+  constexpr int NC = D / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * 2 * kTrRows;
+  const int rep = p.H / p.HKV;
+  const int64_t n_kv = (int64_t)p.n_past + p.T;
+  const int64_t pos0 = (int64_t)split * sp.per * kTrTile;
+  const int n = (int)min((int64_t)sp.per, (n_kv - pos0 + kTrTile - 1) / kTrTile);  // steps of this CTA, at least one
+  const int nt = min(2, (sp.R - r0 + kTrRows - 1) / kTrRows);                      // row tiles in use
+  float* col = (float*)(smem + L::col);
+  float* rowf = (float*)(smem + L::rowf);
+  uint64_t* k_full = (uint64_t*)(smem + L::bars);
+  uint64_t* k_empty = k_full + 1;
+  uint64_t* v_full = k_full + 2;
+  uint64_t* v_empty = k_full + 3;
+  uint64_t* col_full = k_full + 4;          // [kTrSlots]
+  uint64_t* s_full = col_full + kTrSlots;   // [2]
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* p_full = s_full + 4;
+  uint64_t* pv_done = s_full + 6;
+  uint64_t* drain = s_full + 8;
+  uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
+  volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
+
+  if (tid == 0) {
+    mbar_init(k_full, 4);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 4);
+    mbar_init(v_empty, 1);
+    for (int i = 0; i < kTrSlots; i++) mbar_init(&col_full[i], 8);
+    for (int t = 0; t < 2; t++) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_empty[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&pv_done[t], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kTrWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_base)),
+                 "r"(kTrCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // the queries' planes: a warp takes eight rows, four lanes a row
+  for (int g8 = warp; g8 < nt * (kTrRows / 8); g8 += kTrThreads / 32) {
+    const int lr = g8 * 8 + (lane & 7), r = r0 + lr, g = lane >> 3;
+    float x[NC * 8];
+    const int i = r / rep;
+    const float* src = p.q + i * p.q_stride + (int64_t)(kvh * rep + r - i * rep) * D + 8 * g;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < sp.R) {
+          if (vec_q) a = *(const float4*)(src + 32 * c + e);
+          else a = make_float4(src[32 * c + e], src[32 * c + e + 1], src[32 * c + e + 2], src[32 * c + e + 3]);
+        }
+        x[8 * c + e] = a.x, x[8 * c + e + 1] = a.y, x[8 * c + e + 2] = a.z, x[8 * c + e + 3] = a.w;
+      }
+    int e;
+    const bool fine = row_exponent<NC * 8>(x, e);
+    uint8_t* dst = smem + L::q + (lr / kTrRows) * 2 * L::plane_q + ((lr & (kTrRows - 1)) >> 3) * (16 * D) + g * 128 + (lr & 7) * 16;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+      if (fine) split8(&x[8 * c], pow2f(14 - e), hi, lo);
+      *(uint4*)(dst + c * 512) = hi;
+      *(uint4*)(dst + L::plane_q + c * 512) = lo;
+    }
+    // (a query with an infinity or a NaN: every score becomes NaN)
+    if (g == 0) rowf[lr] = fine ? __fmul_rn(__fmul_rn(p.scale, 1.4426950408889634f), pow2f(e - 14)) : __int_as_float(0x7fffffff);
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_base;
+
+  if (warp >= kTrWarpMma) {
+    // ---------------- MMA issue (one thread) ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTrTile >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
+      // (bit 16: B, the values, is dims-major)
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
+      const uint64_t qd = umma_desc(smem_addr(smem + L::q), 128, 16 * D);
+      const uint64_t kd = umma_desc(smem_addr(smem + L::k), 128, 16 * D);
+      const uint64_t vd = umma_desc(smem_addr(smem + L::v), 16 * D, 128);
+      auto scores = [&](int t) {
+        const uint32_t d = tmem + t * kColTile + kColS;
+        const uint64_t qh = qd + (uint64_t)((t * 2 * L::plane_q) >> 4), ql = qh + (uint64_t)(L::plane_q >> 4);
+        const uint64_t kh = kd, kl = kd + (uint64_t)(L::plane_kv >> 4);
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) mma_ss(d, ql + 16 * s, kh + 16 * s, idesc_s, s > 0);
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kl + 16 * s, idesc_s, 1);
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kh + 16 * s, idesc_s, 1);
+        umma_commit(&s_full[t]);
+      };
+      auto values = [&](int t, bool first) {
+        const uint32_t o = tmem + t * kColTile + kColO, ph = tmem + t * kColTile + kColPhi, pl = tmem + t * kColTile + kColPlo;
+        const uint64_t vh = vd, vl = vd + (uint64_t)(L::plane_kv >> 4);
+#pragma unroll
+        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, pl + 8 * s, vh + 2 * D * s, idesc_o, !(first && s == 0));
+#pragma unroll
+        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, ph + 8 * s, vl + 2 * D * s, idesc_o, 1);
+#pragma unroll
+        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, ph + 8 * s, vh + 2 * D * s, idesc_o, 1);
+        umma_commit(&pv_done[t]);
+      };
+      bool ok = tc_wait1(k_full, 0, abort_flag, p.err);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < nt; t++) scores(t);
+        umma_commit(k_empty);
+      }
+      for (int j = 0; j < n && ok; j++) {
+        const uint32_t ph = j & 1;
+        for (int t = 0; t < nt && ok; t++) {
+          // the next step's scores as soon as this one's have been read
+          if (j + 1 < n) {
+            if (t == 0 && !(ok = tc_wait1(k_full, ph ^ 1, abort_flag, p.err))) break;
+            if (!(ok = tc_wait1(&s_empty[t], ph, abort_flag, p.err))) break;
+            tc_fence_after();
+            scores(t);
+            if (t == nt - 1) umma_commit(k_empty);
+          }
+          if (t == 0 && !(ok = tc_wait1(v_full, ph, abort_flag, p.err))) break;
+          if (!(ok = tc_wait1(&p_full[t], ph, abort_flag, p.err))) break;
+          tc_fence_after();
+          values(t, j == 0);
+          if (t == nt - 1) umma_commit(v_empty);
+        }
+      }
+      // every MMA has finished before TMEM and shared memory are given back
+      umma_commit(drain);
+      for (uint32_t it = 0; it < kSpinLimit && !mbar_test(drain, 0); it++) {
+      }
+    }
+  } else if (warp >= kTrWarpK) {
+    // ---------------- keys (warps 8-11) and values (12-15) ----------------
+    const bool is_v = warp >= kTrWarpV;
+    const int w = warp & 3;
+    const void* cache = is_v ? p.cache_v : p.cache_k;
+    uint8_t* planes = smem + (is_v ? L::v : L::k);
+    uint64_t* full = is_v ? v_full : k_full;
+    uint64_t* empty = is_v ? v_empty : k_empty;
+    KvTile<D, Q8> kv, next;
+    if (Q8) kv.load(p, cache, kvh, pos0, n_kv, w, lane);
+    for (int j = 0; j < n; j++) {
+      // (a step of F32 rows takes too many registers to be held twice)
+      if (!Q8) kv.load(p, cache, kvh, pos0 + (int64_t)j * kTrTile, n_kv, w, lane);
+      else if (j + 1 < n) next.load(p, cache, kvh, pos0 + (int64_t)(j + 1) * kTrTile, n_kv, w, lane);
+      int e[2];
+      bool fine[2];
+      float* c = col + (j & (kTrSlots - 1)) * 3 * kTrTile;
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        fine[k] = kv.exponent(k, e[k]);
+        if (lane < 8) {
+          const int at = (w + 4 * k) * 8 + lane;
+          const float bad = __int_as_float(0x7fffffff);
+          if (is_v) {
+            c[kTrTile + at] = fine[k] ? (float)e[k] : bad;
+            // (finite in every case: a masked position's weight is 0 whatever its row holds)
+            c[2 * kTrTile + at] = !fine[k] ? 0.0f : Q8 ? pow2f(-e[k]) : (float)e[k];
+          } else {
+            c[at] = fine[k] ? pow2f(e[k]) : bad;
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&col_full[j & (kTrSlots - 1)]);
+      if (j > 0 && !tc_wait_warp(empty, (j - 1) & 1, abort_flag, p.err)) break;
+      kv.store(planes, w, lane, e, fine);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(full);
+      if (Q8) kv = next;
+    }
+  } else {
+    // ---------------- softmax: one thread per row ----------------
+    const int t = warp >> 2, lr = tid, r = r0 + lr, i = min(r, sp.R - 1) / rep;
+    const uint32_t base = tmem + t * kColTile + ((uint32_t)(32 * (warp & 3)) << 16);
+    float M = -INFINITY, l = 0.0f;  // reference of P and O; sum of the weights (F32 cache: relative to ml)
+    float ml = -INFINITY;
+    bool done = false;
+    if (t < nt) {
+      const float rf = rowf[lr];
+      done = true;
+      for (int j = 0; j < n; j++) {
+        const int64_t pt = pos0 + (int64_t)j * kTrTile;
+        const float* c = col + (j & (kTrSlots - 1)) * 3 * kTrTile;
+        if (!tc_wait_warp(&col_full[j & (kTrSlots - 1)], (j / kTrSlots) & 1, abort_flag, p.err) ||
+            !tc_wait_warp(&s_full[t], j & 1, abort_flag, p.err)) {
+          done = false;
+          break;
+        }
+        tc_fence_after();
+        float x[kTrTile];
+        tmem_ld32(base + kColS, x);
+        tmem_ld32(base + kColS + 32, x + 32);
+        tmem_wait_ld(x);
+        tmem_wait_ld(x + 32);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&s_empty[t]);
+        float mx = -INFINITY, ms = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kTrTile; k += 4) {
+          const float4 kf = *(const float4*)(c + k), ve = *(const float4*)(c + kTrTile + k);
+          x[k] = __fmaf_rn(x[k], __fmul_rn(kf.x, rf), ve.x);
+          x[k + 1] = __fmaf_rn(x[k + 1], __fmul_rn(kf.y, rf), ve.y);
+          x[k + 2] = __fmaf_rn(x[k + 2], __fmul_rn(kf.z, rf), ve.z);
+          x[k + 3] = __fmaf_rn(x[k + 3], __fmul_rn(kf.w, rf), ve.w);
+        }
+        if (pt + kTrTile > p.n_past) {
+          const uint64_t m = attended64(p, i, pt, n_kv);
+#pragma unroll
+          for (int k = 0; k < kTrTile; k++)
+            if (!((m >> k) & 1)) x[k] = -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < kTrTile; k++) mx = fmaxf(mx, x[k]);
+        if (!Q8) {
+#pragma unroll
+          for (int k = 0; k < kTrTile; k++) ms = fmaxf(ms, __fsub_rn(x[k], c[2 * kTrTile + k]));
+        }
+        float f = 1.0f;
+        if (mx > M + 8.0f || (j == 0)) {
+          f = j == 0 ? 1.0f : exp2_approx(__fsub_rn(M, mx));
+          M = mx;
+          if (Q8) l = __fmul_rn(l, f);
+        }
+        const float Ms = M == -INFINITY ? 0.0f : __fsub_rn(M, 7.0f);
+        float mls = 0.0f;
+        if (!Q8) {
+          if (ms > ml) {
+            l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, ms)));
+            ml = ms;
+          }
+          mls = ml == -INFINITY ? 0.0f : ml;
+        }
+        // P and O of the step before have been used
+        if (j > 0) {
+          if (!tc_wait_warp(&pv_done[t], (j - 1) & 1, abort_flag, p.err)) {
+            done = false;
+            break;
+          }
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, f != 1.0f)) {
+#pragma unroll 1
+            for (int o = 0; o < D; o += 32) {
+              float y[32];
+              tmem_ld32(base + kColO + o, y);
+              tmem_wait_ld(y);
+              uint32_t z[32];
+#pragma unroll
+              for (int k = 0; k < 32; k++) z[k] = __float_as_uint(__fmul_rn(y[k], f));
+              tmem_st16(base + kColO + o, z);
+              tmem_st16(base + kColO + o + 16, z + 16);
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < kTrTile; h += 32) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const float4 vf = *(const float4*)(c + 2 * kTrTile + h + k);
+            float pe[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) pe[u] = exp2_approx(__fsub_rn(x[h + k + u], Ms));
+            if (Q8) {
+              l = __fmaf_rn(pe[0], vf.x, l);
+              l = __fmaf_rn(pe[1], vf.y, l);
+              l = __fmaf_rn(pe[2], vf.z, l);
+              l = __fmaf_rn(pe[3], vf.w, l);
+            } else {
+              l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[h + k], vf.x), mls)));
+              l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[h + k + 1], vf.y), mls)));
+              l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[h + k + 2], vf.z), mls)));
+              l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[h + k + 3], vf.w), mls)));
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u += 2) {
+              const __half2 hh = __floats2half2_rn(pe[u], pe[u + 1]);
+              const float2 back = __half22float2(hh);
+              hi[(k + u) / 2] = h2_bits(hh);
+              lo[(k + u) / 2] = h2_bits(__floats2half2_rn(__fsub_rn(pe[u], back.x), __fsub_rn(pe[u + 1], back.y)));
+            }
+          }
+          tmem_st16(base + kColPhi + h / 2, hi);
+          tmem_st16(base + kColPlo + h / 2, lo);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&p_full[t]);
+      }
+      if (done && tc_wait_warp(&pv_done[t], (n - 1) & 1, abort_flag, p.err)) {
+        tc_fence_after();
+        const float Ms = M == -INFINITY ? 0.0f : __fsub_rn(M, 7.0f), mls = Q8 ? Ms : ml == -INFINITY ? 0.0f : ml;
+        float* rec = (float*)p.scratch + (((int64_t)kvh * sp.S + split) * sp.R + r) * (D + 4);
+        float* out = p.out + ((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D;
+        const bool whole = sp.S == 1;
+        // one split: the result itself; a token that attends to nothing has l = 0
+        const float inv = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), exp2_approx(__fsub_rn(Ms, mls)));
+        if (!whole && r < sp.R) *(float4*)rec = make_float4(M == -INFINITY ? -INFINITY : Ms, Q8 ? (M == -INFINITY ? -INFINITY : Ms) : ml, l, 0.0f);
+#pragma unroll 1
+        for (int o = 0; o < D; o += 32) {
+          float y[32];
+          tmem_ld32(base + kColO + o, y);
+          tmem_wait_ld(y);
+          if (r < sp.R) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              if (whole) {
+                out[o + k] = __fmul_rn(y[k], inv);
+                out[o + k + 1] = __fmul_rn(y[k + 1], inv);
+                out[o + k + 2] = __fmul_rn(y[k + 2], inv);
+                out[o + k + 3] = __fmul_rn(y[k + 3], inv);
+              } else {
+                *(float4*)(rec + 4 + o + k) = make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kTrWarpMma) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTrCols));
+  }
+}
+
+// Joins the splits of one row: with a_s = 2^(M_s - max M) and b_s = 2^(m_s - max m),
+// out = sum a_s O_s / sum b_s l_s * 2^(max M - max m). A CTA per row, its warps over
+// the splits, the lanes over the dims.
+constexpr int kTrJoinNT = 128;
+template <int D>
+__global__ void __launch_bounds__(kTrJoinNT) attn_tree_join_kernel(const TreeAttnParams p, const TreeSplit sp) {
+  __shared__ float red[kTrJoinNT / 32][D + 1];
+  pdl_wait();
+  const int r = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float* rec = (const float*)p.scratch + ((int64_t)kvh * sp.S * sp.R + r) * (D + 4);
+  const int64_t step = (int64_t)sp.R * (D + 4);
+  float M = -INFINITY, m = -INFINITY;
+  for (int s = lane; s < sp.S; s += 32) {
+    const float2 h = *(const float2*)(rec + s * step);
+    M = fmaxf(M, h.x);
+    m = fmaxf(m, h.y);
+  }
+  M = warp_max(M);
+  m = warp_max(m);
+  const float Mr = M == -INFINITY ? 0.0f : M, mr = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, acc[D / 32];
+#pragma unroll
+  for (int k = 0; k < D / 32; k++) acc[k] = 0.0f;
+#pragma unroll 4
+  for (int s = warp; s < sp.S; s += kTrJoinNT / 32) {
+    const float* x = rec + s * step;
+    const float4 h = *(const float4*)x;
+    const float a = exp2_approx(__fsub_rn(h.x, Mr));
+    l = __fmaf_rn(h.z, exp2_approx(__fsub_rn(h.y, mr)), l);
+#pragma unroll
+    for (int k = 0; k < D / 32; k++) acc[k] = __fmaf_rn(x[4 + lane + 32 * k], a, acc[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < D / 32; k++) red[warp][lane + 32 * k] = acc[k];
+  if (lane == 0) red[warp][D] = l;
+  __syncthreads();
+  if (tid < D) {
+    float o = red[0][tid];
+    l = red[0][D];
+#pragma unroll
+    for (int w = 1; w < kTrJoinNT / 32; w++) {
+      o = __fadd_rn(o, red[w][tid]);
+      l = __fadd_rn(l, red[w][D]);
+    }
+    const int rep = p.H / p.HKV, i = r / rep;
+    p.out[((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D + tid] =
+        l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(o, l), exp2_approx(__fsub_rn(Mr, mr)));
+  }
+}
+
+constexpr int kTrSms = 148;
+
+int64_t most_splits(int64_t H, int64_t HKV, int64_t n_kv, int64_t T) {
+  const int64_t RG = (T * (H / HKV) + 2 * kTrRows - 1) / (2 * kTrRows), steps = (n_kv + kTrTile - 1) / kTrTile;
+  return std::min(steps, std::max<int64_t>(1, kTrSms / std::max<int64_t>(1, HKV * RG)));
+}
+
+template <int D, bool Q8>
+cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
+  TreeSplit sp{};
+  sp.R = p.T * (p.H / p.HKV);
+  sp.RG = (sp.R + 2 * kTrRows - 1) / (2 * kTrRows);
+  const int64_t n_kv = (int64_t)p.n_past + p.T, steps = (n_kv + kTrTile - 1) / kTrTile;
+  const int64_t most = most_splits(p.H, p.HKV, n_kv, p.T);
+  sp.per = (int32_t)((steps + most - 1) / most);
+  sp.S = (int32_t)((steps + sp.per - 1) / sp.per);
+  const int vec_q = (uintptr_t)p.q % 16 == 0 && p.q_stride % 4 == 0;
+  attn_tree_kernel<D, Q8><<<dim3((unsigned)sp.S, (unsigned)p.HKV, (unsigned)sp.RG), kTrThreads, TrSmem<D>::total, s>>>(p, sp, vec_q);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || sp.S == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)sp.R, (unsigned)p.HKV);
+  cfg.blockDim = dim3(kTrJoinNT);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_tree_join_kernel<D>, p, sp);
+}
+
+template <int D>
+cudaError_t prepare_tree() {
+  const cudaError_t e = cudaFuncSetAttribute(attn_tree_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D>::total);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(attn_tree_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D>::total);
 }
 
 }  // namespace
 
 bool attn_tree_fits(int64_t D, int64_t H, int64_t HKV, int64_t T) {
-  return (D == 32 || D == 64 || D == 96 || D == 128) && H > 0 && HKV > 0 && H % HKV == 0 && H <= 65535 && T >= 0 &&
+  return (D == 32 || D == 64 || D == 96 || D == 128) && H > 0 && HKV > 0 && H % HKV == 0 && H <= 4096 && T >= 0 &&
          T <= kTreeMaxTokens;
 }
 
-size_t attn_tree_scratch_bytes(int64_t H, int64_t HKV, int64_t n_kv, int64_t T, int64_t D) { return 16; }
+// Records of all splits, for up to n_kv rows and T tokens: a KV head's groups of
+// 256 rows times its splits pass kTrSms / HKV only where one group alone does.
+size_t attn_tree_scratch_bytes(int64_t H, int64_t HKV, int64_t n_kv, int64_t T, int64_t D) {
+  const int64_t R = T * (H / HKV), steps = (n_kv + kTrTile - 1) / kTrTile;
+  const int64_t rows = std::min(steps * R, std::max(R, (kTrSms + HKV - 1) / HKV * 2 * kTrRows));
+  return (size_t)(16 + HKV * rows * (D + 4) * 4);
+}
+
+cudaError_t prepare_attn_tree_kernels() {
+  cudaError_t e = prepare_tree<32>();
+  if (e == cudaSuccess) e = prepare_tree<64>();
+  if (e == cudaSuccess) e = prepare_tree<96>();
+  if (e == cudaSuccess) e = prepare_tree<128>();
+  return e;
+}
 
 cudaError_t launch_attn_tree(const TreeAttnParams& p, cudaStream_t s) {
   if (p.T == 0) return cudaSuccess;
-  const dim3 grid((unsigned)p.H, (unsigned)p.T);
-  if (p.q8) attn_tree_kernel<true><<<grid, kTrNT, 0, s>>>(p);
-  else attn_tree_kernel<false><<<grid, kTrNT, 0, s>>>(p);
-  return cudaGetLastError();
+  switch (p.D) {
+    case 32: return p.q8 ? launch_tree<32, true>(p, s) : launch_tree<32, false>(p, s);
+    case 64: return p.q8 ? launch_tree<64, true>(p, s) : launch_tree<64, false>(p, s);
+    case 96: return p.q8 ? launch_tree<96, true>(p, s) : launch_tree<96, false>(p, s);
+    case 128: return p.q8 ? launch_tree<128, true>(p, s) : launch_tree<128, false>(p, s);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
 }  // namespace mi

@@ -463,9 +463,11 @@ struct TreeAttnParams {
   float scale;
   void* scratch;
   float* out;  // [T][H][D]
+  int32_t* err;
 };
 bool attn_tree_fits(int64_t D, int64_t H, int64_t HKV, int64_t T);
 size_t attn_tree_scratch_bytes(int64_t H, int64_t HKV, int64_t n_kv, int64_t T, int64_t D);
+cudaError_t prepare_attn_tree_kernels();  // per device, at init
 cudaError_t launch_attn_tree(const TreeAttnParams& p, cudaStream_t s);
 
 struct LogitsParams {

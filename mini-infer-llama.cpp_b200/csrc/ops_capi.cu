@@ -568,7 +568,7 @@ static int attention_tree_common(const char* name, const float* d_q, int64_t q_s
                  (uintptr_t)d_cache_k % 16 == 0 && (uintptr_t)d_cache_v % 16 == 0 && (uintptr_t)d_scratch % 16 == 0,
              std::string(name) + ": bad arguments (16-byte aligned caches and scratch)");
   MI_REQUIRE(attn_tree_fits(head_dim, n_head, n_head_kv, n_tokens),
-             std::string(name) + ": head_dim 32, 64, 96 or 128, n_head a multiple of n_head_kv, at most 1024 tokens");
+             std::string(name) + ": head_dim 32, 64, 96 or 128, n_head a multiple of n_head_kv and at most 4096, at most 1024 tokens");
   MI_REQUIRE(q_stride >= n_head * head_dim, std::string(name) + ": q_stride below a row");
   MI_REQUIRE(n_past <= n_ctx - n_tokens, std::string(name) + ": rows behind the cache's last");
   MI_CTX(c);
@@ -587,6 +587,7 @@ static int attention_tree_common(const char* name, const float* d_q, int64_t q_s
   p.mask = d_mask;
   p.scale = scale;
   p.scratch = d_scratch;
+  p.err = c->err;
   p.out = d_dst;
   return cuda_status(launch_attn_tree(p, S(s)), name);
 }

@@ -469,7 +469,7 @@ def tree_mask(parents) -> np.ndarray:
 
 
 def attention_tree_scratch(n_head: int, n_head_kv: int, n_kv: int, n_tokens: int, head_dim: int, device="cuda"):
-    """The workspace of attention_tree / attention_tree_q8_0 for up to n_kv = n_past + n_tokens rows."""
+    """The workspace of attention_tree / attention_tree_q8_0 for up to n_kv = n_past + n_tokens rows and n_tokens tokens."""
     torch = _torch()
     nb = lib().mi_cuda_attention_tree_scratch_bytes(n_head, n_head_kv, n_kv, n_tokens, head_dim)
     if nb == 0:

@@ -99,6 +99,11 @@ def test_attention_tree_scratch_bytes():
         for t in (1, 2, 7, 33, 64, 200):
             n = [fn(h, kv, m, t, d) for m in sorted({t, 300, 1000, 1024, 2047, 4096, 5000, 8191, 20000, 32768, 131072, 1 << 20})]
             assert n == sorted(n)
+    # and for fewer tokens
+    for h, kv, d in ((14, 2, 64), (28, 4, 128), (16, 16, 32), (6, 2, 96), (96, 1, 64)):
+        for m in (1024, 32768):
+            n = [fn(h, kv, m, t, d) for t in range(1, 1025)]
+            assert n == sorted(n)
 
 
 @pytest.mark.parametrize("bad", [dict(x=None), dict(out=None), dict(v=0), dict(n=-1), dict(n=65536), dict(stride=99), dict(hist=None),
@@ -612,7 +617,7 @@ class Step:
         self.head = rnd(self.H * self.D, self.V) * 0.2
         self.torch, self.rnd = torch, rnd
         self.caches = [mi_cuda.kv_q8_0_cache(self.n_ctx, self.HKV, self.D) for _ in range(2)]
-        self.scratch = mi_cuda.attention_tree_scratch(self.H, self.HKV, self.n_ctx, 64, self.D)
+        self.scratch = mi_cuda.attention_tree_scratch(self.H, self.HKV, self.n_ctx, self.n_ctx, self.D)
 
     def qkv(self, T):
         return self.rnd(T, (self.H + 2 * self.HKV) * self.D)
