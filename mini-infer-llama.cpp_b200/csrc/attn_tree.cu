@@ -22,12 +22,18 @@
 //     score that makes P (P = 2^(s + e - M)), and the sum of the weights takes it
 //     out again.
 //
-// One CTA: up to 256 rows (two tiles of 128, one TMEM lane each) over one range of
-// positions, 64 at a time. Warps 0-7 softmax (a thread per row), 8-11 convert keys
-// and 12-15 values into the MMAs' layout, 16 issues the MMAs. S (64 columns), P's
-// planes (32 + 32) and O (D) of both tiles fill TMEM at D = 128; the two tiles let
-// one's MMAs run under the other's exponentials. The running maximum M moves only
-// when a score passes it by 2^8 (fp16 holds 2^15), so O is rarely rescaled.
+// One CTA: 128 rows (a TMEM lane each) over one range of positions, 64 a step.
+// Warps 0-7 softmax: two threads per row, 32 positions each; 8-11 convert keys and
+// 12-15 values into the MMAs' layout; 16 issues the MMAs. Everything between two
+// roles is doubled (key and value planes in shared memory; S, P and O in TMEM, all
+// of its 512 columns at D = 128), so the MMAs of one step run under the
+// exponentials of another.
+//
+// A step's O is a product of its own, added to the softmax threads' registers
+// (O = O 2^(M_old - M_new) + O_step): the MMA's accumulation cuts instead of
+// rounding, by half an ulp of the accumulator each time, and over a thousand
+// positions accumulated in TMEM that came to 7e-6 of the result, one-signed. For
+// the same reason the small products (hi lo, lo hi) come first in each step.
 //
 // The positions are split over CTAs to fill the GPU; a second kernel joins the
 // splits' (M, sum, O) records.
@@ -42,24 +48,29 @@ namespace mi {
 namespace {
 
 constexpr int kTrTile = 64;      // positions per step
-constexpr int kTrRows = 128;     // rows per tile (MMA M)
+constexpr int kTrRows = 128;     // rows per CTA (MMA M)
 constexpr int kTrWarpK = 8, kTrWarpV = 12, kTrWarpMma = 16;
-constexpr int kTrThreads = 17 * 32;
-constexpr int kTrSlots = 4;      // steps whose column factors are kept
+constexpr int kTrThreads = 20 * 32;  // (the last three warps complete the MMA warp's group for setmaxnreg)
+constexpr int kTrSlots = 8;      // steps whose column factors are kept (see the roles' waits)
 constexpr uint32_t kTrCols = 512;
-// TMEM columns of a row tile
-constexpr uint32_t kColS = 0, kColPhi = 64, kColPlo = 96, kColO = 128, kColTile = 256;
+// TMEM columns of step j: S at 64 (j & 1), P's planes at 128 + 64 (j & 1) and 32
+// behind it, O at 256 + D (j & 1)
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
+// Registers per thread of the roles: launched with 96 x 640 = 61440, of which
+// 136 x 256 + 80 x 256 + 48 x 128 = 61440 are given out again.
+constexpr int kRegsSoftmax = 136, kRegsConvert = 80, kRegsMma = 48;
 
 template <int D>
 struct TrSmem {
   static constexpr int plane_q = kTrRows * D * 2, plane_kv = kTrTile * D * 2;
-  static constexpr int q = 0;                      // [2 tiles][hi, lo]
-  static constexpr int k = q + 4 * plane_q;        // [hi, lo]
-  static constexpr int v = k + 2 * plane_kv;
-  static constexpr int col = v + 2 * plane_kv;     // float [kTrSlots][3][64]: key factor, value exponent, what takes it out of the sum
-  static constexpr int rowf = col + kTrSlots * 3 * kTrTile * 4;  // float [256]: scale * log2(e) * the row's factor
-  static constexpr int bars = rowf + 2 * kTrRows * 4;
-  static constexpr int n_bars = 4 + kTrSlots + 8 + 1;
+  static constexpr int q = 0;                      // [hi, lo]
+  static constexpr int k = q + 2 * plane_q;        // [step & 1][hi, lo]
+  static constexpr int v = k + 4 * plane_kv;
+  static constexpr int col = v + 4 * plane_kv;     // float [kTrSlots][3][64]: key factor, value exponent, what takes it out of the sum
+  static constexpr int rowf = col + kTrSlots * 3 * kTrTile * 4;  // float [128]: scale * log2(e) * the row's factor
+  static constexpr int mx = rowf + kTrRows * 4;    // float [step & 1][half][128]: the halves' maxima (at the end their sums)
+  static constexpr int bars = mx + 4 * kTrRows * 4;
+  static constexpr int n_bars = 8 + kTrSlots + 10 + 4 + 1;
   static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
   static constexpr int used = misc + 16;
   // above half of an SM's shared memory: two CTAs must not share its TMEM
@@ -68,7 +79,7 @@ struct TrSmem {
 static_assert(TrSmem<128>::total <= 227 * 1024, "shared memory of one CTA");
 
 struct TreeSplit {
-  int32_t R, RG, S, per;  // rows of a KV head, groups of 256, splits, steps of 64 positions per split
+  int32_t R, RG, S, per;  // rows of a KV head, groups of 128, splits, steps of 64 positions per split
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -95,7 +106,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
-#define MI_R8(a, i) a[i], a[i + 1], a[i + 2], a[i + 3], a[i + 4], a[i + 5], a[i + 6], a[i + 7]
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -116,6 +126,21 @@ __device__ __forceinline__ void tmem_wait_ld(float* r) {
                  "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]),
                  "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]),
                  "+f"(r[30]), "+f"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16f(uint32_t addr, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld16(float* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
                :
                : "memory");
 }
@@ -260,26 +285,24 @@ struct KvTile {
   }
 };
 
-// Bit c: whether token t attends to position pos0 + c (c < 64).
-__device__ __forceinline__ uint64_t attended64(const TreeAttnParams& p, int t, int64_t pos0, int64_t n_kv) {
-  uint64_t m = 0;
+// Bit c: whether token t attends to position pos0 + c (c < 32).
+__device__ __forceinline__ uint32_t attended32(const TreeAttnParams& p, int t, int64_t pos0, int64_t n_kv) {
+  uint32_t m = 0;
   const int64_t j0 = pos0 - p.n_past;  // drafted index of bit 0 (negative: cached text)
   if (p.mask) {
     const int words = (p.T + 31) >> 5;
     const uint32_t* row = p.mask + (int64_t)t * words;
-    // words that hold drafted tokens j0 .. j0 + 63
-    for (int w = max(0, (int)max(j0, (int64_t)0) >> 5); w < words && (int64_t)w * 32 < j0 + 64; w++) {
-      const int64_t sh = (int64_t)w * 32 - j0;
-      const uint64_t v = row[w];
-      m |= sh >= 0 ? v << sh : v >> -sh;
-    }
+    // the words that hold drafted tokens j0 .. j0 + 31
+    const int64_t w = j0 >= 0 ? j0 >> 5 : 0, sh = w * 32 - j0;  // -31 .. 0, or above 0
+    if (sh < 32 && w < words) m = sh >= 0 ? row[w] << sh : row[w] >> -sh;
+    if (sh < 0 && w + 1 < words) m |= row[w + 1] << (32 + sh);
   } else {
     const int64_t n = (int64_t)t - j0 + 1;  // drafted tokens 0..t
-    m = n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+    m = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
   }
-  if (j0 < 0) m |= j0 <= -64 ? ~0ull : (1ull << -j0) - 1;
+  if (j0 < 0) m |= j0 <= -32 ? ~0u : (1u << -j0) - 1;
   const int64_t left = n_kv - pos0;
-  if (left < 64) m &= left <= 0 ? 0ull : (1ull << left) - 1;
+  if (left < 32) m &= left <= 0 ? 0u : (1u << left) - 1;
   return m;
 }
 
@@ -290,39 +313,44 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   using L = TrSmem<D>;
   constexpr int NC = D / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * 2 * kTrRows;
+  const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTrRows;
   const int rep = p.H / p.HKV;
   const int64_t n_kv = (int64_t)p.n_past + p.T;
   const int64_t pos0 = (int64_t)split * sp.per * kTrTile;
   const int n = (int)min((int64_t)sp.per, (n_kv - pos0 + kTrTile - 1) / kTrTile);  // steps of this CTA, at least one
-  const int nt = min(2, (sp.R - r0 + kTrRows - 1) / kTrRows);                      // row tiles in use
+  const int nq = min(4, (sp.R - r0 + 31) / 32);  // quadrants of 32 rows in use: two softmax warps each
   float* col = (float*)(smem + L::col);
   float* rowf = (float*)(smem + L::rowf);
-  uint64_t* k_full = (uint64_t*)(smem + L::bars);
-  uint64_t* k_empty = k_full + 1;
-  uint64_t* v_full = k_full + 2;
-  uint64_t* v_empty = k_full + 3;
-  uint64_t* col_full = k_full + 4;          // [kTrSlots]
-  uint64_t* s_full = col_full + kTrSlots;   // [2]
+  float* mxs = (float*)(smem + L::mx);
+  uint64_t* k_full = (uint64_t*)(smem + L::bars);  // each [step & 1]
+  uint64_t* k_empty = k_full + 2;
+  uint64_t* v_full = k_full + 4;
+  uint64_t* v_empty = k_full + 6;
+  uint64_t* col_full = k_full + 8;  // [kTrSlots]
+  uint64_t* s_full = col_full + kTrSlots;
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_full + 4;
-  uint64_t* pv_done = s_full + 6;
-  uint64_t* drain = s_full + 8;
+  uint64_t* o_full = s_full + 6;
+  uint64_t* o_empty = s_full + 8;
+  uint64_t* pair = s_full + 10;  // [quadrant]: its two softmax warps
+  uint64_t* drain = s_full + 14;
   uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
   volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
 
   if (tid == 0) {
-    mbar_init(k_full, 4);
-    mbar_init(k_empty, 1);
-    mbar_init(v_full, 4);
-    mbar_init(v_empty, 1);
-    for (int i = 0; i < kTrSlots; i++) mbar_init(&col_full[i], 8);
-    for (int t = 0; t < 2; t++) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&s_empty[t], 4);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&pv_done[t], 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 2 * nq);
+      mbar_init(&p_full[i], 2 * nq);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 2 * nq);
     }
+    for (int i = 0; i < kTrSlots; i++) mbar_init(&col_full[i], 8);
+    for (int i = 0; i < 4; i++) mbar_init(&pair[i], 2);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -333,8 +361,8 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   // the queries' planes: a warp takes eight rows, four lanes a row
-  for (int g8 = warp; g8 < nt * (kTrRows / 8); g8 += kTrThreads / 32) {
-    const int lr = g8 * 8 + (lane & 7), r = r0 + lr, g = lane >> 3;
+  if (warp < kTrRows / 8) {
+    const int lr = warp * 8 + (lane & 7), r = r0 + lr, g = lane >> 3;
     float x[NC * 8];
     const int i = r / rep;
     const float* src = p.q + i * p.q_stride + (int64_t)(kvh * rep + r - i * rep) * D + 8 * g;
@@ -351,7 +379,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       }
     int e;
     const bool fine = row_exponent<NC * 8>(x, e);
-    uint8_t* dst = smem + L::q + (lr / kTrRows) * 2 * L::plane_q + ((lr & (kTrRows - 1)) >> 3) * (16 * D) + g * 128 + (lr & 7) * 16;
+    uint8_t* dst = smem + L::q + (lr >> 3) * (16 * D) + g * 128 + (lr & 7) * 16;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
       uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
@@ -370,59 +398,55 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
 
   if (warp >= kTrWarpMma) {
     // ---------------- MMA issue (one thread) ----------------
-    if (lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
+    if (warp == kTrWarpMma && lane == 0) {
       constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTrTile >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
       // (bit 16: B, the values, is dims-major)
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
-      const uint64_t qd = umma_desc(smem_addr(smem + L::q), 128, 16 * D);
+      const uint64_t qh = umma_desc(smem_addr(smem + L::q), 128, 16 * D), ql = qh + (uint64_t)(L::plane_q >> 4);
       const uint64_t kd = umma_desc(smem_addr(smem + L::k), 128, 16 * D);
       const uint64_t vd = umma_desc(smem_addr(smem + L::v), 16 * D, 128);
-      auto scores = [&](int t) {
-        const uint32_t d = tmem + t * kColTile + kColS;
-        const uint64_t qh = qd + (uint64_t)((t * 2 * L::plane_q) >> 4), ql = qh + (uint64_t)(L::plane_q >> 4);
-        const uint64_t kh = kd, kl = kd + (uint64_t)(L::plane_kv >> 4);
+      constexpr uint64_t plane = L::plane_kv >> 4;
+      bool ok = true;
+      // step j's scores: into S (j & 1) once step j - 2's have been read
+      auto scores = [&](int j) {
+        const int b = j & 1;
+        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+        if (!(ok = tc_wait1(&k_full[b], ph, abort_flag, p.err))) return;
+        if (j >= 2 && !(ok = tc_wait1(&s_empty[b], ph ^ 1, abort_flag, p.err))) return;
+        tc_fence_after();
+        const uint32_t d = tmem + kColS + 64 * b;
+        const uint64_t kh = kd + 2 * plane * b, kl = kh + plane;
 #pragma unroll
         for (int s = 0; s < D / 16; s++) mma_ss(d, ql + 16 * s, kh + 16 * s, idesc_s, s > 0);
 #pragma unroll
         for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kl + 16 * s, idesc_s, 1);
 #pragma unroll
         for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kh + 16 * s, idesc_s, 1);
-        umma_commit(&s_full[t]);
+        umma_commit(&s_full[b]);
+        umma_commit(&k_empty[b]);
       };
-      auto values = [&](int t, bool first) {
-        const uint32_t o = tmem + t * kColTile + kColO, ph = tmem + t * kColTile + kColPhi, pl = tmem + t * kColTile + kColPlo;
-        const uint64_t vh = vd, vl = vd + (uint64_t)(L::plane_kv >> 4);
-#pragma unroll
-        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, pl + 8 * s, vh + 2 * D * s, idesc_o, !(first && s == 0));
-#pragma unroll
-        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, ph + 8 * s, vl + 2 * D * s, idesc_o, 1);
-#pragma unroll
-        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, ph + 8 * s, vh + 2 * D * s, idesc_o, 1);
-        umma_commit(&pv_done[t]);
-      };
-      bool ok = tc_wait1(k_full, 0, abort_flag, p.err);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < nt; t++) scores(t);
-        umma_commit(k_empty);
-      }
+      scores(0);
+      if (ok && n > 1) scores(1);
       for (int j = 0; j < n && ok; j++) {
-        const uint32_t ph = j & 1;
-        for (int t = 0; t < nt && ok; t++) {
-          // the next step's scores as soon as this one's have been read
-          if (j + 1 < n) {
-            if (t == 0 && !(ok = tc_wait1(k_full, ph ^ 1, abort_flag, p.err))) break;
-            if (!(ok = tc_wait1(&s_empty[t], ph, abort_flag, p.err))) break;
-            tc_fence_after();
-            scores(t);
-            if (t == nt - 1) umma_commit(k_empty);
-          }
-          if (t == 0 && !(ok = tc_wait1(v_full, ph, abort_flag, p.err))) break;
-          if (!(ok = tc_wait1(&p_full[t], ph, abort_flag, p.err))) break;
-          tc_fence_after();
-          values(t, j == 0);
-          if (t == nt - 1) umma_commit(v_empty);
-        }
+        if (j > 0 && j + 1 < n) scores(j + 1);
+        if (!ok) break;
+        const int b = j & 1;
+        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+        if (!(ok = tc_wait1(&v_full[b], ph, abort_flag, p.err))) break;
+        if (j >= 2 && !(ok = tc_wait1(&o_empty[b], ph ^ 1, abort_flag, p.err))) break;
+        if (!(ok = tc_wait1(&p_full[b], ph, abort_flag, p.err))) break;
+        tc_fence_after();
+        const uint32_t o = tmem + kColO + D * b, p_hi = tmem + kColP + 64 * b, p_lo = p_hi + 32;
+        const uint64_t vh = vd + 2 * plane * b, vl = vh + plane;
+#pragma unroll
+        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_lo + 8 * s, vh + 2 * D * s, idesc_o, s > 0);
+#pragma unroll
+        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vl + 2 * D * s, idesc_o, 1);
+#pragma unroll
+        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vh + 2 * D * s, idesc_o, 1);
+        umma_commit(&o_full[b]);
+        umma_commit(&v_empty[b]);
       }
       // every MMA has finished before TMEM and shared memory are given back
       umma_commit(drain);
@@ -431,15 +455,19 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     }
   } else if (warp >= kTrWarpK) {
     // ---------------- keys (warps 8-11) and values (12-15) ----------------
+    // A slot of the column factors is written again eight steps later: after the
+    // planes of seven, which waited for the products of five, whose S was free only
+    // when the softmax had gone past step three.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
     const bool is_v = warp >= kTrWarpV;
     const int w = warp & 3;
     const void* cache = is_v ? p.cache_v : p.cache_k;
-    uint8_t* planes = smem + (is_v ? L::v : L::k);
     uint64_t* full = is_v ? v_full : k_full;
     uint64_t* empty = is_v ? v_empty : k_empty;
     KvTile<D, Q8> kv, next;
     if (Q8) kv.load(p, cache, kvh, pos0, n_kv, w, lane);
     for (int j = 0; j < n; j++) {
+      const int b = j & 1;
       // (a step of F32 rows takes too many registers to be held twice)
       if (!Q8) kv.load(p, cache, kvh, pos0 + (int64_t)j * kTrTile, n_kv, w, lane);
       else if (j + 1 < n) next.load(p, cache, kvh, pos0 + (int64_t)(j + 1) * kTrTile, n_kv, w, lane);
@@ -463,160 +491,172 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       }
       __syncwarp();
       if (lane == 0) mbar_arrive_one(&col_full[j & (kTrSlots - 1)]);
-      if (j > 0 && !tc_wait_warp(empty, (j - 1) & 1, abort_flag, p.err)) break;
-      kv.store(planes, w, lane, e, fine);
+      if (j >= 2 && !tc_wait_warp(&empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort_flag, p.err)) break;
+      kv.store(smem + (is_v ? L::v : L::k) + b * 2 * L::plane_kv, w, lane, e, fine);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_one(full);
+      if (lane == 0) mbar_arrive_one(&full[b]);
       if (Q8) kv = next;
     }
   } else {
-    // ---------------- softmax: one thread per row ----------------
-    const int t = warp >> 2, lr = tid, r = r0 + lr, i = min(r, sp.R - 1) / rep;
-    const uint32_t base = tmem + t * kColTile + ((uint32_t)(32 * (warp & 3)) << 16);
-    float M = -INFINITY, l = 0.0f;  // reference of P and O; sum of the weights (F32 cache: relative to ml)
-    float ml = -INFINITY;
-    bool done = false;
-    if (t < nt) {
+    // ---------------- softmax: two threads per row ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int quad = warp & 3, half = warp >> 2;
+    if (quad < nq) {
+      constexpr int NA = D / 2, HT = kTrTile / 2;
+      const int lr = quad * 32 + lane, r = r0 + lr, i = min(r, sp.R - 1) / rep;
+      const uint32_t base = tmem + ((uint32_t)(32 * quad) << 16);
       const float rf = rowf[lr];
-      done = true;
-      for (int j = 0; j < n; j++) {
-        const int64_t pt = pos0 + (int64_t)j * kTrTile;
-        const float* c = col + (j & (kTrSlots - 1)) * 3 * kTrTile;
-        if (!tc_wait_warp(&col_full[j & (kTrSlots - 1)], (j / kTrSlots) & 1, abort_flag, p.err) ||
-            !tc_wait_warp(&s_full[t], j & 1, abort_flag, p.err)) {
-          done = false;
-          break;
-        }
+      float M = -INFINITY, l = 0.0f;  // the row's maximum; this half's weights (Q8_0: relative to M, F32: to ml)
+      float ml = -INFINITY, f_prev = 1.0f;
+      float acc[NA];
+#pragma unroll
+      for (int k = 0; k < NA; k++) acc[k] = 0.0f;
+      // step j's O into the registers
+      auto take_o = [&](int j, float f) {
+        const int b = j & 1;
+        if (!tc_wait_warp(&o_full[b], (uint32_t)(j >> 1) & 1u, abort_flag, p.err)) return false;
         tc_fence_after();
-        float x[kTrTile];
-        tmem_ld32(base + kColS, x);
-        tmem_ld32(base + kColS + 32, x + 32);
-        tmem_wait_ld(x);
-        tmem_wait_ld(x + 32);
+#pragma unroll
+        for (int o = 0; o < NA; o += 16) {
+          float y[16];
+          tmem_ld16f(base + kColO + D * b + NA * half + o, y);
+          tmem_wait_ld16(y);
+#pragma unroll
+          for (int k = 0; k < 16; k++) acc[o + k] = __fmaf_rn(acc[o + k], f, y[k]);
+        }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(&s_empty[t]);
-        float mx = -INFINITY, ms = -INFINITY;
+        if (lane == 0) mbar_arrive_one(&o_empty[b]);
+        return true;
+      };
+      // the row's other half has come as far (its k-th meeting)
+      auto meet = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&pair[quad]);
+        return tc_wait_warp(&pair[quad], (uint32_t)k & 1u, abort_flag, p.err);
+      };
+      bool ok = true;
+      for (int j = 0; j < n; j++) {
+        const int b = j & 1;
+        const int64_t pt = pos0 + (int64_t)j * kTrTile + half * HT;
+        const float* c = col + (j & (kTrSlots - 1)) * 3 * kTrTile + half * HT;
+        ok = tc_wait_warp(&col_full[j & (kTrSlots - 1)], (uint32_t)(j / kTrSlots) & 1u, abort_flag, p.err) &&
+             tc_wait_warp(&s_full[b], (uint32_t)(j >> 1) & 1u, abort_flag, p.err);
+        if (!ok) break;
+        tc_fence_after();
+        float x[HT];
+        tmem_ld32(base + kColS + 64 * b + half * HT, x);
+        tmem_wait_ld(x);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&s_empty[b]);
 #pragma unroll
-        for (int k = 0; k < kTrTile; k += 4) {
+        for (int k = 0; k < HT; k += 4) {
           const float4 kf = *(const float4*)(c + k), ve = *(const float4*)(c + kTrTile + k);
           x[k] = __fmaf_rn(x[k], __fmul_rn(kf.x, rf), ve.x);
           x[k + 1] = __fmaf_rn(x[k + 1], __fmul_rn(kf.y, rf), ve.y);
           x[k + 2] = __fmaf_rn(x[k + 2], __fmul_rn(kf.z, rf), ve.z);
           x[k + 3] = __fmaf_rn(x[k + 3], __fmul_rn(kf.w, rf), ve.w);
         }
-        if (pt + kTrTile > p.n_past) {
-          const uint64_t m = attended64(p, i, pt, n_kv);
+        if (pt + HT > p.n_past) {
+          const uint32_t m = attended32(p, i, pt, n_kv);
 #pragma unroll
-          for (int k = 0; k < kTrTile; k++)
-            if (!((m >> k) & 1)) x[k] = -INFINITY;
+          for (int k = 0; k < HT; k++)
+            if (!((m >> k) & 1u)) x[k] = -INFINITY;
         }
+        float mx = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < kTrTile; k++) mx = fmaxf(mx, x[k]);
-        if (!Q8) {
-#pragma unroll
-          for (int k = 0; k < kTrTile; k++) ms = fmaxf(ms, __fsub_rn(x[k], c[2 * kTrTile + k]));
-        }
-        float f = 1.0f;
-        if (mx > M + 8.0f || (j == 0)) {
-          f = j == 0 ? 1.0f : exp2_approx(__fsub_rn(M, mx));
-          M = mx;
-          if (Q8) l = __fmul_rn(l, f);
-        }
-        const float Ms = M == -INFINITY ? 0.0f : __fsub_rn(M, 7.0f);
+        for (int k = 0; k < HT; k++) mx = fmaxf(mx, x[k]);
+        // the row's maximum over both halves
+        float* ex = mxs + (b * 2) * kTrRows + lr;
+        ex[half * kTrRows] = mx;
+        if (!(ok = meet(j))) break;
+        const float Mn = fmaxf(M, fmaxf(mx, ex[(half ^ 1) * kTrRows]));
+        // (2^14: the largest weight that fp16 still holds with room)
+        const float Mr = Mn == -INFINITY ? 0.0f : Mn, Ms = __fsub_rn(Mr, 14.0f);
+        const float f = exp2_approx(__fsub_rn(M, Mr));
+        M = Mn;
         float mls = 0.0f;
-        if (!Q8) {
+        if (Q8) {
+          l = __fmul_rn(l, f);
+        } else {
+          float ms = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < HT; k++) ms = fmaxf(ms, __fsub_rn(x[k], c[2 * kTrTile + k]));
           if (ms > ml) {
             l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, ms)));
             ml = ms;
           }
           mls = ml == -INFINITY ? 0.0f : ml;
         }
-        // P and O of the step before have been used
-        if (j > 0) {
-          if (!tc_wait_warp(&pv_done[t], (j - 1) & 1, abort_flag, p.err)) {
-            done = false;
-            break;
-          }
-          tc_fence_after();
-          if (__any_sync(0xffffffffu, f != 1.0f)) {
-#pragma unroll 1
-            for (int o = 0; o < D; o += 32) {
-              float y[32];
-              tmem_ld32(base + kColO + o, y);
-              tmem_wait_ld(y);
-              uint32_t z[32];
+        // P's planes of step j - 2 are free: that step's O has been taken
+        uint32_t hi[HT / 2], lo[HT / 2];
 #pragma unroll
-              for (int k = 0; k < 32; k++) z[k] = __float_as_uint(__fmul_rn(y[k], f));
-              tmem_st16(base + kColO + o, z);
-              tmem_st16(base + kColO + o + 16, z + 16);
-            }
+        for (int k = 0; k < HT; k += 4) {
+          const float4 vf = *(const float4*)(c + 2 * kTrTile + k);
+          float pe[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) pe[u] = exp2_approx(__fsub_rn(x[k + u], Ms));
+          if (Q8) {
+            l = __fmaf_rn(pe[0], vf.x, l);
+            l = __fmaf_rn(pe[1], vf.y, l);
+            l = __fmaf_rn(pe[2], vf.z, l);
+            l = __fmaf_rn(pe[3], vf.w, l);
+          } else {
+            l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[k], vf.x), mls)));
+            l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[k + 1], vf.y), mls)));
+            l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[k + 2], vf.z), mls)));
+            l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[k + 3], vf.w), mls)));
+          }
+#pragma unroll
+          for (int u = 0; u < 4; u += 2) {
+            const __half2 hh = __floats2half2_rn(pe[u], pe[u + 1]);
+            const float2 back = __half22float2(hh);
+            hi[(k + u) / 2] = h2_bits(hh);
+            lo[(k + u) / 2] = h2_bits(__floats2half2_rn(__fsub_rn(pe[u], back.x), __fsub_rn(pe[u + 1], back.y)));
           }
         }
-#pragma unroll
-        for (int h = 0; h < kTrTile; h += 32) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 vf = *(const float4*)(c + 2 * kTrTile + h + k);
-            float pe[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) pe[u] = exp2_approx(__fsub_rn(x[h + k + u], Ms));
-            if (Q8) {
-              l = __fmaf_rn(pe[0], vf.x, l);
-              l = __fmaf_rn(pe[1], vf.y, l);
-              l = __fmaf_rn(pe[2], vf.z, l);
-              l = __fmaf_rn(pe[3], vf.w, l);
-            } else {
-              l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[h + k], vf.x), mls)));
-              l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[h + k + 1], vf.y), mls)));
-              l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[h + k + 2], vf.z), mls)));
-              l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[h + k + 3], vf.w), mls)));
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u += 2) {
-              const __half2 hh = __floats2half2_rn(pe[u], pe[u + 1]);
-              const float2 back = __half22float2(hh);
-              hi[(k + u) / 2] = h2_bits(hh);
-              lo[(k + u) / 2] = h2_bits(__floats2half2_rn(__fsub_rn(pe[u], back.x), __fsub_rn(pe[u + 1], back.y)));
-            }
-          }
-          tmem_st16(base + kColPhi + h / 2, hi);
-          tmem_st16(base + kColPlo + h / 2, lo);
-        }
+        tmem_st16(base + kColP + 64 * b + half * (HT / 2), hi);
+        tmem_st16(base + kColP + 64 * b + 32 + half * (HT / 2), lo);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(&p_full[t]);
+        if (lane == 0) mbar_arrive_one(&p_full[b]);
+        if (j > 0 && !(ok = take_o(j - 1, f_prev))) break;
+        f_prev = f;
       }
-      if (done && tc_wait_warp(&pv_done[t], (n - 1) & 1, abort_flag, p.err)) {
-        tc_fence_after();
-        const float Ms = M == -INFINITY ? 0.0f : __fsub_rn(M, 7.0f), mls = Q8 ? Ms : ml == -INFINITY ? 0.0f : ml;
-        float* rec = (float*)p.scratch + (((int64_t)kvh * sp.S + split) * sp.R + r) * (D + 4);
-        float* out = p.out + ((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D;
-        const bool whole = sp.S == 1;
-        // one split: the result itself; a token that attends to nothing has l = 0
-        const float inv = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), exp2_approx(__fsub_rn(Ms, mls)));
-        if (!whole && r < sp.R) *(float4*)rec = make_float4(M == -INFINITY ? -INFINITY : Ms, Q8 ? (M == -INFINITY ? -INFINITY : Ms) : ml, l, 0.0f);
-#pragma unroll 1
-        for (int o = 0; o < D; o += 32) {
-          float y[32];
-          tmem_ld32(base + kColO + o, y);
-          tmem_wait_ld(y);
-          if (r < sp.R) {
+      if (ok) ok = take_o(n - 1, f_prev);
+      // the halves' sums
+      float m = M == -INFINITY ? -INFINITY : __fsub_rn(M, 14.0f);  // what l is relative to
+      float* ex = mxs + (n & 1) * 2 * kTrRows + lr;  // (not the last step's)
+      if (!Q8 && ok) {
+        ex[half * kTrRows] = ml;
+        if ((ok = meet(n))) {
+          m = fmaxf(ml, ex[(half ^ 1) * kTrRows]);
+          if (ml != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, m)));
+          ex = mxs + ((n + 1) & 1) * 2 * kTrRows + lr;
+        }
+      }
+      if (ok) {
+        ex[half * kTrRows] = l;
+        if ((ok = meet(Q8 ? n : n + 1))) l = __fadd_rn(l, ex[(half ^ 1) * kTrRows]);
+      }
+      if (ok && r < sp.R) {
+        const float Ms = M == -INFINITY ? -INFINITY : __fsub_rn(M, 14.0f);
+        if (sp.S == 1) {
+          // one split: the result itself; a token that attends to nothing has l = 0
+          const float g = Ms == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(Ms, m));
+          const float inv = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), g);
+          float* out = p.out + ((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D + NA * half;
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              if (whole) {
-                out[o + k] = __fmul_rn(y[k], inv);
-                out[o + k + 1] = __fmul_rn(y[k + 1], inv);
-                out[o + k + 2] = __fmul_rn(y[k + 2], inv);
-                out[o + k + 3] = __fmul_rn(y[k + 3], inv);
-              } else {
-                *(float4*)(rec + 4 + o + k) = make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
-              }
-            }
-          }
+          for (int k = 0; k < NA; k++) out[k] = __fmul_rn(acc[k], inv);
+        } else {
+          float* rec = (float*)p.scratch + (((int64_t)kvh * sp.S + split) * sp.R + r) * (D + 4);
+          if (half == 0) *(float4*)rec = make_float4(Ms, m, l, 0.0f);
+#pragma unroll
+          for (int k = 0; k < NA; k += 4)
+            *(float4*)(rec + 4 + NA * half + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
         }
       }
     }
@@ -683,7 +723,7 @@ __global__ void __launch_bounds__(kTrJoinNT) attn_tree_join_kernel(const TreeAtt
 constexpr int kTrSms = 148;
 
 int64_t most_splits(int64_t H, int64_t HKV, int64_t n_kv, int64_t T) {
-  const int64_t RG = (T * (H / HKV) + 2 * kTrRows - 1) / (2 * kTrRows), steps = (n_kv + kTrTile - 1) / kTrTile;
+  const int64_t RG = (T * (H / HKV) + kTrRows - 1) / kTrRows, steps = (n_kv + kTrTile - 1) / kTrTile;
   return std::min(steps, std::max<int64_t>(1, kTrSms / std::max<int64_t>(1, HKV * RG)));
 }
 
@@ -691,7 +731,7 @@ template <int D, bool Q8>
 cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
   TreeSplit sp{};
   sp.R = p.T * (p.H / p.HKV);
-  sp.RG = (sp.R + 2 * kTrRows - 1) / (2 * kTrRows);
+  sp.RG = (sp.R + kTrRows - 1) / kTrRows;
   const int64_t n_kv = (int64_t)p.n_past + p.T, steps = (n_kv + kTrTile - 1) / kTrTile;
   const int64_t most = most_splits(p.H, p.HKV, n_kv, p.T);
   sp.per = (int32_t)((steps + most - 1) / most);
@@ -727,10 +767,10 @@ bool attn_tree_fits(int64_t D, int64_t H, int64_t HKV, int64_t T) {
 }
 
 // Records of all splits, for up to n_kv rows and T tokens: a KV head's groups of
-// 256 rows times its splits pass kTrSms / HKV only where one group alone does.
+// 128 rows times its splits pass kTrSms / HKV only where one group alone does.
 size_t attn_tree_scratch_bytes(int64_t H, int64_t HKV, int64_t n_kv, int64_t T, int64_t D) {
   const int64_t R = T * (H / HKV), steps = (n_kv + kTrTile - 1) / kTrTile;
-  const int64_t rows = std::min(steps * R, std::max(R, (kTrSms + HKV - 1) / HKV * 2 * kTrRows));
+  const int64_t rows = std::min(steps * R, std::max(R, (kTrSms + HKV - 1) / HKV * kTrRows));
   return (size_t)(16 + HKV * rows * (D + 4) * 4);
 }
 
