@@ -52,7 +52,8 @@ constexpr int kTrRows = 128;     // rows per CTA (MMA M)
 constexpr int kTrWarpK = 8, kTrWarpV = 12, kTrWarpMma = 16;
 constexpr int kTrThreads = 20 * 32;  // (the last three warps complete the MMA warp's group for setmaxnreg)
 constexpr int kTrSlots = 8;      // steps whose column factors are kept (see the roles' waits)
-constexpr uint32_t kTrCols = 512;
+constexpr uint32_t kTrCols = 512;  // all of TMEM: its base is 0
+constexpr uint32_t kTmem = 0;
 // TMEM columns of step j: S at 64 (j & 1), P's planes at 128 + 64 (j & 1) and 32
 // behind it, O at 256 + D (j & 1)
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
@@ -86,6 +87,17 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// True in one lane of a converged warp (always the same one).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t y;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(y));
+  return y != 0;
 }
 
 // D (+)= A B, f32 += f16 x f16; A from shared memory or (TS) from TMEM.
@@ -394,12 +406,14 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_base;
 
   if (warp >= kTrWarpMma) {
-    // ---------------- MMA issue (one thread) ----------------
+    // ---------------- MMA issue ----------------
+    // The whole warp runs the loop and one elected lane issues: descriptors then
+    // stay in uniform registers (in a branch of one lane each MMA cost 100 cycles
+    // to issue, three times what it takes to run).
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
-    if (warp == kTrWarpMma && lane == 0) {
+    if (warp == kTrWarpMma) {
       constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTrTile >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
       // (bit 16: B, the values, is dims-major)
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
@@ -407,50 +421,56 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       const uint64_t kd = umma_desc(smem_addr(smem + L::k), 128, 16 * D);
       const uint64_t vd = umma_desc(smem_addr(smem + L::v), 16 * D, 128);
       constexpr uint64_t plane = L::plane_kv >> 4;
-      bool ok = true;
       // step j's scores: into S (j & 1) once step j - 2's have been read
       auto scores = [&](int j) {
         const int b = j & 1;
         const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-        if (!(ok = tc_wait1(&k_full[b], ph, abort_flag, p.err))) return;
-        if (j >= 2 && !(ok = tc_wait1(&s_empty[b], ph ^ 1, abort_flag, p.err))) return;
+        if (!tc_wait_warp(&k_full[b], ph, abort_flag, p.err)) return false;
+        if (j >= 2 && !tc_wait_warp(&s_empty[b], ph ^ 1, abort_flag, p.err)) return false;
         tc_fence_after();
-        const uint32_t d = tmem + kColS + 64 * b;
+        const uint32_t d = kTmem + kColS + 64 * b;
         const uint64_t kh = kd + 2 * plane * b, kl = kh + plane;
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < D / 16; s++) mma_ss(d, ql + 16 * s, kh + 16 * s, idesc_s, s > 0);
+          for (int s = 0; s < D / 16; s++) mma_ss(d, ql + 16 * s, kh + 16 * s, idesc_s, s > 0);
 #pragma unroll
-        for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kl + 16 * s, idesc_s, 1);
+          for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kl + 16 * s, idesc_s, 1);
 #pragma unroll
-        for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kh + 16 * s, idesc_s, 1);
-        umma_commit(&s_full[b]);
-        umma_commit(&k_empty[b]);
+          for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kh + 16 * s, idesc_s, 1);
+          umma_commit(&s_full[b]);
+          umma_commit(&k_empty[b]);
+        }
+        __syncwarp();
+        return true;
       };
-      scores(0);
-      if (ok && n > 1) scores(1);
+      bool ok = scores(0);
+      if (ok && n > 1) ok = scores(1);
       for (int j = 0; j < n && ok; j++) {
-        if (j > 0 && j + 1 < n) scores(j + 1);
-        if (!ok) break;
+        if (j > 0 && j + 1 < n && !(ok = scores(j + 1))) break;
         const int b = j & 1;
         const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-        if (!(ok = tc_wait1(&v_full[b], ph, abort_flag, p.err))) break;
-        if (j >= 2 && !(ok = tc_wait1(&o_empty[b], ph ^ 1, abort_flag, p.err))) break;
-        if (!(ok = tc_wait1(&p_full[b], ph, abort_flag, p.err))) break;
+        if (!(ok = tc_wait_warp(&v_full[b], ph, abort_flag, p.err))) break;
+        if (j >= 2 && !(ok = tc_wait_warp(&o_empty[b], ph ^ 1, abort_flag, p.err))) break;
+        if (!(ok = tc_wait_warp(&p_full[b], ph, abort_flag, p.err))) break;
         tc_fence_after();
-        const uint32_t o = tmem + kColO + D * b, p_hi = tmem + kColP + 64 * b, p_lo = p_hi + 32;
+        const uint32_t o = kTmem + kColO + D * b, p_hi = kTmem + kColP + 64 * b, p_lo = p_hi + 32;
         const uint64_t vh = vd + 2 * plane * b, vl = vh + plane;
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_lo + 8 * s, vh + 2 * D * s, idesc_o, s > 0);
+          for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_lo + 8 * s, vh + 2 * D * s, idesc_o, s > 0);
 #pragma unroll
-        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vl + 2 * D * s, idesc_o, 1);
+          for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vl + 2 * D * s, idesc_o, 1);
 #pragma unroll
-        for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vh + 2 * D * s, idesc_o, 1);
-        umma_commit(&o_full[b]);
-        umma_commit(&v_empty[b]);
+          for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vh + 2 * D * s, idesc_o, 1);
+          umma_commit(&o_full[b]);
+          umma_commit(&v_empty[b]);
+        }
+        __syncwarp();
       }
       // every MMA has finished before TMEM and shared memory are given back
-      umma_commit(drain);
-      for (uint32_t it = 0; it < kSpinLimit && !mbar_test(drain, 0); it++) {
+      if (elect_one()) umma_commit(drain);
+      __syncwarp();
+      for (uint32_t it = 0; it < kSpinLimit && !__all_sync(0xffffffffu, mbar_test(drain, 0)); it++) {
       }
     }
   } else if (warp >= kTrWarpK) {
@@ -505,7 +525,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     if (quad < nq) {
       constexpr int NA = D / 2, HT = kTrTile / 2;
       const int lr = quad * 32 + lane, r = r0 + lr, i = min(r, sp.R - 1) / rep;
-      const uint32_t base = tmem + ((uint32_t)(32 * quad) << 16);
+      const uint32_t base = kTmem + ((uint32_t)(32 * quad) << 16);
       const float rf = rowf[lr];
       float M = -INFINITY, l = 0.0f;  // the row's maximum; this half's weights (Q8_0: relative to M, F32: to ml)
       float ml = -INFINITY, f_prev = 1.0f;
@@ -666,7 +686,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   if (warp == kTrWarpMma) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTrCols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_base), "r"(kTrCols));
   }
 }
 
