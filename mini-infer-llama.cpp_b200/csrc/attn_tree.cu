@@ -71,7 +71,7 @@ struct TrSmem {
   static constexpr int rowf = col + kTrSlots * 3 * kTrTile * 4;  // float [128]: scale * log2(e) * the row's factor
   static constexpr int mx = rowf + kTrRows * 4;    // float [step & 1][half][128]: the halves' maxima (at the end their sums)
   static constexpr int bars = mx + 4 * kTrRows * 4;
-  static constexpr int n_bars = 8 + kTrSlots + 10 + 4 + 1;
+  static constexpr int n_bars = 8 + kTrSlots + 10 + 1;
   static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
   static constexpr int used = misc + 16;
   // above half of an SM's shared memory: two CTAs must not share its TMEM
@@ -344,8 +344,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   uint64_t* p_full = s_full + 4;
   uint64_t* o_full = s_full + 6;
   uint64_t* o_empty = s_full + 8;
-  uint64_t* pair = s_full + 10;  // [quadrant]: its two softmax warps
-  uint64_t* drain = s_full + 14;
+  uint64_t* drain = s_full + 10;
   uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
   volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
 
@@ -362,7 +361,6 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       mbar_init(&o_empty[i], 2 * nq);
     }
     for (int i = 0; i < kTrSlots; i++) mbar_init(&col_full[i], 8);
-    for (int i = 0; i < 4; i++) mbar_init(&pair[i], 2);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -425,8 +423,8 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       auto scores = [&](int j) {
         const int b = j & 1;
         const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-        if (!tc_wait_warp(&k_full[b], ph, abort_flag, p.err)) return false;
-        if (j >= 2 && !tc_wait_warp(&s_empty[b], ph ^ 1, abort_flag, p.err)) return false;
+        if (!tc_wait_ready(&k_full[b], ph, abort_flag, p.err)) return false;
+        if (j >= 2 && !tc_wait_ready(&s_empty[b], ph ^ 1, abort_flag, p.err)) return false;
         tc_fence_after();
         const uint32_t d = kTmem + kColS + 64 * b;
         const uint64_t kh = kd + 2 * plane * b, kl = kh + plane;
@@ -449,9 +447,9 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         if (j > 0 && j + 1 < n && !(ok = scores(j + 1))) break;
         const int b = j & 1;
         const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-        if (!(ok = tc_wait_warp(&v_full[b], ph, abort_flag, p.err))) break;
-        if (j >= 2 && !(ok = tc_wait_warp(&o_empty[b], ph ^ 1, abort_flag, p.err))) break;
-        if (!(ok = tc_wait_warp(&p_full[b], ph, abort_flag, p.err))) break;
+        if (!(ok = tc_wait_ready(&v_full[b], ph, abort_flag, p.err))) break;
+        if (j >= 2 && !(ok = tc_wait_ready(&o_empty[b], ph ^ 1, abort_flag, p.err))) break;
+        if (!(ok = tc_wait_ready(&p_full[b], ph, abort_flag, p.err))) break;
         tc_fence_after();
         const uint32_t o = kTmem + kColO + D * b, p_hi = kTmem + kColP + 64 * b, p_lo = p_hi + 32;
         const uint64_t vh = vd + 2 * plane * b, vl = vh + plane;
@@ -511,7 +509,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       }
       __syncwarp();
       if (lane == 0) mbar_arrive_one(&col_full[j & (kTrSlots - 1)]);
-      if (j >= 2 && !tc_wait_warp(&empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort_flag, p.err)) break;
+      if (j >= 2 && !tc_wait_ready(&empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort_flag, p.err)) break;
       kv.store(smem + (is_v ? L::v : L::k) + b * 2 * L::plane_kv, w, lane, e, fine);
       fence_proxy_async_smem();
       __syncwarp();
@@ -527,7 +525,9 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       const int lr = quad * 32 + lane, r = r0 + lr, i = min(r, sp.R - 1) / rep;
       const uint32_t base = kTmem + ((uint32_t)(32 * quad) << 16);
       const float rf = rowf[lr];
-      float M = -INFINITY, l = 0.0f;  // the row's maximum; this half's weights (Q8_0: relative to M, F32: to ml)
+      const float2 rf2 = make_float2(rf, rf);
+      float M = -INFINITY;                   // the row's maximum
+      float2 l2 = make_float2(0.0f, 0.0f);   // this half's weights (Q8_0: relative to M - 14, F32: to ml)
       float ml = -INFINITY, f_prev = 1.0f;
       float acc[NA];
 #pragma unroll
@@ -535,35 +535,42 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       // step j's O into the registers
       auto take_o = [&](int j, float f) {
         const int b = j & 1;
-        if (!tc_wait_warp(&o_full[b], (uint32_t)(j >> 1) & 1u, abort_flag, p.err)) return false;
+        if (!tc_wait_ready(&o_full[b], (uint32_t)(j >> 1) & 1u, abort_flag, p.err)) return false;
         tc_fence_after();
+        const float2 f2 = make_float2(f, f);
 #pragma unroll
-        for (int o = 0; o < NA; o += 16) {
-          float y[16];
+        for (int o = 0; o < NA; o += 32) {
+          float y[32];
           tmem_ld16f(base + kColO + D * b + NA * half + o, y);
+          if (o + 16 < NA) tmem_ld16f(base + kColO + D * b + NA * half + o + 16, y + 16);
           tmem_wait_ld16(y);
+          if (o + 16 < NA) tmem_wait_ld16(y + 16);
 #pragma unroll
-          for (int k = 0; k < 16; k++) acc[o + k] = __fmaf_rn(acc[o + k], f, y[k]);
+          for (int k = 0; k < 32 && o + k < NA; k += 2) {
+            const float2 a = __ffma2_rn(make_float2(acc[o + k], acc[o + k + 1]), f2, make_float2(y[k], y[k + 1]));
+            acc[o + k] = a.x;
+            acc[o + k + 1] = a.y;
+          }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_one(&o_empty[b]);
         return true;
       };
-      // the row's other half has come as far (its k-th meeting)
-      auto meet = [&](int k) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive_one(&pair[quad]);
-        return tc_wait_warp(&pair[quad], (uint32_t)k & 1u, abort_flag, p.err);
-      };
+      // The row's other half has come as far: once a step and twice at the end, also
+      // by warps that have given up (so that none waits for the other).
+      auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
       bool ok = true;
       for (int j = 0; j < n; j++) {
         const int b = j & 1;
         const int64_t pt = pos0 + (int64_t)j * kTrTile + half * HT;
         const float* c = col + (j & (kTrSlots - 1)) * 3 * kTrTile + half * HT;
-        ok = tc_wait_warp(&col_full[j & (kTrSlots - 1)], (uint32_t)(j / kTrSlots) & 1u, abort_flag, p.err) &&
-             tc_wait_warp(&s_full[b], (uint32_t)(j >> 1) & 1u, abort_flag, p.err);
-        if (!ok) break;
+        ok = ok && tc_wait_ready(&col_full[j & (kTrSlots - 1)], (uint32_t)(j / kTrSlots) & 1u, abort_flag, p.err) &&
+             tc_wait_ready(&s_full[b], (uint32_t)(j >> 1) & 1u, abort_flag, p.err);
+        if (!ok) {
+          meet();
+          continue;
+        }
         tc_fence_after();
         float x[HT];
         tmem_ld32(base + kColS + 64 * b + half * HT, x);
@@ -571,13 +578,13 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_one(&s_empty[b]);
+        // (two elements an instruction where the hardware has one)
+        float2* x2 = (float2*)x;
 #pragma unroll
         for (int k = 0; k < HT; k += 4) {
           const float4 kf = *(const float4*)(c + k), ve = *(const float4*)(c + kTrTile + k);
-          x[k] = __fmaf_rn(x[k], __fmul_rn(kf.x, rf), ve.x);
-          x[k + 1] = __fmaf_rn(x[k + 1], __fmul_rn(kf.y, rf), ve.y);
-          x[k + 2] = __fmaf_rn(x[k + 2], __fmul_rn(kf.z, rf), ve.z);
-          x[k + 3] = __fmaf_rn(x[k + 3], __fmul_rn(kf.w, rf), ve.w);
+          x2[k / 2] = __ffma2_rn(x2[k / 2], __fmul2_rn(make_float2(kf.x, kf.y), rf2), make_float2(ve.x, ve.y));
+          x2[k / 2 + 1] = __ffma2_rn(x2[k / 2 + 1], __fmul2_rn(make_float2(kf.z, kf.w), rf2), make_float2(ve.z, ve.w));
         }
         if (pt + HT > p.n_past) {
           const uint32_t m = attended32(p, i, pt, n_kv);
@@ -585,56 +592,60 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           for (int k = 0; k < HT; k++)
             if (!((m >> k) & 1u)) x[k] = -INFINITY;
         }
-        float mx = -INFINITY;
+        float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int k = 0; k < HT; k++) mx = fmaxf(mx, x[k]);
+        for (int k = 4; k < HT; k += 4)
+#pragma unroll
+          for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], x[k + u]);
+        mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (!(mx[0] == mx[0])) mx[0] = -INFINITY;  // (nothing but NaN)
         // the row's maximum over both halves
         float* ex = mxs + (b * 2) * kTrRows + lr;
-        ex[half * kTrRows] = mx;
-        if (!(ok = meet(j))) break;
-        const float Mn = fmaxf(M, fmaxf(mx, ex[(half ^ 1) * kTrRows]));
+        ex[half * kTrRows] = mx[0];
+        meet();
+        const float Mn = fmaxf(M, fmaxf(mx[0], ex[(half ^ 1) * kTrRows]));
         // (2^14: the largest weight that fp16 still holds with room)
         const float Mr = Mn == -INFINITY ? 0.0f : Mn, Ms = __fsub_rn(Mr, 14.0f);
         const float f = exp2_approx(__fsub_rn(M, Mr));
         M = Mn;
         float mls = 0.0f;
         if (Q8) {
-          l = __fmul_rn(l, f);
+          l2 = __fmul2_rn(l2, make_float2(f, f));
         } else {
           float ms = -INFINITY;
 #pragma unroll
           for (int k = 0; k < HT; k++) ms = fmaxf(ms, __fsub_rn(x[k], c[2 * kTrTile + k]));
           if (ms > ml) {
-            l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, ms)));
+            const float g = exp2_approx(__fsub_rn(ml, ms));
+            l2 = __fmul2_rn(l2, make_float2(g, g));
             ml = ms;
           }
           mls = ml == -INFINITY ? 0.0f : ml;
         }
         // P's planes of step j - 2 are free: that step's O has been taken
+        const float2 neg_ms = make_float2(-Ms, -Ms), one = make_float2(-1.0f, -1.0f);
         uint32_t hi[HT / 2], lo[HT / 2];
 #pragma unroll
         for (int k = 0; k < HT; k += 4) {
           const float4 vf = *(const float4*)(c + 2 * kTrTile + k);
-          float pe[4];
 #pragma unroll
-          for (int u = 0; u < 4; u++) pe[u] = exp2_approx(__fsub_rn(x[k + u], Ms));
-          if (Q8) {
-            l = __fmaf_rn(pe[0], vf.x, l);
-            l = __fmaf_rn(pe[1], vf.y, l);
-            l = __fmaf_rn(pe[2], vf.z, l);
-            l = __fmaf_rn(pe[3], vf.w, l);
-          } else {
-            l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[k], vf.x), mls)));
-            l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[k + 1], vf.y), mls)));
-            l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[k + 2], vf.z), mls)));
-            l = __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(x[k + 3], vf.w), mls)));
-          }
-#pragma unroll
-          for (int u = 0; u < 4; u += 2) {
-            const __half2 hh = __floats2half2_rn(pe[u], pe[u + 1]);
-            const float2 back = __half22float2(hh);
-            hi[(k + u) / 2] = h2_bits(hh);
-            lo[(k + u) / 2] = h2_bits(__floats2half2_rn(__fsub_rn(pe[u], back.x), __fsub_rn(pe[u + 1], back.y)));
+          for (int u = 0; u < 2; u++) {
+            const float2 w = u ? make_float2(vf.z, vf.w) : make_float2(vf.x, vf.y);
+            const float2 d = __fadd2_rn(x2[k / 2 + u], neg_ms);
+            const float2 pe = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+            if (Q8) {
+              l2 = __ffma2_rn(pe, w, l2);
+            } else {
+              const float2 s2 = __fadd2_rn(__ffma2_rn(w, one, x2[k / 2 + u]), make_float2(-mls, -mls));
+              l2 = __fadd2_rn(l2, make_float2(exp2_approx(s2.x), exp2_approx(s2.y)));
+            }
+            // the upper half by cutting to fp16's 11 bits (below 2^-14, a weight of
+            // 2^-28 of the row's largest, its conversion rounds instead)
+            const float2 top = make_float2(__uint_as_float(__float_as_uint(pe.x) & 0xffffe000u),
+                                           __uint_as_float(__float_as_uint(pe.y) & 0xffffe000u));
+            const float2 rest = __ffma2_rn(top, one, pe);
+            hi[k / 2 + u] = h2_bits(__floats2half2_rn(top.x, top.y));
+            lo[k / 2 + u] = h2_bits(__floats2half2_rn(rest.x, rest.y));
           }
         }
         tmem_st16(base + kColP + 64 * b + half * (HT / 2), hi);
@@ -643,25 +654,24 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_one(&p_full[b]);
-        if (j > 0 && !(ok = take_o(j - 1, f_prev))) break;
+        if (j > 0) ok = take_o(j - 1, f_prev);
         f_prev = f;
       }
       if (ok) ok = take_o(n - 1, f_prev);
       // the halves' sums
+      float l = __fadd_rn(l2.x, l2.y);
       float m = M == -INFINITY ? -INFINITY : __fsub_rn(M, 14.0f);  // what l is relative to
       float* ex = mxs + (n & 1) * 2 * kTrRows + lr;  // (not the last step's)
-      if (!Q8 && ok) {
-        ex[half * kTrRows] = ml;
-        if ((ok = meet(n))) {
-          m = fmaxf(ml, ex[(half ^ 1) * kTrRows]);
-          if (ml != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, m)));
-          ex = mxs + ((n + 1) & 1) * 2 * kTrRows + lr;
-        }
+      ex[half * kTrRows] = Q8 ? 0.0f : ml;
+      meet();
+      if (!Q8) {
+        m = fmaxf(ml, ex[(half ^ 1) * kTrRows]);
+        if (ml != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, m)));
       }
-      if (ok) {
-        ex[half * kTrRows] = l;
-        if ((ok = meet(Q8 ? n : n + 1))) l = __fadd_rn(l, ex[(half ^ 1) * kTrRows]);
-      }
+      ex = mxs + ((n + 1) & 1) * 2 * kTrRows + lr;
+      ex[half * kTrRows] = l;
+      meet();
+      l = __fadd_rn(l, ex[(half ^ 1) * kTrRows]);
       if (ok && r < sp.R) {
         const float Ms = M == -INFINITY ? -INFINITY : __fsub_rn(M, 14.0f);
         if (sp.S == 1) {

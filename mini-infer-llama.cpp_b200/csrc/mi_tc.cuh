@@ -79,4 +79,9 @@ __device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity, vol
   }
 }
 
+// The same where the phase has usually completed: looks once before it sleeps.
+__device__ __forceinline__ bool tc_wait_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+  return __all_sync(0xffffffffu, mbar_test(bar, parity)) || tc_wait_warp(bar, parity, abort_flag, err);
+}
+
 }  // namespace mi
