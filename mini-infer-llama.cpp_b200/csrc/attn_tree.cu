@@ -24,10 +24,11 @@
 //
 // One CTA: 128 rows (a TMEM lane each) over one range of positions, 64 a step.
 // Warps 0-7 softmax: two threads per row, 32 positions each; 8-11 convert keys and
-// 12-15 values into the MMAs' layout; 16 issues the MMAs. Everything between two
-// roles is doubled (key and value planes in shared memory; S, P and O in TMEM, all
-// of its 512 columns at D = 128), so the MMAs of one step run under the
-// exponentials of another.
+// 12-15 values into the MMAs' layout; 16 issues the MMAs. Key and value planes (in
+// shared memory), S and P (in TMEM) are doubled, so the MMAs of one step run under
+// the exponentials of another. The queries' planes are copied into TMEM too: as a
+// shared-memory operand they are 4 KB a product beside the keys' 2, and shared
+// memory, not the tensor core, then set the pace (80 cycles a product of 32).
 //
 // A step's O is a product of its own, added to the softmax threads' registers
 // (O = O 2^(M_old - M_new) + O_step): the MMA's accumulation cuts instead of
@@ -54,9 +55,9 @@ constexpr int kTrThreads = 20 * 32;  // (the last three warps complete the MMA w
 constexpr int kTrSlots = 8;      // steps whose column factors are kept (see the roles' waits)
 constexpr uint32_t kTrCols = 512;  // all of TMEM: its base is 0
 constexpr uint32_t kTmem = 0;
-// TMEM columns of step j: S at 64 (j & 1), P's planes at 128 + 64 (j & 1) and 32
-// behind it, O at 256 + D (j & 1)
-constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
+// TMEM columns: step j's S at 64 (j & 1), P's planes at 128 + 64 (j & 1) and 32
+// behind it, O at 256, the queries' planes at 384 and D / 2 behind it
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256, kColQ = 384;
 // Registers per thread of the roles: launched with 96 x 640 = 61440, of which
 // 136 x 256 + 80 x 256 + 48 x 128 = 61440 are given out again.
 constexpr int kRegsSoftmax = 136, kRegsConvert = 80, kRegsMma = 48;
@@ -71,7 +72,7 @@ struct TrSmem {
   static constexpr int rowf = col + kTrSlots * 3 * kTrTile * 4;  // float [128]: scale * log2(e) * the row's factor
   static constexpr int mx = rowf + kTrRows * 4;    // float [step & 1][half][128]: the halves' maxima (at the end their sums)
   static constexpr int bars = mx + 4 * kTrRows * 4;
-  static constexpr int n_bars = 8 + kTrSlots + 10 + 1;
+  static constexpr int n_bars = 8 + kTrSlots + 8 + 2;
   static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
   static constexpr int used = misc + 16;
   // above half of an SM's shared memory: two CTAs must not share its TMEM
@@ -100,15 +101,7 @@ __device__ __forceinline__ bool elect_one() {
   return y != 0;
 }
 
-// D (+)= A B, f32 += f16 x f16; A from shared memory or (TS) from TMEM.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
-      : "memory");
-}
+// D (+)= A B, f32 += f16 x f16; A from TMEM, B from shared memory.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -342,9 +335,9 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   uint64_t* s_full = col_full + kTrSlots;
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_full + 4;
-  uint64_t* o_full = s_full + 6;
-  uint64_t* o_empty = s_full + 8;
-  uint64_t* drain = s_full + 10;
+  uint64_t* o_full = s_full + 6;  // one: O is taken before the next P is handed over
+  uint64_t* q_full = s_full + 7;
+  uint64_t* drain = s_full + 8;
   uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
   volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
 
@@ -357,9 +350,9 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 2 * nq);
       mbar_init(&p_full[i], 2 * nq);
-      mbar_init(&o_full[i], 1);
-      mbar_init(&o_empty[i], 2 * nq);
     }
+    mbar_init(o_full, 1);
+    mbar_init(q_full, 2 * nq);
     for (int i = 0; i < kTrSlots; i++) mbar_init(&col_full[i], 8);
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -415,7 +408,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTrTile >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
       // (bit 16: B, the values, is dims-major)
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
-      const uint64_t qh = umma_desc(smem_addr(smem + L::q), 128, 16 * D), ql = qh + (uint64_t)(L::plane_q >> 4);
+      const uint32_t qh = kTmem + kColQ, ql = qh + D / 2;
       const uint64_t kd = umma_desc(smem_addr(smem + L::k), 128, 16 * D);
       const uint64_t vd = umma_desc(smem_addr(smem + L::v), 16 * D, 128);
       constexpr uint64_t plane = L::plane_kv >> 4;
@@ -430,28 +423,27 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         const uint64_t kh = kd + 2 * plane * b, kl = kh + plane;
         if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < D / 16; s++) mma_ss(d, ql + 16 * s, kh + 16 * s, idesc_s, s > 0);
+          for (int s = 0; s < D / 16; s++) mma_ts(d, ql + 8 * s, kh + 16 * s, idesc_s, s > 0);
 #pragma unroll
-          for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kl + 16 * s, idesc_s, 1);
+          for (int s = 0; s < D / 16; s++) mma_ts(d, qh + 8 * s, kl + 16 * s, idesc_s, 1);
 #pragma unroll
-          for (int s = 0; s < D / 16; s++) mma_ss(d, qh + 16 * s, kh + 16 * s, idesc_s, 1);
+          for (int s = 0; s < D / 16; s++) mma_ts(d, qh + 8 * s, kh + 16 * s, idesc_s, 1);
           umma_commit(&s_full[b]);
           umma_commit(&k_empty[b]);
         }
         __syncwarp();
         return true;
       };
-      bool ok = scores(0);
+      bool ok = tc_wait_ready(q_full, 0, abort_flag, p.err) && scores(0);
       if (ok && n > 1) ok = scores(1);
       for (int j = 0; j < n && ok; j++) {
         if (j > 0 && j + 1 < n && !(ok = scores(j + 1))) break;
         const int b = j & 1;
         const uint32_t ph = (uint32_t)(j >> 1) & 1u;
         if (!(ok = tc_wait_ready(&v_full[b], ph, abort_flag, p.err))) break;
-        if (j >= 2 && !(ok = tc_wait_ready(&o_empty[b], ph ^ 1, abort_flag, p.err))) break;
         if (!(ok = tc_wait_ready(&p_full[b], ph, abort_flag, p.err))) break;
         tc_fence_after();
-        const uint32_t o = kTmem + kColO + D * b, p_hi = kTmem + kColP + 64 * b, p_lo = p_hi + 32;
+        const uint32_t o = kTmem + kColO, p_hi = kTmem + kColP + 64 * b, p_lo = p_hi + 32;
         const uint64_t vh = vd + 2 * plane * b, vl = vh + plane;
         if (elect_one()) {
 #pragma unroll
@@ -460,7 +452,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vl + 2 * D * s, idesc_o, 1);
 #pragma unroll
           for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vh + 2 * D * s, idesc_o, 1);
-          umma_commit(&o_full[b]);
+          umma_commit(o_full);
           umma_commit(&v_empty[b]);
         }
         __syncwarp();
@@ -526,6 +518,25 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       const uint32_t base = kTmem + ((uint32_t)(32 * quad) << 16);
       const float rf = rowf[lr];
       const float2 rf2 = make_float2(rf, rf);
+      // the row's query planes into TMEM (this thread's half of the dims)
+      {
+        const uint8_t* src = smem + L::q + (lr >> 3) * (16 * D) + (lr & 7) * 16 + half * (D / 16) * 128;
+#pragma unroll
+        for (int pl = 0; pl < 2; pl++)
+#pragma unroll
+          for (int o = 0; o < D / 4; o += 8) {
+            const uint4 a = *(const uint4*)(src + pl * L::plane_q + (o / 4) * 128);
+            const uint4 c = *(const uint4*)(src + pl * L::plane_q + (o / 4 + 1) * 128);
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(
+                             base + kColQ + pl * (D / 2) + half * (D / 4) + o),
+                         "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w)
+                         : "memory");
+          }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(q_full);
+      }
       float M = -INFINITY;                   // the row's maximum
       float2 l2 = make_float2(0.0f, 0.0f);   // this half's weights (Q8_0: relative to M - 14, F32: to ml)
       float ml = -INFINITY, f_prev = 1.0f;
@@ -534,15 +545,14 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       for (int k = 0; k < NA; k++) acc[k] = 0.0f;
       // step j's O into the registers
       auto take_o = [&](int j, float f) {
-        const int b = j & 1;
-        if (!tc_wait_ready(&o_full[b], (uint32_t)(j >> 1) & 1u, abort_flag, p.err)) return false;
+        if (!tc_wait_ready(o_full, (uint32_t)j & 1u, abort_flag, p.err)) return false;
         tc_fence_after();
         const float2 f2 = make_float2(f, f);
 #pragma unroll
         for (int o = 0; o < NA; o += 32) {
           float y[32];
-          tmem_ld16f(base + kColO + D * b + NA * half + o, y);
-          if (o + 16 < NA) tmem_ld16f(base + kColO + D * b + NA * half + o + 16, y + 16);
+          tmem_ld16f(base + kColO + NA * half + o, y);
+          if (o + 16 < NA) tmem_ld16f(base + kColO + NA * half + o + 16, y + 16);
           tmem_wait_ld16(y);
           if (o + 16 < NA) tmem_wait_ld16(y + 16);
 #pragma unroll
@@ -552,9 +562,6 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
             acc[o + k + 1] = a.y;
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_one(&o_empty[b]);
         return true;
       };
       // The row's other half has come as far: once a step and twice at the end, also
@@ -650,12 +657,12 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         }
         tmem_st16(base + kColP + 64 * b + half * (HT / 2), hi);
         tmem_st16(base + kColP + 64 * b + 32 + half * (HT / 2), lo);
+        if (j > 0) ok = take_o(j - 1, f_prev);
+        f_prev = f;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_one(&p_full[b]);
-        if (j > 0) ok = take_o(j - 1, f_prev);
-        f_prev = f;
       }
       if (ok) ok = take_o(n - 1, f_prev);
       // the halves' sums
