@@ -17,10 +17,13 @@
 //     is x to 22 bits, and for a Q8_0 value exactly (11 bits of scale times 7 of
 //     quant: hi = fl(d q) and lo = fma(d, q, -hi) is the whole rest). A product
 //     takes three MMAs (hi hi, hi lo, lo hi); what is left out is 2^-22 of it.
-//   * the rows' powers of two leave the products as factors: a position's key
-//     exponent multiplies its column of S, its value exponent e is added to the
-//     score that makes P (P = 2^(s + e - M)), and the sum of the weights takes it
-//     out again.
+//   * the rows' powers of two leave the products as factors: the keys' exponent
+//     multiplies S, the values' exponent e is added to the score that makes P
+//     (P = 2^(s + e - M)), and the sum of the weights takes it out again. The 64
+//     positions of a step share both exponents unless their rows' magnitudes are
+//     more than 2^10 apart or one holds an infinity or a NaN; only then does every
+//     position have its own (a masked row's value then takes nothing from the
+//     others' precision).
 //
 // One CTA: 128 rows (a TMEM lane each) over one range of positions, 64 a step.
 // Warps 0-7 softmax: two threads per row, 32 positions each; 8-11 convert keys and
@@ -69,7 +72,10 @@ struct TrSmem {
   static constexpr int k = q + 2 * plane_q;        // [step & 1][hi, lo]
   static constexpr int v = k + 4 * plane_kv;
   static constexpr int col = v + 4 * plane_kv;     // float [kTrSlots][3][64]: key factor, value exponent, what takes it out of the sum
-  static constexpr int rowf = col + kTrSlots * 3 * kTrTile * 4;  // float [128]: scale * log2(e) * the row's factor
+  static constexpr int info = col + kTrSlots * 3 * kTrTile * 4;  // float [kTrSlots][4]: the step's key factor, value exponent, each whether
+                                                                 // its positions have their own
+  static constexpr int ends = info + kTrSlots * 16;              // int2 [keys, values][step & 1][4 warps]: largest and least exponent
+  static constexpr int rowf = ends + 2 * 2 * 4 * 8;              // float [128]: |scale| * log2(e) * the row's factor
   static constexpr int mx = rowf + kTrRows * 4;    // float [step & 1][half][128]: the halves' maxima (at the end their sums)
   static constexpr int bars = mx + 4 * kTrRows * 4;
   static constexpr int n_bars = 8 + kTrSlots + 8 + 2;
@@ -238,17 +244,20 @@ struct KvTile {
     }
   }
 
-  // The exponent by which row k's planes are scaled down (the row is planes *
-  // 2^e), or false for a row with a NaN scale, an infinity or a NaN.
-  __device__ __forceinline__ bool exponent(int k, int& e) const {
+  // The exponent that brings row k's planes to fp16's range (planes = row * 2^-e),
+  // and whether the row has a value but 0; false for a row with a NaN scale, an
+  // infinity or a NaN.
+  __device__ __forceinline__ bool exponent(int k, int& e, bool& any) const {
     if (Q8) {
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < NC; i++) m = max(m, (uint32_t)d[k][i] & 0x7fffu);
       e = max((int)(m >> 10), 1) - 15;  // the largest scale becomes 1..2 (below it for subnormal ones)
+      any = m != 0;
       return m < 0x7c00u;
     }
     const bool fine = row_exponent<NC * 8>(x[k], e);
+    any = e > -100;
     e -= 14;
     return fine;
   }
@@ -325,6 +334,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   const int n = (int)min((int64_t)sp.per, (n_kv - pos0 + kTrTile - 1) / kTrTile);  // steps of this CTA, at least one
   const int nq = min(4, (sp.R - r0 + 31) / 32);  // quadrants of 32 rows in use: two softmax warps each
   float* col = (float*)(smem + L::col);
+  float* info = (float*)(smem + L::info);
   float* rowf = (float*)(smem + L::rowf);
   float* mxs = (float*)(smem + L::mx);
   uint64_t* k_full = (uint64_t*)(smem + L::bars);  // each [step & 1]
@@ -385,13 +395,13 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     uint8_t* dst = smem + L::q + (lr >> 3) * (16 * D) + g * 128 + (lr & 7) * 16;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-      uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-      if (fine) split8(&x[8 * c], pow2f(14 - e), hi, lo);
+      // (a query with an infinity or a NaN becomes NaN: so do its scores)
+      uint4 hi = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u), lo = make_uint4(0, 0, 0, 0);
+      if (fine) split8(&x[8 * c], p.scale < 0.0f ? -pow2f(14 - e) : pow2f(14 - e), hi, lo);
       *(uint4*)(dst + c * 512) = hi;
       *(uint4*)(dst + L::plane_q + c * 512) = lo;
     }
-    // (a query with an infinity or a NaN: every score becomes NaN)
-    if (g == 0) rowf[lr] = fine ? __fmul_rn(__fmul_rn(p.scale, 1.4426950408889634f), pow2f(e - 14)) : __int_as_float(0x7fffffff);
+    if (g == 0) rowf[lr] = __fmul_rn(__fmul_rn(fabsf(p.scale), 1.4426950408889634f), pow2f(min(e, 127) - 14));
   }
   fence_proxy_async_smem();
   tc_fence_before();
@@ -474,38 +484,73 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     const void* cache = is_v ? p.cache_v : p.cache_k;
     uint64_t* full = is_v ? v_full : k_full;
     uint64_t* empty = is_v ? v_empty : k_empty;
+    int2* ends = (int2*)(smem + L::ends) + (is_v ? 8 : 0);
     KvTile<D, Q8> kv, next;
     if (Q8) kv.load(p, cache, kvh, pos0, n_kv, w, lane);
+    bool ok = true;
     for (int j = 0; j < n; j++) {
-      const int b = j & 1;
+      const int b = j & 1, slot = j & (kTrSlots - 1);
       // (a step of F32 rows takes too many registers to be held twice)
       if (!Q8) kv.load(p, cache, kvh, pos0 + (int64_t)j * kTrTile, n_kv, w, lane);
       else if (j + 1 < n) next.load(p, cache, kvh, pos0 + (int64_t)(j + 1) * kTrTile, n_kv, w, lane);
-      int e[2];
-      bool fine[2];
-      float* c = col + (j & (kTrSlots - 1)) * 3 * kTrTile;
+      int e[2], most = -1000, least = 1000;
+      bool fine[2], bad = false;
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        fine[k] = kv.exponent(k, e[k]);
-        if (lane < 8) {
+        bool any;
+        fine[k] = kv.exponent(k, e[k], any);
+        bad |= !fine[k];
+        if (fine[k] && any) {
+          most = max(most, e[k]);
+          least = min(least, e[k]);
+        }
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      least = __reduce_min_sync(0xffffffffu, least);
+      if (__any_sync(0xffffffffu, bad)) least = -2000;
+      if (lane == 0) ends[b * 4 + w] = make_int2(most, least);
+      // the four warps' exponents (met by warps that have given up too)
+      asm volatile("bar.sync %0, 128;" ::"r"(is_v ? 6 : 5) : "memory");
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int2 o = ends[b * 4 + k];
+        most = max(most, o.x);
+        least = min(least, o.y);
+      }
+      const bool own = least < 1000 && most - least > 10;
+      if (!own) {
+        if (most < -999) most = 0;
+        e[0] = e[1] = most;
+      }
+      float* c = col + slot * 3 * kTrTile;
+      const float nan = __int_as_float(0x7fffffff);
+      if (own && lane < 8) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
           const int at = (w + 4 * k) * 8 + lane;
-          const float bad = __int_as_float(0x7fffffff);
           if (is_v) {
-            c[kTrTile + at] = fine[k] ? (float)e[k] : bad;
+            c[kTrTile + at] = fine[k] ? (float)e[k] : nan;
             // (finite in every case: a masked position's weight is 0 whatever its row holds)
-            c[2 * kTrTile + at] = !fine[k] ? 0.0f : Q8 ? pow2f(-e[k]) : (float)e[k];
+            c[2 * kTrTile + at] = fine[k] ? (float)e[k] : 0.0f;
           } else {
-            c[at] = fine[k] ? pow2f(e[k]) : bad;
+            c[at] = fine[k] ? pow2f(e[k]) : nan;
           }
         }
       }
+      if (w == 0 && lane == 0) {
+        float* o = info + slot * 4 + (is_v ? 2 : 0);
+        o[0] = is_v ? (float)most : pow2f(max(most, -126));
+        o[1] = own ? 1.0f : 0.0f;
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive_one(&col_full[j & (kTrSlots - 1)]);
-      if (j >= 2 && !tc_wait_ready(&empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort_flag, p.err)) break;
-      kv.store(smem + (is_v ? L::v : L::k) + b * 2 * L::plane_kv, w, lane, e, fine);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_one(&full[b]);
+      if (lane == 0) mbar_arrive_one(&col_full[slot]);
+      ok = ok && (j < 2 || tc_wait_ready(&empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort_flag, p.err));
+      if (ok) {
+        kv.store(smem + (is_v ? L::v : L::k) + b * 2 * L::plane_kv, w, lane, e, fine);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&full[b]);
+      }
       if (Q8) kv = next;
     }
   } else {
@@ -517,7 +562,6 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       const int lr = quad * 32 + lane, r = r0 + lr, i = min(r, sp.R - 1) / rep;
       const uint32_t base = kTmem + ((uint32_t)(32 * quad) << 16);
       const float rf = rowf[lr];
-      const float2 rf2 = make_float2(rf, rf);
       // the row's query planes into TMEM (this thread's half of the dims)
       {
         const uint8_t* src = smem + L::q + (lr >> 3) * (16 * D) + (lr & 7) * 16 + half * (D / 16) * 128;
@@ -538,7 +582,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         if (lane == 0) mbar_arrive_one(q_full);
       }
       float M = -INFINITY;                   // the row's maximum
-      float2 l2 = make_float2(0.0f, 0.0f);   // this half's weights (Q8_0: relative to M - 14, F32: to ml)
+      float l = 0.0f;                        // this half's weights (Q8_0: relative to M - 14, F32: to ml)
       float ml = -INFINITY, f_prev = 1.0f;
       float acc[NA];
 #pragma unroll
@@ -587,11 +631,19 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         if (lane == 0) mbar_arrive_one(&s_empty[b]);
         // (two elements an instruction where the hardware has one)
         float2* x2 = (float2*)x;
+        const float4 in = *(const float4*)(info + (j & (kTrSlots - 1)) * 4);
+        const bool own = in.y != 0.0f || in.w != 0.0f;  // the positions have exponents of their own
+        // score + exponent = x * fac + off; the factor stays above 0, so that a masked -inf does
+        float fac = fmaxf(__fmul_rn(in.x, rf), 1e-37f), off = in.z;
+        if (own) {
+          const float kc = in.y != 0.0f ? 0.0f : in.x, vc = in.z;
 #pragma unroll
-        for (int k = 0; k < HT; k += 4) {
-          const float4 kf = *(const float4*)(c + k), ve = *(const float4*)(c + kTrTile + k);
-          x2[k / 2] = __ffma2_rn(x2[k / 2], __fmul2_rn(make_float2(kf.x, kf.y), rf2), make_float2(ve.x, ve.y));
-          x2[k / 2 + 1] = __ffma2_rn(x2[k / 2 + 1], __fmul2_rn(make_float2(kf.z, kf.w), rf2), make_float2(ve.z, ve.w));
+          for (int k = 0; k < HT; k++) {
+            const float kf = in.y != 0.0f ? c[k] : kc, ve = in.w != 0.0f ? c[kTrTile + k] : vc;
+            x[k] = __fmaf_rn(x[k], fmaxf(__fmul_rn(kf, rf), kf == kf ? 1e-37f : kf), ve);
+          }
+          fac = 1.0f;
+          off = 0.0f;
         }
         if (pt + HT > p.n_past) {
           const uint32_t m = attended32(p, i, pt, n_kv);
@@ -601,60 +653,75 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         }
         float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int k = 4; k < HT; k += 4)
+        for (int k = 4; k < HT; k += 8)
 #pragma unroll
-          for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], x[k + u]);
+          for (int u = 0; u < 4; u++) mx[u] = k + 4 < HT ? fmaxf(fmaxf(mx[u], x[k + u]), x[k + 4 + u]) : fmaxf(mx[u], x[k + u]);
         mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if (!(mx[0] == mx[0])) mx[0] = -INFINITY;  // (nothing but NaN)
+        // The references are whole numbers not below the maximum, so that their
+        // differences and those with the exponents are exact (NaN where there is
+        // nothing else: as if nothing were attended, the weights bring it back).
+        mx[0] = mx[0] == mx[0] ? ceilf(__fmaf_ru(mx[0], fac, off)) : -INFINITY;
         // the row's maximum over both halves
         float* ex = mxs + (b * 2) * kTrRows + lr;
         ex[half * kTrRows] = mx[0];
         meet();
         const float Mn = fmaxf(M, fmaxf(mx[0], ex[(half ^ 1) * kTrRows]));
-        // (2^14: the largest weight that fp16 still holds with room)
-        const float Mr = Mn == -INFINITY ? 0.0f : Mn, Ms = __fsub_rn(Mr, 14.0f);
+        // (2^14: the largest weight that fp16 still holds with room; rounded up, and
+        // the sum below down, so that no score of any size gets past it)
+        const float Mr = Mn == -INFINITY ? 0.0f : Mn, Ms = __fsub_ru(Mr, 14.0f);
         const float f = exp2_approx(__fsub_rn(M, Mr));
         M = Mn;
-        float mls = 0.0f;
+        float lr0 = Ms;  // what the weights' sum is relative to
         if (Q8) {
-          l2 = __fmul2_rn(l2, make_float2(f, f));
+          l = __fmul_rn(l, f);
         } else {
+          // the values' exponents reach over all of a float's range: the sum has a
+          // reference of its own, the largest score of this half without them
           float ms = -INFINITY;
+          if (own) {
 #pragma unroll
-          for (int k = 0; k < HT; k++) ms = fmaxf(ms, __fsub_rn(x[k], c[2 * kTrTile + k]));
+            for (int k = 0; k < HT; k++) ms = fmaxf(ms, __fsub_rn(x[k], in.w != 0.0f ? c[2 * kTrTile + k] : in.z));
+            ms = ceilf(ms);
+          } else {
+            ms = __fsub_rn(mx[0], in.z);
+          }
           if (ms > ml) {
-            const float g = exp2_approx(__fsub_rn(ml, ms));
-            l2 = __fmul2_rn(l2, make_float2(g, g));
+            l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, ms)));
             ml = ms;
           }
-          mls = ml == -INFINITY ? 0.0f : ml;
+          lr0 = ml == -INFINITY ? 0.0f : ml;
         }
-        // P's planes of step j - 2 are free: that step's O has been taken
-        const float2 neg_ms = make_float2(-Ms, -Ms), one = make_float2(-1.0f, -1.0f);
-        uint32_t hi[HT / 2], lo[HT / 2];
+        // the factor that takes a value exponent out of a weight and brings it to lr0
+        const float ls = __fsub_rn(Ms, lr0), lf = __fsub_rn(ls, in.z);
+        const bool apart = own || lf > 100.0f;  // (above: weights that count may be below a float's range)
+        if (apart) {
 #pragma unroll
-        for (int k = 0; k < HT; k += 4) {
-          const float4 vf = *(const float4*)(c + 2 * kTrTile + k);
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            const float2 w = u ? make_float2(vf.z, vf.w) : make_float2(vf.x, vf.y);
-            const float2 d = __fadd2_rn(x2[k / 2 + u], neg_ms);
-            const float2 pe = make_float2(exp2_approx(d.x), exp2_approx(d.y));
-            if (Q8) {
-              l2 = __ffma2_rn(pe, w, l2);
-            } else {
-              const float2 s2 = __fadd2_rn(__ffma2_rn(w, one, x2[k / 2 + u]), make_float2(-mls, -mls));
-              l2 = __fadd2_rn(l2, make_float2(exp2_approx(s2.x), exp2_approx(s2.y)));
-            }
-            // the upper half by cutting to fp16's 11 bits (below 2^-14, a weight of
-            // 2^-28 of the row's largest, its conversion rounds instead)
-            const float2 top = make_float2(__uint_as_float(__float_as_uint(pe.x) & 0xffffe000u),
-                                           __uint_as_float(__float_as_uint(pe.y) & 0xffffe000u));
-            const float2 rest = __ffma2_rn(top, one, pe);
-            hi[k / 2 + u] = h2_bits(__floats2half2_rn(top.x, top.y));
-            lo[k / 2 + u] = h2_bits(__floats2half2_rn(rest.x, rest.y));
+          for (int k = 0; k < HT; k++) {
+            const float ve = in.w != 0.0f ? c[2 * kTrTile + k] : in.z, g = __fsub_rn(ls, ve);
+            const float s = own ? x[k] : __fmaf_rn(x[k], fac, off);
+            l = g > 100.0f ? __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(s, ve), lr0)))
+                           : __fmaf_rn(exp2_approx(__fsub_rn(s, Ms)), exp2_approx(g), l);
           }
         }
+        // P's planes of step j - 2 are free: that step's O has been taken
+        const float2 fac2 = make_float2(fac, fac), off2 = make_float2(__fsub_rd(off, Ms), __fsub_rd(off, Ms));
+        const float2 minus = make_float2(-1.0f, -1.0f);
+        float2 sum = make_float2(0.0f, 0.0f);
+        uint32_t hi[HT / 2], lo[HT / 2];
+#pragma unroll
+        for (int k = 0; k < HT / 2; k++) {
+          const float2 d = __ffma2_rn(x2[k], fac2, off2);
+          const float2 pe = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+          sum = __fadd2_rn(sum, pe);
+          // the upper half by cutting to fp16's 11 bits (below 2^-14, a weight of
+          // 2^-28 of the row's largest, its conversion rounds instead)
+          const float2 top = make_float2(__uint_as_float(__float_as_uint(pe.x) & 0xffffe000u),
+                                         __uint_as_float(__float_as_uint(pe.y) & 0xffffe000u));
+          const float2 rest = __ffma2_rn(top, minus, pe);
+          hi[k] = h2_bits(__floats2half2_rn(top.x, top.y));
+          lo[k] = h2_bits(__floats2half2_rn(rest.x, rest.y));
+        }
+        if (!apart) l = __fmaf_rn(__fadd_rn(sum.x, sum.y), exp2_approx(lf), l);
         tmem_st16(base + kColP + 64 * b + half * (HT / 2), hi);
         tmem_st16(base + kColP + 64 * b + 32 + half * (HT / 2), lo);
         if (j > 0) ok = take_o(j - 1, f_prev);
@@ -666,8 +733,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       }
       if (ok) ok = take_o(n - 1, f_prev);
       // the halves' sums
-      float l = __fadd_rn(l2.x, l2.y);
-      float m = M == -INFINITY ? -INFINITY : __fsub_rn(M, 14.0f);  // what l is relative to
+      float m = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);  // what l is relative to
       float* ex = mxs + (n & 1) * 2 * kTrRows + lr;  // (not the last step's)
       ex[half * kTrRows] = Q8 ? 0.0f : ml;
       meet();
@@ -680,7 +746,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       meet();
       l = __fadd_rn(l, ex[(half ^ 1) * kTrRows]);
       if (ok && r < sp.R) {
-        const float Ms = M == -INFINITY ? -INFINITY : __fsub_rn(M, 14.0f);
+        const float Ms = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);
         if (sp.S == 1) {
           // one split: the result itself; a token that attends to nothing has l = 0
           const float g = Ms == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(Ms, m));

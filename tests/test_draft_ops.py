@@ -491,6 +491,38 @@ def test_attention_tree_sizes_of_values(torch, q8):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("H,HKV,D", [(14, 2, 64), (4, 2, 128)])
+def test_attention_tree_rows_of_different_size(torch, q8, H, HKV, D):
+    """Rows whose magnitudes are far apart, and huge rows that only some tokens attend to: the
+    others' results keep the precision of the rows that they do attend to."""
+    T, past = 24, 150
+    q, caches, _, n_ctx = attn_inputs(torch, T, H, HKV, D, past, 6, False)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    size = lambda lo, hi: torch.exp(torch.empty((n_ctx, 1, 1), device="cuda").uniform_(math.log(lo), math.log(hi), generator=g))  # noqa: E731
+    mask = mi_cuda.tree_mask(random_tree(np.random.default_rng(3), T))
+    seen = seen_of(torch, mask, T, past)
+    for ks, vs, huge in ((size(1e-5, 1), size(1e-4, 1e2), 1.0), (size(1, 1), size(1e-3, 1), 5e6), (size(1e-6, 1), size(1, 1), 8e6)):
+        k, v = caches[0] * ks, caches[1] * vs
+        for c in (k, v):  # drafted tokens 0, 7 and 19: huge
+            c[[past, past + 7, past + 19]] *= huge
+        if q8:
+            both = [mi_cuda.kv_q8_0_cache(n_ctx, HKV, D) for _ in range(2)]
+            mi_cuda.kv_append_q8_0(k, v, *both, n_ctx)
+            rows = mi_cuda.kv_read_q8_0(*both, HKV, D, n_ctx, 0, past + T)
+        else:
+            both, rows = (k, v), (k[: past + T], v[: past + T])
+        got = tree(torch, q8, q, both, HKV, n_ctx, past, 0.1, mask)
+        hit = seen[:, [past, past + 7, past + 19]].any(1)
+        assert 0 < int(hit.sum()) < T
+        for part in (hit, ~hit):
+            want, tol = attn_f64(torch, q[part], *rows, seen[part], 0.1)
+            assert float((got[part].double() - want).abs().max()) <= tol
+            if part is not hit or huge == 1.0:
+                assert float((got[part].double() - want).norm()) <= 2e-5 * float(want.norm())
+
+
+@pytest.mark.gpu
 def test_attention_tree_strided_queries_and_offsets_past_32_bits(torch):
     """Queries that are parts of stacked rows; a cache whose last head lies past 2^31 bytes."""
     HKV, D, n_ctx, T, past = 16, 128, 1200000, 3, 700
