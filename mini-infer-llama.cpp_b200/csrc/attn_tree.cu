@@ -26,12 +26,16 @@
 //     others' precision).
 //
 // One CTA: 128 rows (a TMEM lane each) over one range of positions, 64 a step.
-// Warps 0-7 softmax: two threads per row, 32 positions each; 8-11 convert keys and
-// 12-15 values into the MMAs' layout; 16 issues the MMAs. Key and value planes (in
-// shared memory), S and P (in TMEM) are doubled, so the MMAs of one step run under
-// the exponentials of another. The queries' planes are copied into TMEM too: as a
+// Warps 0-15 softmax, in two streams: warps 0-7 take the even steps, 8-15 the odd
+// ones, two threads a row, 32 positions each. A step needs of the one before only
+// its maximum, so one stream's exponentials run beside the other's loads, maxima
+// and waits (all of a row's warps share one scheduler, and steps that all of them
+// took together left the exponential unit idle two thirds of the time). Warps 16-19
+// convert keys and 20-23 values into the MMAs' layout in shared memory, two steps
+// deep; 24 issues the MMAs. The queries' planes are copied into TMEM: as a
 // shared-memory operand they are 4 KB a product beside the keys' 2, and shared
-// memory, not the tensor core, then set the pace (80 cycles a product of 32).
+// memory, not the tensor core, set the pace. S and P's planes (twice each), O and
+// the queries' planes fill TMEM's 512 columns.
 //
 // A step's O is a product of its own, added to the softmax threads' registers
 // (O = O 2^(M_old - M_new) + O_step): the MMA's accumulation cuts instead of
@@ -53,32 +57,35 @@ namespace {
 
 constexpr int kTrTile = 64;      // positions per step
 constexpr int kTrRows = 128;     // rows per CTA (MMA M)
-constexpr int kTrWarpK = 8, kTrWarpV = 12, kTrWarpMma = 16;
-constexpr int kTrThreads = 20 * 32;  // (the last three warps complete the MMA warp's group for setmaxnreg)
-constexpr int kTrSlots = 8;      // steps whose column factors are kept (see the roles' waits)
+constexpr int kTrParts = 4;      // softmax threads per row: two per stream; each holds a quarter of O's dims
+constexpr int kTrWarpK = 16, kTrWarpV = 20, kTrWarpMma = 24;
+constexpr int kTrThreads = 28 * 32;  // (the last three warps complete the MMA warp's group for setmaxnreg)
+constexpr int kTrSlots = 8;      // steps whose exponents are kept (see the roles' waits)
 constexpr uint32_t kTrCols = 512;  // all of TMEM: its base is 0
 constexpr uint32_t kTmem = 0;
 // TMEM columns: step j's S at 64 (j & 1), P's planes at 128 + 64 (j & 1) and 32
-// behind it, O at 256, the queries' planes at 384 and D / 2 behind it
+// behind it, O (two steps' where D <= 64) at 256, the queries' planes at 384
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256, kColQ = 384;
-// Registers per thread of the roles: launched with 96 x 640 = 61440, of which
-// 136 x 256 + 80 x 256 + 48 x 128 = 61440 are given out again.
-constexpr int kRegsSoftmax = 136, kRegsConvert = 80, kRegsMma = 48;
+// Registers per thread of the roles: launched with 72 x 896 = 64512, of which
+// 88 x 512 + 56 x 256 + 40 x 128 = 64512 are given out again.
+constexpr int kRegsSoftmax = 88, kRegsConvert = 56, kRegsMma = 40;
 
 template <int D>
 struct TrSmem {
+  static constexpr int n_o = D <= 64 ? 2 : 1;      // steps whose O TMEM holds
   static constexpr int plane_q = kTrRows * D * 2, plane_kv = kTrTile * D * 2;
   static constexpr int q = 0;                      // [hi, lo]
   static constexpr int k = q + 2 * plane_q;        // [step & 1][hi, lo]
   static constexpr int v = k + 4 * plane_kv;
-  static constexpr int col = v + 4 * plane_kv;     // float [kTrSlots][3][64]: key factor, value exponent, what takes it out of the sum
-  static constexpr int info = col + kTrSlots * 3 * kTrTile * 4;  // float [kTrSlots][4]: the step's key factor, value exponent, each whether
-                                                                 // its positions have their own
-  static constexpr int ends = info + kTrSlots * 16;              // int2 [keys, values][step & 1][4 warps]: largest and least exponent
-  static constexpr int rowf = ends + 2 * 2 * 4 * 8;              // float [128]: |scale| * log2(e) * the row's factor
-  static constexpr int mx = rowf + kTrRows * 4;    // float [step & 1][half][128]: the halves' maxima (at the end their sums)
-  static constexpr int bars = mx + 4 * kTrRows * 4;
-  static constexpr int n_bars = 8 + kTrSlots + 8 + 2;
+  static constexpr int col = v + 4 * plane_kv;     // float [kTrSlots][3][64]: key factor, value exponent, the same where finite
+  static constexpr int info = col + kTrSlots * 3 * kTrTile * 4;  // float [kTrSlots][4]: key factor, whether the positions have
+                                                                 // their own, value exponent, whether they have their own
+  static constexpr int ends = info + kTrSlots * 16;   // int2 [keys, values][step & 1][4 warps]: largest and least exponent
+  static constexpr int rowf = ends + 2 * 2 * 4 * 8;   // float [128]: |scale| * log2(e) * the row's factor
+  static constexpr int mx = rowf + kTrRows * 4;       // float [2][kTrParts][128]: the parts' maxima (at the end their sums)
+  static constexpr int ref = mx + 2 * kTrParts * kTrRows * 4;  // float [step & 1][128]: the rows' references
+  static constexpr int bars = ref + 2 * kTrRows * 4;
+  static constexpr int n_bars = 8 + kTrSlots + 6 + 4 + 8 + 2;
   static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
   static constexpr int used = misc + 16;
   // above half of an SM's shared memory: two CTAs must not share its TMEM
@@ -87,7 +94,7 @@ struct TrSmem {
 static_assert(TrSmem<128>::total <= 227 * 1024, "shared memory of one CTA");
 
 struct TreeSplit {
-  int32_t R, RG, S, per;  // rows of a KV head, groups of 128, splits, steps of 64 positions per split
+  int32_t R, RG, S, per;  // rows of a KV head, groups of 128, splits, steps per split
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -140,18 +147,14 @@ __device__ __forceinline__ void tmem_wait_ld(float* r) {
                :
                : "memory");
 }
-__device__ __forceinline__ void tmem_ld16f(uint32_t addr, float* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-      : "r"(addr));
+__device__ __forceinline__ void tmem_ld8f(uint32_t addr, float* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+               : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait_ld16(float* r) {
+__device__ __forceinline__ void tmem_wait_ld8(float* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
-                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7])
                :
                : "memory");
 }
@@ -203,95 +206,188 @@ __device__ __forceinline__ bool row_exponent(const float* x, int& e) {
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
 
-// 64 positions of one cache (keys or values) of one KV head, by four warps: a
-// warp takes rows of eight positions, lane = position % 8 + 8 * g, and of each 32
-// dims the eight g * 8... -- a block of 32 dims in four lanes, 16-byte pieces of
-// the two planes in core matrices of 8 positions x 8 dims.
+// One cache (keys or values) of one KV head, 64 positions a step by four warps: a
+// warp takes two rows of eight positions (row groups w and w + 4), lane = position %
+// 8 + 8 g, and of each 32 dims the eight from 8 g on. So a block of 32 dims lies in
+// four lanes, and a lane's eight are a 16-byte piece of each plane: core matrices of
+// 8 positions x 8 dims.
+//
+// The exponent of a row (planes = row * 2^-e brings it to fp16's range) is that of
+// its largest scale, or for F32 of its largest value.
 template <int D, bool Q8>
-struct KvTile {
-  static constexpr int NC = D / 32;
-  // what a lane holds of its two rows
-  uint2 q[Q8 ? 2 : 1][Q8 ? NC : 1];
-  uint16_t d[Q8 ? 2 : 1][Q8 ? NC : 1];
-  float x[Q8 ? 1 : 2][Q8 ? 1 : NC * 8];
+struct KvRows;
 
-  __device__ __forceinline__ void load(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv,
-                                       int w, int lane) {
+// Q8_0: what store() has used is requested for the next step at once, so that a
+// step's rows are a whole step under way.
+template <int D>
+struct KvRows<D, true> {
+  static constexpr int NC = D / 32, ND = (NC + 1) / 2;
+  uint2 q[2][NC];
+  uint32_t d[2][ND];   // two scales a word
+  uint32_t all[2][ND]; // the scales of positions lane and lane + 32 of the step: every warp finds its exponents itself
+  const uint8_t* qs;   // the head's quants and scales from this CTA's first position on
+  const uint16_t* ds;
+  int64_t left;        // positions from there on
+
+  static __device__ __forceinline__ void scales(const uint16_t* s, bool in, uint32_t (&o)[ND]) {
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+      o[i] = !in ? 0u : NC % 2 == 0 ? *(const uint32_t*)(s + 2 * i) : s[2 * i] | (2 * i + 1 < NC ? (uint32_t)s[2 * i + 1] << 16 : 0u);
+  }
+  __device__ __forceinline__ void load_all(int at, int lane) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) scales(ds + (int64_t)(at + lane + 32 * k) * NC, at + lane + 32 * k < left, all[k]);
+  }
+  __device__ __forceinline__ void load_row(int k, int at, int w, int lane) {
+    const int pos = at + (w + 4 * k) * 8 + (lane & 7);
+    const bool in = pos < left;
+    scales(ds + (int64_t)pos * NC, in, d[k]);
+#pragma unroll
+    for (int i = 0; i < NC; i++)
+      q[k][i] = in ? *(const uint2*)(qs + (int64_t)pos * D + 8 * (lane >> 3) + 32 * i) : make_uint2(0u, 0u);
+  }
+  __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int w, int lane) {
+    const int64_t at = (int64_t)kvh * p.n_ctx + pos0;
+    qs = (const uint8_t*)cache + at * D;
+    ds = (const uint16_t*)((const uint8_t*)cache + (int64_t)p.HKV * p.n_ctx * D) + at * NC;
+    left = n_kv - pos0;
+    load_all(0, lane);
+    load_row(0, 0, w, lane);
+    load_row(1, 0, w, lane);
+  }
+  static __device__ __forceinline__ bool exponent(const uint32_t (&s)[ND], int& e, bool& any) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < ND; i++) m = max(m, max(s[i] & 0x7fffu, (s[i] >> 16) & 0x7fffu));
+    e = max((int)(m >> 10), 1) - 15;  // the largest scale becomes 1..2 (below it for subnormal ones)
+    any = m != 0;
+    return m < 0x7c00u;
+  }
+  // The largest and least exponent of the step's rows that have a value but 0 (least
+  // is -2000 where a row has a NaN scale, an infinity or a NaN) and this lane's rows'.
+  __device__ __forceinline__ void exponents(int at, int w, int lane, int2*, int, int& most, int& least, int (&e)[2], bool (&fine)[2]) {
+    bool bad = false;
+    most = -1000;
+    least = 1000;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-      const int64_t pos = pos0 + (w + 4 * k) * 8 + (lane & 7);
-      const int g = lane >> 3;
-      const bool in = pos < n_kv;
-      if (Q8) {
-        const int64_t at = (int64_t)kvh * p.n_ctx + (in ? pos : 0);
-        const uint8_t* qs = (const uint8_t*)cache + at * D + 8 * g;
-        const uint16_t* ds = (const uint16_t*)((const uint8_t*)cache + (int64_t)p.HKV * p.n_ctx * D) + at * NC;
-#pragma unroll
-        for (int i = 0; i < NC; i++) {
-          q[k][i] = in ? *(const uint2*)(qs + 32 * i) : make_uint2(0u, 0u);
-          d[k][i] = in ? ds[i] : (uint16_t)0;
-        }
-      } else {
-        const float* src = (const float*)cache + ((in ? pos : 0) * p.HKV + kvh) * D + 8 * g;
-#pragma unroll
-        for (int i = 0; i < NC; i++) {
-          const float4 a = in ? *(const float4*)(src + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-          const float4 b = in ? *(const float4*)(src + 32 * i + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-          float* o = &x[k][8 * i];
-          o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
-        }
+      int x;
+      bool any;
+      const bool f = exponent(all[k], x, any);
+      bad |= !f;
+      if (f && any) {
+        most = max(most, x);
+        least = min(least, x);
       }
     }
-  }
-
-  // The exponent that brings row k's planes to fp16's range (planes = row * 2^-e),
-  // and whether the row has a value but 0; false for a row with a NaN scale, an
-  // infinity or a NaN.
-  __device__ __forceinline__ bool exponent(int k, int& e, bool& any) const {
-    if (Q8) {
-      uint32_t m = 0;
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (__any_sync(0xffffffffu, bad)) least = -2000;
+    load_all(at + kTrTile, lane);
 #pragma unroll
-      for (int i = 0; i < NC; i++) m = max(m, (uint32_t)d[k][i] & 0x7fffu);
-      e = max((int)(m >> 10), 1) - 15;  // the largest scale becomes 1..2 (below it for subnormal ones)
-      any = m != 0;
-      return m < 0x7c00u;
+    for (int k = 0; k < 2; k++) {
+      bool any;
+      fine[k] = exponent(d[k], e[k], any);
     }
-    const bool fine = row_exponent<NC * 8>(x[k], e);
-    any = e > -100;
-    e -= 14;
-    return fine;
   }
+  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&e)[2], const bool (&fine)[2]) {
+    constexpr int plane = kTrTile * D * 2;
+    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      uint8_t* dst = planes + (w + 4 * k) * (16 * D) + (lane >> 3) * 128 + (lane & 7) * 16;
+      // 2^-e: fp16 holds 2^14 down to 2^-15
+      const __half down = __float2half_rn(fine[k] ? pow2f(-e[k]) : 0.0f);
+#pragma unroll
+      for (int i = 0; i < NC; i++) {
+        const __half s = __ushort_as_half(fine[k] ? (uint16_t)(i & 1 ? d[k][i / 2] >> 16 : d[k][i / 2]) : (uint16_t)0);
+        const __half2 f = __half2half2(__hmul_rn(s, down));
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint32_t b = j < 2 ? q[k][i].x : q[k][i].y;
+          // two signed bytes as fp16: 1024 + (byte + 128) - 1152
+          const uint32_t t = __byte_perm(b, 0x64646464u, j & 1 ? 0x7362 : 0x5140) ^ 0x00800080u;
+          const __half2 n = __hsub2_rn(*reinterpret_cast<const __half2*>(&t), off);
+          const __half2 hh = __hmul2_rn(n, f);
+          h[j] = h2_bits(hh);
+          l[j] = h2_bits(__hfma2(n, f, __hneg2(hh)));
+        }
+        *(uint4*)(dst + i * 512) = make_uint4(h[0], h[1], h[2], h[3]);
+        *(uint4*)(dst + plane + i * 512) = make_uint4(l[0], l[1], l[2], l[3]);
+      }
+      load_row(k, at + kTrTile, w, lane);
+    }
+  }
+};
 
-  __device__ __forceinline__ void store(uint8_t* planes, int w, int lane, const int (&e)[2], const bool (&fine)[2]) const {
+// F32: a step's rows would take too many registers; they are read for their
+// exponents and again for their planes.
+template <int D>
+struct KvRows<D, false> {
+  static constexpr int NC = D / 32;
+  const float* rows;  // the head's, from this CTA's first position on
+  int64_t row, left;  // floats between positions; positions
+
+  __device__ __forceinline__ void load_row(int pos, int lane, float (&x)[NC * 8]) const {
+    const bool in = pos < left;
+    const float* src = rows + (int64_t)pos * row + 8 * (lane >> 3);
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+      const float4 a = in ? *(const float4*)(src + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 b = in ? *(const float4*)(src + 32 * i + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float* o = &x[8 * i];
+      o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
+    }
+  }
+  __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int, int) {
+    row = (int64_t)p.HKV * D;
+    rows = (const float*)cache + pos0 * row + (int64_t)kvh * D;
+    left = n_kv - pos0;
+  }
+  // (as above; `ends` [4]: what the four warps found, met at barrier `id`, also by
+  // warps that have given up)
+  __device__ __forceinline__ void exponents(int at, int w, int lane, int2* ends, int id, int& most, int& least, int (&e)[2],
+                                            bool (&fine)[2]) const {
+    bool bad = false;
+    most = -1000;
+    least = 1000;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      float x[NC * 8];
+      load_row(at + (w + 4 * k) * 8 + (lane & 7), lane, x);
+      fine[k] = row_exponent<NC * 8>(x, e[k]);
+      bad |= !fine[k];
+      const bool any = e[k] > -100;
+      e[k] -= 14;
+      if (fine[k] && any) {
+        most = max(most, e[k]);
+        least = min(least, e[k]);
+      }
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (__any_sync(0xffffffffu, bad)) least = -2000;
+    if (lane == 0) ends[w] = make_int2(most, least);
+    asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int2 o = ends[k];
+      most = max(most, o.x);
+      least = min(least, o.y);
+    }
+  }
+  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&e)[2], const bool (&fine)[2]) const {
     constexpr int plane = kTrTile * D * 2;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       uint8_t* dst = planes + (w + 4 * k) * (16 * D) + (lane >> 3) * 128 + (lane & 7) * 16;
+      float x[NC * 8];
+      load_row(at + (w + 4 * k) * 8 + (lane & 7), lane, x);
 #pragma unroll
       for (int i = 0; i < NC; i++) {
         uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (fine[k]) {
-          if (Q8) {
-            const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-            // 2^-e: fp16 holds 2^14 down to 2^-15
-            const __half2 f = __half2half2(__hmul_rn(__ushort_as_half(d[k][i]), __float2half_rn(pow2f(-e[k]))));
-            uint32_t h[4], l[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const uint32_t b = j < 2 ? q[k][i].x : q[k][i].y;
-              // two signed bytes as fp16: 1024 + (byte + 128) - 1152
-              const uint32_t t = __byte_perm(b, 0x64646464u, j & 1 ? 0x7362 : 0x5140) ^ 0x00800080u;
-              const __half2 n = __hsub2_rn(*reinterpret_cast<const __half2*>(&t), off);
-              const __half2 hh = __hmul2_rn(n, f);
-              h[j] = h2_bits(hh);
-              l[j] = h2_bits(__hfma2(n, f, __hneg2(hh)));
-            }
-            hi = make_uint4(h[0], h[1], h[2], h[3]);
-            lo = make_uint4(l[0], l[1], l[2], l[3]);
-          } else {
-            split8(&x[k][8 * i], pow2f(-e[k]), hi, lo);
-          }
-        }
+        if (fine[k]) split8(&x[8 * i], pow2f(-e[k]), hi, lo);
         *(uint4*)(dst + i * 512) = hi;
         *(uint4*)(dst + plane + i * 512) = lo;
       }
@@ -332,22 +428,25 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   const int64_t n_kv = (int64_t)p.n_past + p.T;
   const int64_t pos0 = (int64_t)split * sp.per * kTrTile;
   const int n = (int)min((int64_t)sp.per, (n_kv - pos0 + kTrTile - 1) / kTrTile);  // steps of this CTA, at least one
-  const int nq = min(4, (sp.R - r0 + 31) / 32);  // quadrants of 32 rows in use: two softmax warps each
+  const int nq = min(4, (sp.R - r0 + 31) / 32);  // quadrants of 32 rows in use: kTrParts softmax warps each
   float* col = (float*)(smem + L::col);
   float* info = (float*)(smem + L::info);
   float* rowf = (float*)(smem + L::rowf);
   float* mxs = (float*)(smem + L::mx);
-  uint64_t* k_full = (uint64_t*)(smem + L::bars);  // each [step & 1]
+  float* ref = (float*)(smem + L::ref);
+  uint64_t* k_full = (uint64_t*)(smem + L::bars);  // these four [step & 1]
   uint64_t* k_empty = k_full + 2;
   uint64_t* v_full = k_full + 4;
   uint64_t* v_empty = k_full + 6;
   uint64_t* col_full = k_full + 8;  // [kTrSlots]
-  uint64_t* s_full = col_full + kTrSlots;
+  uint64_t* s_full = col_full + kTrSlots;  // these three [step & 1]
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_full + 4;
-  uint64_t* o_full = s_full + 6;  // one: O is taken before the next P is handed over
-  uint64_t* q_full = s_full + 7;
-  uint64_t* drain = s_full + 8;
+  uint64_t* o_full = s_full + 6;  // these two [step % n_o]
+  uint64_t* o_empty = s_full + 8;
+  uint64_t* ref_full = s_full + 10;  // [step & 1][quadrant]
+  uint64_t* q_full = s_full + 18;
+  uint64_t* drain = s_full + 19;
   uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
   volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
 
@@ -360,10 +459,12 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 2 * nq);
       mbar_init(&p_full[i], 2 * nq);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], kTrParts * nq);
     }
-    mbar_init(o_full, 1);
-    mbar_init(q_full, 2 * nq);
     for (int i = 0; i < kTrSlots; i++) mbar_init(&col_full[i], 8);
+    for (int i = 0; i < 8; i++) mbar_init(&ref_full[i], 2);
+    mbar_init(q_full, kTrParts * nq);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -422,16 +523,18 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       const uint64_t kd = umma_desc(smem_addr(smem + L::k), 128, 16 * D);
       const uint64_t vd = umma_desc(smem_addr(smem + L::v), 16 * D, 128);
       constexpr uint64_t plane = L::plane_kv >> 4;
-      // step j's scores: into S (j & 1) once step j - 2's have been read
+      // step j's scores, once step j - 2's have been read
       auto scores = [&](int j) {
         const int b = j & 1;
         const uint32_t ph = (uint32_t)(j >> 1) & 1u;
         if (!tc_wait_ready(&k_full[b], ph, abort_flag, p.err)) return false;
         if (j >= 2 && !tc_wait_ready(&s_empty[b], ph ^ 1, abort_flag, p.err)) return false;
         tc_fence_after();
-        const uint32_t d = kTmem + kColS + 64 * b;
-        const uint64_t kh = kd + 2 * plane * b, kl = kh + plane;
         if (elect_one()) {
+          const uint32_t d = kTmem + kColS + 64 * b;
+          uint64_t kh = kd + 2 * plane * b;
+          asm volatile("" : "+l"(kh));  // (the 24 descriptors are formed here, not kept in registers)
+          const uint64_t kl = kh + plane;
 #pragma unroll
           for (int s = 0; s < D / 16; s++) mma_ts(d, ql + 8 * s, kh + 16 * s, idesc_s, s > 0);
 #pragma unroll
@@ -448,21 +551,24 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       if (ok && n > 1) ok = scores(1);
       for (int j = 0; j < n && ok; j++) {
         if (j > 0 && j + 1 < n && !(ok = scores(j + 1))) break;
-        const int b = j & 1;
+        const int b = j & 1, ob = j % L::n_o;
         const uint32_t ph = (uint32_t)(j >> 1) & 1u;
         if (!(ok = tc_wait_ready(&v_full[b], ph, abort_flag, p.err))) break;
+        if (j >= L::n_o && !(ok = tc_wait_ready(&o_empty[ob], (uint32_t)(j / L::n_o - 1) & 1u, abort_flag, p.err))) break;
         if (!(ok = tc_wait_ready(&p_full[b], ph, abort_flag, p.err))) break;
         tc_fence_after();
-        const uint32_t o = kTmem + kColO, p_hi = kTmem + kColP + 64 * b, p_lo = p_hi + 32;
-        const uint64_t vh = vd + 2 * plane * b, vl = vh + plane;
         if (elect_one()) {
+          const uint32_t o = kTmem + kColO + D * ob, p_hi = kTmem + kColP + 64 * b, p_lo = p_hi + 32;
+          uint64_t vh = vd + 2 * plane * b;
+          asm volatile("" : "+l"(vh));
+          const uint64_t vl = vh + plane;
 #pragma unroll
           for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_lo + 8 * s, vh + 2 * D * s, idesc_o, s > 0);
 #pragma unroll
           for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vl + 2 * D * s, idesc_o, 1);
 #pragma unroll
           for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vh + 2 * D * s, idesc_o, 1);
-          umma_commit(o_full);
+          umma_commit(&o_full[ob]);
           umma_commit(&v_empty[b]);
         }
         __syncwarp();
@@ -474,10 +580,11 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       }
     }
   } else if (warp >= kTrWarpK) {
-    // ---------------- keys (warps 8-11) and values (12-15) ----------------
-    // A slot of the column factors is written again eight steps later: after the
-    // planes of seven, which waited for the products of five, whose S was free only
-    // when the softmax had gone past step three.
+    // ---------------- keys (warps 16-19) and values (20-23) ----------------
+    // A step's exponents go out before its planes, which wait for the products that
+    // read those of two steps ago. Their slot is written again eight steps later:
+    // after the planes of seven, which waited for the scores of five and so of four,
+    // for which the step's own stream had read the scores of two.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
     const bool is_v = warp >= kTrWarpV;
     const int w = warp & 3;
@@ -485,38 +592,14 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     uint64_t* full = is_v ? v_full : k_full;
     uint64_t* empty = is_v ? v_empty : k_empty;
     int2* ends = (int2*)(smem + L::ends) + (is_v ? 8 : 0);
-    KvTile<D, Q8> kv, next;
-    if (Q8) kv.load(p, cache, kvh, pos0, n_kv, w, lane);
+    KvRows<D, Q8> kv;
+    kv.begin(p, cache, kvh, pos0, n_kv, w, lane);
     bool ok = true;
     for (int j = 0; j < n; j++) {
       const int b = j & 1, slot = j & (kTrSlots - 1);
-      // (a step of F32 rows takes too many registers to be held twice)
-      if (!Q8) kv.load(p, cache, kvh, pos0 + (int64_t)j * kTrTile, n_kv, w, lane);
-      else if (j + 1 < n) next.load(p, cache, kvh, pos0 + (int64_t)(j + 1) * kTrTile, n_kv, w, lane);
-      int e[2], most = -1000, least = 1000;
-      bool fine[2], bad = false;
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        bool any;
-        fine[k] = kv.exponent(k, e[k], any);
-        bad |= !fine[k];
-        if (fine[k] && any) {
-          most = max(most, e[k]);
-          least = min(least, e[k]);
-        }
-      }
-      most = __reduce_max_sync(0xffffffffu, most);
-      least = __reduce_min_sync(0xffffffffu, least);
-      if (__any_sync(0xffffffffu, bad)) least = -2000;
-      if (lane == 0) ends[b * 4 + w] = make_int2(most, least);
-      // the four warps' exponents (met by warps that have given up too)
-      asm volatile("bar.sync %0, 128;" ::"r"(is_v ? 6 : 5) : "memory");
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int2 o = ends[b * 4 + k];
-        most = max(most, o.x);
-        least = min(least, o.y);
-      }
+      int e[2], most, least;
+      bool fine[2];
+      kv.exponents(j * kTrTile, w, lane, ends + b * 4, is_v ? 10 : 9, most, least, e, fine);
       const bool own = least < 1000 && most - least > 10;
       if (!own) {
         if (most < -999) most = 0;
@@ -546,34 +629,32 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       if (lane == 0) mbar_arrive_one(&col_full[slot]);
       ok = ok && (j < 2 || tc_wait_ready(&empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort_flag, p.err));
       if (ok) {
-        kv.store(smem + (is_v ? L::v : L::k) + b * 2 * L::plane_kv, w, lane, e, fine);
+        kv.store(j * kTrTile, smem + (is_v ? L::v : L::k) + b * 2 * L::plane_kv, w, lane, e, fine);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive_one(&full[b]);
       }
-      if (Q8) kv = next;
     }
   } else {
-    // ---------------- softmax: two threads per row ----------------
+    // ---------------- softmax: two streams of two threads per row ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, part = warp >> 2, stream = part >> 1;
     if (quad < nq) {
-      constexpr int NA = D / 2, HT = kTrTile / 2;
+      constexpr int NA = D / kTrParts, HT = kTrTile / 2;
       const int lr = quad * 32 + lane, r = r0 + lr, i = min(r, sp.R - 1) / rep;
       const uint32_t base = kTmem + ((uint32_t)(32 * quad) << 16);
       const float rf = rowf[lr];
-      // the row's query planes into TMEM (this thread's half of the dims)
+      // the row's query planes into TMEM (this thread's quarter of the dims)
       {
-        const uint8_t* src = smem + L::q + (lr >> 3) * (16 * D) + (lr & 7) * 16 + half * (D / 16) * 128;
+        const uint8_t* src = smem + L::q + (lr >> 3) * (16 * D) + (lr & 7) * 16 + part * (D / 32) * 128;
 #pragma unroll
         for (int pl = 0; pl < 2; pl++)
 #pragma unroll
-          for (int o = 0; o < D / 4; o += 8) {
-            const uint4 a = *(const uint4*)(src + pl * L::plane_q + (o / 4) * 128);
-            const uint4 c = *(const uint4*)(src + pl * L::plane_q + (o / 4 + 1) * 128);
-            asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(
-                             base + kColQ + pl * (D / 2) + half * (D / 4) + o),
-                         "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w)
+          for (int o = 0; o < D / 32; o++) {
+            const uint4 a = *(const uint4*)(src + pl * L::plane_q + o * 128);
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             base + kColQ + pl * (D / 2) + part * (D / 8) + o * 4),
+                         "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w)
                          : "memory");
           }
         tmem_wait_st();
@@ -581,57 +662,68 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive_one(q_full);
       }
-      float M = -INFINITY;                   // the row's maximum
-      float l = 0.0f;                        // this half's weights (Q8_0: relative to M - 14, F32: to ml)
-      float ml = -INFINITY, f_prev = 1.0f;
+      float M = -INFINITY;   // the row's reference (of the last step that this thread knows of)
+      float l = 0.0f;        // this part's weights (Q8_0: relative to Ml - 14, F32: to ml)
+      float Ml = -INFINITY, ml = -INFINITY, f_own = 1.0f;
       float acc[NA];
 #pragma unroll
       for (int k = 0; k < NA; k++) acc[k] = 0.0f;
-      // step j's O into the registers
+      // step j's O into the registers, which so far are relative to a reference of
+      // 1 / f times its
       auto take_o = [&](int j, float f) {
-        if (!tc_wait_ready(o_full, (uint32_t)j & 1u, abort_flag, p.err)) return false;
+        const int ob = j % L::n_o;
+        if (!tc_wait_ready(&o_full[ob], (uint32_t)(j / L::n_o) & 1u, abort_flag, p.err)) return false;
         tc_fence_after();
         const float2 f2 = make_float2(f, f);
+        float y[NA];
 #pragma unroll
-        for (int o = 0; o < NA; o += 32) {
-          float y[32];
-          tmem_ld16f(base + kColO + NA * half + o, y);
-          if (o + 16 < NA) tmem_ld16f(base + kColO + NA * half + o + 16, y + 16);
-          tmem_wait_ld16(y);
-          if (o + 16 < NA) tmem_wait_ld16(y + 16);
+        for (int o = 0; o < NA; o += 8) tmem_ld8f(base + kColO + D * ob + NA * part + o, y + o);
 #pragma unroll
-          for (int k = 0; k < 32 && o + k < NA; k += 2) {
-            const float2 a = __ffma2_rn(make_float2(acc[o + k], acc[o + k + 1]), f2, make_float2(y[k], y[k + 1]));
-            acc[o + k] = a.x;
-            acc[o + k + 1] = a.y;
-          }
+        for (int o = 0; o < NA; o += 8) tmem_wait_ld8(y + o);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&o_empty[ob]);
+#pragma unroll
+        for (int k = 0; k < NA; k += 2) {
+          const float2 a = __ffma2_rn(make_float2(acc[k], acc[k + 1]), f2, make_float2(y[k], y[k + 1]));
+          acc[k] = a.x;
+          acc[k + 1] = a.y;
         }
         return true;
       };
-      // The row's other half has come as far: once a step and twice at the end, also
-      // by warps that have given up (so that none waits for the other).
-      auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
+      // The reference that the other stream has set for step j; the factor from the
+      // one before it, `from`.
+      auto other_ref = [&](int j, float from, float& f) {
+        if (!tc_wait_ready(&ref_full[(j & 1) * 4 + quad], (uint32_t)(j >> 1) & 1u, abort_flag, p.err)) return false;
+        M = ref[(j & 1) * kTrRows + lr];
+        f = exp2_approx(__fsub_rn(from, M == -INFINITY ? 0.0f : M));
+        return true;
+      };
+      // The stream's other half of the row has come as far: once a step, also by
+      // warps that have given up (so that none waits for another).
+      auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad + 4 * stream) : "memory"); };
       bool ok = true;
-      for (int j = 0; j < n; j++) {
-        const int b = j & 1;
-        const int64_t pt = pos0 + (int64_t)j * kTrTile + half * HT;
-        const float* c = col + (j & (kTrSlots - 1)) * 3 * kTrTile + half * HT;
-        ok = ok && tc_wait_ready(&col_full[j & (kTrSlots - 1)], (uint32_t)(j / kTrSlots) & 1u, abort_flag, p.err) &&
-             tc_wait_ready(&s_full[b], (uint32_t)(j >> 1) & 1u, abort_flag, p.err);
+      for (int j = stream; j < n; j += 2) {
+        const int slot = j & (kTrSlots - 1), b = stream;
+        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+        const int64_t pt = pos0 + (int64_t)j * kTrTile + (part & 1) * HT;
+        const float* c = col + slot * 3 * kTrTile + (part & 1) * HT;
+        ok = ok && tc_wait_ready(&col_full[slot], (uint32_t)(j / kTrSlots) & 1u, abort_flag, p.err) &&
+             tc_wait_ready(&s_full[b], ph, abort_flag, p.err);
         if (!ok) {
           meet();
           continue;
         }
         tc_fence_after();
         float x[HT];
-        tmem_ld32(base + kColS + 64 * b + half * HT, x);
+        tmem_ld32(base + kColS + 64 * b + (part & 1) * HT, x);
         tmem_wait_ld(x);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_one(&s_empty[b]);
         // (two elements an instruction where the hardware has one)
         float2* x2 = (float2*)x;
-        const float4 in = *(const float4*)(info + (j & (kTrSlots - 1)) * 4);
+        const float4 in = *(const float4*)(info + slot * 4);
         const bool own = in.y != 0.0f || in.w != 0.0f;  // the positions have exponents of their own
         // score + exponent = x * fac + off; the factor stays above 0, so that a masked -inf does
         float fac = fmaxf(__fmul_rn(in.x, rf), 1e-37f), off = in.z;
@@ -661,22 +753,30 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         // differences and those with the exponents are exact (NaN where there is
         // nothing else: as if nothing were attended, the weights bring it back).
         mx[0] = mx[0] == mx[0] ? ceilf(__fmaf_ru(mx[0], fac, off)) : -INFINITY;
-        // the row's maximum over both halves
-        float* ex = mxs + (b * 2) * kTrRows + lr;
-        ex[half * kTrRows] = mx[0];
+        // the row's maximum over the stream's two halves and the steps before
+        float* ex = mxs + (((j >> 1) & 1) * kTrParts + 2 * stream) * kTrRows + lr;
+        ex[(part & 1) * kTrRows] = mx[0];
         meet();
-        const float Mn = fmaxf(M, fmaxf(mx[0], ex[(half ^ 1) * kTrRows]));
+        float f_other = 1.0f;
+        if (j > 0) ok = other_ref(j - 1, M, f_other);
+        const float Mn = fmaxf(M, fmaxf(ex[0], ex[kTrRows]));
+        if ((part & 1) == 0) ref[b * kTrRows + lr] = Mn;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&ref_full[b * 4 + quad]);
         // (2^14: the largest weight that fp16 still holds with room; rounded up, and
         // the sum below down, so that no score of any size gets past it)
         const float Mr = Mn == -INFINITY ? 0.0f : Mn, Ms = __fsub_ru(Mr, 14.0f);
-        const float f = exp2_approx(__fsub_rn(M, Mr));
+        // this stream's last O; with it its P's columns are free
+        if (j >= 2) ok = ok && take_o(j - 2, f_own);
+        f_own = exp2_approx(__fsub_rn(M, Mr));
         M = Mn;
         float lr0 = Ms;  // what the weights' sum is relative to
         if (Q8) {
-          l = __fmul_rn(l, f);
+          l = __fmul_rn(l, exp2_approx(__fsub_rn(Ml, Mr)));
+          Ml = Mn;
         } else {
           // the values' exponents reach over all of a float's range: the sum has a
-          // reference of its own, the largest score of this half without them
+          // reference of its own, the largest score of this part without them
           float ms = -INFINITY;
           if (own) {
 #pragma unroll
@@ -703,7 +803,6 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
                            : __fmaf_rn(exp2_approx(__fsub_rn(s, Ms)), exp2_approx(g), l);
           }
         }
-        // P's planes of step j - 2 are free: that step's O has been taken
         const float2 fac2 = make_float2(fac, fac), off2 = make_float2(__fsub_rd(off, Ms), __fsub_rd(off, Ms));
         const float2 minus = make_float2(-1.0f, -1.0f);
         float2 sum = make_float2(0.0f, 0.0f);
@@ -722,44 +821,58 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           lo[k] = h2_bits(__floats2half2_rn(rest.x, rest.y));
         }
         if (!apart) l = __fmaf_rn(__fadd_rn(sum.x, sum.y), exp2_approx(lf), l);
-        tmem_st16(base + kColP + 64 * b + half * (HT / 2), hi);
-        tmem_st16(base + kColP + 64 * b + 32 + half * (HT / 2), lo);
-        if (j > 0) ok = take_o(j - 1, f_prev);
-        f_prev = f;
+        tmem_st16(base + kColP + 64 * b + (part & 1) * (HT / 2), hi);
+        tmem_st16(base + kColP + 64 * b + 32 + (part & 1) * (HT / 2), lo);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_one(&p_full[b]);
+        // the other stream's last O
+        if (j > 0) ok = ok && take_o(j - 1, f_other);
       }
-      if (ok) ok = take_o(n - 1, f_prev);
-      // the halves' sums
+      // the steps after this stream's last but one
+      const int last = n - 1 - ((n - 1 - stream) & 1);  // this stream's last step (-1: it has none)
+      if (last >= 0) ok = ok && take_o(last, f_own);
+      if (last + 1 < n) {
+        float f = 1.0f;
+        ok = ok && other_ref(last + 1, M, f) && take_o(last + 1, f);
+      }
+      if (Q8 && l != 0.0f) l = __fmul_rn(l, exp2_approx(__fsub_rn(Ml, M)));
+      // the parts' sums (a barrier of the quadrant's four warps)
+      auto meet4 = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(11 + quad) : "memory"); };
       float m = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);  // what l is relative to
-      float* ex = mxs + (n & 1) * 2 * kTrRows + lr;  // (not the last step's)
-      ex[half * kTrRows] = Q8 ? 0.0f : ml;
-      meet();
-      if (!Q8) {
-        m = fmaxf(ml, ex[(half ^ 1) * kTrRows]);
-        if (ml != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, m)));
+      meet4();  // (the last steps' maxima have been read)
+      float* ex = mxs + lr;
+      ex[part * kTrRows] = ml;
+      ex[(kTrParts + part) * kTrRows] = l;
+      meet4();
+      if (Q8) {
+        l = __fadd_rn(__fadd_rn(ex[4 * kTrRows], ex[5 * kTrRows]), __fadd_rn(ex[6 * kTrRows], ex[7 * kTrRows]));
+      } else {
+        m = fmaxf(fmaxf(ex[0], ex[kTrRows]), fmaxf(ex[2 * kTrRows], ex[3 * kTrRows]));
+        l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kTrParts; k++)
+          if (ex[k * kTrRows] != -INFINITY)
+            l = __fmaf_rn(ex[(kTrParts + k) * kTrRows], exp2_approx(__fsub_rn(ex[k * kTrRows], m)), l);
+          else
+            l = __fadd_rn(l, ex[(kTrParts + k) * kTrRows]);
       }
-      ex = mxs + ((n + 1) & 1) * 2 * kTrRows + lr;
-      ex[half * kTrRows] = l;
-      meet();
-      l = __fadd_rn(l, ex[(half ^ 1) * kTrRows]);
       if (ok && r < sp.R) {
         const float Ms = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);
         if (sp.S == 1) {
           // one split: the result itself; a token that attends to nothing has l = 0
           const float g = Ms == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(Ms, m));
           const float inv = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), g);
-          float* out = p.out + ((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D + NA * half;
+          float* out = p.out + ((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D + NA * part;
 #pragma unroll
           for (int k = 0; k < NA; k++) out[k] = __fmul_rn(acc[k], inv);
         } else {
           float* rec = (float*)p.scratch + (((int64_t)kvh * sp.S + split) * sp.R + r) * (D + 4);
-          if (half == 0) *(float4*)rec = make_float4(Ms, m, l, 0.0f);
+          if (part == 0) *(float4*)rec = make_float4(Ms, m, l, 0.0f);
 #pragma unroll
           for (int k = 0; k < NA; k += 4)
-            *(float4*)(rec + 4 + NA * half + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+            *(float4*)(rec + 4 + NA * part + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
         }
       }
     }
