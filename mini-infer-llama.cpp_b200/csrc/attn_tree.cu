@@ -25,17 +25,18 @@
 //     position have its own (a masked row's value then takes nothing from the
 //     others' precision).
 //
-// One CTA: 128 rows (a TMEM lane each) over one range of positions, 64 a step.
-// Warps 0-15 softmax, in two streams: warps 0-7 take the even steps, 8-15 the odd
-// ones, two threads a row, 32 positions each. A step needs of the one before only
-// its maximum, so one stream's exponentials run beside the other's loads, maxima
-// and waits (all of a row's warps share one scheduler, and steps that all of them
-// took together left the exponential unit idle two thirds of the time). Warps 16-19
-// convert keys and 20-23 values into the MMAs' layout in shared memory, two steps
-// deep; 24 issues the MMAs. The queries' planes are copied into TMEM: as a
-// shared-memory operand they are 4 KB a product beside the keys' 2, and shared
-// memory, not the tensor core, set the pace. S and P's planes (twice each), O and
-// the queries' planes fill TMEM's 512 columns.
+// One CTA: 128 rows (a TMEM lane each) over one range of positions, 128 a step.
+// Warps 0-15 softmax: four threads per row, 32 positions each; 16-19 convert keys
+// and 20-23 values into the MMAs' layout in shared memory; 24 issues the MMAs. The
+// queries' planes are copied into TMEM: as a shared-memory operand they are 4 KB a
+// product beside the keys' 4, and shared memory, not the tensor core, set the pace.
+// S, P's planes, O and the queries' planes fill TMEM's 512 columns at D = 128. The
+// next step's scores run under a step's exponentials and its P V under the next
+// one's.
+//
+// What bounds it: the softmax threads (some 20 instructions a pair of scores and
+// the round trips of a step; steps of 64 positions took 1.4 us, nearly as long as
+// steps of 128) with the MMAs close behind.
 //
 // A step's O is a product of its own, added to the softmax threads' registers
 // (O = O 2^(M_old - M_new) + O_step): the MMA's accumulation cuts instead of
@@ -55,16 +56,16 @@ namespace mi {
 
 namespace {
 
-constexpr int kTrTile = 64;      // positions per step
+constexpr int kTrTile = 128;     // positions per step
+constexpr int kTrHalf = 64;      // ... that share their exponents
+constexpr int kTrParts = 4;      // softmax threads per row: 32 positions each, and a quarter of O's dims
 constexpr int kTrRows = 128;     // rows per CTA (MMA M)
-constexpr int kTrParts = 4;      // softmax threads per row: two per stream; each holds a quarter of O's dims
 constexpr int kTrWarpK = 16, kTrWarpV = 20, kTrWarpMma = 24;
 constexpr int kTrThreads = 28 * 32;  // (the last three warps complete the MMA warp's group for setmaxnreg)
-constexpr int kTrSlots = 8;      // steps whose exponents are kept (see the roles' waits)
+constexpr int kTrSlots = 4;      // steps whose exponents are kept (see the roles' waits)
 constexpr uint32_t kTrCols = 512;  // all of TMEM: its base is 0
 constexpr uint32_t kTmem = 0;
-// TMEM columns: step j's S at 64 (j & 1), P's planes at 128 + 64 (j & 1) and 32
-// behind it, O (two steps' where D <= 64) at 256, the queries' planes at 384
+// TMEM columns: S, P's planes (64 + 64), O, the queries' planes (D / 2 each)
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256, kColQ = 384;
 // Registers per thread of the roles: launched with 72 x 896 = 64512, of which
 // 88 x 512 + 56 x 256 + 40 x 128 = 64512 are given out again.
@@ -72,20 +73,18 @@ constexpr int kRegsSoftmax = 88, kRegsConvert = 56, kRegsMma = 40;
 
 template <int D>
 struct TrSmem {
-  static constexpr int n_o = D <= 64 ? 2 : 1;      // steps whose O TMEM holds
   static constexpr int plane_q = kTrRows * D * 2, plane_kv = kTrTile * D * 2;
   static constexpr int q = 0;                      // [hi, lo]
-  static constexpr int k = q + 2 * plane_q;        // [step & 1][hi, lo]
-  static constexpr int v = k + 4 * plane_kv;
-  static constexpr int col = v + 4 * plane_kv;     // float [kTrSlots][3][64]: key factor, value exponent, the same where finite
-  static constexpr int info = col + kTrSlots * 3 * kTrTile * 4;  // float [kTrSlots][4]: key factor, whether the positions have
-                                                                 // their own, value exponent, whether they have their own
-  static constexpr int ends = info + kTrSlots * 16;   // int2 [keys, values][step & 1][4 warps]: largest and least exponent
-  static constexpr int rowf = ends + 2 * 2 * 4 * 8;   // float [128]: |scale| * log2(e) * the row's factor
-  static constexpr int mx = rowf + kTrRows * 4;       // float [2][kTrParts][128]: the parts' maxima (at the end their sums)
-  static constexpr int ref = mx + 2 * kTrParts * kTrRows * 4;  // float [step & 1][128]: the rows' references
-  static constexpr int bars = ref + 2 * kTrRows * 4;
-  static constexpr int n_bars = 8 + kTrSlots + 6 + 4 + 8 + 2;
+  static constexpr int k = q + 2 * plane_q;        // [hi, lo]
+  static constexpr int v = k + 2 * plane_kv;
+  static constexpr int col = v + 2 * plane_kv;     // float [kTrSlots][half][3][64]: key factor, value exponent, the same where finite
+  static constexpr int info = col + kTrSlots * 2 * 3 * kTrHalf * 4;  // float [kTrSlots][half][4]: key factor, whether the positions have
+                                                                     // their own, value exponent, whether they have their own
+  static constexpr int ends = info + kTrSlots * 2 * 16;  // int2 [keys, values][step & 1][half][4 warps]: largest and least exponent
+  static constexpr int rowf = ends + 2 * 2 * 2 * 4 * 8;  // float [128]: |scale| * log2(e) * the row's factor
+  static constexpr int mx = rowf + kTrRows * 4;    // float [step & 1][part][128]: the parts' maxima (at the end their sums)
+  static constexpr int bars = mx + 2 * kTrParts * kTrRows * 4;
+  static constexpr int n_bars = 4 + 2 * kTrSlots + 6;
   static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
   static constexpr int used = misc + 16;
   // above half of an SM's shared memory: two CTAs must not share its TMEM
@@ -206,45 +205,59 @@ __device__ __forceinline__ bool row_exponent(const float* x, int& e) {
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
 
-// One cache (keys or values) of one KV head, 64 positions a step by four warps: a
-// warp takes two rows of eight positions (row groups w and w + 4), lane = position %
-// 8 + 8 g, and of each 32 dims the eight from 8 g on. So a block of 32 dims lies in
-// four lanes, and a lane's eight are a 16-byte piece of each plane: core matrices of
-// 8 positions x 8 dims.
+// One cache (keys or values) of one KV head, 128 positions a step by four warps: a
+// warp takes four rows of eight positions (row groups w + 4 k, k < 4; k < 2 in the
+// step's first half), lane = position % 8 + 8 g, and of each 32 dims the eight from
+// 8 g on. So a block of 32 dims lies in four lanes, and a lane's eight are a 16-byte
+// piece of each plane: core matrices of 8 positions x 8 dims.
 //
 // The exponent of a row (planes = row * 2^-e brings it to fp16's range) is that of
 // its largest scale, or for F32 of its largest value.
 template <int D, bool Q8>
 struct KvRows;
 
-// Q8_0: what store() has used is requested for the next step at once, so that a
-// step's rows are a whole step under way.
+// Q8_0: two of a warp's rows are in registers, the next two on their way to L2; a
+// row that store() has converted makes room for the one after the next.
 template <int D>
 struct KvRows<D, true> {
   static constexpr int NC = D / 32, ND = (NC + 1) / 2;
   uint2 q[2][NC];
-  uint32_t d[2][ND];   // two scales a word
-  uint32_t all[2][ND]; // the scales of positions lane and lane + 32 of the step: every warp finds its exponents itself
-  const uint8_t* qs;   // the head's quants and scales from this CTA's first position on
+  uint32_t d[2][ND];    // two scales a word
+  uint32_t all[4][ND];  // the scales of the step's positions lane + 32 k: every warp finds the exponents itself
+  const uint8_t* qs;    // the head's quants and scales from this CTA's first position on
   const uint16_t* ds;
-  int64_t left;        // positions from there on
+  int64_t left;         // positions from there on
 
   static __device__ __forceinline__ void scales(const uint16_t* s, bool in, uint32_t (&o)[ND]) {
 #pragma unroll
     for (int i = 0; i < ND; i++)
       o[i] = !in ? 0u : NC % 2 == 0 ? *(const uint32_t*)(s + 2 * i) : s[2 * i] | (2 * i + 1 < NC ? (uint32_t)s[2 * i + 1] << 16 : 0u);
   }
+  // the largest scale becomes 1..2 (below it for subnormal ones); false for a NaN scale
+  static __device__ __forceinline__ bool exponent(const uint32_t (&s)[ND], int& e, bool& any) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < ND; i++) m = max(m, max(s[i] & 0x7fffu, (s[i] >> 16) & 0x7fffu));
+    e = max((int)(m >> 10), 1) - 15;
+    any = m != 0;
+    return m < 0x7c00u;
+  }
   __device__ __forceinline__ void load_all(int at, int lane) {
 #pragma unroll
-    for (int k = 0; k < 2; k++) scales(ds + (int64_t)(at + lane + 32 * k) * NC, at + lane + 32 * k < left, all[k]);
+    for (int k = 0; k < 4; k++) scales(ds + (int64_t)(at + lane + 32 * k) * NC, at + lane + 32 * k < left, all[k]);
   }
+  // the warp's row k of the step at `at`
   __device__ __forceinline__ void load_row(int k, int at, int w, int lane) {
     const int pos = at + (w + 4 * k) * 8 + (lane & 7);
     const bool in = pos < left;
-    scales(ds + (int64_t)pos * NC, in, d[k]);
+    const uint8_t* src = qs + (int64_t)pos * D + 8 * (lane >> 3);
+    scales(ds + (int64_t)pos * NC, in, d[k & 1]);
 #pragma unroll
-    for (int i = 0; i < NC; i++)
-      q[k][i] = in ? *(const uint2*)(qs + (int64_t)pos * D + 8 * (lane >> 3) + 32 * i) : make_uint2(0u, 0u);
+    for (int i = 0; i < NC; i++) q[k & 1][i] = in ? *(const uint2*)(src + 32 * i) : make_uint2(0u, 0u);
+    if (k < 2 && pos + 64 < left && lane < 8) {
+#pragma unroll
+      for (int i = 0; i < D; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 64 * D + i));
+    }
   }
   __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int w, int lane) {
     const int64_t at = (int64_t)kvh * p.n_ctx + pos0;
@@ -255,59 +268,60 @@ struct KvRows<D, true> {
     load_row(0, 0, w, lane);
     load_row(1, 0, w, lane);
   }
-  static __device__ __forceinline__ bool exponent(const uint32_t (&s)[ND], int& e, bool& any) {
-    uint32_t m = 0;
+  // The largest and least exponent of each half's rows that have a value but 0
+  // (least is -2000 where a row has a NaN scale); those of rows that have their own
+  // go to put(half, position in it, exponent, whether it is no NaN).
+  template <class Own, class Put>
+  __device__ __forceinline__ void exponents(int at, int w, int lane, int2*, int, int (&most)[2], bool (&own)[2], Own judge, Put put) {
 #pragma unroll
-    for (int i = 0; i < ND; i++) m = max(m, max(s[i] & 0x7fffu, (s[i] >> 16) & 0x7fffu));
-    e = max((int)(m >> 10), 1) - 15;  // the largest scale becomes 1..2 (below it for subnormal ones)
-    any = m != 0;
-    return m < 0x7c00u;
-  }
-  // The largest and least exponent of the step's rows that have a value but 0 (least
-  // is -2000 where a row has a NaN scale, an infinity or a NaN) and this lane's rows'.
-  __device__ __forceinline__ void exponents(int at, int w, int lane, int2*, int, int& most, int& least, int (&e)[2], bool (&fine)[2]) {
-    bool bad = false;
-    most = -1000;
-    least = 1000;
+    for (int h = 0; h < 2; h++) {
+      bool bad = false;
+      int e[2], hi = -1000, lo = 1000;
+      bool fine[2];
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-      int x;
-      bool any;
-      const bool f = exponent(all[k], x, any);
-      bad |= !f;
-      if (f && any) {
-        most = max(most, x);
-        least = min(least, x);
+      for (int k = 0; k < 2; k++) {
+        bool any;
+        fine[k] = exponent(all[2 * h + k], e[k], any);
+        bad |= !fine[k];
+        if (fine[k] && any) {
+          hi = max(hi, e[k]);
+          lo = min(lo, e[k]);
+        }
+      }
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      if (__any_sync(0xffffffffu, bad)) lo = -2000;
+      most[h] = hi;
+      own[h] = judge(hi, lo);
+      if (own[h] && (lane >> 3) == w) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) put(h, lane + 32 * k, e[k], fine[k]);
       }
     }
-    most = __reduce_max_sync(0xffffffffu, most);
-    least = __reduce_min_sync(0xffffffffu, least);
-    if (__any_sync(0xffffffffu, bad)) least = -2000;
     load_all(at + kTrTile, lane);
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      bool any;
-      fine[k] = exponent(d[k], e[k], any);
-    }
   }
-  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&e)[2], const bool (&fine)[2]) {
+  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&most)[2], const bool (&own)[2]) {
     constexpr int plane = kTrTile * D * 2;
     const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
+    for (int k = 0; k < 4; k++) {
       uint8_t* dst = planes + (w + 4 * k) * (16 * D) + (lane >> 3) * 128 + (lane & 7) * 16;
+      int e = most[k >> 1];
+      bool fine = true, any;
+      if (own[k >> 1]) fine = exponent(d[k & 1], e, any);
       // 2^-e: fp16 holds 2^14 down to 2^-15
-      const __half down = __float2half_rn(fine[k] ? pow2f(-e[k]) : 0.0f);
+      const __half down = __float2half_rn(fine ? pow2f(-e) : 0.0f);
 #pragma unroll
       for (int i = 0; i < NC; i++) {
-        const __half s = __ushort_as_half(fine[k] ? (uint16_t)(i & 1 ? d[k][i / 2] >> 16 : d[k][i / 2]) : (uint16_t)0);
+        const uint32_t sd = d[k & 1][i / 2];
+        const __half s = __ushort_as_half(fine ? (uint16_t)(i & 1 ? sd >> 16 : sd) : (uint16_t)0);
         const __half2 f = __half2half2(__hmul_rn(s, down));
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const uint32_t b = j < 2 ? q[k][i].x : q[k][i].y;
+          const uint32_t b = (j < 2 ? q[k & 1][i].x : q[k & 1][i].y) ^ 0x80808080u;
           // two signed bytes as fp16: 1024 + (byte + 128) - 1152
-          const uint32_t t = __byte_perm(b, 0x64646464u, j & 1 ? 0x7362 : 0x5140) ^ 0x00800080u;
+          const uint32_t t = __byte_perm(b, 0x64646464u, j & 1 ? 0x7362 : 0x5140);
           const __half2 n = __hsub2_rn(*reinterpret_cast<const __half2*>(&t), off);
           const __half2 hh = __hmul2_rn(n, f);
           h[j] = h2_bits(hh);
@@ -316,7 +330,8 @@ struct KvRows<D, true> {
         *(uint4*)(dst + i * 512) = make_uint4(h[0], h[1], h[2], h[3]);
         *(uint4*)(dst + plane + i * 512) = make_uint4(l[0], l[1], l[2], l[3]);
       }
-      load_row(k, at + kTrTile, w, lane);
+      if (k < 2) load_row(k + 2, at, w, lane);
+      else load_row(k - 2, at + kTrTile, w, lane);
     }
   }
 };
@@ -345,49 +360,70 @@ struct KvRows<D, false> {
     rows = (const float*)cache + pos0 * row + (int64_t)kvh * D;
     left = n_kv - pos0;
   }
-  // (as above; `ends` [4]: what the four warps found, met at barrier `id`, also by
-  // warps that have given up)
-  __device__ __forceinline__ void exponents(int at, int w, int lane, int2* ends, int id, int& most, int& least, int (&e)[2],
-                                            bool (&fine)[2]) const {
-    bool bad = false;
-    most = -1000;
-    least = 1000;
+  // (as above; `ends` [half][4]: what the four warps found, met at barrier `id`, also
+  // by warps that have given up)
+  template <class Own, class Put>
+  __device__ __forceinline__ void exponents(int at, int w, int lane, int2* ends, int id, int (&most)[2], bool (&own)[2], Own judge,
+                                            Put put) const {
+    int e[4];
+    bool fine[4];
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-      float x[NC * 8];
-      load_row(at + (w + 4 * k) * 8 + (lane & 7), lane, x);
-      fine[k] = row_exponent<NC * 8>(x, e[k]);
-      bad |= !fine[k];
-      const bool any = e[k] > -100;
-      e[k] -= 14;
-      if (fine[k] && any) {
-        most = max(most, e[k]);
-        least = min(least, e[k]);
+    for (int h = 0; h < 2; h++) {
+      bool bad = false;
+      int hi = -1000, lo = 1000;
+#pragma unroll
+      for (int k = 2 * h; k < 2 * h + 2; k++) {
+        float x[NC * 8];
+        load_row(at + (w + 4 * k) * 8 + (lane & 7), lane, x);
+        fine[k] = row_exponent<NC * 8>(x, e[k]);
+        bad |= !fine[k];
+        const bool any = e[k] > -100;
+        e[k] -= 14;
+        if (fine[k] && any) {
+          hi = max(hi, e[k]);
+          lo = min(lo, e[k]);
+        }
       }
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      if (__any_sync(0xffffffffu, bad)) lo = -2000;
+      if (lane == 0) ends[h * 4 + w] = make_int2(hi, lo);
     }
-    most = __reduce_max_sync(0xffffffffu, most);
-    least = __reduce_min_sync(0xffffffffu, least);
-    if (__any_sync(0xffffffffu, bad)) least = -2000;
-    if (lane == 0) ends[w] = make_int2(most, least);
     asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int2 o = ends[k];
-      most = max(most, o.x);
-      least = min(least, o.y);
+    for (int h = 0; h < 2; h++) {
+      int hi = -1000, lo = 1000;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int2 o = ends[h * 4 + k];
+        hi = max(hi, o.x);
+        lo = min(lo, o.y);
+      }
+      most[h] = hi;
+      own[h] = judge(hi, lo);
+      if (own[h] && lane < 8) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) put(h, (w + 4 * k) * 8 + lane, e[2 * h + k], fine[2 * h + k]);
+      }
     }
   }
-  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&e)[2], const bool (&fine)[2]) const {
+  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&most)[2], const bool (&own)[2]) const {
     constexpr int plane = kTrTile * D * 2;
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
+    for (int k = 0; k < 4; k++) {
       uint8_t* dst = planes + (w + 4 * k) * (16 * D) + (lane >> 3) * 128 + (lane & 7) * 16;
       float x[NC * 8];
       load_row(at + (w + 4 * k) * 8 + (lane & 7), lane, x);
+      int e = most[k >> 1];
+      bool fine = true;
+      if (own[k >> 1]) {
+        fine = row_exponent<NC * 8>(x, e);
+        e -= 14;
+      }
 #pragma unroll
       for (int i = 0; i < NC; i++) {
         uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (fine[k]) split8(&x[8 * i], pow2f(-e[k]), hi, lo);
+        if (fine) split8(&x[8 * i], pow2f(-e), hi, lo);
         *(uint4*)(dst + i * 512) = hi;
         *(uint4*)(dst + plane + i * 512) = lo;
       }
@@ -433,37 +469,30 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   float* info = (float*)(smem + L::info);
   float* rowf = (float*)(smem + L::rowf);
   float* mxs = (float*)(smem + L::mx);
-  float* ref = (float*)(smem + L::ref);
-  uint64_t* k_full = (uint64_t*)(smem + L::bars);  // these four [step & 1]
-  uint64_t* k_empty = k_full + 2;
-  uint64_t* v_full = k_full + 4;
-  uint64_t* v_empty = k_full + 6;
-  uint64_t* col_full = k_full + 8;  // [kTrSlots]
-  uint64_t* s_full = col_full + kTrSlots;  // these three [step & 1]
-  uint64_t* s_empty = s_full + 2;
-  uint64_t* p_full = s_full + 4;
-  uint64_t* o_full = s_full + 6;  // these two [step % n_o]
-  uint64_t* o_empty = s_full + 8;
-  uint64_t* ref_full = s_full + 10;  // [step & 1][quadrant]
-  uint64_t* q_full = s_full + 18;
-  uint64_t* drain = s_full + 19;
+  uint64_t* k_full = (uint64_t*)(smem + L::bars);
+  uint64_t* k_empty = k_full + 1;
+  uint64_t* v_full = k_full + 2;
+  uint64_t* v_empty = k_full + 3;
+  uint64_t* col_full = k_full + 4;  // [kTrSlots][half]
+  uint64_t* s_full = col_full + 2 * kTrSlots;
+  uint64_t* s_empty = s_full + 1;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = s_full + 3;
+  uint64_t* q_full = s_full + 4;
+  uint64_t* drain = s_full + 5;
   uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
   volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
 
   if (tid == 0) {
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&k_full[i], 4);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 4);
-      mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], 2 * nq);
-      mbar_init(&p_full[i], 2 * nq);
-      mbar_init(&o_full[i], 1);
-      mbar_init(&o_empty[i], kTrParts * nq);
-    }
-    for (int i = 0; i < kTrSlots; i++) mbar_init(&col_full[i], 8);
-    for (int i = 0; i < 8; i++) mbar_init(&ref_full[i], 2);
+    mbar_init(k_full, 4);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 4);
+    mbar_init(v_empty, 1);
+    for (int i = 0; i < 2 * kTrSlots; i++) mbar_init(&col_full[i], 8);
+    mbar_init(s_full, 1);
+    mbar_init(s_empty, kTrParts * nq);
+    mbar_init(p_full, kTrParts * nq);
+    mbar_init(o_full, 1);
     mbar_init(q_full, kTrParts * nq);
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -523,16 +552,14 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       const uint64_t kd = umma_desc(smem_addr(smem + L::k), 128, 16 * D);
       const uint64_t vd = umma_desc(smem_addr(smem + L::v), 16 * D, 128);
       constexpr uint64_t plane = L::plane_kv >> 4;
-      // step j's scores, once step j - 2's have been read
+      // step j's scores, once the step before's have been read
       auto scores = [&](int j) {
-        const int b = j & 1;
-        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-        if (!tc_wait_ready(&k_full[b], ph, abort_flag, p.err)) return false;
-        if (j >= 2 && !tc_wait_ready(&s_empty[b], ph ^ 1, abort_flag, p.err)) return false;
+        if (!tc_wait_ready(k_full, (uint32_t)j & 1u, abort_flag, p.err)) return false;
+        if (j > 0 && !tc_wait_ready(s_empty, (uint32_t)(j - 1) & 1u, abort_flag, p.err)) return false;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t d = kTmem + kColS + 64 * b;
-          uint64_t kh = kd + 2 * plane * b;
+          constexpr uint32_t d = kTmem + kColS;
+          uint64_t kh = kd;
           asm volatile("" : "+l"(kh));  // (the 24 descriptors are formed here, not kept in registers)
           const uint64_t kl = kh + plane;
 #pragma unroll
@@ -541,25 +568,22 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           for (int s = 0; s < D / 16; s++) mma_ts(d, qh + 8 * s, kl + 16 * s, idesc_s, 1);
 #pragma unroll
           for (int s = 0; s < D / 16; s++) mma_ts(d, qh + 8 * s, kh + 16 * s, idesc_s, 1);
-          umma_commit(&s_full[b]);
-          umma_commit(&k_empty[b]);
+          umma_commit(s_full);
+          umma_commit(k_empty);
         }
         __syncwarp();
         return true;
       };
       bool ok = tc_wait_ready(q_full, 0, abort_flag, p.err) && scores(0);
-      if (ok && n > 1) ok = scores(1);
       for (int j = 0; j < n && ok; j++) {
-        if (j > 0 && j + 1 < n && !(ok = scores(j + 1))) break;
-        const int b = j & 1, ob = j % L::n_o;
-        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-        if (!(ok = tc_wait_ready(&v_full[b], ph, abort_flag, p.err))) break;
-        if (j >= L::n_o && !(ok = tc_wait_ready(&o_empty[ob], (uint32_t)(j / L::n_o - 1) & 1u, abort_flag, p.err))) break;
-        if (!(ok = tc_wait_ready(&p_full[b], ph, abort_flag, p.err))) break;
+        if (j + 1 < n && !(ok = scores(j + 1))) break;
+        const uint32_t ph = (uint32_t)j & 1u;
+        if (!(ok = tc_wait_ready(v_full, ph, abort_flag, p.err))) break;
+        if (!(ok = tc_wait_ready(p_full, ph, abort_flag, p.err))) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t o = kTmem + kColO + D * ob, p_hi = kTmem + kColP + 64 * b, p_lo = p_hi + 32;
-          uint64_t vh = vd + 2 * plane * b;
+          constexpr uint32_t o = kTmem + kColO, p_hi = kTmem + kColP, p_lo = p_hi + kTrTile / 2;
+          uint64_t vh = vd;
           asm volatile("" : "+l"(vh));
           const uint64_t vl = vh + plane;
 #pragma unroll
@@ -568,8 +592,8 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vl + 2 * D * s, idesc_o, 1);
 #pragma unroll
           for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vh + 2 * D * s, idesc_o, 1);
-          umma_commit(&o_full[ob]);
-          umma_commit(&v_empty[b]);
+          umma_commit(o_full);
+          umma_commit(v_empty);
         }
         __syncwarp();
       }
@@ -582,65 +606,61 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   } else if (warp >= kTrWarpK) {
     // ---------------- keys (warps 16-19) and values (20-23) ----------------
     // A step's exponents go out before its planes, which wait for the products that
-    // read those of two steps ago. Their slot is written again eight steps later:
-    // after the planes of seven, which waited for the scores of five and so of four,
-    // for which the step's own stream had read the scores of two.
+    // read the last ones. Their slot is written again four steps later: after the
+    // planes of three, which waited for the scores of two, which the softmax had
+    // read the scores of one for, done with the step itself.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
     const bool is_v = warp >= kTrWarpV;
     const int w = warp & 3;
     const void* cache = is_v ? p.cache_v : p.cache_k;
+    uint8_t* planes = smem + (is_v ? L::v : L::k);
     uint64_t* full = is_v ? v_full : k_full;
     uint64_t* empty = is_v ? v_empty : k_empty;
-    int2* ends = (int2*)(smem + L::ends) + (is_v ? 8 : 0);
+    int2* ends = (int2*)(smem + L::ends) + (is_v ? 16 : 0);
     KvRows<D, Q8> kv;
     kv.begin(p, cache, kvh, pos0, n_kv, w, lane);
     bool ok = true;
     for (int j = 0; j < n; j++) {
-      const int b = j & 1, slot = j & (kTrSlots - 1);
-      int e[2], most, least;
-      bool fine[2];
-      kv.exponents(j * kTrTile, w, lane, ends + b * 4, is_v ? 10 : 9, most, least, e, fine);
-      const bool own = least < 1000 && most - least > 10;
-      if (!own) {
-        if (most < -999) most = 0;
-        e[0] = e[1] = most;
-      }
-      float* c = col + slot * 3 * kTrTile;
-      const float nan = __int_as_float(0x7fffffff);
-      if (own && lane < 8) {
+      const int slot = j & (kTrSlots - 1);
+      int most[2];
+      bool own[2];
+      kv.exponents(
+          j * kTrTile, w, lane, ends + (j & 1) * 8, is_v ? 6 : 5, most, own,
+          [](int hi, int lo) { return lo < 1000 && hi - lo > 10; },
+          [&](int h, int at, int e, bool fine) {
+            float* c = col + (slot * 2 + h) * 3 * kTrHalf;
+            const float nan = __int_as_float(0x7fffffff);
+            if (is_v) {
+              c[kTrHalf + at] = fine ? (float)e : nan;
+              // (finite in every case: a masked position's weight is 0 whatever its row holds)
+              c[2 * kTrHalf + at] = fine ? (float)e : 0.0f;
+            } else {
+              c[at] = fine ? pow2f(e) : nan;
+            }
+          });
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          const int at = (w + 4 * k) * 8 + lane;
-          if (is_v) {
-            c[kTrTile + at] = fine[k] ? (float)e[k] : nan;
-            // (finite in every case: a masked position's weight is 0 whatever its row holds)
-            c[2 * kTrTile + at] = fine[k] ? (float)e[k] : 0.0f;
-          } else {
-            c[at] = fine[k] ? pow2f(e[k]) : nan;
-          }
-        }
-      }
-      if (w == 0 && lane == 0) {
-        float* o = info + slot * 4 + (is_v ? 2 : 0);
-        o[0] = is_v ? (float)most : pow2f(max(most, -126));
-        o[1] = own ? 1.0f : 0.0f;
+      for (int h = 0; h < 2; h++) {
+        if (most[h] < -999) most[h] = 0;  // (nothing but zeros)
+        if (w == 0 && lane == 0)
+          *(float2*)(info + (slot * 2 + h) * 4 + (is_v ? 2 : 0)) =
+              make_float2(is_v ? (float)most[h] : pow2f(most[h]), own[h] ? 1.0f : 0.0f);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_one(&col_full[slot]);
-      ok = ok && (j < 2 || tc_wait_ready(&empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort_flag, p.err));
+      if (lane < 2) mbar_arrive_one(&col_full[slot * 2 + lane]);
+      ok = ok && (j == 0 || tc_wait_ready(empty, (uint32_t)(j - 1) & 1u, abort_flag, p.err));
       if (ok) {
-        kv.store(j * kTrTile, smem + (is_v ? L::v : L::k) + b * 2 * L::plane_kv, w, lane, e, fine);
+        kv.store(j * kTrTile, planes, w, lane, most, own);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(&full[b]);
+        if (lane == 0) mbar_arrive_one(full);
       }
     }
   } else {
-    // ---------------- softmax: two streams of two threads per row ----------------
+    // ---------------- softmax: four threads per row ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    const int quad = warp & 3, part = warp >> 2, stream = part >> 1;
+    const int quad = warp & 3, part = warp >> 2;
     if (quad < nq) {
-      constexpr int NA = D / kTrParts, HT = kTrTile / 2;
+      constexpr int NA = D / kTrParts, HT = kTrTile / kTrParts;
       const int lr = quad * 32 + lane, r = r0 + lr, i = min(r, sp.R - 1) / rep;
       const uint32_t base = kTmem + ((uint32_t)(32 * quad) << 16);
       const float rf = rowf[lr];
@@ -662,27 +682,22 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive_one(q_full);
       }
-      float M = -INFINITY;   // the row's reference (of the last step that this thread knows of)
-      float l = 0.0f;        // this part's weights (Q8_0: relative to Ml - 14, F32: to ml)
-      float Ml = -INFINITY, ml = -INFINITY, f_own = 1.0f;
+      float M = -INFINITY;                   // the row's maximum
+      float l = 0.0f;                        // this part's weights (Q8_0: relative to M - 14, F32: to ml)
+      float ml = -INFINITY, f_prev = 1.0f;
       float acc[NA];
 #pragma unroll
       for (int k = 0; k < NA; k++) acc[k] = 0.0f;
-      // step j's O into the registers, which so far are relative to a reference of
-      // 1 / f times its
+      // step j's O into the registers
       auto take_o = [&](int j, float f) {
-        const int ob = j % L::n_o;
-        if (!tc_wait_ready(&o_full[ob], (uint32_t)(j / L::n_o) & 1u, abort_flag, p.err)) return false;
+        if (!tc_wait_ready(o_full, (uint32_t)j & 1u, abort_flag, p.err)) return false;
         tc_fence_after();
         const float2 f2 = make_float2(f, f);
         float y[NA];
 #pragma unroll
-        for (int o = 0; o < NA; o += 8) tmem_ld8f(base + kColO + D * ob + NA * part + o, y + o);
+        for (int o = 0; o < NA; o += 8) tmem_ld8f(base + kColO + NA * part + o, y + o);
 #pragma unroll
         for (int o = 0; o < NA; o += 8) tmem_wait_ld8(y + o);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_one(&o_empty[ob]);
 #pragma unroll
         for (int k = 0; k < NA; k += 2) {
           const float2 a = __ffma2_rn(make_float2(acc[k], acc[k + 1]), f2, make_float2(y[k], y[k + 1]));
@@ -691,36 +706,27 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         }
         return true;
       };
-      // The reference that the other stream has set for step j; the factor from the
-      // one before it, `from`.
-      auto other_ref = [&](int j, float from, float& f) {
-        if (!tc_wait_ready(&ref_full[(j & 1) * 4 + quad], (uint32_t)(j >> 1) & 1u, abort_flag, p.err)) return false;
-        M = ref[(j & 1) * kTrRows + lr];
-        f = exp2_approx(__fsub_rn(from, M == -INFINITY ? 0.0f : M));
-        return true;
-      };
-      // The stream's other half of the row has come as far: once a step, also by
-      // warps that have given up (so that none waits for another).
-      auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad + 4 * stream) : "memory"); };
+      // The row's other parts have come as far: once a step and twice at the end, also
+      // by warps that have given up (so that none waits for another).
+      auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + quad) : "memory"); };
       bool ok = true;
-      for (int j = stream; j < n; j += 2) {
-        const int slot = j & (kTrSlots - 1), b = stream;
-        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-        const int64_t pt = pos0 + (int64_t)j * kTrTile + (part & 1) * HT;
-        const float* c = col + slot * 3 * kTrTile + (part & 1) * HT;
+      for (int j = 0; j < n; j++) {
+        const int slot = (j & (kTrSlots - 1)) * 2 + (part >> 1);
+        const int64_t pt = pos0 + (int64_t)j * kTrTile + part * HT;
+        const float* c = col + slot * 3 * kTrHalf + (part & 1) * HT;
         ok = ok && tc_wait_ready(&col_full[slot], (uint32_t)(j / kTrSlots) & 1u, abort_flag, p.err) &&
-             tc_wait_ready(&s_full[b], ph, abort_flag, p.err);
+             tc_wait_ready(s_full, (uint32_t)j & 1u, abort_flag, p.err);
         if (!ok) {
           meet();
           continue;
         }
         tc_fence_after();
         float x[HT];
-        tmem_ld32(base + kColS + 64 * b + (part & 1) * HT, x);
+        tmem_ld32(base + kColS + part * HT, x);
         tmem_wait_ld(x);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(&s_empty[b]);
+        if (lane == 0) mbar_arrive_one(s_empty);
         // (two elements an instruction where the hardware has one)
         float2* x2 = (float2*)x;
         const float4 in = *(const float4*)(info + slot * 4);
@@ -731,7 +737,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           const float kc = in.y != 0.0f ? 0.0f : in.x, vc = in.z;
 #pragma unroll
           for (int k = 0; k < HT; k++) {
-            const float kf = in.y != 0.0f ? c[k] : kc, ve = in.w != 0.0f ? c[kTrTile + k] : vc;
+            const float kf = in.y != 0.0f ? c[k] : kc, ve = in.w != 0.0f ? c[kTrHalf + k] : vc;
             x[k] = __fmaf_rn(x[k], fmaxf(__fmul_rn(kf, rf), kf == kf ? 1e-37f : kf), ve);
           }
           fac = 1.0f;
@@ -753,34 +759,26 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         // differences and those with the exponents are exact (NaN where there is
         // nothing else: as if nothing were attended, the weights bring it back).
         mx[0] = mx[0] == mx[0] ? ceilf(__fmaf_ru(mx[0], fac, off)) : -INFINITY;
-        // the row's maximum over the stream's two halves and the steps before
-        float* ex = mxs + (((j >> 1) & 1) * kTrParts + 2 * stream) * kTrRows + lr;
-        ex[(part & 1) * kTrRows] = mx[0];
+        // the row's maximum over its parts
+        float* ex = mxs + (j & 1) * kTrParts * kTrRows + lr;
+        ex[part * kTrRows] = mx[0];
         meet();
-        float f_other = 1.0f;
-        if (j > 0) ok = other_ref(j - 1, M, f_other);
-        const float Mn = fmaxf(M, fmaxf(ex[0], ex[kTrRows]));
-        if ((part & 1) == 0) ref[b * kTrRows + lr] = Mn;
-        __syncwarp();
-        if (lane == 0) mbar_arrive_one(&ref_full[b * 4 + quad]);
+        const float Mn = fmaxf(fmaxf(fmaxf(M, ex[0]), fmaxf(ex[kTrRows], ex[2 * kTrRows])), ex[3 * kTrRows]);
         // (2^14: the largest weight that fp16 still holds with room; rounded up, and
         // the sum below down, so that no score of any size gets past it)
         const float Mr = Mn == -INFINITY ? 0.0f : Mn, Ms = __fsub_ru(Mr, 14.0f);
-        // this stream's last O; with it its P's columns are free
-        if (j >= 2) ok = ok && take_o(j - 2, f_own);
-        f_own = exp2_approx(__fsub_rn(M, Mr));
+        const float f = exp2_approx(__fsub_rn(M, Mr));
         M = Mn;
         float lr0 = Ms;  // what the weights' sum is relative to
         if (Q8) {
-          l = __fmul_rn(l, exp2_approx(__fsub_rn(Ml, Mr)));
-          Ml = Mn;
+          l = __fmul_rn(l, f);
         } else {
           // the values' exponents reach over all of a float's range: the sum has a
           // reference of its own, the largest score of this part without them
           float ms = -INFINITY;
           if (own) {
 #pragma unroll
-            for (int k = 0; k < HT; k++) ms = fmaxf(ms, __fsub_rn(x[k], in.w != 0.0f ? c[2 * kTrTile + k] : in.z));
+            for (int k = 0; k < HT; k++) ms = fmaxf(ms, __fsub_rn(x[k], in.w != 0.0f ? c[2 * kTrHalf + k] : in.z));
             ms = ceilf(ms);
           } else {
             ms = __fsub_rn(mx[0], in.z);
@@ -797,7 +795,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         if (apart) {
 #pragma unroll
           for (int k = 0; k < HT; k++) {
-            const float ve = in.w != 0.0f ? c[2 * kTrTile + k] : in.z, g = __fsub_rn(ls, ve);
+            const float ve = in.w != 0.0f ? c[2 * kTrHalf + k] : in.z, g = __fsub_rn(ls, ve);
             const float s = own ? x[k] : __fmaf_rn(x[k], fac, off);
             l = g > 100.0f ? __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(s, ve), lr0)))
                            : __fmaf_rn(exp2_approx(__fsub_rn(s, Ms)), exp2_approx(g), l);
@@ -821,43 +819,30 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           lo[k] = h2_bits(__floats2half2_rn(rest.x, rest.y));
         }
         if (!apart) l = __fmaf_rn(__fadd_rn(sum.x, sum.y), exp2_approx(lf), l);
-        tmem_st16(base + kColP + 64 * b + (part & 1) * (HT / 2), hi);
-        tmem_st16(base + kColP + 64 * b + 32 + (part & 1) * (HT / 2), lo);
+        // the step before's O; with it P's columns are free
+        if (j > 0) ok = take_o(j - 1, f_prev);
+        f_prev = f;
+        tmem_st16(base + kColP + part * (HT / 2), hi);
+        tmem_st16(base + kColP + kTrTile / 2 + part * (HT / 2), lo);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(&p_full[b]);
-        // the other stream's last O
-        if (j > 0) ok = ok && take_o(j - 1, f_other);
+        if (lane == 0) mbar_arrive_one(p_full);
       }
-      // the steps after this stream's last but one
-      const int last = n - 1 - ((n - 1 - stream) & 1);  // this stream's last step (-1: it has none)
-      if (last >= 0) ok = ok && take_o(last, f_own);
-      if (last + 1 < n) {
-        float f = 1.0f;
-        ok = ok && other_ref(last + 1, M, f) && take_o(last + 1, f);
-      }
-      if (Q8 && l != 0.0f) l = __fmul_rn(l, exp2_approx(__fsub_rn(Ml, M)));
-      // the parts' sums (a barrier of the quadrant's four warps)
-      auto meet4 = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(11 + quad) : "memory"); };
+      if (ok) ok = take_o(n - 1, f_prev);
+      // the parts' sums
       float m = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);  // what l is relative to
-      meet4();  // (the last steps' maxima have been read)
-      float* ex = mxs + lr;
+      float* ex = mxs + (n & 1) * kTrParts * kTrRows + lr;  // (not the last step's)
       ex[part * kTrRows] = ml;
-      ex[(kTrParts + part) * kTrRows] = l;
-      meet4();
-      if (Q8) {
-        l = __fadd_rn(__fadd_rn(ex[4 * kTrRows], ex[5 * kTrRows]), __fadd_rn(ex[6 * kTrRows], ex[7 * kTrRows]));
-      } else {
+      meet();
+      if (!Q8) {
         m = fmaxf(fmaxf(ex[0], ex[kTrRows]), fmaxf(ex[2 * kTrRows], ex[3 * kTrRows]));
-        l = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kTrParts; k++)
-          if (ex[k * kTrRows] != -INFINITY)
-            l = __fmaf_rn(ex[(kTrParts + k) * kTrRows], exp2_approx(__fsub_rn(ex[k * kTrRows], m)), l);
-          else
-            l = __fadd_rn(l, ex[(kTrParts + k) * kTrRows]);
+        if (ml != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(ml, m)));
       }
+      ex = mxs + ((n + 1) & 1) * kTrParts * kTrRows + lr;
+      ex[part * kTrRows] = l;
+      meet();
+      l = __fadd_rn(__fadd_rn(ex[0], ex[kTrRows]), __fadd_rn(ex[2 * kTrRows], ex[3 * kTrRows]));
       if (ok && r < sp.R) {
         const float Ms = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);
         if (sp.S == 1) {
