@@ -249,8 +249,8 @@ size_t mi_cuda_kv_q8_0_bytes(int64_t n_ctx, int64_t n_head_kv, int64_t head_dim)
  * given (n_past is then not used): a negative slot skips the token, of two tokens
  * with one slot the later is kept, and a slot >= n_ctx is skipped and sets the
  * device error word to MI_CUDA_ERR_ARG (mi_cuda_device_error). Other rows stay as
- * they are. Per 32 values d = fp16(max|x| / 127), at most 65504, and
- * q = rint(x / d) in [-127, 127] (0 where d is 0); a block with an infinity or a
+ * they are. Per 32 values d = fp16(max|x| * (1 / 127 as a float)), at most
+ * 65504, and q = rint(x / d) in [-127, 127] (0 where d is 0); a block with an infinity or a
  * NaN is stored as d = NaN. Caches 16-byte aligned. */
 int mi_cuda_kv_append_q8_0(const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride,
                            int64_t head_dim, int64_t n_head_kv, int64_t n_tokens, int64_t n_ctx,

@@ -719,6 +719,7 @@ cudaError_t prepare_kernels() {
   if (e == cudaSuccess) e = prepare_persist_kernel(optin);
   if (e == cudaSuccess) e = prepare_attn_split_kernels();
   if (e == cudaSuccess) e = prepare_attn_tree_kernels();
+  if (e == cudaSuccess) e = prepare_logits_kernels();
   if (e == cudaSuccess) e = prepare_attn_long_kernels(optin);
   return e;
 }

@@ -7,17 +7,21 @@
 // run of positions as two contiguous ranges; 34/32 bytes per value.
 //
 // Block of 32 values of a row:
-//   d = fp16(min(max|x| / 127, 65504)),  q = clamp(rint(x / d), -127, 127),  q = 0 where d = 0.
-// q rounds against the d that is stored, so a value is off by d / 2 at most (a
-// fp16 below amax / 127 makes |x| / d pass 127 by 2^-11 of it, which rounds to
-// 127; only subnormal scales reach the clamp). An infinity or a NaN makes d NaN
+//   d = fp16(min(max|x| * fl(1 / 127), 65504)),  q = clamp(rint(x / d), -127, 127),  q = 0 where d = 0.
+// (The product with the float nearest 1 / 127 is off by 2^-24 of the quotient at
+// most, which picks the other neighbour of d only where both are as good.) q rounds
+// against the d that is stored, so a value is off by d / 2 at most: a d below
+// max|x| / 127 makes |x| / d pass 127 by 2^-11 of it, which rounds to 127; only
+// subnormal and saturated scales reach the clamp. An infinity or a NaN makes d NaN
 // and q 0: the whole block reads back as NaN.
 //
-// The float32 quotients give exactly the integers that 64-bit ones give: a
-// rounding border is (k + 1/2) d with at most 20 significant bits, a float x
-// beside it is at least one of its own ulps away, and that moves the quotient by
-// more than half an ulp of k + 1/2. The same holds for amax / 127 and the
-// borders between two fp16 values.
+// The float32 quotient x / d gives exactly the integer that a 64-bit one gives: a
+// rounding border is (k + 1/2) d with at most 20 significant bits, a float x beside
+// it is at least one of its own ulps away, and that moves the quotient by more than
+// half an ulp of k + 1/2.
+//
+// Both kernels pass over their data once; HBM bounds them for many rows, launch and
+// latency for few. Each thread has four 16-byte pieces of four rows under way.
 #include <algorithm>
 
 #include "mi_device.cuh"
@@ -27,7 +31,13 @@ namespace mi {
 namespace {
 
 constexpr int kKvNT = 256;
-constexpr int kKvTokens = 8;  // tokens per CTA of the append
+constexpr int kKvAhead = 4;  // rows that a thread has under way
+
+// A CTA's threads are tiled over a row's 16-byte pieces (`width` of them, all of the
+// row where it has no more than the CTA has threads) and over rows.
+struct KvTiling {
+  int32_t pieces, width, rows;  // of a row; of a CTA; rows of a CTA at a time
+};
 
 // Eight lanes hold a block, four values each.
 __device__ __forceinline__ void quantise_block(const float (&x)[4], bool store, int8_t* q, __half* d, int lane8) {
@@ -42,7 +52,7 @@ __device__ __forceinline__ void quantise_block(const float (&x)[4], bool store, 
 #pragma unroll
   for (int s = 4; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
   const bool finite = m <= 3.402823466e38f;
-  const __half dh = finite ? __float2half_rn(fminf(__fdiv_rn(m, 127.0f), 65504.0f)) : __ushort_as_half(0x7e00);
+  const __half dh = finite ? __float2half_rn(fminf(__fmul_rn(m, 1.0f / 127.0f), 65504.0f)) : __ushort_as_half(0x7e00);
   const float df = __half2float(dh);
   uint32_t word = 0;
   if (df > 0.0f) {  // (NaN: no)
@@ -58,91 +68,123 @@ __device__ __forceinline__ void quantise_block(const float (&x)[4], bool store, 
   }
 }
 
-// VEC: rows are 16-byte aligned (float4 loads).
+// VEC: rows are 16-byte aligned (float4 loads). Grid (rows, pieces of a row, keys /
+// values); eight threads hold a block of 32.
 template <bool VEC>
-__global__ void __launch_bounds__(kKvNT) kv_append_q8_kernel(const KvAppendParams p) {
-  __shared__ int32_t row[kKvTokens];
-  const int64_t t0 = (int64_t)blockIdx.x * kKvTokens;
-  const int nt = (int)min((int64_t)kKvTokens, p.n_tokens - t0);
-  if (threadIdx.x < nt) {
-    const int64_t t = t0 + threadIdx.x;
-    int32_t r = p.slots ? p.slots[t] : (int32_t)(p.n_past + t);
-    if (r >= p.n_ctx) {
-      atomicExch(p.err, 1 /* MI_CUDA_ERR_ARG */);
-      r = -1;
+__global__ void __launch_bounds__(kKvNT) kv_append_q8_kernel(const KvAppendParams p, const KvTiling g) {
+  extern __shared__ int32_t row[];  // cache row of each of the CTA's tokens, -1: none
+  const int nt_cta = g.rows * kKvAhead;
+  const int64_t t0 = (int64_t)blockIdx.x * nt_cta;
+  const int nt = (int)min((int64_t)nt_cta, p.n_tokens - t0);
+  const bool is_v = blockIdx.z;
+  const int tid = threadIdx.x, r = tid / g.width, piece = blockIdx.y * g.width + tid - r * g.width;
+  const bool live = r < g.rows && piece < g.pieces;
+  const float* src = (is_v ? p.v : p.k) + (int64_t)piece * 4;
+  const int64_t stride = is_v ? p.v_stride : p.k_stride;
+  float x[kKvAhead][4];
+#pragma unroll
+  for (int u = 0; u < kKvAhead; u++) {
+    const int i = r + u * g.rows;
+    if (live && i < nt) {
+      if (VEC) {
+        const float4 f = *(const float4*)(src + (t0 + i) * stride);
+        x[u][0] = f.x, x[u][1] = f.y, x[u][2] = f.z, x[u][3] = f.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[u][e] = src[(t0 + i) * stride + e];
+      }
+    } else {
+      x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
     }
-    row[threadIdx.x] = r;
+  }
+  for (int i = tid; i < nt; i += kKvNT) {
+    int32_t s = p.slots ? p.slots[t0 + i] : (int32_t)(p.n_past + t0 + i);
+    if (s >= p.n_ctx) {
+      atomicExch(p.err, 1 /* MI_CUDA_ERR_ARG */);
+      s = -1;
+    }
+    row[i] = s;
   }
   __syncthreads();
   if (p.slots) {  // a later token with the same slot wins
-    for (int64_t j = t0 + 1 + threadIdx.x; j < p.n_tokens; j += kKvNT) {
-      const int32_t r = p.slots[j];
-      if (r >= 0)
-        for (int i = 0; i < nt; i++)
-          if (t0 + i < j && p.slots[t0 + i] == r) row[i] = -1;
+    for (int64_t j = t0 + 1 + tid; j < p.n_tokens; j += kKvNT) {
+      const int32_t s = p.slots[j];
+      if (s >= 0)
+        for (int i = 0; i < nt && t0 + i < j; i++)
+          if (p.slots[t0 + i] == s) row[i] = -1;
     }
     __syncthreads();
   }
-  const int nb = p.D / 32, per_row = p.HKV * nb;  // blocks of a token's row
-  const int items = nt * per_row * 2;
-  const int lane8 = threadIdx.x & 7;
+  const int nb = p.D / 32, blk = piece >> 3, h = blk / nb, b = blk - h * nb, lane8 = tid & 7;
   const int64_t plane = (int64_t)p.HKV * p.n_ctx * p.D;
-  for (int i0 = 0; i0 < items; i0 += kKvNT / 8) {  // (whole warps stay for the shuffles)
-    const int it = i0 + (threadIdx.x >> 3);
-    const bool live = it < items;
-    const int which = live ? it / (nt * per_row) : 0, rem = live ? it - which * nt * per_row : 0;
-    const int i = rem / per_row, blk = rem - i * per_row, h = blk / nb, b = blk - h * nb;
-    const float* src = (which ? p.v + (t0 + i) * p.v_stride : p.k + (t0 + i) * p.k_stride) + blk * 32 + lane8 * 4;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    const int32_t r = live ? row[i] : -1;
-    if (r >= 0) {
-      if (VEC) {
-        const float4 f = *(const float4*)src;
-        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-      } else {
+  uint8_t* c = is_v ? p.cache_v : p.cache_k;
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = src[e];
-      }
-    }
-    uint8_t* c = which ? p.cache_v : p.cache_k;
-    const int64_t at = (int64_t)h * p.n_ctx + (r < 0 ? 0 : r);
-    quantise_block(x, r >= 0, (int8_t*)c + at * p.D + b * 32, (__half*)(c + plane) + at * nb + b, lane8);
+  for (int u = 0; u < kKvAhead; u++) {  // (whole warps stay for the shuffles)
+    const int i = r + u * g.rows;
+    const int32_t s = live && i < nt ? row[i] : -1;
+    const int64_t at = (int64_t)h * p.n_ctx + (s < 0 ? 0 : s);
+    quantise_block(x[u], s >= 0, (int8_t*)c + at * p.D + b * 32, (__half*)(c + plane) + at * nb + b, lane8);
   }
 }
 
-__global__ void __launch_bounds__(kKvNT) kv_read_q8_kernel(const KvReadParams p) {
-  const int nb = p.D / 32;
-  const int64_t plane = (int64_t)p.HKV * p.n_ctx * p.D;
-  const uint8_t* c = blockIdx.y ? p.cache_v : p.cache_k;
-  float* out = blockIdx.y ? p.v : p.k;
-  const int64_t n4 = p.n_rows * p.HKV * p.D / 4, row4 = (int64_t)p.HKV * p.D / 4;
-  for (int64_t i = (int64_t)blockIdx.x * kKvNT + threadIdx.x; i < n4; i += (int64_t)gridDim.x * kKvNT) {
-    const int64_t r = i / row4;
-    const int e = (int)(i - r * row4) * 4, h = e / p.D, o = e - h * p.D;
-    const int64_t at = (int64_t)h * p.n_ctx + p.first + r;
-    const char4 q = *(const char4*)(c + at * p.D + o);
-    const float d = __half2float(((const __half*)(c + plane))[at * nb + (o >> 5)]);
-    *(float4*)(out + 4 * i) = make_float4(__fmul_rn((float)q.x, d), __fmul_rn((float)q.y, d), __fmul_rn((float)q.z, d),
-                                          __fmul_rn((float)q.w, d));
+__global__ void __launch_bounds__(kKvNT) kv_read_q8_kernel(const KvReadParams p, const KvTiling g) {
+  const bool is_v = blockIdx.z;
+  const int tid = threadIdx.x, r = tid / g.width, piece = blockIdx.y * g.width + tid - r * g.width;
+  if (r >= g.rows || piece >= g.pieces) return;
+  const int nb = p.D / 32, blk = piece >> 3, h = blk / nb, b = blk - h * nb;
+  const int64_t plane = (int64_t)p.HKV * p.n_ctx * p.D, at = (int64_t)h * p.n_ctx + p.first;
+  const uint8_t* c = is_v ? p.cache_v : p.cache_k;
+  const uint8_t* qs = c + at * p.D + b * 32 + (piece & 7) * 4;
+  const __half* ds = (const __half*)(c + plane) + at * nb + b;
+  float* out = (is_v ? p.v : p.k) + (int64_t)piece * 4;
+  const int64_t i0 = (int64_t)blockIdx.x * g.rows * kKvAhead + r;
+  char4 q[kKvAhead];
+  float d[kKvAhead];
+#pragma unroll
+  for (int u = 0; u < kKvAhead; u++) {
+    const int64_t i = i0 + u * g.rows;
+    if (i < p.n_rows) {
+      q[u] = *(const char4*)(qs + i * p.D);
+      d[u] = __half2float(ds[i * nb]);
+    }
   }
+#pragma unroll
+  for (int u = 0; u < kKvAhead; u++) {
+    const int64_t i = i0 + u * g.rows;
+    if (i < p.n_rows)
+      *(float4*)(out + i * g.pieces * 4) = make_float4(__fmul_rn((float)q[u].x, d[u]), __fmul_rn((float)q[u].y, d[u]),
+                                                       __fmul_rn((float)q[u].z, d[u]), __fmul_rn((float)q[u].w, d[u]));
+  }
+}
+
+KvTiling kv_tiling(int32_t HKV, int32_t D) {
+  KvTiling g{};
+  g.pieces = HKV * (D / 4);
+  g.width = std::min(g.pieces, kKvNT);
+  g.rows = kKvNT / g.width;
+  return g;
+}
+dim3 kv_grid(const KvTiling& g, int64_t n) {
+  const int64_t per = g.rows * kKvAhead;
+  return dim3((unsigned)((n + per - 1) / per), (unsigned)((g.pieces + g.width - 1) / g.width), 2);
 }
 
 }  // namespace
 
 cudaError_t launch_kv_append_q8(const KvAppendParams& p, cudaStream_t s) {
   if (p.n_tokens == 0) return cudaSuccess;
-  const unsigned grid = (unsigned)((p.n_tokens + kKvTokens - 1) / kKvTokens);
+  const KvTiling g = kv_tiling(p.HKV, p.D);
+  const size_t smem = (size_t)g.rows * kKvAhead * 4;
   const bool vec = ((uintptr_t)p.k | (uintptr_t)p.v) % 16 == 0 && p.k_stride % 4 == 0 && p.v_stride % 4 == 0;
-  if (vec) kv_append_q8_kernel<true><<<grid, kKvNT, 0, s>>>(p);
-  else kv_append_q8_kernel<false><<<grid, kKvNT, 0, s>>>(p);
+  if (vec) kv_append_q8_kernel<true><<<kv_grid(g, p.n_tokens), kKvNT, smem, s>>>(p, g);
+  else kv_append_q8_kernel<false><<<kv_grid(g, p.n_tokens), kKvNT, smem, s>>>(p, g);
   return cudaGetLastError();
 }
 
 cudaError_t launch_kv_read_q8(const KvReadParams& p, cudaStream_t s) {
   if (p.n_rows == 0) return cudaSuccess;
-  const int64_t n4 = p.n_rows * p.HKV * p.D / 4;
-  const dim3 grid((unsigned)std::min<int64_t>((n4 + kKvNT - 1) / kKvNT, 148 * 8), 2);
-  kv_read_q8_kernel<<<grid, kKvNT, 0, s>>>(p);
+  const KvTiling g = kv_tiling(p.HKV, p.D);
+  kv_read_q8_kernel<<<kv_grid(g, p.n_rows), kKvNT, 0, s>>>(p, g);
   return cudaGetLastError();
 }
 

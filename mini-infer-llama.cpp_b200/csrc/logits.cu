@@ -3,15 +3,23 @@
 // first maximum of the raw logits (ref src/model_qwen2.cpp:690-700).
 //
 // Row r, token j with logit l, c = how often j is in the row's history:
-//   x = l;                          c > 0: x = (l > 0 ? l / repeat : l * repeat) - (c * frequency + presence)
-//   x += sum of the biases of j (in the list's order);   x = -inf where the allowed bit of j is 0
+//   x = l;  c > 0: x = (l > 0 ? l / repeat : l * repeat) - (c * frequency + presence)
+//   x += sum of the biases of j (in the list's order);  x = -inf where the allowed bit of j is 0
 // token = the lowest j of the largest x, -1 where no x is above -inf.
 //
 // A row is one thread-block cluster: CTA c takes a contiguous part of the
 // vocabulary and counts the history's tokens that fall into it in shared memory
-// (integer adds: their order does not matter), so the counts never exist in
-// global memory and a row is one pass, 8 bytes per token; the CTAs' winners meet
-// in the first CTA's shared memory.
+// (integer adds: their order does not matter), so the counts never exist in global
+// memory. The tokens with a count or a bias are few: they are listed when they are
+// first met, computed from the list, and left out of the dense pass. (Computed
+// inside it they cost every warp that met one the divisions of all its lanes, 60 us
+// for 64 rows of 152064 with 4093 ids of history; computed by the thread of their
+// history entry, 48 us.) The CTAs' winners meet in the first CTA's shared memory.
+// A row is one pass, 8 bytes per token.
+//
+// Bound by HBM for many rows (8.1 bytes per token of the vocabulary), by the
+// latency of the phases (history, dense pass, winners) for few: then a row takes
+// 16 CTAs instead of 8.
 #include <algorithm>
 
 #include "mi_device.cuh"
@@ -21,79 +29,197 @@ namespace mi {
 namespace {
 
 constexpr int kLgNT = 512;
-constexpr int kLgCluster = 8;
-constexpr int kLgSlice = 2048;  // tokens counted at a time
+constexpr int kLgMaxCluster = 16;
+constexpr int kLgBias = 512;     // biases of a CTA's part that are kept in shared memory
+constexpr int kLgList = 2048;    // tokens of a part with a count or a bias that are listed
+constexpr int kLgAhead = 4;      // 16-byte pieces that a thread has under way
 
-__global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParams p) {
-  __shared__ int32_t cnt[kLgSlice];
-  __shared__ float bias[kLgSlice];
-  __shared__ int32_t owner[kLgSlice];
-  __shared__ float wv[kLgNT / 32];
-  __shared__ int32_t wi[kLgNT / 32];
-  __shared__ float cv[kLgCluster];
-  __shared__ int32_t ci[kLgCluster];
+// Count words: 16 bits, or 32 for histories that 15 bits do not count. The top bit
+// marks a token with a bias. add() and mark() tell whether the word was 0.
+constexpr int64_t kLgNarrow = 32767;  // the longest history for 16-bit words
+template <bool WIDE>
+struct Counts;
+template <>
+struct Counts<false> {
+  static constexpr int bytes = 2;
+  static constexpr uint32_t count = 0x7fffu, biased = 0x8000u;
+  static __device__ __forceinline__ bool add(uint32_t* w, int i) {
+    return (atomicAdd(w + (i >> 1), 1u << (16 * (i & 1))) >> (16 * (i & 1)) & 0xffffu) == 0;
+  }
+  static __device__ __forceinline__ bool mark(uint32_t* w, int i) {
+    return (atomicOr(w + (i >> 1), biased << (16 * (i & 1))) >> (16 * (i & 1)) & 0xffffu) == 0;
+  }
+  static __device__ __forceinline__ uint32_t word(const uint32_t* w, int i) { return ((const uint16_t*)w)[i]; }
+  // bit k: whether word i + k is not 0 (i a multiple of 4)
+  static __device__ __forceinline__ uint32_t any4(const uint32_t* w, int i) {
+    const uint2 v = *(const uint2*)((const uint16_t*)w + i);
+    if ((v.x | v.y) == 0) return 0;
+    return (v.x & 0xffffu ? 1u : 0u) | (v.x >> 16 ? 2u : 0u) | (v.y & 0xffffu ? 4u : 0u) | (v.y >> 16 ? 8u : 0u);
+  }
+};
+template <>
+struct Counts<true> {
+  static constexpr int bytes = 4;
+  static constexpr uint32_t count = 0x7fffffffu, biased = 0x80000000u;
+  static __device__ __forceinline__ bool add(uint32_t* w, int i) { return atomicAdd(w + i, 1u) == 0; }
+  static __device__ __forceinline__ bool mark(uint32_t* w, int i) { return atomicOr(w + i, biased) == 0; }
+  static __device__ __forceinline__ uint32_t word(const uint32_t* w, int i) { return w[i]; }
+  static __device__ __forceinline__ uint32_t any4(const uint32_t* w, int i) {
+    const uint4 v = *(const uint4*)(w + i);
+    return (v.x ? 1u : 0u) | (v.y ? 2u : 0u) | (v.z ? 4u : 0u) | (v.w ? 8u : 0u);
+  }
+};
+constexpr int kLgSlice = 20480;  // tokens counted at a time (a multiple of 32)
+
+struct LgSmem {
+  float cv[kLgMaxCluster], wv[kLgNT / 32];
+  int32_t ci[kLgMaxCluster], wi[kLgNT / 32];
+  int32_t bias_of[kLgNT / 32 + 1];
+  int32_t n_list;
+  int32_t list[kLgList];
+  int32_t bias_id[kLgBias];
+  float bias[kLgBias];
+};
+
+// VEC: rows are 16-byte aligned, so four tokens a thread at a time.
+template <bool WIDE, bool VEC>
+__global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParams p, const int cluster, const int slice) {
+  using C = Counts<WIDE>;
+  extern __shared__ __align__(16) uint32_t cnt[];
+  __shared__ LgSmem sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_ctarank();
-  cluster_arrive_relaxed();  // (every CTA runs before any stores into another's shared memory)
-  const int64_t row = blockIdx.x / kLgCluster;
-  const int64_t V = p.n_vocab;
-  const int64_t per = ((V + kLgCluster - 1) / kLgCluster + 31) / 32 * 32;
+  if (p.tokens) cluster_arrive_relaxed();  // (every CTA runs before any stores into another's shared memory)
+  const int64_t row = blockIdx.x / cluster, V = p.n_vocab;
+  const int64_t per = ((V + cluster - 1) / cluster + 31) / 32 * 32;
   const int64_t v0 = min(V, (int64_t)rank * per), v1 = min(V, v0 + per);
   const float* x = p.logits + row * p.stride;
   float* y = p.out + row * V;
-  const int32_t* hist = p.hist + row * p.hist_stride;
+  const int32_t* hist = p.hist + (p.n_hist ? row * p.hist_stride : 0);
   const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
-  float best = -INFINITY;
-  int32_t best_i = -1;
-  for (int64_t s0 = v0; s0 < v1; s0 += kLgSlice) {
-    const int n = (int)min((int64_t)kLgSlice, v1 - s0);
-    for (int i = tid; i < n; i += kLgNT) {
-      cnt[i] = 0;
-      bias[i] = 0.0f;
-      owner[i] = 0x7fffffff;
-    }
-    __syncthreads();
-    for (int64_t i = tid; i < p.n_hist; i += kLgNT) {
-      const int64_t u = (int64_t)hist[i] - s0;
-      if (u >= 0 && u < n) atomicAdd(&cnt[u], 1);
-    }
-    // biases in the list's order: of the entries for one token in a chunk the
-    // first adds, then the next (one round where no token is named twice)
-    for (int64_t b0 = 0; b0 < p.n_bias; b0 += kLgNT) {
-      const int64_t i = b0 + tid;
-      const int64_t u = i < p.n_bias ? (int64_t)p.bias_ids[i] - s0 : -1;
-      bool todo = u >= 0 && u < n;
-      while (__syncthreads_or(todo)) {
-        if (todo) atomicMin(&owner[u], tid);
+  const bool special = p.n_hist > 0 || p.n_bias > 0;
+  float best = -INFINITY, best_s = -INFINITY;  // of the dense pass, which goes up, and of the others
+  int32_t best_i = -1, best_si = -1;
+  for (int64_t s0 = v0; s0 < v1; s0 += slice) {
+    const int n = (int)min((int64_t)slice, v1 - s0);
+    // the dense pass's first pieces are under way while the special tokens are seen to
+    constexpr int W = VEC ? 4 : 1;
+    const int np = n / W;  // (VEC: V is a multiple of 4, and so is n)
+    float f[kLgAhead][W];
+    uint32_t a[kLgAhead];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int u = 0; u < kLgAhead; u++) {
+        const int i = i0 + u * kLgNT;
+        if (i >= np) continue;
+        if (VEC) {
+          const float4 v = *(const float4*)(x + s0 + 4 * i);
+          f[u][0] = v.x, f[u][W > 1 ? 1 : 0] = v.y, f[u][W > 2 ? 2 : 0] = v.z, f[u][W > 3 ? 3 : 0] = v.w;
+        } else {
+          f[u][0] = x[s0 + i];
+        }
+        a[u] = allowed ? allowed[(s0 + W * i) >> 5] >> ((W * i) & 31) : 15u;
+      }
+    };
+    load(tid);
+    if (special) {
+      for (int i = tid; i < (n * C::bytes + 15) / 16; i += kLgNT) ((uint4*)cnt)[i] = make_uint4(0, 0, 0, 0);
+      if (tid == 0) sm.n_list = 0;
+      __syncthreads();
+      auto met = [&](int u) {  // the first entry of token s0 + u
+        const int at = atomicAdd(&sm.n_list, 1);
+        if (at < kLgList) sm.list[at] = u;
+      };
+      for (int64_t i0 = tid; i0 < p.n_hist; i0 += 8 * kLgNT) {
+        int32_t h[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[e] = i0 + e * kLgNT < p.n_hist ? hist[i0 + e * kLgNT] : -1;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int64_t u = (int64_t)h[e] - s0;
+          if (u >= 0 && u < n && C::add(cnt, (int)u)) met((int)u);
+        }
+      }
+      // the part's biases in the list's order; above kLgBias of them the caller's list is read
+      int n_bias = 0;
+      for (int64_t b0 = 0; b0 < p.n_bias; b0 += kLgNT) {
+        const int64_t i = b0 + tid;
+        const int64_t u = i < p.n_bias ? (int64_t)p.bias_ids[i] - s0 : -1;
+        const bool in = u >= 0 && u < n;
+        const uint32_t m = __ballot_sync(0xffffffffu, in);
+        if (lane == 0) sm.bias_of[warp] = __popc(m);
         __syncthreads();
-        const bool mine = todo && owner[u] == tid;
+        int at = n_bias + __popc(m & ((1u << lane) - 1)), all = 0;
+        for (int w = 0; w < kLgNT / 32; w++) {
+          if (w < warp) at += sm.bias_of[w];
+          all += sm.bias_of[w];
+        }
+        if (in) {
+          if (C::mark(cnt, (int)u)) met((int)u);
+          if (at < kLgBias) {
+            sm.bias_id[at] = (int32_t)u;
+            sm.bias[at] = p.bias[i];
+          }
+        }
+        n_bias += all;
         __syncthreads();
-        if (mine) {
-          bias[u] = __fadd_rn(bias[u], p.bias[i]);
-          owner[u] = 0x7fffffff;
-          todo = false;
+      }
+      __syncthreads();
+      auto one = [&](int u) {  // token s0 + u
+        const uint32_t c = C::word(cnt, u);
+        const int64_t j = s0 + u;
+        float v = x[j];
+        if (c & C::count)
+          v = __fsub_rn(v > 0.0f ? __fdiv_rn(v, p.repeat) : __fmul_rn(v, p.repeat),
+                        __fadd_rn(__fmul_rn((float)(c & C::count), p.frequency), p.presence));
+        if (c & C::biased) {
+          float b = 0.0f;
+          if (n_bias <= kLgBias) {
+            for (int e = 0; e < n_bias; e++)
+              if (sm.bias_id[e] == u) b = __fadd_rn(b, sm.bias[e]);
+          } else {
+            for (int64_t e = 0; e < p.n_bias; e++)
+              if ((int64_t)p.bias_ids[e] - s0 == u) b = __fadd_rn(b, p.bias[e]);
+          }
+          v = __fadd_rn(v, b);
+        }
+        if (allowed && !((allowed[j >> 5] >> (j & 31)) & 1u)) v = -INFINITY;
+        y[j] = v;
+        if (v > best_s || (v == best_s && (int32_t)j < best_si)) best_s = v, best_si = (int32_t)j;
+      };
+      const int n_list = sm.n_list;
+      if (n_list <= kLgList) {
+        for (int i = tid; i < n_list; i += kLgNT) one(sm.list[i]);
+      } else {  // more than the list holds: every word is looked at
+        for (int i = tid; i < n; i += kLgNT)
+          if (C::word(cnt, i)) one(i);
+      }
+    }
+    for (int i0 = tid; i0 < np; i0 += kLgNT * kLgAhead) {
+      if (i0 != tid) load(i0);
+#pragma unroll
+      for (int u = 0; u < kLgAhead; u++) {
+        const int i = i0 + u * kLgNT;
+        if (i >= np) continue;
+        const int32_t j = (int32_t)(s0 + W * i);
+        uint32_t skip = 0;  // tokens that are done
+        if (special) skip = VEC ? C::any4(cnt, 4 * i) : (C::word(cnt, i) ? 1u : 0u);
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+          if (!((a[u] >> k) & 1u)) f[u][k] = -INFINITY;
+          if (f[u][k] > best && !((skip >> k) & 1u)) best = f[u][k], best_i = j + k;
+        }
+        if (VEC && skip == 0) {
+          *(float4*)(y + j) = make_float4(f[u][0], f[u][W > 1 ? 1 : 0], f[u][W > 2 ? 2 : 0], f[u][W > 3 ? 3 : 0]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < W; k++)
+            if (!((skip >> k) & 1u)) y[j + k] = f[u][k];
         }
       }
     }
     __syncthreads();
-    for (int i = tid; i < n; i += kLgNT) {
-      const int64_t j = s0 + i;
-      float v = x[j];
-      const int c = cnt[i];
-      if (c > 0)
-        v = __fsub_rn(v > 0.0f ? __fdiv_rn(v, p.repeat) : __fmul_rn(v, p.repeat),
-                      __fadd_rn(__fmul_rn((float)c, p.frequency), p.presence));
-      if (p.n_bias) v = __fadd_rn(v, bias[i]);
-      if (allowed && !((allowed[j >> 5] >> (j & 31)) & 1u)) v = -INFINITY;
-      y[j] = v;
-      if (v > best) {
-        best = v;
-        best_i = (int32_t)j;
-      }
-    }
-    __syncthreads();
   }
-  cluster_wait_acquire();
   if (!p.tokens) return;
   auto take = [&](float v, int32_t i) {
     if (i >= 0 && (v > best || best_i < 0 || (v == best && i < best_i))) {
@@ -101,6 +227,7 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
       best_i = i;
     }
   };
+  take(best_s, best_si);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) {
     const float v = __shfl_xor_sync(0xffffffffu, best, s);
@@ -108,40 +235,71 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
     take(v, i);
   }
   if (lane == 0) {
-    wv[warp] = best;
-    wi[warp] = best_i;
+    sm.wv[warp] = best;
+    sm.wi[warp] = best_i;
   }
   __syncthreads();
+  cluster_wait_acquire();
   if (tid == 0) {
-    for (int w = 1; w < kLgNT / 32; w++) take(wv[w], wi[w]);
+    for (int w = 1; w < kLgNT / 32; w++) take(sm.wv[w], sm.wi[w]);
     // into the first CTA's shared memory
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dsmem_addr(&cv[rank], 0)), "f"(best) : "memory");
-    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(dsmem_addr(&ci[rank], 0)), "r"(best_i) : "memory");
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dsmem_addr(&sm.cv[rank], 0)), "f"(best) : "memory");
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(dsmem_addr(&sm.ci[rank], 0)), "r"(best_i) : "memory");
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (rank == 0 && tid == 0) {
     best_i = -1;
     best = -INFINITY;
-    for (int c = 0; c < kLgCluster; c++) take(cv[c], ci[c]);
+    for (int c = 0; c < cluster; c++) take(sm.cv[c], sm.ci[c]);
     p.tokens[row] = best_i;
   }
 }
 
-}  // namespace
-
-cudaError_t launch_logits_process(const LogitsParams& p, int64_t n_rows, cudaStream_t s) {
-  if (n_rows == 0) return cudaSuccess;
+template <bool WIDE, bool VEC>
+cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, int cluster, int slice, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(n_rows * kLgCluster));
+  cfg.gridDim = dim3((unsigned)(n_rows * cluster));
   cfg.blockDim = dim3(kLgNT);
+  cfg.dynamicSmemBytes = p.n_hist || p.n_bias ? (size_t)slice * Counts<WIDE>::bytes : 0;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kLgCluster;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, logits_process_kernel, p);
+  return cudaLaunchKernelEx(&cfg, logits_process_kernel<WIDE, VEC>, p, cluster, slice);
+}
+
+template <bool WIDE, bool VEC>
+cudaError_t prepare_logits() {
+  cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kLgSlice * Counts<WIDE>::bytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e;
+}
+
+}  // namespace
+
+// (clusters of 16 CTAs need an attribute; per device, at init)
+cudaError_t prepare_logits_kernels() {
+  cudaError_t e = prepare_logits<false, false>();
+  if (e == cudaSuccess) e = prepare_logits<false, true>();
+  if (e == cudaSuccess) e = prepare_logits<true, false>();
+  if (e == cudaSuccess) e = prepare_logits<true, true>();
+  return e;
+}
+
+cudaError_t launch_logits_process(const LogitsParams& p, int64_t n_rows, cudaStream_t s) {
+  if (n_rows == 0) return cudaSuccess;
+  const int cluster = n_rows * 16 <= 148 ? 16 : 8;
+  const int64_t per = ((p.n_vocab + cluster - 1) / cluster + 31) / 32 * 32;
+  const int slice = (int)std::min<int64_t>(per, kLgSlice);
+  const bool vec = ((uintptr_t)p.logits | (uintptr_t)p.out) % 16 == 0 && p.stride % 4 == 0 && p.n_vocab % 4 == 0;
+  if (p.n_hist <= kLgNarrow)
+    return vec ? launch_logits<false, true>(p, n_rows, cluster, slice, s) : launch_logits<false, false>(p, n_rows, cluster, slice, s);
+  return vec ? launch_logits<true, true>(p, n_rows, cluster, slice, s) : launch_logits<true, false>(p, n_rows, cluster, slice, s);
 }
 
 }  // namespace mi

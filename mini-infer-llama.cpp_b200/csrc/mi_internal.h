@@ -426,7 +426,7 @@ struct QkRopeParams {
   const int32_t* pos;  // nullptr: n_past + t
   float* q_out;        // dense
   float* k_out;
-  double freq[kRopeMaxDim / 2];  // set by the launcher: radians per position of each pair
+  double turns[kRopeMaxDim / 2];  // set by the launcher: turns per position of each pair
 };
 cudaError_t launch_qk_norm_rope(QkRopeParams& p, float freq_base, cudaStream_t s);
 
@@ -484,6 +484,7 @@ struct LogitsParams {
   float* out;       // dense rows
   int32_t* tokens;  // optional
 };
+cudaError_t prepare_logits_kernels();  // per device, at init
 cudaError_t launch_logits_process(const LogitsParams& p, int64_t n_rows, cudaStream_t s);
 
 // ---------------------------------------------------------------------------

@@ -615,7 +615,7 @@ int mi_cuda_logits_process(const float* d_logits, int64_t stride, int64_t n_voca
   MI_REQUIRE(d_logits && d_dst && n_vocab > 0 && n_vocab < (1ll << 31) - 65536 && n_rows >= 0 && n_rows <= 65535 &&
                  stride >= n_vocab && stride < (1ll << 40),
              "mi_cuda_logits_process: bad arguments");
-  MI_REQUIRE(n_hist >= 0 && n_hist < (1ll << 31) && (n_hist == 0 || d_hist) && (hist_stride == 0 || hist_stride >= n_hist),
+  MI_REQUIRE(n_hist >= 0 && n_hist < (1ll << 30) && (n_hist == 0 || d_hist) && (hist_stride == 0 || hist_stride >= n_hist),
              "mi_cuda_logits_process: a history of n_hist tokens, rows hist_stride apart (0: one for all)");
   MI_REQUIRE(n_bias >= 0 && n_bias < (1ll << 31) && (n_bias == 0 || (d_bias_ids && d_bias)),
              "mi_cuda_logits_process: n_bias without biases");

@@ -143,9 +143,15 @@ def init(device: int = 0) -> None:
 # torch plumbing
 # ---------------------------------------------------------------------------
 
+_torch_ = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_
+    if _torch_ is None:
+        import torch
+        _torch_ = torch
+    return _torch_
 
 
 def _p(t) -> int | None:
@@ -333,76 +339,102 @@ def argmax(x):
 # of a tree over a cache, logits processing
 # ---------------------------------------------------------------------------
 
-def _arg(t, name: str, dtypes, shape=None, dense_from: int = 0):
-    """Checks a tensor argument: on a GPU, one of `dtypes`, `shape` (None: any
-    size of that dimension), dense from dimension `dense_from` on."""
-    if not t.is_cuda:
-        raise ValueError(f"{name}: a CUDA tensor is needed")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name}: {t.dtype} where {' or '.join(map(str, dtypes))} is needed")
-    if shape is not None:
-        if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-            raise ValueError(f"{name}: shape {tuple(t.shape)} where {shape} is needed")
-    if not t.is_contiguous():
-        want = 1
-        for n, st in zip(reversed(t.shape[dense_from:]), reversed(t.stride()[dense_from:])):
-            if n != 1 and st != want:
-                raise ValueError(f"{name}: strides {t.stride()} (dense from dimension {dense_from} on is needed)")
-            want *= n
-    return t
+class _Rt:
+    """What every call below needs of torch and the library, looked up once (a
+    drafted step is tens of calls of a few microseconds each)."""
+
+    def __init__(self):
+        torch = _torch()
+        c = torch._C
+        torch.cuda.init()
+        self.L, self.empty = lib(), torch.empty
+        self.f32, self.u8, self.i32, self.u32 = torch.float32, torch.uint8, torch.int32, torch.uint32
+        self.stream, self.device, self.set_device = c._cuda_getCurrentRawStream, c._cuda_getDevice, torch.cuda.set_device
 
 
-def _row_stride(t) -> int:
-    """Elements between the rows of dimension 0 (of a single row: the row itself)."""
-    return t.stride(0) if t.shape[0] > 1 else t.numel()
+_rt_ = None
 
 
-class _on:
-    """Makes the tensors' device the current one for a call and gives its current
-    stream; refuses tensors of several devices."""
+def _rt() -> _Rt:
+    global _rt_
+    if _rt_ is None:
+        _rt_ = _Rt()
+    return _rt_
 
-    __slots__ = ("dev", "back")
 
-    def __init__(self, *tensors):
-        dev = tensors[0].get_device()
-        for t in tensors:
-            if t is not None and t.get_device() != dev:
-                raise ValueError("the tensors are on several devices")
-        self.dev = dev
+def _bad(name: str, t, want: str):
+    raise ValueError(f"{name}: {want} is needed, not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
-    def __enter__(self):
-        cuda = _torch().cuda
-        now = cuda.current_device()
-        self.back = now if now != self.dev else -1
-        if self.back >= 0:
-            cuda.set_device(self.dev)
-        return cuda.current_stream(self.dev).cuda_stream
 
-    def __exit__(self, *exc):
-        if self.back >= 0:
-            _torch().cuda.set_device(self.back)
+def _rows3(t, name: str):
+    """(rows, heads, head_dim, floats between rows) of F32 rows [n, heads, head_dim],
+    each row dense (views of stacked rows may be given)."""
+    if not t.is_cuda or t.dim() != 3 or t.dtype is not _torch().float32:
+        _bad(name, t, "an F32 CUDA tensor of [rows, heads, head_dim]")
+    n, h, d = t.shape
+    a, b, c = t.stride()
+    if (c != 1 and d > 1) or (b != d and h > 1):
+        _bad(name, t, "dense rows")
+    return n, h, d, a if n > 1 else h * d
+
+
+def _dense(t, name: str, dtype, shape):
+    """A dense CUDA tensor of `dtype` (two may be named) and `shape`."""
+    if not t.is_cuda or (t.dtype is not dtype and (type(dtype) is not tuple or t.dtype not in dtype)) or t.shape != shape \
+            or not t.is_contiguous():
+        _bad(name, t, f"a dense CUDA tensor of {dtype} {tuple(shape)}")
+
+
+def _on(dev: int, *tensors):
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("the tensors are on several devices")
+
+
+def _run(fn, dev: int, *args):
+    """fn(*args, the device's current stream) with `dev` as the current device."""
+    r = _rt()
+    now = r.device()
+    if now == dev:
+        rc = fn(*args, r.stream(dev))
+    else:
+        r.set_device(dev)
+        try:
+            rc = fn(*args, r.stream(dev))
+        finally:
+            r.set_device(now)
+    if rc:
+        check(rc)
 
 
 def qk_norm_rope(q, k, q_norm, k_norm, eps: float, n_past: int, n_dims: int, freq_base: float, pos=None,
                  q_out=None, k_out=None):
     """q [T, H, D] and k [T, HKV, D] (views of stacked rows may be given) normed per
     head (q_norm / k_norm [D], or None) and rotated to position pos[t] (or n_past + t)."""
-    torch = _torch()
-    f32 = (torch.float32,)
-    T, H, D = _arg(q, "q", f32, (None, None, None), 1).shape
-    HKV = _arg(k, "k", f32, (T, None, D), 1).shape[1]
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t is not None:
-            _arg(t, name, f32, (D,))
+    T, H, D, qs = _rows3(q, "q")
+    Tk, HKV, Dk, ks = _rows3(k, "k")
+    if Tk != T or Dk != D:
+        _bad("k", k, f"[{T}, heads, {D}]")
+    r = _rt()
+    if q_norm is not None:
+        _dense(q_norm, "q_norm", r.f32, (D,))
+    if k_norm is not None:
+        _dense(k_norm, "k_norm", r.f32, (D,))
     if pos is not None:
-        _arg(pos, "pos", (torch.int32,), (T,))
-    q_out = torch.empty((T, H, D), dtype=torch.float32, device=q.device) if q_out is None else _arg(q_out, "q_out", f32, (T, H, D))
-    k_out = torch.empty((T, HKV, D), dtype=torch.float32, device=q.device) if k_out is None else _arg(k_out, "k_out", f32, (T, HKV, D))
-    if T == 0:
-        return q_out, k_out
-    with _on(q, k, q_norm, k_norm, pos, q_out, k_out) as s:
-        check(lib().mi_cuda_qk_norm_rope(_p(q), _row_stride(q), _p(k), _row_stride(k), _p(q_norm), _p(k_norm), eps, D, H, HKV,
-                                         T, _p(pos), n_past, n_dims, freq_base, _p(q_out), _p(k_out), s))
+        _dense(pos, "pos", r.i32, (T,))
+    if q_out is None:
+        q_out = q.new_empty((T, H, D))
+    else:
+        _dense(q_out, "q_out", r.f32, (T, H, D))
+    if k_out is None:
+        k_out = q.new_empty((T, HKV, D))
+    else:
+        _dense(k_out, "k_out", r.f32, (T, HKV, D))
+    dev = q.get_device()
+    _on(dev, k, q_norm, k_norm, pos, q_out, k_out)
+    if T:
+        _run(r.L.mi_cuda_qk_norm_rope, dev, q.data_ptr(), qs, k.data_ptr(), ks, _p(q_norm), _p(k_norm), eps, D, H, HKV, T, _p(pos),
+             n_past, n_dims, freq_base, q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
@@ -414,42 +446,45 @@ def kv_q8_0_cache(n_ctx: int, n_head_kv: int, head_dim: int, device="cuda"):
     return _torch().zeros(nb, dtype=_torch().uint8, device=device)
 
 
-def _kv_q8_0_arg(t, name: str, n_ctx: int, n_head_kv: int, head_dim: int):
+def _kv_q8_0_args(cache_k, cache_v, n_ctx: int, n_head_kv: int, head_dim: int):
     nb = lib().mi_cuda_kv_q8_0_bytes(n_ctx, n_head_kv, head_dim)
     if nb == 0:
-        raise ValueError(f"{name}: no Q8_0 cache of {n_ctx} rows of {n_head_kv} heads of {head_dim}")
-    if _arg(t, name, (_torch().uint8,)).numel() != nb:
-        raise ValueError(f"{name}: {t.numel()} bytes where the cache has {nb}")
+        raise ValueError(f"no Q8_0 cache of {n_ctx} rows of {n_head_kv} heads of {head_dim}")
+    u8 = _torch().uint8
+    _dense(cache_k, "cache_k", u8, (nb,))
+    _dense(cache_v, "cache_v", u8, (nb,))
 
 
 def kv_append_q8_0(k, v, cache_k, cache_v, n_ctx: int, n_past: int = 0, slots=None):
     """Quantises k and v [T, HKV, D] into cache rows n_past + t, or slots[t] (int32; negative: skipped)."""
-    torch = _torch()
-    T, HKV, D = _arg(k, "k", (torch.float32,), (None, None, None), 1).shape
-    _arg(v, "v", (torch.float32,), (T, HKV, D), 1)
-    _kv_q8_0_arg(cache_k, "cache_k", n_ctx, HKV, D)
-    _kv_q8_0_arg(cache_v, "cache_v", n_ctx, HKV, D)
+    T, HKV, D, ks = _rows3(k, "k")
+    Tv, Hv, Dv, vs = _rows3(v, "v")
+    if Tv != T or Hv != HKV or Dv != D:
+        _bad("v", v, f"[{T}, {HKV}, {D}]")
+    _kv_q8_0_args(cache_k, cache_v, n_ctx, HKV, D)
+    r = _rt()
     if slots is not None:
-        _arg(slots, "slots", (torch.int32,), (T,))
-    if T == 0:
-        return
-    with _on(k, v, cache_k, cache_v, slots) as s:
-        check(lib().mi_cuda_kv_append_q8_0(_p(k), _row_stride(k), _p(v), _row_stride(v), D, HKV, T, n_ctx, n_past, _p(slots),
-                                           _p(cache_k), _p(cache_v), s))
+        _dense(slots, "slots", r.i32, (T,))
+    dev = k.get_device()
+    _on(dev, v, cache_k, cache_v, slots)
+    if T:
+        _run(r.L.mi_cuda_kv_append_q8_0, dev, k.data_ptr(), ks, v.data_ptr(), vs, D, HKV, T, n_ctx, n_past, _p(slots),
+             cache_k.data_ptr(), cache_v.data_ptr())
 
 
 def kv_read_q8_0(cache_k, cache_v, n_head_kv: int, head_dim: int, n_ctx: int, first: int, n_rows: int):
     """Cache rows [first, first + n_rows) as F32 tensors (k, v) of [n_rows, n_head_kv, head_dim]."""
-    torch = _torch()
-    _kv_q8_0_arg(cache_k, "cache_k", n_ctx, n_head_kv, head_dim)
-    _kv_q8_0_arg(cache_v, "cache_v", n_ctx, n_head_kv, head_dim)
+    _kv_q8_0_args(cache_k, cache_v, n_ctx, n_head_kv, head_dim)
     if first < 0 or n_rows < 0 or first + n_rows > n_ctx:
         raise ValueError(f"rows [{first}, {first + n_rows}) of a cache of {n_ctx}")
-    k = torch.empty((n_rows, n_head_kv, head_dim), dtype=torch.float32, device=cache_k.device)
-    v = torch.empty((n_rows, n_head_kv, head_dim), dtype=torch.float32, device=cache_k.device)
+    r = _rt()
+    k = r.empty((n_rows, n_head_kv, head_dim), dtype=r.f32, device=cache_k.device)
+    v = r.empty((n_rows, n_head_kv, head_dim), dtype=r.f32, device=cache_k.device)
+    dev = cache_k.get_device()
+    _on(dev, cache_v)
     if n_rows:
-        with _on(cache_k, cache_v) as s:
-            check(lib().mi_cuda_kv_read_q8_0(_p(cache_k), _p(cache_v), head_dim, n_head_kv, n_ctx, first, n_rows, _p(k), _p(v), s))
+        _run(r.L.mi_cuda_kv_read_q8_0, dev, cache_k.data_ptr(), cache_v.data_ptr(), head_dim, n_head_kv, n_ctx, first, n_rows,
+             k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -477,41 +512,51 @@ def attention_tree_scratch(n_head: int, n_head_kv: int, n_kv: int, n_tokens: int
     return torch.empty(nb, dtype=torch.uint8, device=device)
 
 
-def _attention_tree(fn, q, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch):
-    torch = _torch()
+def _attention_tree(name, q, qs, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch):
+    r = _rt()
     T, H, D = q.shape
     if mask is not None:
-        _arg(mask, "mask", (torch.int32, torch.uint32), (T, (T + 31) // 32))
-    out = torch.empty((T, H, D), dtype=torch.float32, device=q.device)
+        _dense(mask, "mask", (r.i32, r.u32), (T, (T + 31) // 32))
+    out = q.new_empty((T, H, D))
     if T == 0:
         return out
     if scratch is None:
         scratch = attention_tree_scratch(H, n_head_kv, n_past + T, T, D, q.device)
-    elif _arg(scratch, "scratch", (torch.uint8,)).numel() < lib().mi_cuda_attention_tree_scratch_bytes(H, n_head_kv, n_past + T, T, D):
-        raise ValueError("scratch: too small (attention_tree_scratch)")
-    with _on(q, cache_k, cache_v, mask, scratch) as s:
-        check(fn(_p(q), _row_stride(q), _p(cache_k), _p(cache_v), D, H, n_head_kv, n_ctx, n_past, T, _p(mask), scale_,
-                 _p(scratch), _p(out), s))
+    else:
+        nb = r.L.mi_cuda_attention_tree_scratch_bytes(H, n_head_kv, n_past + T, T, D)
+        if not scratch.is_cuda or scratch.dtype is not r.u8 or not scratch.is_contiguous() or scratch.numel() < nb:
+            _bad("scratch", scratch, f"a dense CUDA tensor of at least {nb} bytes (attention_tree_scratch)")
+    dev = q.get_device()
+    _on(dev, cache_k, cache_v, mask, scratch)
+    _run(getattr(r.L, name), dev, q.data_ptr(), qs, cache_k.data_ptr(), cache_v.data_ptr(), D, H, n_head_kv, n_ctx, n_past, T,
+         _p(mask), scale_, scratch.data_ptr(), out.data_ptr())
     return out
 
 
 def attention_tree(q, cache_k, cache_v, n_head_kv: int, n_past: int, scale_: float, mask=None, scratch=None):
     """Attention of drafted tokens q [T, H, D] over F32 caches [n_ctx, HKV, D] whose rows
     n_past + j hold the drafted tokens' own; mask as tree_mask gives it (None: causal)."""
-    torch = _torch()
-    f32 = (torch.float32,)
-    D = _arg(q, "q", f32, (None, None, None), 1).shape[2]
-    n_ctx = _arg(cache_k, "cache_k", f32, (None, n_head_kv, D)).shape[0]
-    _arg(cache_v, "cache_v", f32, (n_ctx, n_head_kv, D))
-    return _attention_tree(lib().mi_cuda_attention_tree, q, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch)
+    _, _, D, qs = _rows3(q, "q")
+    f32, n_ctx = _torch().float32, cache_k.shape[0]
+    _dense(cache_k, "cache_k", f32, (n_ctx, n_head_kv, D))
+    _dense(cache_v, "cache_v", f32, (n_ctx, n_head_kv, D))
+    return _attention_tree("mi_cuda_attention_tree", q, qs, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch)
 
 
 def attention_tree_q8_0(q, cache_k, cache_v, n_head_kv: int, n_ctx: int, n_past: int, scale_: float, mask=None, scratch=None):
     """attention_tree over Q8_0 caches (kv_q8_0_cache, kv_append_q8_0)."""
-    D = _arg(q, "q", (_torch().float32,), (None, None, None), 1).shape[2]
-    _kv_q8_0_arg(cache_k, "cache_k", n_ctx, n_head_kv, D)
-    _kv_q8_0_arg(cache_v, "cache_v", n_ctx, n_head_kv, D)
-    return _attention_tree(lib().mi_cuda_attention_tree_q8_0, q, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch)
+    _, _, D, qs = _rows3(q, "q")
+    _kv_q8_0_args(cache_k, cache_v, n_ctx, n_head_kv, D)
+    return _attention_tree("mi_cuda_attention_tree_q8_0", q, qs, cache_k, cache_v, n_head_kv, n_ctx, n_past, scale_, mask, scratch)
+
+
+def _rows_of(t, name: str, dtype, rows: int, least: int) -> int:
+    """Elements between the rows of t [rows, m] (0 for [m], one row for all), each dense, m >= least."""
+    d = t.dim()
+    if not t.is_cuda or (t.dtype is not dtype and (type(dtype) is not tuple or t.dtype not in dtype)) or d not in (1, 2) \
+            or (d == 2 and t.shape[0] != rows) or t.shape[-1] < least or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        _bad(name, t, f"a CUDA tensor of {dtype}, [{rows}, m] or [m] with m >= {least}, with dense rows")
+    return 0 if d == 1 else t.stride(0) if rows > 1 else t.shape[1]
 
 
 def logits_process(logits, hist=None, repeat: float = 1.0, frequency: float = 0.0, presence: float = 0.0, bias_ids=None,
@@ -520,32 +565,33 @@ def logits_process(logits, hist=None, repeat: float = 1.0, frequency: float = 0.
     are padding), biases (int32 ids and F32 values) and a mask of allowed tokens (bits of
     int32 [words] or [rows, words]) on logits [rows, V]: (processed logits, greedy tokens
     int32 [rows], -1 where nothing is left). out may be the logits themselves."""
-    torch = _torch()
-    n, V = _arg(logits, "logits", (torch.float32,), (None, None), 1).shape
-    i32 = (torch.int32,)
-
-    def rows_of(t, name, dtypes, least):
-        if t.dim() == 2 and t.shape[0] != n or t.dim() not in (1, 2) or t.shape[-1] < least:
-            raise ValueError(f"{name}: shape {tuple(t.shape)} for {n} rows of {V} tokens")
-        _arg(t, name, dtypes, None, t.dim() - 1)
-        return 0 if t.dim() == 1 else _row_stride(t)
-
-    hs = rows_of(hist, "hist", i32, 0) if hist is not None else 0
-    nh = hist.shape[-1] if hist is not None else 0
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype is not _torch().float32 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        _bad("logits", logits, "an F32 CUDA tensor of [rows, vocabulary] with dense rows")
+    n, V = logits.shape
+    ls = logits.stride(0) if n > 1 else V
+    r = _rt()
+    hs = nh = nb = als = 0
+    if hist is not None:
+        hs, nh = _rows_of(hist, "hist", r.i32, n, 0), hist.shape[-1]
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
-    nb = 0
     if bias is not None:
-        nb = _arg(bias, "bias", (torch.float32,), (None,)).shape[0]
-        _arg(bias_ids, "bias_ids", i32, (nb,))
-    als = rows_of(allowed, "allowed", (torch.int32, torch.uint32), (V + 31) // 32) if allowed is not None else 0
-    out = torch.empty((n, V), dtype=torch.float32, device=logits.device) if out is None else _arg(out, "out", (torch.float32,), (n, V))
-    tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
+        nb = bias.numel()
+        _dense(bias, "bias", r.f32, (nb,))
+        _dense(bias_ids, "bias_ids", r.i32, (nb,))
+    if allowed is not None:
+        als = _rows_of(allowed, "allowed", (r.i32, r.u32), n, (V + 31) // 32)
+    if out is None:
+        out = logits.new_empty((n, V))
+    else:
+        _dense(out, "out", r.f32, (n, V))
+    tokens = r.empty(n, dtype=r.i32, device=logits.device)
+    dev = logits.get_device()
+    _on(dev, hist, bias_ids, bias, allowed, out)
     if n:
-        with _on(logits, hist, bias_ids, bias, allowed, out) as s:
-            check(lib().mi_cuda_logits_process(_p(logits), _row_stride(logits), V, n, _p(hist) if nh else None, nh, hs if nh else 0,
-                                               repeat, frequency, presence, _p(bias_ids) if nb else None, _p(bias) if nb else None, nb,
-                                               _p(allowed), als, _p(out), _p(tokens), s))
+        _run(r.L.mi_cuda_logits_process, dev, logits.data_ptr(), ls, V, n, hist.data_ptr() if nh else None, nh, hs if nh else 0,
+             repeat, frequency, presence, bias_ids.data_ptr() if nb else None, bias.data_ptr() if nb else None, nb,
+             _p(allowed), als, out.data_ptr(), tokens.data_ptr())
     return out, tokens
 
 

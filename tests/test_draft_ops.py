@@ -164,7 +164,7 @@ def quantise_f64(torch, x):
     """[T, HKV, D] -> (q int8 [HKV, T, D], d fp16 [HKV, T, D / 32])."""
     b = x.double().transpose(0, 1).unflatten(-1, (-1, 32))
     top = b.abs().amax(-1, keepdim=True)
-    d = (top / 127).clamp(max=65504.0).half()
+    d = (top.float() * torch.tensor(1 / 127, dtype=torch.float32, device=x.device)).clamp(max=65504.0).half()  # the header's product
     f = d.double()
     q = torch.where(f > 0, torch.round(b / torch.where(f > 0, f, 1.0)).clamp(-127, 127), 0.0)
     bad = ~torch.isfinite(b).all(-1, keepdim=True)
@@ -567,7 +567,8 @@ def check_logits(torch, x, out, tokens, hist, repeat, freq, pres, ids, bias, all
 @pytest.mark.parametrize("n,V,nh,nb,mask", [(1, 151936, 300, 0, False), (3, 151936, 2000, 50, True), (2, 152064, 0, 7, False),
                                             (5, 257, 40, 9, True), (4, 1, 3, 2, True), (2, 31, 0, 0, True), (2, 33, 100, 0, False),
                                             (7, 50001, 999, 300, True), (64, 2048, 64, 1, True), (1, 600001, 70, 3, True),
-                                            (2, 8192, 5000, 2000, False)])
+                                            (2, 8192, 5000, 2000, False), (1, 5003, 40000, 20, True), (2, 4096, 70001, 3, False),
+                                            (9, 40000, 32767, 5, True), (10, 40000, 32768, 700, False)])
 @pytest.mark.parametrize("form", ["rows", "shared", "strided"])
 def test_logits_process(torch, n, V, nh, nb, mask, form):
     rng = np.random.default_rng(V + nh)
