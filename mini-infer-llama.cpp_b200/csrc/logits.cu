@@ -28,7 +28,7 @@ namespace mi {
 
 namespace {
 
-constexpr int kLgNT = 512;
+constexpr int kLgMaxNT = 512;
 constexpr int kLgMaxCluster = 16;
 constexpr int kLgBias = 512;     // biases of a CTA's part that are kept in shared memory
 constexpr int kLgList = 2048;    // tokens of a part with a count or a bias that are listed
@@ -72,18 +72,18 @@ struct Counts<true> {
 constexpr int kLgSlice = 20480;  // tokens counted at a time (a multiple of 32)
 
 struct LgSmem {
-  float cv[kLgMaxCluster], wv[kLgNT / 32];
-  int32_t ci[kLgMaxCluster], wi[kLgNT / 32];
-  int32_t bias_of[kLgNT / 32 + 1];
+  float cv[kLgMaxCluster], wv[kLgMaxNT / 32];
+  int32_t ci[kLgMaxCluster], wi[kLgMaxNT / 32];
+  int32_t bias_of[kLgMaxNT / 32];
   int32_t n_list;
   int32_t list[kLgList];
   int32_t bias_id[kLgBias];
   float bias[kLgBias];
 };
 
-// VEC: rows are 16-byte aligned, so four tokens a thread at a time.
-template <bool WIDE, bool VEC>
-__global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParams p, const int cluster, const int slice) {
+// VEC: rows are 16-byte aligned, so four tokens a thread at a time. NT threads.
+template <int NT, bool WIDE, bool VEC>
+__global__ void __launch_bounds__(NT) logits_process_kernel(const LogitsParams p, const int cluster, const int slice) {
   using C = Counts<WIDE>;
   extern __shared__ __align__(16) uint32_t cnt[];
   __shared__ LgSmem sm;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
     auto load = [&](int i0) {
 #pragma unroll
       for (int u = 0; u < kLgAhead; u++) {
-        const int i = i0 + u * kLgNT;
+        const int i = i0 + u * NT;
         if (i >= np) continue;
         if (VEC) {
           const float4 v = *(const float4*)(x + s0 + 4 * i);
@@ -123,17 +123,17 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
     };
     load(tid);
     if (special) {
-      for (int i = tid; i < (n * C::bytes + 15) / 16; i += kLgNT) ((uint4*)cnt)[i] = make_uint4(0, 0, 0, 0);
+      for (int i = tid; i < (n * C::bytes + 15) / 16; i += NT) ((uint4*)cnt)[i] = make_uint4(0, 0, 0, 0);
       if (tid == 0) sm.n_list = 0;
       __syncthreads();
       auto met = [&](int u) {  // the first entry of token s0 + u
         const int at = atomicAdd(&sm.n_list, 1);
         if (at < kLgList) sm.list[at] = u;
       };
-      for (int64_t i0 = tid; i0 < p.n_hist; i0 += 8 * kLgNT) {
+      for (int64_t i0 = tid; i0 < p.n_hist; i0 += 8 * NT) {
         int32_t h[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) h[e] = i0 + e * kLgNT < p.n_hist ? hist[i0 + e * kLgNT] : -1;
+        for (int e = 0; e < 8; e++) h[e] = i0 + e * NT < p.n_hist ? hist[i0 + e * NT] : -1;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const int64_t u = (int64_t)h[e] - s0;
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
       }
       // the part's biases in the list's order; above kLgBias of them the caller's list is read
       int n_bias = 0;
-      for (int64_t b0 = 0; b0 < p.n_bias; b0 += kLgNT) {
+      for (int64_t b0 = 0; b0 < p.n_bias; b0 += NT) {
         const int64_t i = b0 + tid;
         const int64_t u = i < p.n_bias ? (int64_t)p.bias_ids[i] - s0 : -1;
         const bool in = u >= 0 && u < n;
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
         if (lane == 0) sm.bias_of[warp] = __popc(m);
         __syncthreads();
         int at = n_bias + __popc(m & ((1u << lane) - 1)), all = 0;
-        for (int w = 0; w < kLgNT / 32; w++) {
+        for (int w = 0; w < NT / 32; w++) {
           if (w < warp) at += sm.bias_of[w];
           all += sm.bias_of[w];
         }
@@ -189,17 +189,17 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
       };
       const int n_list = sm.n_list;
       if (n_list <= kLgList) {
-        for (int i = tid; i < n_list; i += kLgNT) one(sm.list[i]);
+        for (int i = tid; i < n_list; i += NT) one(sm.list[i]);
       } else {  // more than the list holds: every word is looked at
-        for (int i = tid; i < n; i += kLgNT)
+        for (int i = tid; i < n; i += NT)
           if (C::word(cnt, i)) one(i);
       }
     }
-    for (int i0 = tid; i0 < np; i0 += kLgNT * kLgAhead) {
+    for (int i0 = tid; i0 < np; i0 += NT * kLgAhead) {
       if (i0 != tid) load(i0);
 #pragma unroll
       for (int u = 0; u < kLgAhead; u++) {
-        const int i = i0 + u * kLgNT;
+        const int i = i0 + u * NT;
         if (i >= np) continue;
         const int32_t j = (int32_t)(s0 + W * i);
         uint32_t skip = 0;  // tokens that are done
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
   __syncthreads();
   cluster_wait_acquire();
   if (tid == 0) {
-    for (int w = 1; w < kLgNT / 32; w++) take(sm.wv[w], sm.wi[w]);
+    for (int w = 1; w < NT / 32; w++) take(sm.wv[w], sm.wi[w]);
     // into the first CTA's shared memory
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dsmem_addr(&sm.cv[rank], 0)), "f"(best) : "memory");
     asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(dsmem_addr(&sm.ci[rank], 0)), "r"(best_i) : "memory");
@@ -255,11 +255,11 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
   }
 }
 
-template <bool WIDE, bool VEC>
+template <int NT, bool WIDE, bool VEC>
 cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, int cluster, int slice, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_rows * cluster));
-  cfg.blockDim = dim3(kLgNT);
+  cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = p.n_hist || p.n_bias ? (size_t)slice * Counts<WIDE>::bytes : 0;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -268,38 +268,51 @@ cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, int cluster, in
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, logits_process_kernel<WIDE, VEC>, p, cluster, slice);
+  return cudaLaunchKernelEx(&cfg, logits_process_kernel<NT, WIDE, VEC>, p, cluster, slice);
 }
 
-template <bool WIDE, bool VEC>
+template <int NT, bool WIDE, bool VEC>
 cudaError_t prepare_logits() {
-  cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<NT, WIDE, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        kLgSlice * Counts<WIDE>::bytes);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(logits_process_kernel<NT, WIDE, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   return e;
+}
+
+template <int NT>
+cudaError_t prepare_nt() {
+  cudaError_t e = prepare_logits<NT, false, false>();
+  if (e == cudaSuccess) e = prepare_logits<NT, false, true>();
+  if (e == cudaSuccess) e = prepare_logits<NT, true, false>();
+  if (e == cudaSuccess) e = prepare_logits<NT, true, true>();
+  return e;
+}
+
+template <int NT>
+cudaError_t launch_nt(const LogitsParams& p, int64_t n_rows, int cluster, cudaStream_t s) {
+  const int64_t per = ((p.n_vocab + cluster - 1) / cluster + 31) / 32 * 32;
+  const int slice = (int)std::min<int64_t>(per, kLgSlice);
+  const bool vec = ((uintptr_t)p.logits | (uintptr_t)p.out) % 16 == 0 && p.stride % 4 == 0 && p.n_vocab % 4 == 0;
+  if (p.n_hist <= kLgNarrow)
+    return vec ? launch_logits<NT, false, true>(p, n_rows, cluster, slice, s) : launch_logits<NT, false, false>(p, n_rows, cluster, slice, s);
+  return vec ? launch_logits<NT, true, true>(p, n_rows, cluster, slice, s) : launch_logits<NT, true, false>(p, n_rows, cluster, slice, s);
 }
 
 }  // namespace
 
 // (clusters of 16 CTAs need an attribute; per device, at init)
 cudaError_t prepare_logits_kernels() {
-  cudaError_t e = prepare_logits<false, false>();
-  if (e == cudaSuccess) e = prepare_logits<false, true>();
-  if (e == cudaSuccess) e = prepare_logits<true, false>();
-  if (e == cudaSuccess) e = prepare_logits<true, true>();
-  return e;
+  const cudaError_t e = prepare_nt<256>();
+  return e == cudaSuccess ? prepare_nt<512>() : e;
 }
 
+// Few rows: 16 CTAs of 512 threads a row (one row of 151936: 7.3 us). As soon as
+// those do not all run at once (64 rows: two waves, 39 us), 8 CTAs of 256, of which
+// an SM holds four.
 cudaError_t launch_logits_process(const LogitsParams& p, int64_t n_rows, cudaStream_t s) {
   if (n_rows == 0) return cudaSuccess;
-  const int cluster = n_rows * 16 <= 148 ? 16 : 8;
-  const int64_t per = ((p.n_vocab + cluster - 1) / cluster + 31) / 32 * 32;
-  const int slice = (int)std::min<int64_t>(per, kLgSlice);
-  const bool vec = ((uintptr_t)p.logits | (uintptr_t)p.out) % 16 == 0 && p.stride % 4 == 0 && p.n_vocab % 4 == 0;
-  if (p.n_hist <= kLgNarrow)
-    return vec ? launch_logits<false, true>(p, n_rows, cluster, slice, s) : launch_logits<false, false>(p, n_rows, cluster, slice, s);
-  return vec ? launch_logits<true, true>(p, n_rows, cluster, slice, s) : launch_logits<true, false>(p, n_rows, cluster, slice, s);
+  return n_rows * 16 <= 148 ? launch_nt<512>(p, n_rows, 16, s) : launch_nt<256>(p, n_rows, 8, s);
 }
 
 }  // namespace mi

@@ -617,6 +617,13 @@ def test_logits_process_values(torch):
         check_logits(torch, x, out, tok, hist, repeat, freq, pres, None, None, None)
     out, tok = mi_cuda.logits_process(X)
     assert torch.equal(out.view(torch.int32), X.view(torch.int32)) and tok.tolist()[:2] == [17, -1]
+    # more tokens with a count in one part than its list holds
+    V2 = 151936
+    x2 = (np.random.default_rng(5).standard_normal((11, V2)) * 3).astype(np.float32)
+    hist2 = np.arange(1000, 31000, dtype=np.int32)
+    for rows in (1, 11):
+        out, tok = mi_cuda.logits_process(torch.from_numpy(x2[:rows]).cuda(), hist=torch.from_numpy(hist2).cuda(), repeat=1.3, presence=0.5)
+        check_logits(torch, x2[:rows], out, tok, hist2, 1.3, 0.0, 0.5, None, None, None)
     # one token named by every bias: the list's order
     ids = torch.full((1500,), 321, dtype=torch.int32, device="cuda")
     bias = np.random.default_rng(0).standard_normal(1500).astype(np.float32) * 1000
