@@ -1,0 +1,451 @@
+// Tree attention with few rows over a Q8_0 cache: one token of decode, or a draft of
+// a token or two (n_rep query heads of a KV head times T tokens). The same formula
+// and records as attn_tree.cu, whose 128-row tiles would be almost empty here; what
+// counts is how soon the last byte of the cache has been asked for.
+//
+// A warp takes 16 positions at a time and eight rows for its columns, so a tile of
+// the two products is one m16n8 tensor-core tile: S^T = K Q^T and O^T = V^T P^T. The
+// cache goes from global memory straight into the MMAs' registers:
+//   * a lane's eight bytes of a block of 32 dims are two k-steps of K's operand (the
+//     queries are held in the same order of dims, as fp16 pairs hi + lo);
+//   * four bytes of each of four positions, transposed by byte permutes, are two
+//     k-steps of V^T's.
+// int8 is exact in fp16, so S needs two MMAs (hi, lo) per step and block, the block's
+// scale multiplies its sum in float, and P carries the values' scales: P d_v 2^(13 -
+// E), E the largest scale's exponent of the step, again as hi + lo, turned from S's
+// layout into the operand's by an 8 x 8 transpose.
+//
+// Four warps per CTA, each with its own running maxima, sums and O in registers. The
+// CTA's warps meet in shared memory and the CTAs of a cluster in distributed shared
+// memory, so up to 16 steps (2048 positions, D <= 64) are one launch; longer caches
+// leave one record per cluster for the join.
+//
+// Bound by latency: a step's loads, its two products, the two reductions and, past
+// 2048 positions, the join: one token of 14 / 2 heads of 64 takes 5.9 us at 2000
+// positions and 11.3 us at 32000 (8.7 MB of cache, 0.8 TB/s).
+#include <algorithm>
+
+#include "attn_tree.cuh"
+
+namespace mi {
+
+namespace {
+
+constexpr int kFewNT = 128;
+constexpr int kFewWarps = kFewNT / 32;
+
+// positions that a warp has in registers at a time, in tiles of 16
+template <int D>
+constexpr int kFewTiles = D <= 64 ? 2 : 1;
+template <int D>
+constexpr int kFewStep = kFewWarps * 16 * kFewTiles<D>;  // positions of a CTA's step
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Two bytes of b (chosen by `sel` against 0x64), each already offset by 128, as fp16:
+// 1024 + (byte + 128) - 1152.
+__device__ __forceinline__ uint32_t bytes_to_h2(uint32_t b, uint32_t sel) {
+  const uint32_t t = __byte_perm(b, 0x64646464u, sel);
+  return h2_bits(__hsub2_rn(*reinterpret_cast<const __half2*>(&t), __floats2half2_rn(1152.0f, 1152.0f)));
+}
+__device__ __forceinline__ float dsmem_ld(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(dsmem_addr(p, rank)) : "memory");
+  return v;
+}
+
+template <int D, int NR>
+struct FewSmem {
+  static constexpr int R = 8 * NR;
+  float part[kFewWarps][R][D];  // the warps' O, then (in [0]) the CTA's
+  float m[kFewWarps][R], l[kFewWarps][R], scale[kFewWarps][R];
+  float cm[R], cl[R];           // the CTA's
+};
+
+// NR: groups of eight rows. Grid (splits, KV heads, groups of 8 NR rows), clusters
+// along the splits.
+template <int D, int NR>
+__global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant__ TreeAttnParams p, const TreeSplit sp,
+                                                          const int cluster) {
+  constexpr int NC = D / 32, ND = (NC + 1) / 2, PT = kFewTiles<D>, step = kFewStep<D>;
+  extern __shared__ __align__(16) uint8_t few_raw[];
+  FewSmem<D, NR>& sm = *reinterpret_cast<FewSmem<D, NR>*>(few_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y, r0 = blockIdx.z * 8 * NR, rep = p.H / p.HKV;
+  const int64_t n_kv = (int64_t)p.n_past + p.T;
+  const int64_t begin = (int64_t)blockIdx.x * sp.per * step, end = min(n_kv, begin + (int64_t)sp.per * step);
+  const int64_t head = (int64_t)kvh * p.n_ctx, plane = (int64_t)p.HKV * p.n_ctx * D;
+  const uint8_t* kq = (const uint8_t*)p.cache_k + head * D;
+  const uint8_t* vq = (const uint8_t*)p.cache_v + head * D;
+  const uint16_t* ks = (const uint16_t*)((const uint8_t*)p.cache_k + plane) + head * NC;
+  const uint16_t* vs = (const uint16_t*)((const uint8_t*)p.cache_v + plane) + head * NC;
+
+  // what a step holds of the cache
+  uint2 K[PT][2][NC];                  // positions g, g + 8; eight bytes of each block
+  uint32_t V[PT][4][NC];               // positions 2t, 2t + 1, 2t + 8, 2t + 9; four bytes of each block
+  uint32_t dk[PT][2][ND], dv[PT][2][ND];  // scales of positions g, g + 8, two a word
+  auto scales = [&](const uint16_t* s, int64_t pos, bool in, uint32_t (&o)[ND]) {
+    s += pos * NC;
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+      o[i] = !in ? 0u : NC % 2 == 0 ? *(const uint32_t*)(s + 2 * i) : s[2 * i] | (2 * i + 1 < NC ? (uint32_t)s[2 * i + 1] << 16 : 0u);
+  };
+  auto load = [&](int64_t b) {
+#pragma unroll
+    for (int q = 0; q < PT; q++) {
+      const int64_t tp = b + (warp * PT + q) * 16;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int64_t pos = tp + g + 8 * h;
+        const bool in = pos < end;
+        scales(ks, pos, in, dk[q][h]);
+        scales(vs, pos, in, dv[q][h]);
+#pragma unroll
+        for (int c = 0; c < NC; c++) K[q][h][c] = in ? *(const uint2*)(kq + pos * D + 32 * c + 8 * t) : make_uint2(0u, 0u);
+      }
+#pragma unroll
+      for (int h = 0; h < 4; h++) {
+        const int64_t pos = tp + 2 * t + (h & 1) + 4 * (h & 2);
+#pragma unroll
+        for (int c = 0; c < NC; c++) V[q][h][c] = pos < end ? *(const uint32_t*)(vq + pos * D + 32 * c + 4 * g) : 0u;
+      }
+    }
+  };
+  if (begin < end) load(begin);
+
+  // the queries: row 8n + g, the dims that this lane's key bytes stand for
+  uint32_t qh[NR][NC][4], ql[NR][NC][4];
+  float rf[NR][2];  // |scale| * log2(e) * the factor of rows 8n + 2t, 8n + 2t + 1
+  int tok[NR][2];
+#pragma unroll
+  for (int n = 0; n < NR; n++) {
+    const int r = min(r0 + 8 * n + g, sp.R - 1), i = r / rep;
+    const float* src = p.q + i * p.q_stride + (int64_t)(kvh * rep + r - i * rep) * D + 8 * t;
+    float x[NC][8], m = 0.0f;
+    bool fine = true;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x[c][e] = src[32 * c + e];
+        m = fmaxf(m, fabsf(x[c][e]));
+        fine &= fabsf(x[c][e]) <= 3.402823466e38f;
+      }
+    if (!fine) m = INFINITY;
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    fine = m <= 3.402823466e38f;
+    // (the row's largest value becomes 2^14..2^15; a row with an infinity or a NaN: NaN)
+    const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127);
+    const float f = p.scale < 0.0f ? -pow2f(14 - ex) : pow2f(14 - ex);
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float a = __fmul_rn(x[c][2 * e], f), b = __fmul_rn(x[c][2 * e + 1], f);
+        const __half2 hh = __floats2half2_rn(a, b);
+        const float2 back = __half22float2(hh);
+        qh[n][c][e] = fine ? h2_bits(hh) : 0x7e007e00u;
+        ql[n][c][e] = fine ? h2_bits(__floats2half2_rn(__fsub_rn(a, back.x), __fsub_rn(b, back.y))) : 0u;
+      }
+    const float own = __fmul_rn(__fmul_rn(fabsf(p.scale), 1.4426950408889634f), pow2f(ex - 14));
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      rf[n][u] = __shfl_sync(0xffffffffu, own, 4 * (2 * t + u));
+      tok[n][u] = min(r0 + 8 * n + 2 * t + u, sp.R - 1) / rep;
+    }
+  }
+
+  float M[NR][2], l[NR][2], acc[NR][NC][2][4];
+  int E = 0;  // O is in units of 2^(E - 13)
+#pragma unroll
+  for (int n = 0; n < NR; n++) {
+    M[n][0] = M[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc[n][c][i][k] = 0.0f;
+  }
+  for (int64_t b = begin; b < end; b += step) {
+    if (b != begin) load(b);
+    // ---- scores, in units of log2: x[tile][row group][position g + 8 (k / 2), row 2t + k % 2]
+    float x[PT][NR][4];
+#pragma unroll
+    for (int q = 0; q < PT; q++) {
+#pragma unroll
+      for (int n = 0; n < NR; n++) x[q][n][0] = x[q][n][1] = x[q][n][2] = x[q][n][3] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        uint32_t a[2][4];  // [row g / g + 8][byte pair]
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t w0 = K[q][h][c].x ^ 0x80808080u, w1 = K[q][h][c].y ^ 0x80808080u;
+          a[h][0] = bytes_to_h2(w0, 0x5140);
+          a[h][1] = bytes_to_h2(w0, 0x7362);
+          a[h][2] = bytes_to_h2(w1, 0x5140);
+          a[h][3] = bytes_to_h2(w1, 0x7362);
+        }
+        const float s0 = __half2float(__ushort_as_half((uint16_t)(c & 1 ? dk[q][0][c / 2] >> 16 : dk[q][0][c / 2])));
+        const float s1 = __half2float(__ushort_as_half((uint16_t)(c & 1 ? dk[q][1][c / 2] >> 16 : dk[q][1][c / 2])));
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816(s, a[0][0], a[1][0], a[0][1], a[1][1], ql[n][c][0], ql[n][c][1]);
+          mma16816(s, a[0][2], a[1][2], a[0][3], a[1][3], ql[n][c][2], ql[n][c][3]);
+          mma16816(s, a[0][0], a[1][0], a[0][1], a[1][1], qh[n][c][0], qh[n][c][1]);
+          mma16816(s, a[0][2], a[1][2], a[0][3], a[1][3], qh[n][c][2], qh[n][c][3]);
+          x[q][n][0] = __fmaf_rn(s[0], s0, x[q][n][0]);
+          x[q][n][1] = __fmaf_rn(s[1], s0, x[q][n][1]);
+          x[q][n][2] = __fmaf_rn(s[2], s1, x[q][n][2]);
+          x[q][n][3] = __fmaf_rn(s[3], s1, x[q][n][3]);
+        }
+      }
+    }
+    // ---- masks, maxima
+    uint32_t seen[PT][NR];  // bit k: x[..][k] is attended to
+    float fac[NR][2];
+    uint32_t top = 0;  // the values' largest scale
+#pragma unroll
+    for (int q = 0; q < PT; q++)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < ND; i++) top = max(top, max(dv[q][h][i] & 0x7fffu, (dv[q][h][i] >> 16) & 0x7fffu));
+    const int En = max((int)(__reduce_max_sync(0xffffffffu, top) >> 10), 1) - 15;
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int q = 0; q < PT; q++) {
+        const int64_t tp = b + (warp * PT + q) * 16;
+        seen[q][n] = 15u;
+        if (tp + 16 > p.n_past) {
+          const uint32_t m0 = attended32(p, tok[n][0], tp, end) >> g, m1 = attended32(p, tok[n][1], tp, end) >> g;
+          seen[q][n] = (m0 & 1u) | (m1 & 1u) << 1 | (m0 >> 8 & 1u) << 2 | (m1 >> 8 & 1u) << 3;
+        } else if (tp + 16 > end) {
+          seen[q][n] = (tp + g < end ? 3u : 0u) | (tp + g + 8 < end ? 12u : 0u);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          x[q][n][k] = (seen[q][n] >> k) & 1u ? __fmul_rn(x[q][n][k], rf[n][k & 1]) : -INFINITY;
+          mx[k & 1] = fmaxf(mx[k & 1], x[q][n][k]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int s = 4; s < 32; s *= 2) mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], s));
+        const float Mn = fmaxf(M[n][u], mx[u]), Mr = Mn == -INFINITY ? 0.0f : Mn;
+        const float f = exp2_approx(__fsub_rn(M[n][u], Mr));
+        fac[n][u] = __fmul_rn(f, pow2f(E - En));
+        l[n][u] = __fmul_rn(l[n][u], f);
+        M[n][u] = Mn;
+        // weights
+#pragma unroll
+        for (int q = 0; q < PT; q++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float& y = x[q][n][2 * h + u];
+            y = exp2_approx(__fsub_rn(y, Mr));
+            l[n][u] = __fadd_rn(l[n][u], y);
+          }
+      }
+    }
+    E = En;
+    const float unit = pow2f(13 - En);
+    // ---- O = O fac + P V
+#pragma unroll
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) acc[n][c][i][k] = __fmul_rn(acc[n][c][i][k], fac[n][k & 1]);
+#pragma unroll
+    for (int q = 0; q < PT; q++)
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        // V^T: dims 32c + 4g + e of positions 2t, 2t + 1 (v[0][e]) and 2t + 8, 2t + 9 (v[1][e])
+        uint32_t v[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t w0 = V[q][2 * h][c] ^ 0x80808080u, w1 = V[q][2 * h + 1][c] ^ 0x80808080u;
+          const uint32_t lo = __byte_perm(w0, w1, 0x5140), hi = __byte_perm(w0, w1, 0x7362);
+          v[h][0] = bytes_to_h2(lo, 0x4140);
+          v[h][1] = bytes_to_h2(lo, 0x4342);
+          v[h][2] = bytes_to_h2(hi, 0x4140);
+          v[h][3] = bytes_to_h2(hi, 0x4342);
+        }
+        const float s0 = __fmul_rn(__half2float(__ushort_as_half((uint16_t)(c & 1 ? dv[q][0][c / 2] >> 16 : dv[q][0][c / 2]))), unit);
+        const float s1 = __fmul_rn(__half2float(__ushort_as_half((uint16_t)(c & 1 ? dv[q][1][c / 2] >> 16 : dv[q][1][c / 2]))), unit);
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+          float w[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) w[k] = (seen[q][n] >> k) & 1u ? __fmul_rn(x[q][n][k], k < 2 ? s0 : s1) : 0.0f;
+          const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+          const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+          const uint32_t b0 = transpose8x8(h2_bits(h0)), b1 = transpose8x8(h2_bits(h1));
+          const uint32_t c0 = transpose8x8(h2_bits(__floats2half2_rn(__fsub_rn(w[0], f0.x), __fsub_rn(w[1], f0.y))));
+          const uint32_t c1 = transpose8x8(h2_bits(__floats2half2_rn(__fsub_rn(w[2], f1.x), __fsub_rn(w[3], f1.y))));
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            mma16816(acc[n][c][i], v[0][2 * i], v[0][2 * i + 1], v[1][2 * i], v[1][2 * i + 1], c0, c1);
+            mma16816(acc[n][c][i], v[0][2 * i], v[0][2 * i + 1], v[1][2 * i], v[1][2 * i + 1], b0, b1);
+          }
+        }
+      }
+  }
+  // ---- the CTA's warps
+#pragma unroll
+  for (int n = 0; n < NR; n++) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+      for (int s = 4; s < 32; s *= 2) l[n][u] = __fadd_rn(l[n][u], __shfl_xor_sync(0xffffffffu, l[n][u], s));
+      if (g == 0) {
+        sm.m[warp][8 * n + 2 * t + u] = M[n][u];
+        sm.l[warp][8 * n + 2 * t + u] = l[n][u];
+        sm.scale[warp][8 * n + 2 * t + u] = pow2f(E - 13);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          sm.part[warp][8 * n + 2 * t + (k & 1)][32 * c + 4 * g + 2 * i + (k >> 1)] = acc[n][c][i][k];
+  }
+  __syncthreads();
+  for (int e = tid; e < 8 * NR * D; e += kFewNT) {
+    const int r = e / D, d = e - r * D;
+    float m = sm.m[0][r];
+#pragma unroll
+    for (int w = 1; w < kFewWarps; w++) m = fmaxf(m, sm.m[w][r]);
+    const float mr = m == -INFINITY ? 0.0f : m;
+    float o = 0.0f, s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; w++) {
+      const float f = exp2_approx(__fsub_rn(sm.m[w][r], mr));
+      o = __fmaf_rn(sm.part[w][r][d], __fmul_rn(f, sm.scale[w][r]), o);
+      s = __fmaf_rn(sm.l[w][r], f, s);
+    }
+    sm.part[0][r][d] = o;  // (read by this thread alone)
+    if (d == 0) {
+      sm.cm[r] = m;
+      sm.cl[r] = s;
+    }
+  }
+  // ---- the cluster's CTAs: each takes a share of the (row, dim) pairs
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int rank = (int)cluster_ctarank(), c_id = blockIdx.x / cluster;
+  for (int e = rank * kFewNT + tid; e < 8 * NR * D; e += cluster * kFewNT) {
+    const int r = e / D, d = e - r * D, row = r0 + r;
+    if (row >= sp.R) break;  // (rows go up)
+    float m = -INFINITY;
+    for (int c = 0; c < cluster; c++) m = fmaxf(m, dsmem_ld(&sm.cm[r], c));
+    const float mr = m == -INFINITY ? 0.0f : m;
+    float o = 0.0f, s = 0.0f;
+    for (int c = 0; c < cluster; c++) {
+      const float f = exp2_approx(__fsub_rn(dsmem_ld(&sm.cm[r], c), mr));
+      o = __fmaf_rn(dsmem_ld(&sm.part[0][r][d], c), f, o);
+      s = __fmaf_rn(dsmem_ld(&sm.cl[r], c), f, s);
+    }
+    if (sp.S == 1) {
+      const int i = row / rep;
+      p.out[((int64_t)i * p.H + kvh * rep + (row - i * rep)) * D + d] = s == 0.0f ? 0.0f : __fdiv_rn(o, s);
+    } else {
+      float* rec = (float*)p.scratch + (((int64_t)kvh * sp.S + c_id) * sp.R + row) * (D + 4);
+      rec[4 + d] = o;
+      if (d == 0) *(float4*)rec = make_float4(m, m, s, 0.0f);
+    }
+  }
+  // (no CTA leaves while another reads its shared memory)
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int D, int NR>
+cudaError_t launch_few(const TreeAttnParams& p, cudaStream_t s) {
+  TreeSplit sp{};
+  sp.R = p.T * (p.H / p.HKV);
+  sp.RG = (sp.R + 8 * NR - 1) / (8 * NR);
+  const int64_t n_kv = (int64_t)p.n_past + p.T, steps = (n_kv + kFewStep<D> - 1) / kFewStep<D>;
+  // one cluster where it holds every step; else clusters of 8 (fewer where a KV
+  // head's share of the GPU has no room for them), as many as run at once
+  int cluster = 1;
+  const int64_t room = std::max<int64_t>(1, kTrSms * (D <= 64 ? 4 : 2) / ((int64_t)p.HKV * sp.RG));
+  if (steps <= 16) {
+    while (cluster < steps) cluster *= 2;
+    sp.per = 1;
+    sp.S = 1;
+  } else {
+    cluster = 8;
+    while (cluster > room) cluster /= 2;
+    const int64_t ctas = room / cluster * cluster;
+    sp.per = (int32_t)((steps + ctas - 1) / ctas);
+    sp.S = (int32_t)((steps + (int64_t)sp.per * cluster - 1) / ((int64_t)sp.per * cluster));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(sp.S * cluster), (unsigned)p.HKV, (unsigned)sp.RG);
+  cfg.blockDim = dim3(kFewNT);
+  cfg.dynamicSmemBytes = sizeof(FewSmem<D, NR>);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_few_kernel<D, NR>, p, sp, cluster);
+  if (e != cudaSuccess || sp.S == 1) return e;
+  return launch_tree_join<D>(p, sp, s);
+}
+
+template <int D, int NR>
+cudaError_t prepare_few() {
+  cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(FewSmem<D, NR>));
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_few_kernel<D, NR>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e;
+}
+
+}  // namespace
+
+cudaError_t prepare_attn_few_kernels() {
+  cudaError_t e = prepare_few<32, 1>();
+  if (e == cudaSuccess) e = prepare_few<32, 2>();
+  if (e == cudaSuccess) e = prepare_few<64, 1>();
+  if (e == cudaSuccess) e = prepare_few<64, 2>();
+  if (e == cudaSuccess) e = prepare_few<96, 1>();
+  if (e == cudaSuccess) e = prepare_few<96, 2>();
+  if (e == cudaSuccess) e = prepare_few<128, 1>();
+  if (e == cudaSuccess) e = prepare_few<128, 2>();
+  return e;
+}
+
+cudaError_t launch_attn_few(const TreeAttnParams& p, cudaStream_t s) {
+  const bool one = p.T * (p.H / p.HKV) <= 8;
+  switch (p.D) {
+    case 32: return one ? launch_few<32, 1>(p, s) : launch_few<32, 2>(p, s);
+    case 64: return one ? launch_few<64, 1>(p, s) : launch_few<64, 2>(p, s);
+    case 96: return one ? launch_few<96, 1>(p, s) : launch_few<96, 2>(p, s);
+    case 128: return one ? launch_few<128, 1>(p, s) : launch_few<128, 2>(p, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace mi

@@ -46,10 +46,9 @@
 //
 // The positions are split over CTAs to fill the GPU; a second kernel joins the
 // splits' (M, sum, O) records.
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
+#include "attn_tree.cuh"
 #include "mi_tc.cuh"
 
 namespace mi {
@@ -91,16 +90,6 @@ struct TrSmem {
   static constexpr int total = used > 120 * 1024 ? used : 120 * 1024;
 };
 static_assert(TrSmem<128>::total <= 227 * 1024, "shared memory of one CTA");
-
-struct TreeSplit {
-  int32_t R, RG, S, per;  // rows of a KV head, groups of 128, splits, steps per split
-};
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // True in one lane of a converged warp (always the same one).
 __device__ __forceinline__ bool elect_one() {
@@ -167,8 +156,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
 // Eight floats (scaled) as the two fp16 planes' 16-byte pieces.
 __device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4& lo) {
   uint32_t h[4], l[4];
@@ -203,8 +190,6 @@ __device__ __forceinline__ bool row_exponent(const float* x, int& e) {
   e = max((int)(__float_as_uint(m) >> 23) - 127, -100);
   return m <= 3.402823466e38f;
 }
-__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
-
 // One cache (keys or values) of one KV head, 128 positions a step by four warps: a
 // warp takes four rows of eight positions (row groups w + 4 k, k < 4; k < 2 in the
 // step's first half), lane = position % 8 + 8 g, and of each 32 dims the eight from
@@ -430,27 +415,6 @@ struct KvRows<D, false> {
     }
   }
 };
-
-// Bit c: whether token t attends to position pos0 + c (c < 32).
-__device__ __forceinline__ uint32_t attended32(const TreeAttnParams& p, int t, int64_t pos0, int64_t n_kv) {
-  uint32_t m = 0;
-  const int64_t j0 = pos0 - p.n_past;  // drafted index of bit 0 (negative: cached text)
-  if (p.mask) {
-    const int words = (p.T + 31) >> 5;
-    const uint32_t* row = p.mask + (int64_t)t * words;
-    // the words that hold drafted tokens j0 .. j0 + 31
-    const int64_t w = j0 >= 0 ? j0 >> 5 : 0, sh = w * 32 - j0;  // -31 .. 0, or above 0
-    if (sh < 32 && w < words) m = sh >= 0 ? row[w] << sh : row[w] >> -sh;
-    if (sh < 0 && w + 1 < words) m |= row[w + 1] << (32 + sh);
-  } else {
-    const int64_t n = (int64_t)t - j0 + 1;  // drafted tokens 0..t
-    m = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
-  }
-  if (j0 < 0) m |= j0 <= -32 ? ~0u : (1u << -j0) - 1;
-  const int64_t left = n_kv - pos0;
-  if (left < 32) m &= left <= 0 ? 0u : (1u << left) - 1;
-  return m;
-}
 
 template <int D, bool Q8>
 __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_constant__ TreeAttnParams p,
@@ -871,58 +835,6 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   }
 }
 
-// Joins the splits of one row: with a_s = 2^(M_s - max M) and b_s = 2^(m_s - max m),
-// out = sum a_s O_s / sum b_s l_s * 2^(max M - max m). A CTA per row, its warps over
-// the splits, the lanes over the dims.
-constexpr int kTrJoinNT = 128;
-template <int D>
-__global__ void __launch_bounds__(kTrJoinNT) attn_tree_join_kernel(const TreeAttnParams p, const TreeSplit sp) {
-  __shared__ float red[kTrJoinNT / 32][D + 1];
-  pdl_wait();
-  const int r = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float* rec = (const float*)p.scratch + ((int64_t)kvh * sp.S * sp.R + r) * (D + 4);
-  const int64_t step = (int64_t)sp.R * (D + 4);
-  float M = -INFINITY, m = -INFINITY;
-  for (int s = lane; s < sp.S; s += 32) {
-    const float2 h = *(const float2*)(rec + s * step);
-    M = fmaxf(M, h.x);
-    m = fmaxf(m, h.y);
-  }
-  M = warp_max(M);
-  m = warp_max(m);
-  const float Mr = M == -INFINITY ? 0.0f : M, mr = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[D / 32];
-#pragma unroll
-  for (int k = 0; k < D / 32; k++) acc[k] = 0.0f;
-#pragma unroll 4
-  for (int s = warp; s < sp.S; s += kTrJoinNT / 32) {
-    const float* x = rec + s * step;
-    const float4 h = *(const float4*)x;
-    const float a = exp2_approx(__fsub_rn(h.x, Mr));
-    l = __fmaf_rn(h.z, exp2_approx(__fsub_rn(h.y, mr)), l);
-#pragma unroll
-    for (int k = 0; k < D / 32; k++) acc[k] = __fmaf_rn(x[4 + lane + 32 * k], a, acc[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < D / 32; k++) red[warp][lane + 32 * k] = acc[k];
-  if (lane == 0) red[warp][D] = l;
-  __syncthreads();
-  if (tid < D) {
-    float o = red[0][tid];
-    l = red[0][D];
-#pragma unroll
-    for (int w = 1; w < kTrJoinNT / 32; w++) {
-      o = __fadd_rn(o, red[w][tid]);
-      l = __fadd_rn(l, red[w][D]);
-    }
-    const int rep = p.H / p.HKV, i = r / rep;
-    p.out[((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D + tid] =
-        l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(o, l), exp2_approx(__fsub_rn(Mr, mr)));
-  }
-}
-
-constexpr int kTrSms = 148;
-
 int64_t most_splits(int64_t H, int64_t HKV, int64_t n_kv, int64_t T) {
   const int64_t RG = (T * (H / HKV) + kTrRows - 1) / kTrRows, steps = (n_kv + kTrTile - 1) / kTrTile;
   return std::min(steps, std::max<int64_t>(1, kTrSms / std::max<int64_t>(1, HKV * RG)));
@@ -941,16 +853,7 @@ cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
   attn_tree_kernel<D, Q8><<<dim3((unsigned)sp.S, (unsigned)p.HKV, (unsigned)sp.RG), kTrThreads, TrSmem<D>::total, s>>>(p, sp, vec_q);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || sp.S == 1) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)sp.R, (unsigned)p.HKV);
-  cfg.blockDim = dim3(kTrJoinNT);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_tree_join_kernel<D>, p, sp);
+  return launch_tree_join<D>(p, sp, s);
 }
 
 template <int D>
@@ -983,8 +886,19 @@ cudaError_t prepare_attn_tree_kernels() {
   return e;
 }
 
+// Whether attn_few.cu is the faster one for R rows of a KV head. Up to 8 rows it
+// always is (one token, us here / there: 4.8 / 9.7 at 500 positions, 11.3 / 18.5 at
+// 32000 with 14 / 2 heads of 64, 22.7 / 36.6 with 28 / 4 heads of 128); each further
+// 16 rows are another pass over the cache there, which 14 rows repay up to some
+// 16000 positions (16.1 / 18.3 at 8000, 46.4 / 36.7 at 32000, heads of 128) and 28
+// up to some 8000 of 64 dims (10.9 / 12.6 at 8000; heads of 128 19.7 / 19.0).
+static bool few_rows(int64_t R, int64_t n_kv, int64_t D) {
+  return R <= 8 || (R <= 16 && n_kv <= 16384) || (R <= 32 && n_kv * D <= (1 << 19));
+}
+
 cudaError_t launch_attn_tree(const TreeAttnParams& p, cudaStream_t s) {
   if (p.T == 0) return cudaSuccess;
+  if (p.q8 && few_rows((int64_t)p.T * (p.H / p.HKV), (int64_t)p.n_past + p.T, p.D)) return launch_attn_few(p, s);
   switch (p.D) {
     case 32: return p.q8 ? launch_tree<32, true>(p, s) : launch_tree<32, false>(p, s);
     case 64: return p.q8 ? launch_tree<64, true>(p, s) : launch_tree<64, false>(p, s);

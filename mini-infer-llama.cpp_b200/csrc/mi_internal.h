@@ -467,6 +467,9 @@ struct TreeAttnParams {
 };
 bool attn_tree_fits(int64_t D, int64_t H, int64_t HKV, int64_t T);
 size_t attn_tree_scratch_bytes(int64_t H, int64_t HKV, int64_t n_kv, int64_t T, int64_t D);
+// Few rows over a Q8_0 cache (attn_few.cu).
+cudaError_t prepare_attn_few_kernels();  // per device, at init
+cudaError_t launch_attn_few(const TreeAttnParams& p, cudaStream_t s);
 cudaError_t prepare_attn_tree_kernels();  // per device, at init
 cudaError_t launch_attn_tree(const TreeAttnParams& p, cudaStream_t s);
 

@@ -421,7 +421,9 @@ def test_attention_tree(torch, q8, H, HKV, D, T, past):
 @pytest.mark.gpu
 @pytest.mark.parametrize("q8", [False, True])
 @pytest.mark.parametrize("H,HKV,D,T,past", [(14, 2, 64, 1, 32767), (14, 2, 64, 64, 20001), (28, 4, 128, 11, 16389), (16, 16, 32, 1, 9000),
-                                            (6, 2, 96, 300, 5000), (14, 2, 64, 1024, 1500), (14, 2, 64, 7, 131071)])
+                                            (6, 2, 96, 300, 5000), (14, 2, 64, 1024, 1500), (14, 2, 64, 7, 131071),
+                                            (28, 4, 128, 1, 40000), (14, 2, 64, 2, 16000), (14, 2, 64, 2, 16383), (28, 4, 128, 4, 4092),
+                                            (28, 4, 128, 4, 4093), (16, 16, 32, 8, 131071), (4, 2, 96, 4, 60001)])
 def test_attention_tree_long(torch, q8, H, HKV, D, T, past):
     q, caches, rows, n_ctx = attn_inputs(torch, T, H, HKV, D, past, 3, q8)
     mask = mi_cuda.tree_mask(random_tree(np.random.default_rng(T), T))
