@@ -61,7 +61,7 @@ constexpr int kTrParts = 4;      // softmax threads per row: 32 positions each, 
 constexpr int kTrRows = 128;     // rows per CTA (MMA M)
 constexpr int kTrWarpK = 16, kTrWarpV = 20, kTrWarpMma = 24;
 constexpr int kTrThreads = 28 * 32;  // (the last three warps complete the MMA warp's group for setmaxnreg)
-constexpr int kTrSlots = 4;      // steps whose exponents are kept (see the roles' waits)
+constexpr int kTrSlots = 8;      // steps whose exponents are kept (see the roles' waits)
 constexpr uint32_t kTrCols = 512;  // all of TMEM: its base is 0
 constexpr uint32_t kTmem = 0;
 // TMEM columns: S, P's planes (64 + 64), O, the queries' planes (D / 2 each)
@@ -72,22 +72,22 @@ constexpr int kRegsSoftmax = 88, kRegsConvert = 56, kRegsMma = 40;
 
 template <int D>
 struct TrSmem {
-  static constexpr int plane_q = kTrRows * D * 2, plane_kv = kTrTile * D * 2;
-  static constexpr int q = 0;                      // [hi, lo]
-  static constexpr int k = q + 2 * plane_q;        // [hi, lo]
-  static constexpr int v = k + 2 * plane_kv;
-  static constexpr int col = v + 2 * plane_kv;     // float [kTrSlots][half][3][64]: key factor, value exponent, the same where finite
+  static constexpr int n_k = 2, n_v = D <= 64 ? 2 : 1;  // steps whose planes there is room for
+  static constexpr int plane = kTrTile * D * 2;
+  static constexpr int k = 0;                      // [step % n_k][hi, lo]; at the end float [128][D + 4], the rows' records
+  static constexpr int v = k + n_k * 2 * plane;    // [step % n_v][hi, lo]
+  static constexpr int col = v + n_v * 2 * plane;  // float [kTrSlots][half][3][64]: key factor, value exponent, the same where finite
   static constexpr int info = col + kTrSlots * 2 * 3 * kTrHalf * 4;  // float [kTrSlots][half][4]: key factor, whether the positions have
                                                                      // their own, value exponent, whether they have their own
   static constexpr int ends = info + kTrSlots * 2 * 16;  // int2 [keys, values][step & 1][half][4 warps]: largest and least exponent
-  static constexpr int rowf = ends + 2 * 2 * 2 * 4 * 8;  // float [128]: |scale| * log2(e) * the row's factor
-  static constexpr int mx = rowf + kTrRows * 4;    // float [step & 1][part][128]: the parts' maxima (at the end their sums)
+  static constexpr int mx = ends + 2 * 2 * 2 * 4 * 8;    // float [2][part][128]: the parts' maxima (at the end their sums)
   static constexpr int bars = mx + 2 * kTrParts * kTrRows * 4;
-  static constexpr int n_bars = 4 + 2 * kTrSlots + 6;
+  static constexpr int n_bars = 2 * n_k + 2 * n_v + 2 * kTrSlots + 7;
   static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
   static constexpr int used = misc + 16;
   // above half of an SM's shared memory: two CTAs must not share its TMEM
   static constexpr int total = used > 120 * 1024 ? used : 120 * 1024;
+  static_assert(kTrRows * (D + 4) * 4 <= v + n_v * 2 * plane, "the records fit where the planes were");
 };
 static_assert(TrSmem<128>::total <= 227 * 1024, "shared memory of one CTA");
 
@@ -146,6 +146,10 @@ __device__ __forceinline__ void tmem_wait_ld8(float* r) {
                :
                : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t addr, uint4 a) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -171,7 +175,7 @@ __device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// A row of floats held by four lanes (lane bits 3 and 4), N values each: the
+// A cached row of floats held by four lanes (lane bits 3 and 4), N values each: the
 // exponent e that brings its largest magnitude to [2^14, 2^15) as 2^(14 - e), or
 // false where the row holds an infinity or a NaN. Rows below 2^-100 keep e = -100:
 // their halves lose bits below 2^-138, nothing that a float sum of products shows.
@@ -201,8 +205,8 @@ __device__ __forceinline__ bool row_exponent(const float* x, int& e) {
 template <int D, bool Q8>
 struct KvRows;
 
-// Q8_0: two of a warp's rows are in registers, the next two on their way to L2; a
-// row that store() has converted makes room for the one after the next.
+// Q8_0: two of a warp's rows are in registers; a row that store() has converted makes
+// room for the one after the next.
 template <int D>
 struct KvRows<D, true> {
   static constexpr int NC = D / 32, ND = (NC + 1) / 2;
@@ -239,10 +243,6 @@ struct KvRows<D, true> {
     scales(ds + (int64_t)pos * NC, in, d[k & 1]);
 #pragma unroll
     for (int i = 0; i < NC; i++) q[k & 1][i] = in ? *(const uint2*)(src + 32 * i) : make_uint2(0u, 0u);
-    if (k < 2 && pos + 64 < left && lane < 8) {
-#pragma unroll
-      for (int i = 0; i < D; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 64 * D + i));
-    }
   }
   __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int w, int lane) {
     const int64_t at = (int64_t)kvh * p.n_ctx + pos0;
@@ -421,7 +421,6 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
                                                                   const TreeSplit sp, const int vec_q) {
   extern __shared__ __align__(1024) uint8_t smem[];
   using L = TrSmem<D>;
-  constexpr int NC = D / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTrRows;
   const int rep = p.H / p.HKV;
@@ -431,76 +430,43 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   const int nq = min(4, (sp.R - r0 + 31) / 32);  // quadrants of 32 rows in use: kTrParts softmax warps each
   float* col = (float*)(smem + L::col);
   float* info = (float*)(smem + L::info);
-  float* rowf = (float*)(smem + L::rowf);
   float* mxs = (float*)(smem + L::mx);
-  uint64_t* k_full = (uint64_t*)(smem + L::bars);
-  uint64_t* k_empty = k_full + 1;
-  uint64_t* v_full = k_full + 2;
-  uint64_t* v_empty = k_full + 3;
-  uint64_t* col_full = k_full + 4;  // [kTrSlots][half]
+  uint64_t* k_full = (uint64_t*)(smem + L::bars);  // [step % n_k]
+  uint64_t* k_empty = k_full + L::n_k;
+  uint64_t* v_full = k_empty + L::n_k;  // [step % n_v]
+  uint64_t* v_empty = v_full + L::n_v;
+  uint64_t* col_full = v_empty + L::n_v;  // [kTrSlots][half]
   uint64_t* s_full = col_full + 2 * kTrSlots;
   uint64_t* s_empty = s_full + 1;
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = s_full + 3;
-  uint64_t* q_full = s_full + 4;
-  uint64_t* drain = s_full + 5;
+  uint64_t* t_full = s_full + 4;  // TMEM is there
+  uint64_t* q_full = s_full + 5;
+  uint64_t* drain = s_full + 6;
   uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
   volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
 
   if (tid == 0) {
-    mbar_init(k_full, 4);
-    mbar_init(k_empty, 1);
-    mbar_init(v_full, 4);
-    mbar_init(v_empty, 1);
+    for (int i = 0; i < L::n_k; i++) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < L::n_v; i++) {
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], 1);
+    }
     for (int i = 0; i < 2 * kTrSlots; i++) mbar_init(&col_full[i], 8);
     mbar_init(s_full, 1);
     mbar_init(s_empty, kTrParts * nq);
     mbar_init(p_full, kTrParts * nq);
     mbar_init(o_full, 1);
+    mbar_init(t_full, 1);
     mbar_init(q_full, kTrParts * nq);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kTrWarpMma) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_base)),
-                 "r"(kTrCols));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  // the queries' planes: a warp takes eight rows, four lanes a row
-  if (warp < kTrRows / 8) {
-    const int lr = warp * 8 + (lane & 7), r = r0 + lr, g = lane >> 3;
-    float x[NC * 8];
-    const int i = r / rep;
-    const float* src = p.q + i * p.q_stride + (int64_t)(kvh * rep + r - i * rep) * D + 8 * g;
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < sp.R) {
-          if (vec_q) a = *(const float4*)(src + 32 * c + e);
-          else a = make_float4(src[32 * c + e], src[32 * c + e + 1], src[32 * c + e + 2], src[32 * c + e + 3]);
-        }
-        x[8 * c + e] = a.x, x[8 * c + e + 1] = a.y, x[8 * c + e + 2] = a.z, x[8 * c + e + 3] = a.w;
-      }
-    int e;
-    const bool fine = row_exponent<NC * 8>(x, e);
-    uint8_t* dst = smem + L::q + (lr >> 3) * (16 * D) + g * 128 + (lr & 7) * 16;
-#pragma unroll
-    for (int c = 0; c < NC; c++) {
-      // (a query with an infinity or a NaN becomes NaN: so do its scores)
-      uint4 hi = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u), lo = make_uint4(0, 0, 0, 0);
-      if (fine) split8(&x[8 * c], p.scale < 0.0f ? -pow2f(14 - e) : pow2f(14 - e), hi, lo);
-      *(uint4*)(dst + c * 512) = hi;
-      *(uint4*)(dst + L::plane_q + c * 512) = lo;
-    }
-    if (g == 0) rowf[lr] = __fmul_rn(__fmul_rn(fabsf(p.scale), 1.4426950408889634f), pow2f(min(e, 127) - 14));
-  }
-  fence_proxy_async_smem();
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
 
   if (warp >= kTrWarpMma) {
     // ---------------- MMA issue ----------------
@@ -509,21 +475,28 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     // to issue, three times what it takes to run).
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
     if (warp == kTrWarpMma) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_base)),
+                   "r"(kTrCols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(t_full);
       constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTrTile >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
       // (bit 16: B, the values, is dims-major)
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
       const uint32_t qh = kTmem + kColQ, ql = qh + D / 2;
       const uint64_t kd = umma_desc(smem_addr(smem + L::k), 128, 16 * D);
       const uint64_t vd = umma_desc(smem_addr(smem + L::v), 16 * D, 128);
-      constexpr uint64_t plane = L::plane_kv >> 4;
+      constexpr uint64_t plane = L::plane >> 4;
       // step j's scores, once the step before's have been read
       auto scores = [&](int j) {
-        if (!tc_wait_ready(k_full, (uint32_t)j & 1u, abort_flag, p.err)) return false;
+        const int b = j % L::n_k;
+        if (!tc_wait_ready(&k_full[b], (uint32_t)(j / L::n_k) & 1u, abort_flag, p.err)) return false;
         if (j > 0 && !tc_wait_ready(s_empty, (uint32_t)(j - 1) & 1u, abort_flag, p.err)) return false;
         tc_fence_after();
         if (elect_one()) {
           constexpr uint32_t d = kTmem + kColS;
-          uint64_t kh = kd;
+          uint64_t kh = kd + 2 * plane * b;
           asm volatile("" : "+l"(kh));  // (the 24 descriptors are formed here, not kept in registers)
           const uint64_t kl = kh + plane;
 #pragma unroll
@@ -533,7 +506,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
 #pragma unroll
           for (int s = 0; s < D / 16; s++) mma_ts(d, qh + 8 * s, kh + 16 * s, idesc_s, 1);
           umma_commit(s_full);
-          umma_commit(k_empty);
+          umma_commit(&k_empty[b]);
         }
         __syncwarp();
         return true;
@@ -541,13 +514,13 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       bool ok = tc_wait_ready(q_full, 0, abort_flag, p.err) && scores(0);
       for (int j = 0; j < n && ok; j++) {
         if (j + 1 < n && !(ok = scores(j + 1))) break;
-        const uint32_t ph = (uint32_t)j & 1u;
-        if (!(ok = tc_wait_ready(v_full, ph, abort_flag, p.err))) break;
-        if (!(ok = tc_wait_ready(p_full, ph, abort_flag, p.err))) break;
+        const int b = j % L::n_v;
+        if (!(ok = tc_wait_ready(&v_full[b], (uint32_t)(j / L::n_v) & 1u, abort_flag, p.err))) break;
+        if (!(ok = tc_wait_ready(p_full, (uint32_t)j & 1u, abort_flag, p.err))) break;
         tc_fence_after();
         if (elect_one()) {
           constexpr uint32_t o = kTmem + kColO, p_hi = kTmem + kColP, p_lo = p_hi + kTrTile / 2;
-          uint64_t vh = vd;
+          uint64_t vh = vd + 2 * plane * b;
           asm volatile("" : "+l"(vh));
           const uint64_t vl = vh + plane;
 #pragma unroll
@@ -557,7 +530,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
 #pragma unroll
           for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vh + 2 * D * s, idesc_o, 1);
           umma_commit(o_full);
-          umma_commit(v_empty);
+          umma_commit(&v_empty[b]);
         }
         __syncwarp();
       }
@@ -566,18 +539,34 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       __syncwarp();
       for (uint32_t it = 0; it < kSpinLimit && !__all_sync(0xffffffffu, mbar_test(drain, 0)); it++) {
       }
+    } else if (warp < kTrWarpMma + 3) {
+      // Two of the other warps of the group ask for the whole range, keys and values,
+      // ahead of the converters (whose first read of a line from HBM takes 2 us).
+      const void* cache = warp == kTrWarpMma + 1 ? p.cache_k : p.cache_v;
+      const int64_t pend = min(n_kv, pos0 + (int64_t)n * kTrTile);
+      if (Q8) {
+        const uint8_t* src = (const uint8_t*)cache + ((int64_t)kvh * p.n_ctx + pos0) * D;
+        for (int64_t o = (int64_t)lane * 4096; o < (pend - pos0) * D; o += 32 * 4096)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + o),
+                       "r"((uint32_t)min((int64_t)4096, (pend - pos0) * D - o))
+                       : "memory");
+      } else {
+        const float* src = (const float*)cache + (int64_t)kvh * D;
+        for (int64_t pos = pos0 + lane; pos < pend; pos += 32)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + pos * p.HKV * D), "n"(D * 4) : "memory");
+      }
     }
   } else if (warp >= kTrWarpK) {
     // ---------------- keys (warps 16-19) and values (20-23) ----------------
     // A step's exponents go out before its planes, which wait for the products that
-    // read the last ones. Their slot is written again four steps later: after the
-    // planes of three, which waited for the scores of two, which the softmax had
-    // read the scores of one for, done with the step itself.
+    // read the planes there before. Their slot is written again eight steps later:
+    // after the planes of seven, for which the scores of five were done, for which
+    // the softmax had read those of four, and so had long left the step itself.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
     const bool is_v = warp >= kTrWarpV;
     const int w = warp & 3;
     const void* cache = is_v ? p.cache_v : p.cache_k;
-    uint8_t* planes = smem + (is_v ? L::v : L::k);
+    const int nb = is_v ? L::n_v : L::n_k;
     uint64_t* full = is_v ? v_full : k_full;
     uint64_t* empty = is_v ? v_empty : k_empty;
     int2* ends = (int2*)(smem + L::ends) + (is_v ? 16 : 0);
@@ -611,12 +600,13 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       }
       __syncwarp();
       if (lane < 2) mbar_arrive_one(&col_full[slot * 2 + lane]);
-      ok = ok && (j == 0 || tc_wait_ready(empty, (uint32_t)(j - 1) & 1u, abort_flag, p.err));
+      const int b = j % nb;
+      ok = ok && (j < nb || tc_wait_ready(&empty[b], (uint32_t)(j / nb - 1) & 1u, abort_flag, p.err));
       if (ok) {
-        kv.store(j * kTrTile, planes, w, lane, most, own);
+        kv.store(j * kTrTile, smem + (is_v ? L::v : L::k) + b * 2 * L::plane, w, lane, most, own);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(full);
+        if (lane == 0) mbar_arrive_one(&full[b]);
       }
     }
   } else {
@@ -627,24 +617,51 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       constexpr int NA = D / kTrParts, HT = kTrTile / kTrParts;
       const int lr = quad * 32 + lane, r = r0 + lr, i = min(r, sp.R - 1) / rep;
       const uint32_t base = kTmem + ((uint32_t)(32 * quad) << 16);
-      const float rf = rowf[lr];
+      // The row's other parts have come as far: twice before the steps, once in each and
+      // twice behind them, also by warps that have given up (so that none waits for another).
+      auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + quad) : "memory"); };
+      bool ok = true;
       // the row's query planes into TMEM (this thread's quarter of the dims)
+      float rf;  // |scale| * log2(e) * the row's factor
       {
-        const uint8_t* src = smem + L::q + (lr >> 3) * (16 * D) + (lr & 7) * 16 + part * (D / 32) * 128;
+        float x[NA], m = 0.0f;
+        bool fine = true;
+        const float* src = p.q + i * p.q_stride + (int64_t)(kvh * rep + min(r, sp.R - 1) - i * rep) * D + NA * part;
 #pragma unroll
-        for (int pl = 0; pl < 2; pl++)
+        for (int k = 0; k < NA; k += 4) {
+          const float4 a = vec_q ? *(const float4*)(src + k) : make_float4(src[k], src[k + 1], src[k + 2], src[k + 3]);
+          x[k] = a.x, x[k + 1] = a.y, x[k + 2] = a.z, x[k + 3] = a.w;
+        }
 #pragma unroll
-          for (int o = 0; o < D / 32; o++) {
-            const uint4 a = *(const uint4*)(src + pl * L::plane_q + o * 128);
-            asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                             base + kColQ + pl * (D / 2) + part * (D / 8) + o * 4),
-                         "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w)
-                         : "memory");
+        for (int k = 0; k < NA; k++) {
+          m = fmaxf(m, fabsf(x[k]));
+          fine &= fabsf(x[k]) <= 3.402823466e38f;
+        }
+        float* ex = mxs + lr;
+        ex[part * kTrRows] = fine ? m : INFINITY;
+        meet();
+        m = fmaxf(fmaxf(ex[0], ex[kTrRows]), fmaxf(ex[2 * kTrRows], ex[3 * kTrRows]));
+        meet();
+        fine = m <= 3.402823466e38f;
+        const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127);
+        rf = __fmul_rn(__fmul_rn(fabsf(p.scale), 1.4426950408889634f), pow2f(e - 14));
+        ok = tc_wait_ready(t_full, 0, abort_flag, p.err);
+        if (ok) {
+          tc_fence_after();
+          const float f = p.scale < 0.0f ? -pow2f(14 - e) : pow2f(14 - e);
+#pragma unroll
+          for (int k = 0; k < NA; k += 8) {
+            // (a query with an infinity or a NaN becomes NaN: so do its scores)
+            uint4 hi = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u), lo = make_uint4(0, 0, 0, 0);
+            if (fine) split8(&x[k], f, hi, lo);
+            tmem_st4(base + kColQ + part * (NA / 2) + k / 2, hi);
+            tmem_st4(base + kColQ + D / 2 + part * (NA / 2) + k / 2, lo);
           }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_one(q_full);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_one(q_full);
+        }
       }
       float M = -INFINITY;                   // the row's maximum
       float l = 0.0f;                        // this part's weights (Q8_0: relative to M - 14, F32: to ml)
@@ -670,10 +687,6 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         }
         return true;
       };
-      // The row's other parts have come as far: once a step and twice at the end, also
-      // by warps that have given up (so that none waits for another).
-      auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + quad) : "memory"); };
-      bool ok = true;
       for (int j = 0; j < n; j++) {
         const int slot = (j & (kTrSlots - 1)) * 2 + (part >> 1);
         const int64_t pt = pos0 + (int64_t)j * kTrTile + part * HT;
@@ -807,27 +820,40 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       ex[part * kTrRows] = l;
       meet();
       l = __fadd_rn(__fadd_rn(ex[0], ex[kTrRows]), __fadd_rn(ex[2 * kTrRows], ex[3 * kTrRows]));
-      if (ok && r < sp.R) {
-        const float Ms = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);
-        if (sp.S == 1) {
-          // one split: the result itself; a token that attends to nothing has l = 0
-          const float g = Ms == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(Ms, m));
-          const float inv = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), g);
-          float* out = p.out + ((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D + NA * part;
+      // The rows into shared memory (every product that read the planes there is done:
+      // O has been taken), as records or, with one split, as results; a token that
+      // attends to nothing has l = 0.
+      const float Ms = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);
+      float* rec = (float*)(smem + L::k) + lr * (D + 4);
+      float inv = 1.0f;
+      if (sp.S == 1) inv = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), Ms == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(Ms, m)));
+      if (ok) {
+        if (part == 0) *(float4*)rec = make_float4(Ms, m, l, 0.0f);
 #pragma unroll
-          for (int k = 0; k < NA; k++) out[k] = __fmul_rn(acc[k], inv);
-        } else {
-          float* rec = (float*)p.scratch + (((int64_t)kvh * sp.S + split) * sp.R + r) * (D + 4);
-          if (part == 0) *(float4*)rec = make_float4(Ms, m, l, 0.0f);
-#pragma unroll
-          for (int k = 0; k < NA; k += 4)
-            *(float4*)(rec + 4 + NA * part + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
-        }
+        for (int k = 0; k < NA; k += 4)
+          *(float4*)(rec + 4 + NA * part + k) =
+              make_float4(__fmul_rn(acc[k], inv), __fmul_rn(acc[k + 1], inv), __fmul_rn(acc[k + 2], inv), __fmul_rn(acc[k + 3], inv));
       }
     }
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag == 0) {
+    // out of it in rows: the records of a CTA's rows are contiguous
+    const int rows = min(kTrRows, sp.R - r0);
+    const float* rec = (const float*)(smem + L::k);
+    if (sp.S == 1) {
+      for (int e = tid; e < rows * (D / 4); e += kTrThreads) {
+        const int lr = e / (D / 4), d = (e - lr * (D / 4)) * 4, r = r0 + lr, i = r / rep;
+        const float4 v = *(const float4*)(rec + lr * (D + 4) + 4 + d);
+        float* out = p.out + ((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D + d;
+        out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
+      }
+    } else {
+      float4* dst = (float4*)((float*)p.scratch + (((int64_t)kvh * sp.S + split) * sp.R + r0) * (D + 4));
+      for (int e = tid; e < rows * (D / 4 + 1); e += kTrThreads) dst[e] = ((const float4*)rec)[e];
+    }
+  }
   if (warp == kTrWarpMma) {
     __syncwarp();
     tc_fence_after();
