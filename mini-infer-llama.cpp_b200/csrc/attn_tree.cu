@@ -38,6 +38,14 @@
 // the round trips of a step; steps of 64 positions took 1.4 us, nearly as long as
 // steps of 128) with the MMAs close behind.
 //
+// More than one tile of rows: two CTAs of a cluster take two tiles over the same
+// positions as one pair (cta_group::2). One of them issues the MMAs of both, 256 rows
+// each; B is split between their shared memories, so each converts half of a step's
+// keys (64 positions) and half of its values (half of the dims). With a CTA by itself
+// the conversion is 40 % of the issued instructions and, at D = 128, there is no room
+// for a second step's values; stores or bulk copies of converted planes into the
+// other CTAs' shared memory took longer than converting them again.
+//
 // A step's O is a product of its own, added to the softmax threads' registers
 // (O = O 2^(M_old - M_new) + O_step): the MMA's accumulation cuts instead of
 // rounding, by half an ulp of the accumulator each time, and over a thousand
@@ -70,26 +78,41 @@ constexpr uint32_t kColS = 0, kColP = 128, kColO = 256, kColQ = 384;
 // 88 x 512 + 56 x 256 + 40 x 128 = 64512 are given out again.
 constexpr int kRegsSoftmax = 88, kRegsConvert = 56, kRegsMma = 40;
 
-template <int D>
+// PAIR: two CTAs share the products' B operand.
+template <int D, bool PAIR>
 struct TrSmem {
-  static constexpr int n_k = 2, n_v = D <= 64 ? 2 : 1;  // steps whose planes there is room for
-  static constexpr int plane = kTrTile * D * 2;
+  static constexpr int n_k = 2, n_v = PAIR || D <= 64 ? 2 : 1;  // steps whose planes there is room for
+  static constexpr int plane = kTrTile * D * 2 / (PAIR ? 2 : 1);  // of a CTA's share of the keys or the values
   static constexpr int k = 0;                      // [step % n_k][hi, lo]; at the end float [128][D + 4], the rows' records
-  static constexpr int v = k + n_k * 2 * plane;    // [step % n_v][hi, lo]
+  static constexpr int v = k + n_k * 2 * plane;    // [step % n_v][hi, lo]; before the first step the queries
   static constexpr int col = v + n_v * 2 * plane;  // float [kTrSlots][half][3][64]: key factor, value exponent, the same where finite
   static constexpr int info = col + kTrSlots * 2 * 3 * kTrHalf * 4;  // float [kTrSlots][half][4]: key factor, whether the positions have
                                                                      // their own, value exponent, whether they have their own
   static constexpr int ends = info + kTrSlots * 2 * 16;  // int2 [keys, values][step & 1][half][4 warps]: largest and least exponent
   static constexpr int mx = ends + 2 * 2 * 2 * 4 * 8;    // float [2][part][128]: the parts' maxima (at the end their sums)
   static constexpr int bars = mx + 2 * kTrParts * kTrRows * 4;
-  static constexpr int n_bars = 2 * n_k + 2 * n_v + 2 * kTrSlots + 7;
+  static constexpr int n_bars = 2 * n_k + 2 * n_v + 2 * kTrSlots + 8;
   static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
   static constexpr int used = misc + 16;
   // above half of an SM's shared memory: two CTAs must not share its TMEM
   static constexpr int total = used > 120 * 1024 ? used : 120 * 1024;
   static_assert(kTrRows * (D + 4) * 4 <= v + n_v * 2 * plane, "the records fit where the planes were");
+  static_assert(kTrRows * D * 4 <= n_v * 2 * plane, "the queries fit where the values will be");
+  static_assert(total <= 227 * 1024, "shared memory of one CTA");
 };
-static_assert(TrSmem<128>::total <= 227 * 1024, "shared memory of one CTA");
+
+// Arrives on a barrier of the CTA that issues (its shared::cluster address). What the
+// barrier stands for is in TMEM, behind tcgen05.wait and fence, or in this CTA's own
+// shared memory, behind the fence to the async proxy: it has been performed before
+// this, and nothing else has to be made visible (a release for the whole cluster
+// waited for the loads in flight as well, 900 to 1250 cycles each time).
+__device__ __forceinline__ void arrive_lead(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // True in one lane of a converged warp (always the same one).
 __device__ __forceinline__ bool elect_one() {
@@ -102,14 +125,34 @@ __device__ __forceinline__ bool elect_one() {
   return y != 0;
 }
 
-// D (+)= A B, f32 += f16 x f16; A from TMEM, B from shared memory.
+// D (+)= A B, f32 += f16 x f16; A from TMEM, B from shared memory (of both CTAs).
+template <bool PAIR>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
-      : "memory");
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+        : "memory");
+}
+// Arrives on `bar` (of both CTAs) when the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  if (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    umma_commit(bar);
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* r) {
@@ -194,28 +237,30 @@ __device__ __forceinline__ bool row_exponent(const float* x, int& e) {
   e = max((int)(__float_as_uint(m) >> 23) - 127, -100);
   return m <= 3.402823466e38f;
 }
-// One cache (keys or values) of one KV head, 128 positions a step by four warps: a
-// warp takes four rows of eight positions (row groups w + 4 k, k < 4; k < 2 in the
-// step's first half), lane = position % 8 + 8 g, and of each 32 dims the eight from
-// 8 g on. So a block of 32 dims lies in four lanes, and a lane's eight are a 16-byte
-// piece of each plane: core matrices of 8 positions x 8 dims.
+// A CTA's share of one cache (keys or values) of one KV head, by four warps: of a
+// step's 128 positions NK * 4 row groups of eight, of their dims CH pieces of eight
+// (all of both by itself; in a pair half the groups of the keys, half the pieces of
+// the values). A warp takes groups w + 4 k, k < NK; lane = position % 8 + 8 g, and
+// pieces g + 4 i. A piece is 16 bytes of each plane: core matrices of 8 positions x
+// 8 dims.
 //
 // The exponent of a row (planes = row * 2^-e brings it to fp16's range) is that of
 // its largest scale, or for F32 of its largest value.
-template <int D, bool Q8>
+template <int D, bool Q8, int NK, int CH>
 struct KvRows;
 
-// Q8_0: two of a warp's rows are in registers; a row that store() has converted makes
+// Q8_0: two of a warp's rows are in registers; a row that has been converted makes
 // room for the one after the next.
-template <int D>
-struct KvRows<D, true> {
-  static constexpr int NC = D / 32, ND = (NC + 1) / 2;
-  uint2 q[2][NC];
+template <int D, int NK, int CH>
+struct KvRows<D, true, NK, CH> {
+  static constexpr int NC = D / 32, ND = (NC + 1) / 2, NI = (CH + 3) / 4;
+  uint2 q[2][NI];
   uint32_t d[2][ND];    // two scales a word
   uint32_t all[4][ND];  // the scales of the step's positions lane + 32 k: every warp finds the exponents itself
-  const uint8_t* qs;    // the head's quants and scales from this CTA's first position on
+  const uint8_t* qs;    // the head's quants (this share's dims) and scales from this CTA's first position on
   const uint16_t* ds;
   int64_t left;         // positions from there on
+  int row0, ch0;        // this share's first position of a step, first piece
 
   static __device__ __forceinline__ void scales(const uint16_t* s, bool in, uint32_t (&o)[ND]) {
 #pragma unroll
@@ -235,23 +280,26 @@ struct KvRows<D, true> {
 #pragma unroll
     for (int k = 0; k < 4; k++) scales(ds + (int64_t)(at + lane + 32 * k) * NC, at + lane + 32 * k < left, all[k]);
   }
-  // the warp's row k of the step at `at`
-  __device__ __forceinline__ void load_row(int k, int at, int w, int lane) {
-    const int pos = at + (w + 4 * k) * 8 + (lane & 7);
+  // row k of the step at `at` into buffer b
+  __device__ __forceinline__ void load_row(int k, int b, int at, int w, int lane) {
+    const int pos = at + row0 + (w + 4 * k) * 8 + (lane & 7), g = lane >> 3;
     const bool in = pos < left;
-    const uint8_t* src = qs + (int64_t)pos * D + 8 * (lane >> 3);
-    scales(ds + (int64_t)pos * NC, in, d[k & 1]);
+    const uint8_t* src = qs + (int64_t)pos * D + 8 * g;
+    scales(ds + (int64_t)pos * NC, in, d[b]);
 #pragma unroll
-    for (int i = 0; i < NC; i++) q[k & 1][i] = in ? *(const uint2*)(src + 32 * i) : make_uint2(0u, 0u);
+    for (int i = 0; i < NI; i++) q[b][i] = in && g + 4 * i < CH ? *(const uint2*)(src + 32 * i) : make_uint2(0u, 0u);
   }
-  __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int w, int lane) {
+  __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int w, int lane,
+                                        int first_row, int first_piece) {
     const int64_t at = (int64_t)kvh * p.n_ctx + pos0;
-    qs = (const uint8_t*)cache + at * D;
+    row0 = first_row;
+    ch0 = first_piece;
+    qs = (const uint8_t*)cache + at * D + 8 * ch0;
     ds = (const uint16_t*)((const uint8_t*)cache + (int64_t)p.HKV * p.n_ctx * D) + at * NC;
     left = n_kv - pos0;
     load_all(0, lane);
-    load_row(0, 0, w, lane);
-    load_row(1, 0, w, lane);
+    load_row(0, 0, 0, w, lane);
+    load_row(1, 1, 0, w, lane);
   }
   // The largest and least exponent of each half's rows that have a value but 0
   // (least is -2000 where a row has a NaN scale); those of rows that have their own
@@ -285,65 +333,86 @@ struct KvRows<D, true> {
     }
     load_all(at + kTrTile, lane);
   }
-  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&most)[2], const bool (&own)[2]) {
-    constexpr int plane = kTrTile * D * 2;
+  // row k, in buffer b
+  __device__ __forceinline__ void convert(int k, int b, uint8_t* planes, int w, int lane, const int (&most)[2], const bool (&own)[2]) const {
     const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+    const int g = lane >> 3;
+    const bool second = row0 + 32 * k >= kTrHalf;  // of the step's halves
+    int e = second ? most[1] : most[0];
+    bool fine = true, any;
+    if (second ? own[1] : own[0]) fine = exponent(d[b], e, any);
+    // 2^-e: fp16 holds 2^14 down to 2^-15
+    const __half down = __float2half_rn(fine ? pow2f(-e) : 0.0f);
+    uint8_t* dst = planes + (w + 4 * k) * (CH * 128) + g * 128 + (lane & 7) * 16;
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      uint8_t* dst = planes + (w + 4 * k) * (16 * D) + (lane >> 3) * 128 + (lane & 7) * 16;
-      int e = most[k >> 1];
-      bool fine = true, any;
-      if (own[k >> 1]) fine = exponent(d[k & 1], e, any);
-      // 2^-e: fp16 holds 2^14 down to 2^-15
-      const __half down = __float2half_rn(fine ? pow2f(-e) : 0.0f);
+    for (int i = 0; i < NI; i++) {
+      const int blk = (ch0 + g + 4 * i) >> 2;
+      uint32_t sd = d[b][0];
 #pragma unroll
-      for (int i = 0; i < NC; i++) {
-        const uint32_t sd = d[k & 1][i / 2];
-        const __half s = __ushort_as_half(fine ? (uint16_t)(i & 1 ? sd >> 16 : sd) : (uint16_t)0);
-        const __half2 f = __half2half2(__hmul_rn(s, down));
-        uint32_t h[4], l[4];
+      for (int u = 1; u < ND; u++) sd = (blk >> 1) == u ? d[b][u] : sd;
+      const __half s = __ushort_as_half(fine ? (uint16_t)(blk & 1 ? sd >> 16 : sd) : (uint16_t)0);
+      const __half2 f = __half2half2(__hmul_rn(s, down));
+      uint32_t h[4], l[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint32_t b = (j < 2 ? q[k & 1][i].x : q[k & 1][i].y) ^ 0x80808080u;
-          // two signed bytes as fp16: 1024 + (byte + 128) - 1152
-          const uint32_t t = __byte_perm(b, 0x64646464u, j & 1 ? 0x7362 : 0x5140);
-          const __half2 n = __hsub2_rn(*reinterpret_cast<const __half2*>(&t), off);
-          const __half2 hh = __hmul2_rn(n, f);
-          h[j] = h2_bits(hh);
-          l[j] = h2_bits(__hfma2(n, f, __hneg2(hh)));
-        }
-        *(uint4*)(dst + i * 512) = make_uint4(h[0], h[1], h[2], h[3]);
-        *(uint4*)(dst + plane + i * 512) = make_uint4(l[0], l[1], l[2], l[3]);
+      for (int j = 0; j < 4; j++) {
+        const uint32_t x = (j < 2 ? q[b][i].x : q[b][i].y) ^ 0x80808080u;
+        // two signed bytes as fp16: 1024 + (byte + 128) - 1152
+        const uint32_t t = __byte_perm(x, 0x64646464u, j & 1 ? 0x7362 : 0x5140);
+        const __half2 n = __hsub2_rn(*reinterpret_cast<const __half2*>(&t), off);
+        const __half2 hh = __hmul2_rn(n, f);
+        h[j] = h2_bits(hh);
+        l[j] = h2_bits(__hfma2(n, f, __hneg2(hh)));
       }
-      if (k < 2) load_row(k + 2, at, w, lane);
-      else load_row(k - 2, at + kTrTile, w, lane);
+      if (CH % 4 == 0 || g + 4 * i < CH) {
+        *(uint4*)(dst + i * 512) = make_uint4(h[0], h[1], h[2], h[3]);
+        *(uint4*)(dst + NK * 4 * CH * 128 + i * 512) = make_uint4(l[0], l[1], l[2], l[3]);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&most)[2], const bool (&own)[2]) {
+#pragma unroll 1
+    for (int u = 0; u < NK; u += 2) {
+      // (the row that a buffer takes next: two on, or this one of the next step)
+      const int next = NK == 4 ? u ^ 2 : u, to = NK == 4 && u == 0 ? at : at + kTrTile;
+      convert(u, 0, planes, w, lane, most, own);
+      load_row(next, 0, to, w, lane);
+      convert(u + 1, 1, planes, w, lane, most, own);
+      load_row(next + 1, 1, to, w, lane);
     }
   }
 };
 
 // F32: a step's rows would take too many registers; they are read for their
-// exponents and again for their planes.
-template <int D>
-struct KvRows<D, false> {
-  static constexpr int NC = D / 32;
+// exponents (all of them) and again for their planes.
+template <int D, int NK, int CH>
+struct KvRows<D, false, NK, CH> {
+  static constexpr int NC = D / 32, NI = (CH + 3) / 4;
   const float* rows;  // the head's, from this CTA's first position on
   int64_t row, left;  // floats between positions; positions
+  int row0, ch0;
 
-  __device__ __forceinline__ void load_row(int pos, int lane, float (&x)[NC * 8]) const {
+  // pieces g + 4 i (i < N) of a row from `first` on, up to `end`
+  template <int N>
+  __device__ __forceinline__ void load_row(int pos, int first, int end, int lane, float (&x)[N * 8]) const {
+    const int g = lane >> 3;
     const bool in = pos < left;
-    const float* src = rows + (int64_t)pos * row + 8 * (lane >> 3);
+    const float* src = rows + (int64_t)pos * row + 8 * (first + g);
 #pragma unroll
-    for (int i = 0; i < NC; i++) {
-      const float4 a = in ? *(const float4*)(src + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 b = in ? *(const float4*)(src + 32 * i + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < N; i++) {
+      const bool here = in && first + g + 4 * i < end;
+      const float4 a = here ? *(const float4*)(src + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 b = here ? *(const float4*)(src + 32 * i + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
       float* o = &x[8 * i];
       o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
     }
   }
-  __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int, int) {
+  __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int, int,
+                                        int first_row, int first_piece) {
     row = (int64_t)p.HKV * D;
     rows = (const float*)cache + pos0 * row + (int64_t)kvh * D;
     left = n_kv - pos0;
+    row0 = first_row;
+    ch0 = first_piece;
   }
   // (as above; `ends` [half][4]: what the four warps found, met at barrier `id`, also
   // by warps that have given up)
@@ -359,7 +428,7 @@ struct KvRows<D, false> {
 #pragma unroll
       for (int k = 2 * h; k < 2 * h + 2; k++) {
         float x[NC * 8];
-        load_row(at + (w + 4 * k) * 8 + (lane & 7), lane, x);
+        load_row<NC>(at + (w + 4 * k) * 8 + (lane & 7), 0, D / 8, lane, x);
         fine[k] = row_exponent<NC * 8>(x, e[k]);
         bad |= !fine[k];
         const bool any = e[k] > -100;
@@ -393,41 +462,114 @@ struct KvRows<D, false> {
     }
   }
   __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&most)[2], const bool (&own)[2]) const {
-    constexpr int plane = kTrTile * D * 2;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      uint8_t* dst = planes + (w + 4 * k) * (16 * D) + (lane >> 3) * 128 + (lane & 7) * 16;
-      float x[NC * 8];
-      load_row(at + (w + 4 * k) * 8 + (lane & 7), lane, x);
-      int e = most[k >> 1];
+    const int g = lane >> 3;
+#pragma unroll 1
+    for (int k = 0; k < NK; k++) {
+      const int in_step = row0 + (w + 4 * k) * 8 + (lane & 7);
+      const bool second = row0 + 32 * k >= kTrHalf;
+      int e = second ? most[1] : most[0];
       bool fine = true;
-      if (own[k >> 1]) {
+      if (second ? own[1] : own[0]) {
+        float x[NC * 8];
+        load_row<NC>(at + in_step, 0, D / 8, lane, x);
         fine = row_exponent<NC * 8>(x, e);
         e -= 14;
       }
+      float x[NI * 8];
+      load_row<NI>(at + in_step, ch0, ch0 + CH, lane, x);
+      uint8_t* dst = planes + (w + 4 * k) * (CH * 128) + g * 128 + (lane & 7) * 16;
 #pragma unroll
-      for (int i = 0; i < NC; i++) {
+      for (int i = 0; i < NI; i++) {
         uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
         if (fine) split8(&x[8 * i], pow2f(-e), hi, lo);
-        *(uint4*)(dst + i * 512) = hi;
-        *(uint4*)(dst + plane + i * 512) = lo;
+        if (CH % 4 == 0 || g + 4 * i < CH) {
+          *(uint4*)(dst + i * 512) = hi;
+          *(uint4*)(dst + NK * 4 * CH * 128 + i * 512) = lo;
+        }
       }
     }
   }
 };
 
-template <int D, bool Q8>
+// What a converting warp needs of its CTA.
+struct TrConvert {
+  int64_t pos0, n_kv;
+  int kvh, n, w, lane, rank;
+  const void* cache;
+  uint8_t* planes;  // [buffers][hi, lo]
+  int buffers;
+  uint64_t *empty, *col_full;
+  uint32_t full;    // shared::cluster address of the issuing CTA's barriers
+  float *col, *info;
+  int2* ends;
+  volatile int* abort_flag;
+};
+
+// The keys (or values) of every step. A step's exponents go out before its planes,
+// which wait for the products that read the planes there before. Their slot is
+// written again eight steps later: after the planes of seven, for which the scores of
+// five were done, for which the softmax had read those of four, and so had long left
+// the step itself.
+template <int D, bool Q8, bool PAIR, bool IS_V>
+__device__ __forceinline__ void convert_role(const TreeAttnParams& p, const TrConvert& r, uint64_t* queries_done, bool wait_queries) {
+  constexpr int NK = PAIR && !IS_V ? 2 : 4, CH = PAIR && IS_V ? D / 16 : D / 8, plane = NK * 4 * CH * 128;
+  KvRows<D, Q8, NK, CH> kv;
+  kv.begin(p, r.cache, r.kvh, r.pos0, r.n_kv, r.w, r.lane, PAIR && !IS_V ? r.rank * kTrHalf : 0, PAIR && IS_V ? r.rank * CH : 0);
+  bool ok = true;
+  for (int j = 0; j < r.n; j++) {
+    const int slot = j & (kTrSlots - 1), b = j % r.buffers;
+    int most[2];
+    bool own[2];
+    kv.exponents(
+        j * kTrTile, r.w, r.lane, r.ends + (j & 1) * 8, IS_V ? 6 : 5, most, own, [](int hi, int lo) { return lo < 1000 && hi - lo > 10; },
+        [&](int h, int at, int e, bool fine) {
+          float* c = r.col + (slot * 2 + h) * 3 * kTrHalf;
+          const float nan = __int_as_float(0x7fffffff);
+          if (IS_V) {
+            c[kTrHalf + at] = fine ? (float)e : nan;
+            // (finite in every case: a masked position's weight is 0 whatever its row holds)
+            c[2 * kTrHalf + at] = fine ? (float)e : 0.0f;
+          } else {
+            c[at] = fine ? pow2f(e) : nan;
+          }
+        });
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if (most[h] < -999) most[h] = 0;  // (nothing but zeros)
+      if (r.w == 0 && r.lane == 0)
+        *(float2*)(r.info + (slot * 2 + h) * 4 + (IS_V ? 2 : 0)) =
+            make_float2(IS_V ? (float)most[h] : pow2f(most[h]), own[h] ? 1.0f : 0.0f);
+    }
+    __syncwarp();
+    if (r.lane < 2) mbar_arrive_one(&r.col_full[slot * 2 + r.lane]);
+    ok = ok && (j < r.buffers || tc_wait_ready(&r.empty[b], (uint32_t)(j / r.buffers - 1) & 1u, r.abort_flag, p.err));
+    // (the first values lie where the queries were)
+    if (IS_V && j == 0 && wait_queries) ok = ok && tc_wait_ready(queries_done, 0, r.abort_flag, p.err);
+    if (ok) {
+      kv.store(j * kTrTile, r.planes + b * 2 * plane, r.w, r.lane, most, own);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (r.lane == 0) arrive_lead(r.full + 8 * b);
+    }
+  }
+}
+
+template <int D, bool Q8, bool PAIR>
 __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_constant__ TreeAttnParams p,
                                                                   const TreeSplit sp, const int vec_q) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  using L = TrSmem<D>;
+  using L = TrSmem<D, PAIR>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTrRows;
+  const int split = blockIdx.z, kvh = blockIdx.y, r0 = blockIdx.x * kTrRows;
   const int rep = p.H / p.HKV;
   const int64_t n_kv = (int64_t)p.n_past + p.T;
   const int64_t pos0 = (int64_t)split * sp.per * kTrTile;
   const int n = (int)min((int64_t)sp.per, (n_kv - pos0 + kTrTile - 1) / kTrTile);  // steps of this CTA, at least one
-  const int nq = min(4, (sp.R - r0 + 31) / 32);  // quadrants of 32 rows in use: kTrParts softmax warps each
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;  // CTA 0 of a pair issues the MMAs
+  // quadrants of 32 rows in use, kTrParts softmax warps each: here (none, where a pair
+  // has no second tile) and in the pair
+  const int nq = max(0, min(4, (sp.R - r0 + 31) / 32));
+  const int nq_all = PAIR ? max(0, min(8, (sp.R - (r0 - rank * kTrRows) + 31) / 32)) : nq;
   float* col = (float*)(smem + L::col);
   float* info = (float*)(smem + L::info);
   float* mxs = (float*)(smem + L::mx);
@@ -441,32 +583,39 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = s_full + 3;
   uint64_t* t_full = s_full + 4;  // TMEM is there
-  uint64_t* q_full = s_full + 5;
+  uint64_t* q_full = s_full + 5;  // the queries are in TMEM (of both CTAs)
   uint64_t* drain = s_full + 6;
+  uint64_t* q_here = s_full + 7;  // ... of this one
   uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
   volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
 
+  // Barriers that the issuing warp waits on lie in CTA 0 and count both CTAs' warps;
+  // its commits arrive in both.
   if (tid == 0) {
     for (int i = 0; i < L::n_k; i++) {
-      mbar_init(&k_full[i], 4);
+      mbar_init(&k_full[i], PAIR ? 8 : 4);
       mbar_init(&k_empty[i], 1);
     }
     for (int i = 0; i < L::n_v; i++) {
-      mbar_init(&v_full[i], 4);
+      mbar_init(&v_full[i], PAIR ? 8 : 4);
       mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2 * kTrSlots; i++) mbar_init(&col_full[i], 8);
     mbar_init(s_full, 1);
-    mbar_init(s_empty, kTrParts * nq);
-    mbar_init(p_full, kTrParts * nq);
+    mbar_init(s_empty, kTrParts * nq_all);
+    mbar_init(p_full, kTrParts * nq_all);
     mbar_init(o_full, 1);
     mbar_init(t_full, 1);
-    mbar_init(q_full, kTrParts * nq);
+    mbar_init(q_full, kTrParts * nq_all + (PAIR ? 2 : 1));
     mbar_init(drain, 1);
+    mbar_init(q_here, max(1, kTrParts * nq));
     *abort_flag = 0;
     fence_mbar_init();
   }
-  __syncthreads();
+  if (PAIR) cluster_sync_all();
+  else __syncthreads();
+  auto lead = [](uint64_t* bar) { return dsmem_addr(bar, 0); };
+  const uint32_t s_empty0 = lead(s_empty), p_full0 = lead(p_full), q_full0 = lead(q_full);
 
   if (warp >= kTrWarpMma) {
     // ---------------- MMA issue ----------------
@@ -475,18 +624,28 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     // to issue, three times what it takes to run).
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
     if (warp == kTrWarpMma) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_base)),
-                   "r"(kTrCols));
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+      if (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_base)), "r"(kTrCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+      } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_base)), "r"(kTrCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+      }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_one(t_full);
-      constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTrTile >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
+      if (lane == 0) {
+        mbar_arrive_one(t_full);
+        arrive_lead(q_full0);
+      }
+      constexpr uint32_t M = kTrRows * (PAIR ? 2 : 1);
+      constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTrTile >> 3) << 17) | ((M >> 4) << 24);
       // (bit 16: B, the values, is dims-major)
-      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTrRows >> 4) << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((M >> 4) << 24);
+      // bytes between the values' groups of eight positions
+      constexpr uint32_t v_group = (uint32_t)(D / 8) * 128 / (PAIR ? 2 : 1);
       const uint32_t qh = kTmem + kColQ, ql = qh + D / 2;
       const uint64_t kd = umma_desc(smem_addr(smem + L::k), 128, 16 * D);
-      const uint64_t vd = umma_desc(smem_addr(smem + L::v), 16 * D, 128);
+      const uint64_t vd = umma_desc(smem_addr(smem + L::v), v_group, 128);
       constexpr uint64_t plane = L::plane >> 4;
       // step j's scores, once the step before's have been read
       auto scores = [&](int j) {
@@ -500,18 +659,18 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           asm volatile("" : "+l"(kh));  // (the 24 descriptors are formed here, not kept in registers)
           const uint64_t kl = kh + plane;
 #pragma unroll
-          for (int s = 0; s < D / 16; s++) mma_ts(d, ql + 8 * s, kh + 16 * s, idesc_s, s > 0);
+          for (int s = 0; s < D / 16; s++) mma_ts<PAIR>(d, ql + 8 * s, kh + 16 * s, idesc_s, s > 0);
 #pragma unroll
-          for (int s = 0; s < D / 16; s++) mma_ts(d, qh + 8 * s, kl + 16 * s, idesc_s, 1);
+          for (int s = 0; s < D / 16; s++) mma_ts<PAIR>(d, qh + 8 * s, kl + 16 * s, idesc_s, 1);
 #pragma unroll
-          for (int s = 0; s < D / 16; s++) mma_ts(d, qh + 8 * s, kh + 16 * s, idesc_s, 1);
-          umma_commit(s_full);
-          umma_commit(&k_empty[b]);
+          for (int s = 0; s < D / 16; s++) mma_ts<PAIR>(d, qh + 8 * s, kh + 16 * s, idesc_s, 1);
+          mma_commit<PAIR>(s_full);
+          mma_commit<PAIR>(&k_empty[b]);
         }
         __syncwarp();
         return true;
       };
-      bool ok = tc_wait_ready(q_full, 0, abort_flag, p.err) && scores(0);
+      bool ok = rank == 0 && tc_wait_ready(q_full, 0, abort_flag, p.err) && scores(0);
       for (int j = 0; j < n && ok; j++) {
         if (j + 1 < n && !(ok = scores(j + 1))) break;
         const int b = j % L::n_v;
@@ -524,20 +683,20 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           asm volatile("" : "+l"(vh));
           const uint64_t vl = vh + plane;
 #pragma unroll
-          for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_lo + 8 * s, vh + 2 * D * s, idesc_o, s > 0);
+          for (int s = 0; s < kTrTile / 16; s++) mma_ts<PAIR>(o, p_lo + 8 * s, vh + (v_group >> 3) * s, idesc_o, s > 0);
 #pragma unroll
-          for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vl + 2 * D * s, idesc_o, 1);
+          for (int s = 0; s < kTrTile / 16; s++) mma_ts<PAIR>(o, p_hi + 8 * s, vl + (v_group >> 3) * s, idesc_o, 1);
 #pragma unroll
-          for (int s = 0; s < kTrTile / 16; s++) mma_ts(o, p_hi + 8 * s, vh + 2 * D * s, idesc_o, 1);
-          umma_commit(o_full);
-          umma_commit(&v_empty[b]);
+          for (int s = 0; s < kTrTile / 16; s++) mma_ts<PAIR>(o, p_hi + 8 * s, vh + (v_group >> 3) * s, idesc_o, 1);
+          mma_commit<PAIR>(o_full);
+          mma_commit<PAIR>(&v_empty[b]);
         }
         __syncwarp();
       }
       // every MMA has finished before TMEM and shared memory are given back
-      if (elect_one()) umma_commit(drain);
+      if (rank == 0 && elect_one()) mma_commit<PAIR>(drain);
       __syncwarp();
-      for (uint32_t it = 0; it < kSpinLimit && !__all_sync(0xffffffffu, mbar_test(drain, 0)); it++) {
+      for (uint32_t it = 0; it < kSpinLimit && !__all_sync(0xffffffffu, mbar_try_wait_sleep(drain, 0)); it++) {
       }
     } else if (warp < kTrWarpMma + 3) {
       // Two of the other warps of the group ask for the whole range, keys and values,
@@ -558,57 +717,28 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     }
   } else if (warp >= kTrWarpK) {
     // ---------------- keys (warps 16-19) and values (20-23) ----------------
-    // A step's exponents go out before its planes, which wait for the products that
-    // read the planes there before. Their slot is written again eight steps later:
-    // after the planes of seven, for which the scores of five were done, for which
-    // the softmax had read those of four, and so had long left the step itself.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
     const bool is_v = warp >= kTrWarpV;
-    const int w = warp & 3;
-    const void* cache = is_v ? p.cache_v : p.cache_k;
-    const int nb = is_v ? L::n_v : L::n_k;
-    uint64_t* full = is_v ? v_full : k_full;
-    uint64_t* empty = is_v ? v_empty : k_empty;
-    int2* ends = (int2*)(smem + L::ends) + (is_v ? 16 : 0);
-    KvRows<D, Q8> kv;
-    kv.begin(p, cache, kvh, pos0, n_kv, w, lane);
-    bool ok = true;
-    for (int j = 0; j < n; j++) {
-      const int slot = j & (kTrSlots - 1);
-      int most[2];
-      bool own[2];
-      kv.exponents(
-          j * kTrTile, w, lane, ends + (j & 1) * 8, is_v ? 6 : 5, most, own,
-          [](int hi, int lo) { return lo < 1000 && hi - lo > 10; },
-          [&](int h, int at, int e, bool fine) {
-            float* c = col + (slot * 2 + h) * 3 * kTrHalf;
-            const float nan = __int_as_float(0x7fffffff);
-            if (is_v) {
-              c[kTrHalf + at] = fine ? (float)e : nan;
-              // (finite in every case: a masked position's weight is 0 whatever its row holds)
-              c[2 * kTrHalf + at] = fine ? (float)e : 0.0f;
-            } else {
-              c[at] = fine ? pow2f(e) : nan;
-            }
-          });
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if (most[h] < -999) most[h] = 0;  // (nothing but zeros)
-        if (w == 0 && lane == 0)
-          *(float2*)(info + (slot * 2 + h) * 4 + (is_v ? 2 : 0)) =
-              make_float2(is_v ? (float)most[h] : pow2f(most[h]), own[h] ? 1.0f : 0.0f);
-      }
-      __syncwarp();
-      if (lane < 2) mbar_arrive_one(&col_full[slot * 2 + lane]);
-      const int b = j % nb;
-      ok = ok && (j < nb || tc_wait_ready(&empty[b], (uint32_t)(j / nb - 1) & 1u, abort_flag, p.err));
-      if (ok) {
-        kv.store(j * kTrTile, smem + (is_v ? L::v : L::k) + b * 2 * L::plane, w, lane, most, own);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_one(&full[b]);
-      }
-    }
+    TrConvert r;
+    r.pos0 = pos0;
+    r.n_kv = n_kv;
+    r.kvh = kvh;
+    r.n = n;
+    r.w = warp & 3;
+    r.lane = lane;
+    r.rank = rank;
+    r.cache = is_v ? p.cache_v : p.cache_k;
+    r.planes = smem + (is_v ? L::v : L::k);
+    r.buffers = is_v ? L::n_v : L::n_k;
+    r.empty = is_v ? v_empty : k_empty;
+    r.full = lead(is_v ? v_full : k_full);
+    r.col_full = col_full;
+    r.col = col;
+    r.info = info;
+    r.ends = (int2*)(smem + L::ends) + (is_v ? 16 : 0);
+    r.abort_flag = abort_flag;
+    if (is_v) convert_role<D, Q8, PAIR, true>(p, r, q_here, nq > 0);
+    else convert_role<D, Q8, PAIR, false>(p, r, q_here, false);
   } else {
     // ---------------- softmax: four threads per row ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -626,11 +756,28 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       {
         float x[NA], m = 0.0f;
         bool fine = true;
-        const float* src = p.q + i * p.q_stride + (int64_t)(kvh * rep + min(r, sp.R - 1) - i * rep) * D + NA * part;
+        // read along the rows (a row a lane would be 32 lines a request), turned where
+        // the first values will be: this warp's 32 rows x NA floats
+        constexpr int NP = NA / 4;
+        float4* turn = (float4*)(smem + L::v) + (part * 4 + quad) * 32 * NP;
+        auto place = [](int row, int c) { return row * NP + (NP == 8 || NP == 4 ? c ^ (row & (NP - 1)) : c); };
+        float4 got[NP];
 #pragma unroll
-        for (int k = 0; k < NA; k += 4) {
-          const float4 a = vec_q ? *(const float4*)(src + k) : make_float4(src[k], src[k + 1], src[k + 2], src[k + 3]);
-          x[k] = a.x, x[k + 1] = a.y, x[k + 2] = a.z, x[k + 3] = a.w;
+        for (int u = 0; u < NP; u++) {
+          const int e = lane + 32 * u, row = e / NP, c = e - row * NP, rr = min(r0 + quad * 32 + row, sp.R - 1), ti = rr / rep;
+          const float* src = p.q + ti * p.q_stride + (int64_t)(kvh * rep + rr - ti * rep) * D + NA * part + 4 * c;
+          got[u] = vec_q ? *(const float4*)src : make_float4(src[0], src[1], src[2], src[3]);
+        }
+#pragma unroll
+        for (int u = 0; u < NP; u++) {
+          const int e = lane + 32 * u, row = e / NP;
+          turn[place(row, e - row * NP)] = got[u];
+        }
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < NP; c++) {
+          const float4 a = turn[place(lane, c)];
+          x[4 * c] = a.x, x[4 * c + 1] = a.y, x[4 * c + 2] = a.z, x[4 * c + 3] = a.w;
         }
 #pragma unroll
         for (int k = 0; k < NA; k++) {
@@ -660,7 +807,10 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_one(q_full);
+          if (lane == 0) {
+            mbar_arrive_one(q_here);
+            arrive_lead(q_full0);
+          }
         }
       }
       float M = -INFINITY;                   // the row's maximum
@@ -703,7 +853,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         tmem_wait_ld(x);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(s_empty);
+        if (lane == 0) arrive_lead(s_empty0);
         // (two elements an instruction where the hardware has one)
         float2* x2 = (float2*)x;
         const float4 in = *(const float4*)(info + slot * 4);
@@ -804,7 +954,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(p_full);
+        if (lane == 0) arrive_lead(p_full0);
       }
       if (ok) ok = take_o(n - 1, f_prev);
       // the parts' sums
@@ -837,7 +987,8 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync_all();  // (neither CTA leaves, or gives up its TMEM, before the other has finished)
+  else __syncthreads();
   if (*abort_flag == 0) {
     // out of it in rows: the records of a CTA's rows are contiguous
     const int rows = min(kTrRows, sp.R - r0);
@@ -857,13 +1008,33 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   if (warp == kTrWarpMma) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_base), "r"(kTrCols));
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(*tmem_base), "r"(kTrCols));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_base), "r"(kTrCols));
   }
 }
 
+// Splits of a KV head's positions: one CTA (or pair) per SM (or two).
 int64_t most_splits(int64_t H, int64_t HKV, int64_t n_kv, int64_t T) {
   const int64_t RG = (T * (H / HKV) + kTrRows - 1) / kTrRows, steps = (n_kv + kTrTile - 1) / kTrTile;
-  return std::min(steps, std::max<int64_t>(1, kTrSms / std::max<int64_t>(1, HKV * RG)));
+  const int64_t ctas = RG == 1 ? 1 : (RG + 1) / 2 * 2;
+  return std::min(steps, std::max<int64_t>(1, kTrSms / std::max<int64_t>(1, HKV * ctas)));
+}
+
+template <int D, bool Q8, bool PAIR>
+cudaError_t launch_tiles(const TreeAttnParams& p, const TreeSplit& sp, cudaStream_t s) {
+  const int vec_q = (uintptr_t)p.q % 16 == 0 && p.q_stride % 4 == 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(PAIR ? (sp.RG + 1) / 2 * 2 : sp.RG), (unsigned)p.HKV, (unsigned)sp.S);
+  cfg.blockDim = dim3(kTrThreads);
+  cfg.dynamicSmemBytes = TrSmem<D, PAIR>::total;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : 1;  // (a pair lies along x: along z the launch is refused)
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_tree_kernel<D, Q8, PAIR>, p, sp, vec_q);
 }
 
 template <int D, bool Q8>
@@ -875,18 +1046,22 @@ cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
   const int64_t most = most_splits(p.H, p.HKV, n_kv, p.T);
   sp.per = (int32_t)((steps + most - 1) / most);
   sp.S = (int32_t)((steps + sp.per - 1) / sp.per);
-  const int vec_q = (uintptr_t)p.q % 16 == 0 && p.q_stride % 4 == 0;
-  attn_tree_kernel<D, Q8><<<dim3((unsigned)sp.S, (unsigned)p.HKV, (unsigned)sp.RG), kTrThreads, TrSmem<D>::total, s>>>(p, sp, vec_q);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = sp.RG == 1 ? launch_tiles<D, Q8, false>(p, sp, s) : launch_tiles<D, Q8, true>(p, sp, s);
   if (e != cudaSuccess || sp.S == 1) return e;
   return launch_tree_join<D>(p, sp, s);
 }
 
+template <int D, bool Q8>
+cudaError_t prepare_tiles() {
+  const cudaError_t e = cudaFuncSetAttribute(attn_tree_kernel<D, Q8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             TrSmem<D, false>::total);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(attn_tree_kernel<D, Q8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D, true>::total);
+}
 template <int D>
 cudaError_t prepare_tree() {
-  const cudaError_t e = cudaFuncSetAttribute(attn_tree_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D>::total);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(attn_tree_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D>::total);
+  const cudaError_t e = prepare_tiles<D, false>();
+  return e == cudaSuccess ? prepare_tiles<D, true>() : e;
 }
 
 }  // namespace
