@@ -1,11 +1,11 @@
-// Tree attention with few rows over a Q8_0 cache: one token of decode, or a draft of
-// a token or two (n_rep query heads of a KV head times T tokens). The same formula
-// and records as attn_tree.cu, whose 128-row tiles would be almost empty here; what
-// counts is how soon the last byte of the cache has been asked for.
+// Tree attention with few rows: one token of decode, or a draft of a token or two
+// (n_rep query heads of a KV head times T tokens). The same formula and records as
+// attn_tree.cu, whose 128-row tiles would be almost empty here; what counts is how
+// soon the last byte of the cache has been asked for.
 //
 // A warp takes 16 positions at a time and eight rows for its columns, so a tile of
 // the two products is one m16n8 tensor-core tile: S^T = K Q^T and O^T = V^T P^T. The
-// cache goes from global memory straight into the MMAs' registers:
+// cache goes from global memory straight into the MMAs' registers. From a Q8_0 cache:
 //   * a lane's eight bytes of a block of 32 dims are two k-steps of K's operand (the
 //     queries are held in the same order of dims, as fp16 pairs hi + lo);
 //   * four bytes of each of four positions, transposed by byte permutes, are two
@@ -14,6 +14,13 @@
 // scale multiplies its sum in float, and P carries the values' scales: P d_v 2^(13 -
 // E), E the largest scale's exponent of the step, again as hi + lo, turned from S's
 // layout into the operand's by an 8 x 8 transpose.
+//
+// From an F32 cache the same tiles as m16n8k8 of tf32, every operand as hi + lo (11
+// bits each: 2^-21 of a value is left out) and three MMAs a product; tf32 has float's
+// range, so nothing has to be scaled. The queries' planes lie in shared memory, the
+// registers are full of cache. A position whose values hold an infinity or a NaN
+// counts with zeros, and with a weight of NaN where it is attended to: a masked
+// weight, 0, takes nothing from it.
 //
 // Four warps per CTA, each with its own running maxima, sums and O in registers. The
 // CTA's warps meet in shared memory and the CTAs of a cluster in distributed shared
@@ -35,16 +42,27 @@ constexpr int kFewNT = 128;
 constexpr int kFewWarps = kFewNT / 32;
 
 // positions that a warp has in registers at a time, in tiles of 16
-template <int D>
-constexpr int kFewTiles = D <= 64 ? 2 : 1;
-template <int D>
-constexpr int kFewStep = kFewWarps * 16 * kFewTiles<D>;  // positions of a CTA's step
+template <int D, bool Q8>
+constexpr int kFewTiles = D <= (Q8 ? 64 : 32) ? 2 : 1;
+template <int D, bool Q8>
+constexpr int kFewStep = kFewWarps * 16 * kFewTiles<D, Q8>;  // positions of a CTA's step
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo as tf32: hi is cut (a rounded one could leave float's range), lo rounded
+// (the MMA drops the bits behind its eleventh).
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi))) + 0x1000u;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -63,46 +81,45 @@ __device__ __forceinline__ float dsmem_ld(const float* p, uint32_t rank) {
   return v;
 }
 
-template <int D, int NR>
+template <int D, int NR, bool Q8>
 struct FewSmem {
   static constexpr int R = 8 * NR;
   float part[kFewWarps][R][D];  // the warps' O, then (in [0]) the CTA's
   float m[kFewWarps][R], l[kFewWarps][R], scale[kFewWarps][R];
   float cm[R], cl[R];           // the CTA's
+  uint4 q[Q8 ? 1 : NR][Q8 ? 1 : D / 32][4][Q8 ? 1 : 32];  // F32: [hi, hi, lo, lo] of a lane's eight dims of each block
 };
 
-// NR: groups of eight rows. Grid (splits, KV heads, groups of 8 NR rows), clusters
-// along the splits.
-template <int D, int NR>
-__global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant__ TreeAttnParams p, const TreeSplit sp,
-                                                          const int cluster) {
-  constexpr int NC = D / 32, ND = (NC + 1) / 2, PT = kFewTiles<D>, step = kFewStep<D>;
-  extern __shared__ __align__(16) uint8_t few_raw[];
-  FewSmem<D, NR>& sm = *reinterpret_cast<FewSmem<D, NR>*>(few_raw);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.y, r0 = blockIdx.z * 8 * NR, rep = p.H / p.HKV;
-  const int64_t n_kv = (int64_t)p.n_past + p.T;
-  const int64_t begin = (int64_t)blockIdx.x * sp.per * step, end = min(n_kv, begin + (int64_t)sp.per * step);
-  const int64_t head = (int64_t)kvh * p.n_ctx, plane = (int64_t)p.HKV * p.n_ctx * D;
-  const uint8_t* kq = (const uint8_t*)p.cache_k + head * D;
-  const uint8_t* vq = (const uint8_t*)p.cache_v + head * D;
-  const uint16_t* ks = (const uint16_t*)((const uint8_t*)p.cache_k + plane) + head * NC;
-  const uint16_t* vs = (const uint16_t*)((const uint8_t*)p.cache_v + plane) + head * NC;
+// What a warp holds of the cache: PT tiles of 16 positions.
+template <int D, bool Q8>
+struct FewCache;
 
-  // what a step holds of the cache
+template <int D>
+struct FewCache<D, true> {
+  static constexpr int NC = D / 32, ND = (NC + 1) / 2, PT = kFewTiles<D, true>;
   uint2 K[PT][2][NC];                  // positions g, g + 8; eight bytes of each block
   uint32_t V[PT][4][NC];               // positions 2t, 2t + 1, 2t + 8, 2t + 9; four bytes of each block
   uint32_t dk[PT][2][ND], dv[PT][2][ND];  // scales of positions g, g + 8, two a word
-  auto scales = [&](const uint16_t* s, int64_t pos, bool in, uint32_t (&o)[ND]) {
+  const uint8_t *kq, *vq;
+  const uint16_t *ks, *vs;
+
+  __device__ __forceinline__ FewCache(const TreeAttnParams& p, int kvh) {
+    const int64_t head = (int64_t)kvh * p.n_ctx, plane = (int64_t)p.HKV * p.n_ctx * D;
+    kq = (const uint8_t*)p.cache_k + head * D;
+    vq = (const uint8_t*)p.cache_v + head * D;
+    ks = (const uint16_t*)((const uint8_t*)p.cache_k + plane) + head * NC;
+    vs = (const uint16_t*)((const uint8_t*)p.cache_v + plane) + head * NC;
+  }
+  static __device__ __forceinline__ void scales(const uint16_t* s, int64_t pos, bool in, uint32_t (&o)[ND]) {
     s += pos * NC;
 #pragma unroll
     for (int i = 0; i < ND; i++)
       o[i] = !in ? 0u : NC % 2 == 0 ? *(const uint32_t*)(s + 2 * i) : s[2 * i] | (2 * i + 1 < NC ? (uint32_t)s[2 * i + 1] << 16 : 0u);
-  };
-  auto load = [&](int64_t b) {
+  }
+  __device__ __forceinline__ void load(int64_t at, int64_t end, int g, int t) {
 #pragma unroll
     for (int q = 0; q < PT; q++) {
-      const int64_t tp = b + (warp * PT + q) * 16;
+      const int64_t tp = at + q * 16;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const int64_t pos = tp + g + 8 * h;
@@ -119,11 +136,69 @@ __global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant_
         for (int c = 0; c < NC; c++) V[q][h][c] = pos < end ? *(const uint32_t*)(vq + pos * D + 32 * c + 4 * g) : 0u;
       }
     }
-  };
-  if (begin < end) load(begin);
+  }
+};
+
+template <int D>
+struct FewCache<D, false> {
+  static constexpr int NC = D / 32, PT = kFewTiles<D, false>;
+  float K[PT][2][NC][8];  // positions g, g + 8; eight dims of each block
+  float V[PT][4][NC][4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9; four dims of each block
+  const float *k, *v;
+  int64_t row;
+
+  __device__ __forceinline__ FewCache(const TreeAttnParams& p, int kvh) {
+    k = (const float*)p.cache_k + (int64_t)kvh * D;
+    v = (const float*)p.cache_v + (int64_t)kvh * D;
+    row = (int64_t)p.HKV * D;
+  }
+  static __device__ __forceinline__ void load4(float* to, const float* from, bool in) {
+    const float4 x = in ? *(const float4*)from : make_float4(0.f, 0.f, 0.f, 0.f);
+    to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+  }
+  __device__ __forceinline__ void load(int64_t at, int64_t end, int g, int t) {
+#pragma unroll
+    for (int q = 0; q < PT; q++) {
+      const int64_t tp = at + q * 16;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int64_t pos = tp + g + 8 * h;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          load4(&K[q][h][c][0], k + pos * row + 32 * c + 8 * t, pos < end);
+          load4(&K[q][h][c][4], k + pos * row + 32 * c + 8 * t + 4, pos < end);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 4; h++) {
+        const int64_t pos = tp + 2 * t + (h & 1) + 4 * (h & 2);
+#pragma unroll
+        for (int c = 0; c < NC; c++) load4(V[q][h][c], v + pos * row + 32 * c + 4 * g, pos < end);
+      }
+    }
+  }
+};
+
+// NR: groups of eight rows. Grid (splits, KV heads, groups of 8 NR rows), clusters
+// along the splits.
+//
+// Registers: one group over a Q8_0 cache for 4 CTAs of an SM (3 of 96 and 128 dims; 2
+// took 36 us for a token over 32000 positions of 28 / 4 heads of 128, 3 take 23).
+template <int D, int NR, bool Q8>
+__global__ void __launch_bounds__(kFewNT, NR == 1 && Q8 ? (D <= 64 ? 4 : 3) : 1) attn_few_kernel(const __grid_constant__ TreeAttnParams p, const TreeSplit sp,
+                                                          const int cluster) {
+  constexpr int NC = D / 32, PT = kFewTiles<D, Q8>, step = kFewStep<D, Q8>;
+  extern __shared__ __align__(16) uint8_t few_raw[];
+  FewSmem<D, NR, Q8>& sm = *reinterpret_cast<FewSmem<D, NR, Q8>*>(few_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y, r0 = blockIdx.z * 8 * NR, rep = p.H / p.HKV;
+  const int64_t n_kv = (int64_t)p.n_past + p.T;
+  const int64_t begin = (int64_t)blockIdx.x * sp.per * step, end = min(n_kv, begin + (int64_t)sp.per * step);
+  FewCache<D, Q8> kv(p, kvh);
+  if (begin < end) kv.load(begin + warp * PT * 16, end, g, t);
 
   // the queries: row 8n + g, the dims that this lane's key bytes stand for
-  uint32_t qh[NR][NC][4], ql[NR][NC][4];
+  uint32_t qh[Q8 ? NR : 1][NC][4], ql[Q8 ? NR : 1][NC][4];  // (F32: in shared memory)
   float rf[NR][2];  // |scale| * log2(e) * the factor of rows 8n + 2t, 8n + 2t + 1
   int tok[NR][2];
 #pragma unroll
@@ -144,20 +219,36 @@ __global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant_
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     fine = m <= 3.402823466e38f;
-    // (the row's largest value becomes 2^14..2^15; a row with an infinity or a NaN: NaN)
-    const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127);
-    const float f = p.scale < 0.0f ? -pow2f(14 - ex) : pow2f(14 - ex);
+    // The row's largest value becomes 2^14..2^15; with an F32 cache 2^-9..2^-8, so that
+    // no score leaves a float's range. A row with an infinity or a NaN: NaN.
+    constexpr int up = Q8 ? 14 : -9;
+    const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), Q8 ? 127 : 117);
+    const float f = p.scale < 0.0f ? -pow2f(up - ex) : pow2f(up - ex);
 #pragma unroll
-    for (int c = 0; c < NC; c++)
+    for (int c = 0; c < NC; c++) {
+      if constexpr (Q8) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float a = __fmul_rn(x[c][2 * e], f), b = __fmul_rn(x[c][2 * e + 1], f);
-        const __half2 hh = __floats2half2_rn(a, b);
-        const float2 back = __half22float2(hh);
-        qh[n][c][e] = fine ? h2_bits(hh) : 0x7e007e00u;
-        ql[n][c][e] = fine ? h2_bits(__floats2half2_rn(__fsub_rn(a, back.x), __fsub_rn(b, back.y))) : 0u;
+        for (int e = 0; e < 4; e++) {
+          const float a = __fmul_rn(x[c][2 * e], f), b = __fmul_rn(x[c][2 * e + 1], f);
+          const __half2 hh = __floats2half2_rn(a, b);
+          const float2 back = __half22float2(hh);
+          qh[n][c][e] = fine ? h2_bits(hh) : 0x7e007e00u;
+          ql[n][c][e] = fine ? h2_bits(__floats2half2_rn(__fsub_rn(a, back.x), __fsub_rn(b, back.y))) : 0u;
+        }
+      } else if (c % kFewWarps == warp) {
+        uint32_t h[8], l[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          split_tf32(__fmul_rn(x[c][e], f), h[e], l[e]);
+          if (!fine) h[e] = 0x7fc00000u;
+        }
+        sm.q[n][c][0][lane] = make_uint4(h[0], h[1], h[2], h[3]);
+        sm.q[n][c][1][lane] = make_uint4(h[4], h[5], h[6], h[7]);
+        sm.q[n][c][2][lane] = make_uint4(l[0], l[1], l[2], l[3]);
+        sm.q[n][c][3][lane] = make_uint4(l[4], l[5], l[6], l[7]);
       }
-    const float own = __fmul_rn(__fmul_rn(fabsf(p.scale), 1.4426950408889634f), pow2f(ex - 14));
+    }
+    const float own = __fmul_rn(__fmul_rn(fabsf(p.scale), 1.4426950408889634f), pow2f(ex - up));
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       rf[n][u] = __shfl_sync(0xffffffffu, own, 4 * (2 * t + u));
@@ -165,8 +256,10 @@ __global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant_
     }
   }
 
+  if (!Q8) __syncthreads();
+
   float M[NR][2], l[NR][2], acc[NR][NC][2][4];
-  int E = 0;  // O is in units of 2^(E - 13)
+  int E = 13;  // O is in units of 2^(E - 13)
 #pragma unroll
   for (int n = 0; n < NR; n++) {
     M[n][0] = M[n][1] = -INFINITY;
@@ -179,51 +272,81 @@ __global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant_
         for (int k = 0; k < 4; k++) acc[n][c][i][k] = 0.0f;
   }
   for (int64_t b = begin; b < end; b += step) {
-    if (b != begin) load(b);
+    if (b != begin) kv.load(b + warp * PT * 16, end, g, t);
     // ---- scores, in units of log2: x[tile][row group][position g + 8 (k / 2), row 2t + k % 2]
     float x[PT][NR][4];
 #pragma unroll
     for (int q = 0; q < PT; q++) {
+      if constexpr (Q8) {
 #pragma unroll
-      for (int n = 0; n < NR; n++) x[q][n][0] = x[q][n][1] = x[q][n][2] = x[q][n][3] = 0.0f;
+        for (int n = 0; n < NR; n++) x[q][n][0] = x[q][n][1] = x[q][n][2] = x[q][n][3] = 0.0f;
 #pragma unroll
-      for (int c = 0; c < NC; c++) {
-        uint32_t a[2][4];  // [row g / g + 8][byte pair]
+        for (int c = 0; c < NC; c++) {
+          uint32_t a[2][4];  // [row g / g + 8][byte pair]
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t w0 = K[q][h][c].x ^ 0x80808080u, w1 = K[q][h][c].y ^ 0x80808080u;
-          a[h][0] = bytes_to_h2(w0, 0x5140);
-          a[h][1] = bytes_to_h2(w0, 0x7362);
-          a[h][2] = bytes_to_h2(w1, 0x5140);
-          a[h][3] = bytes_to_h2(w1, 0x7362);
+          for (int h = 0; h < 2; h++) {
+            const uint32_t w0 = kv.K[q][h][c].x ^ 0x80808080u, w1 = kv.K[q][h][c].y ^ 0x80808080u;
+            a[h][0] = bytes_to_h2(w0, 0x5140);
+            a[h][1] = bytes_to_h2(w0, 0x7362);
+            a[h][2] = bytes_to_h2(w1, 0x5140);
+            a[h][3] = bytes_to_h2(w1, 0x7362);
+          }
+          const float s0 = __half2float(__ushort_as_half((uint16_t)(c & 1 ? kv.dk[q][0][c / 2] >> 16 : kv.dk[q][0][c / 2])));
+          const float s1 = __half2float(__ushort_as_half((uint16_t)(c & 1 ? kv.dk[q][1][c / 2] >> 16 : kv.dk[q][1][c / 2])));
+#pragma unroll
+          for (int n = 0; n < NR; n++) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            mma16816(s, a[0][0], a[1][0], a[0][1], a[1][1], ql[n][c][0], ql[n][c][1]);
+            mma16816(s, a[0][2], a[1][2], a[0][3], a[1][3], ql[n][c][2], ql[n][c][3]);
+            mma16816(s, a[0][0], a[1][0], a[0][1], a[1][1], qh[n][c][0], qh[n][c][1]);
+            mma16816(s, a[0][2], a[1][2], a[0][3], a[1][3], qh[n][c][2], qh[n][c][3]);
+            x[q][n][0] = __fmaf_rn(s[0], s0, x[q][n][0]);
+            x[q][n][1] = __fmaf_rn(s[1], s0, x[q][n][1]);
+            x[q][n][2] = __fmaf_rn(s[2], s1, x[q][n][2]);
+            x[q][n][3] = __fmaf_rn(s[3], s1, x[q][n][3]);
+          }
         }
-        const float s0 = __half2float(__ushort_as_half((uint16_t)(c & 1 ? dk[q][0][c / 2] >> 16 : dk[q][0][c / 2])));
-        const float s1 = __half2float(__ushort_as_half((uint16_t)(c & 1 ? dk[q][1][c / 2] >> 16 : dk[q][1][c / 2])));
+      } else {
+        float s[NR][3][4];  // lo hi, hi lo, hi hi
 #pragma unroll
-        for (int n = 0; n < NR; n++) {
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16816(s, a[0][0], a[1][0], a[0][1], a[1][1], ql[n][c][0], ql[n][c][1]);
-          mma16816(s, a[0][2], a[1][2], a[0][3], a[1][3], ql[n][c][2], ql[n][c][3]);
-          mma16816(s, a[0][0], a[1][0], a[0][1], a[1][1], qh[n][c][0], qh[n][c][1]);
-          mma16816(s, a[0][2], a[1][2], a[0][3], a[1][3], qh[n][c][2], qh[n][c][3]);
-          x[q][n][0] = __fmaf_rn(s[0], s0, x[q][n][0]);
-          x[q][n][1] = __fmaf_rn(s[1], s0, x[q][n][1]);
-          x[q][n][2] = __fmaf_rn(s[2], s1, x[q][n][2]);
-          x[q][n][3] = __fmaf_rn(s[3], s1, x[q][n][3]);
-        }
+        for (int n = 0; n < NR; n++)
+#pragma unroll
+          for (int i = 0; i < 12; i++) s[n][i / 4][i % 4] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {  // dims 8t + 2e, 8t + 2e + 1 of the block
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) split_tf32(kv.K[q][i & 1][c][2 * e + (i >> 1)], h[i], l[i]);
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+              const uint2 bh = ((const uint2*)&sm.q[n][c][e >> 1][lane])[e & 1], bl = ((const uint2*)&sm.q[n][c][2 + (e >> 1)][lane])[e & 1];
+              mma1688(s[n][0], l, bh.x, bh.y);
+              mma1688(s[n][1], h, bl.x, bl.y);
+              mma1688(s[n][2], h, bh.x, bh.y);
+            }
+          }
+#pragma unroll
+        for (int n = 0; n < NR; n++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) x[q][n][k] = __fadd_rn(s[n][2][k], __fadd_rn(s[n][0][k], s[n][1][k]));
       }
     }
     // ---- masks, maxima
     uint32_t seen[PT][NR];  // bit k: x[..][k] is attended to
     float fac[NR][2];
-    uint32_t top = 0;  // the values' largest scale
+    int En = 13;
+    if constexpr (Q8) {
+      uint32_t top = 0;  // the values' largest scale
 #pragma unroll
-    for (int q = 0; q < PT; q++)
+      for (int q = 0; q < PT; q++)
 #pragma unroll
-      for (int h = 0; h < 2; h++)
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int i = 0; i < ND; i++) top = max(top, max(dv[q][h][i] & 0x7fffu, (dv[q][h][i] >> 16) & 0x7fffu));
-    const int En = max((int)(__reduce_max_sync(0xffffffffu, top) >> 10), 1) - 15;
+          for (int i = 0; i < FewCache<D, Q8>::ND; i++) top = max(top, max(kv.dv[q][h][i] & 0x7fffu, (kv.dv[q][h][i] >> 16) & 0x7fffu));
+      En = max((int)(__reduce_max_sync(0xffffffffu, top) >> 10), 1) - 15;
+    }
 #pragma unroll
     for (int n = 0; n < NR; n++) {
       float mx[2] = {-INFINITY, -INFINITY};
@@ -249,7 +372,7 @@ __global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant_
         for (int s = 4; s < 32; s *= 2) mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], s));
         const float Mn = fmaxf(M[n][u], mx[u]), Mr = Mn == -INFINITY ? 0.0f : Mn;
         const float f = exp2_approx(__fsub_rn(M[n][u], Mr));
-        fac[n][u] = __fmul_rn(f, pow2f(E - En));
+        fac[n][u] = Q8 ? __fmul_rn(f, pow2f(E - En)) : f;
         l[n][u] = __fmul_rn(l[n][u], f);
         M[n][u] = Mn;
         // weights
@@ -264,50 +387,112 @@ __global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant_
       }
     }
     E = En;
-    const float unit = pow2f(13 - En);
     // ---- O = O fac + P V
+    if constexpr (Q8) {
+      const float unit = pow2f(13 - En);
 #pragma unroll
-    for (int n = 0; n < NR; n++)
+      for (int q = 0; q < PT; q++)
 #pragma unroll
-      for (int c = 0; c < NC; c++)
+        for (int c = 0; c < NC; c++) {
+          // V^T: dims 32c + 4g + e of positions 2t, 2t + 1 (v[0][e]) and 2t + 8, 2t + 9 (v[1][e])
+          uint32_t v[2][4];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+          for (int h = 0; h < 2; h++) {
+            const uint32_t w0 = kv.V[q][2 * h][c] ^ 0x80808080u, w1 = kv.V[q][2 * h + 1][c] ^ 0x80808080u;
+            const uint32_t lo = __byte_perm(w0, w1, 0x5140), hi = __byte_perm(w0, w1, 0x7362);
+            v[h][0] = bytes_to_h2(lo, 0x4140);
+            v[h][1] = bytes_to_h2(lo, 0x4342);
+            v[h][2] = bytes_to_h2(hi, 0x4140);
+            v[h][3] = bytes_to_h2(hi, 0x4342);
+          }
+          const float s0 = __fmul_rn(__half2float(__ushort_as_half((uint16_t)(c & 1 ? kv.dv[q][0][c / 2] >> 16 : kv.dv[q][0][c / 2]))), unit);
+          const float s1 = __fmul_rn(__half2float(__ushort_as_half((uint16_t)(c & 1 ? kv.dv[q][1][c / 2] >> 16 : kv.dv[q][1][c / 2]))), unit);
 #pragma unroll
-          for (int k = 0; k < 4; k++) acc[n][c][i][k] = __fmul_rn(acc[n][c][i][k], fac[n][k & 1]);
+          for (int n = 0; n < NR; n++) {
+            float w[4];
 #pragma unroll
-    for (int q = 0; q < PT; q++)
+            for (int k = 0; k < 4; k++) w[k] = (seen[q][n] >> k) & 1u ? __fmul_rn(x[q][n][k], k < 2 ? s0 : s1) : 0.0f;
+            const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+            const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+            const uint32_t b0 = transpose8x8(h2_bits(h0)), b1 = transpose8x8(h2_bits(h1));
+            const uint32_t c0 = transpose8x8(h2_bits(__floats2half2_rn(__fsub_rn(w[0], f0.x), __fsub_rn(w[1], f0.y))));
+            const uint32_t c1 = transpose8x8(h2_bits(__floats2half2_rn(__fsub_rn(w[2], f1.x), __fsub_rn(w[3], f1.y))));
 #pragma unroll
-      for (int c = 0; c < NC; c++) {
-        // V^T: dims 32c + 4g + e of positions 2t, 2t + 1 (v[0][e]) and 2t + 8, 2t + 9 (v[1][e])
-        uint32_t v[2][4];
+            for (int i = 0; i < 2; i++) {
+              // (a sum of its own for every 16 positions: the MMA cuts what it accumulates, and
+              // one-signed, 4e-6 of the result over 2000 positions a warp)
+              float o[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(o, v[0][2 * i], v[0][2 * i + 1], v[1][2 * i], v[1][2 * i + 1], c0, c1);
+              mma16816(o, v[0][2 * i], v[0][2 * i + 1], v[1][2 * i], v[1][2 * i + 1], b0, b1);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t w0 = V[q][2 * h][c] ^ 0x80808080u, w1 = V[q][2 * h + 1][c] ^ 0x80808080u;
-          const uint32_t lo = __byte_perm(w0, w1, 0x5140), hi = __byte_perm(w0, w1, 0x7362);
-          v[h][0] = bytes_to_h2(lo, 0x4140);
-          v[h][1] = bytes_to_h2(lo, 0x4342);
-          v[h][2] = bytes_to_h2(hi, 0x4140);
-          v[h][3] = bytes_to_h2(hi, 0x4342);
-        }
-        const float s0 = __fmul_rn(__half2float(__ushort_as_half((uint16_t)(c & 1 ? dv[q][0][c / 2] >> 16 : dv[q][0][c / 2]))), unit);
-        const float s1 = __fmul_rn(__half2float(__ushort_as_half((uint16_t)(c & 1 ? dv[q][1][c / 2] >> 16 : dv[q][1][c / 2]))), unit);
-#pragma unroll
-        for (int n = 0; n < NR; n++) {
-          float w[4];
-#pragma unroll
-          for (int k = 0; k < 4; k++) w[k] = (seen[q][n] >> k) & 1u ? __fmul_rn(x[q][n][k], k < 2 ? s0 : s1) : 0.0f;
-          const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
-          const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-          const uint32_t b0 = transpose8x8(h2_bits(h0)), b1 = transpose8x8(h2_bits(h1));
-          const uint32_t c0 = transpose8x8(h2_bits(__floats2half2_rn(__fsub_rn(w[0], f0.x), __fsub_rn(w[1], f0.y))));
-          const uint32_t c1 = transpose8x8(h2_bits(__floats2half2_rn(__fsub_rn(w[2], f1.x), __fsub_rn(w[3], f1.y))));
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            mma16816(acc[n][c][i], v[0][2 * i], v[0][2 * i + 1], v[1][2 * i], v[1][2 * i + 1], c0, c1);
-            mma16816(acc[n][c][i], v[0][2 * i], v[0][2 * i + 1], v[1][2 * i], v[1][2 * i + 1], b0, b1);
+              for (int k = 0; k < 4; k++)
+                acc[n][c][i][k] = q == 0 ? __fmaf_rn(acc[n][c][i][k], fac[n][k & 1], o[k]) : __fadd_rn(acc[n][c][i][k], o[k]);
+            }
           }
         }
+    } else {
+#pragma unroll
+      for (int q = 0; q < PT; q++) {
+        // positions whose values are not all finite
+        uint32_t bad = 0;
+#pragma unroll
+        for (int h = 0; h < 4; h++) {
+          float z = 0.0f;
+#pragma unroll
+          for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) z = __fmaf_rn(kv.V[q][h][c][e], 0.0f, z);
+          if (z != 0.0f) bad |= 1u << (2 * t + (h & 1) + 4 * (h & 2));
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        if (bad) {
+#pragma unroll
+          for (int h = 0; h < 4; h++)
+            if (bad >> (2 * t + (h & 1) + 4 * (h & 2)) & 1u)
+#pragma unroll
+              for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) kv.V[q][h][c][e] = 0.0f;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {  // positions 8h .. 8h + 7
+          uint32_t wh[NR][2], wl[NR][2];  // weights of positions 8h + 2t, 8h + 2t + 1, row g
+#pragma unroll
+          for (int n = 0; n < NR; n++) {
+            float w[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+              w[u] = (seen[q][n] >> (2 * h + u)) & 1u ? x[q][n][2 * h + u] : 0.0f;
+              if (bad && (bad >> (8 * h + g) & 1u) && ((seen[q][n] >> (2 * h + u)) & 1u)) w[u] = __int_as_float(0x7fffffff);
+            }
+            const uint32_t a = __float_as_uint(w[0]), b = __float_as_uint(w[1]);
+            const uint32_t top = transpose8x8(__byte_perm(a, b, 0x7632)), low = transpose8x8(__byte_perm(a, b, 0x5410));
+            split_tf32(__uint_as_float(__byte_perm(low, top, 0x5410)), wh[n][0], wl[n][0]);
+            split_tf32(__uint_as_float(__byte_perm(low, top, 0x7632)), wh[n][1], wl[n][1]);
+          }
+#pragma unroll
+          for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              uint32_t vh[4], vl[4];
+#pragma unroll
+              for (int k = 0; k < 4; k++) split_tf32(kv.V[q][2 * h + (k >> 1)][c][2 * i + (k & 1)], vh[k], vl[k]);
+#pragma unroll
+              for (int n = 0; n < NR; n++) {
+                // (a sum of its own for every eight positions: the MMA cuts what it
+                // accumulates, and one-signed; over 2000 positions that was 2e-5)
+                float o[4] = {0.f, 0.f, 0.f, 0.f};
+                mma1688(o, vl, wh[n][0], wh[n][1]);
+                mma1688(o, vh, wl[n][0], wl[n][1]);
+                mma1688(o, vh, wh[n][0], wh[n][1]);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                  acc[n][c][i][k] = q == 0 && h == 0 ? __fmaf_rn(acc[n][c][i][k], fac[n][k & 1], o[k]) : __fadd_rn(acc[n][c][i][k], o[k]);
+              }
+            }
+        }
       }
+    }
   }
   // ---- the CTA's warps
 #pragma unroll
@@ -379,12 +564,12 @@ __global__ void __launch_bounds__(kFewNT) attn_few_kernel(const __grid_constant_
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <int D, int NR>
+template <int D, int NR, bool Q8>
 cudaError_t launch_few(const TreeAttnParams& p, cudaStream_t s) {
   TreeSplit sp{};
   sp.R = p.T * (p.H / p.HKV);
   sp.RG = (sp.R + 8 * NR - 1) / (8 * NR);
-  const int64_t n_kv = (int64_t)p.n_past + p.T, steps = (n_kv + kFewStep<D> - 1) / kFewStep<D>;
+  const int64_t n_kv = (int64_t)p.n_past + p.T, steps = (n_kv + kFewStep<D, Q8> - 1) / kFewStep<D, Q8>;
   // one cluster where it holds every step; else clusters of 8 (fewer where a KV
   // head's share of the GPU has no room for them), as many as run at once
   int cluster = 1;
@@ -403,7 +588,7 @@ cudaError_t launch_few(const TreeAttnParams& p, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(sp.S * cluster), (unsigned)p.HKV, (unsigned)sp.RG);
   cfg.blockDim = dim3(kFewNT);
-  cfg.dynamicSmemBytes = sizeof(FewSmem<D, NR>);
+  cfg.dynamicSmemBytes = sizeof(FewSmem<D, NR, Q8>);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -411,39 +596,47 @@ cudaError_t launch_few(const TreeAttnParams& p, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_few_kernel<D, NR>, p, sp, cluster);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_few_kernel<D, NR, Q8>, p, sp, cluster);
   if (e != cudaSuccess || sp.S == 1) return e;
   return launch_tree_join<D>(p, sp, s);
 }
 
-template <int D, int NR>
+template <int D, int NR, bool Q8>
 cudaError_t prepare_few() {
-  cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(FewSmem<D, NR>));
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_few_kernel<D, NR>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<D, NR, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(FewSmem<D, NR, Q8>));
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_few_kernel<D, NR, Q8>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   return e;
+}
+
+template <int D>
+cudaError_t prepare_few_of() {
+  cudaError_t e = prepare_few<D, 1, true>();
+  if (e == cudaSuccess) e = prepare_few<D, 2, true>();
+  if (e == cudaSuccess) e = prepare_few<D, 1, false>();
+  return e == cudaSuccess ? prepare_few<D, 2, false>() : e;
+}
+template <int D>
+cudaError_t launch_few_of(const TreeAttnParams& p, cudaStream_t s) {
+  const bool one = p.T * (p.H / p.HKV) <= 8;
+  if (p.q8) return one ? launch_few<D, 1, true>(p, s) : launch_few<D, 2, true>(p, s);
+  return one ? launch_few<D, 1, false>(p, s) : launch_few<D, 2, false>(p, s);
 }
 
 }  // namespace
 
 cudaError_t prepare_attn_few_kernels() {
-  cudaError_t e = prepare_few<32, 1>();
-  if (e == cudaSuccess) e = prepare_few<32, 2>();
-  if (e == cudaSuccess) e = prepare_few<64, 1>();
-  if (e == cudaSuccess) e = prepare_few<64, 2>();
-  if (e == cudaSuccess) e = prepare_few<96, 1>();
-  if (e == cudaSuccess) e = prepare_few<96, 2>();
-  if (e == cudaSuccess) e = prepare_few<128, 1>();
-  if (e == cudaSuccess) e = prepare_few<128, 2>();
-  return e;
+  cudaError_t e = prepare_few_of<32>();
+  if (e == cudaSuccess) e = prepare_few_of<64>();
+  if (e == cudaSuccess) e = prepare_few_of<96>();
+  return e == cudaSuccess ? prepare_few_of<128>() : e;
 }
 
 cudaError_t launch_attn_few(const TreeAttnParams& p, cudaStream_t s) {
-  const bool one = p.T * (p.H / p.HKV) <= 8;
   switch (p.D) {
-    case 32: return one ? launch_few<32, 1>(p, s) : launch_few<32, 2>(p, s);
-    case 64: return one ? launch_few<64, 1>(p, s) : launch_few<64, 2>(p, s);
-    case 96: return one ? launch_few<96, 1>(p, s) : launch_few<96, 2>(p, s);
-    case 128: return one ? launch_few<128, 1>(p, s) : launch_few<128, 2>(p, s);
+    case 32: return launch_few_of<32>(p, s);
+    case 64: return launch_few_of<64>(p, s);
+    case 96: return launch_few_of<96>(p, s);
+    case 128: return launch_few_of<128>(p, s);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -1087,19 +1087,26 @@ cudaError_t prepare_attn_tree_kernels() {
   return e;
 }
 
-// Whether attn_few.cu is the faster one for R rows of a KV head. Up to 8 rows it
+// Whether attn_few.cu is the faster one for R rows of a KV head. Q8_0: up to 8 rows it
 // always is (one token, us here / there: 4.8 / 9.7 at 500 positions, 11.3 / 18.5 at
 // 32000 with 14 / 2 heads of 64, 22.7 / 36.6 with 28 / 4 heads of 128); each further
 // 16 rows are another pass over the cache there, which 14 rows repay up to some
 // 16000 positions (16.1 / 18.3 at 8000, 46.4 / 36.7 at 32000, heads of 128) and 28
 // up to some 8000 of 64 dims (10.9 / 12.6 at 8000; heads of 128 19.7 / 19.0).
-static bool few_rows(int64_t R, int64_t n_kv, int64_t D) {
-  return R <= 8 || (R <= 16 && n_kv <= 16384) || (R <= 32 && n_kv * D <= (1 << 19));
+//
+// Over an F32 cache (28 / 4 heads of 128, 14 / 2 of 64 and 6 / 2 of 96): up to 8 rows
+// always (12.5 / 21.0 at 2000 positions of 128, 78 / 98 at 32000), up to 16 until the
+// one pass over the cache takes longer than the converters (29 / 36 at 8000, 114 / 98
+// at 32000), and with more passes while the cache is small (63 rows of 64 over 2000
+// 11.9 / 14.2, 91 rows 20.2 / 14.8; 126 rows of 128 over 100 16.7 / 22.2).
+static bool few_rows(bool q8, int64_t R, int64_t n_kv, int64_t HKV, int64_t D) {
+  if (q8) return R <= 8 || (R <= 16 && n_kv <= 16384) || (R <= 32 && n_kv * D <= (1 << 19));
+  return R <= 8 || (R <= 128 && (R + 15) / 16 * n_kv * HKV * D <= (R <= 16 ? 1 << 23 : R <= 64 ? 1 << 20 : 1 << 19));
 }
 
 cudaError_t launch_attn_tree(const TreeAttnParams& p, cudaStream_t s) {
   if (p.T == 0) return cudaSuccess;
-  if (p.q8 && few_rows((int64_t)p.T * (p.H / p.HKV), (int64_t)p.n_past + p.T, p.D)) return launch_attn_few(p, s);
+  if (few_rows(p.q8, (int64_t)p.T * (p.H / p.HKV), (int64_t)p.n_past + p.T, p.HKV, p.D)) return launch_attn_few(p, s);
   switch (p.D) {
     case 32: return p.q8 ? launch_tree<32, true>(p, s) : launch_tree<32, false>(p, s);
     case 64: return p.q8 ? launch_tree<64, true>(p, s) : launch_tree<64, false>(p, s);
