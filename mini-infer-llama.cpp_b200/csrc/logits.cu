@@ -17,9 +17,10 @@
 // history entry, 48 us.) The CTAs' winners meet in the first CTA's shared memory.
 // A row is one pass, 8 bytes per token.
 //
-// Bound by HBM for many rows (8.1 bytes per token of the vocabulary), by the
-// latency of the phases (history, dense pass, winners) for few: then a row takes
-// 16 CTAs instead of 8.
+// Bound for many rows by HBM (8.1 bytes per token of the vocabulary: 64 rows of 152064
+// without history or biases take 14 us, 5.6 TB/s) and by the phases before the dense
+// pass (4093 ids of history and 300 biases: 23 us), for few rows by the latency of all
+// phases.
 #include <algorithm>
 
 #include "mi_device.cuh"
@@ -28,14 +29,14 @@ namespace mi {
 
 namespace {
 
-constexpr int kLgMaxNT = 512;
+constexpr int kLgNT = 512;
 constexpr int kLgMaxCluster = 16;
 constexpr int kLgBias = 512;     // biases of a CTA's part that are kept in shared memory
 constexpr int kLgList = 2048;    // tokens of a part with a count or a bias that are listed
 constexpr int kLgAhead = 4;      // 16-byte pieces that a thread has under way
 
 // Count words: 16 bits, or 32 for histories that 15 bits do not count. The top bit
-// marks a token with a bias. add() and mark() tell whether the word was 0.
+// marks a token with a bias. add() and mark() give the word as it was.
 constexpr int64_t kLgNarrow = 32767;  // the longest history for 16-bit words
 template <bool WIDE>
 struct Counts;
@@ -43,11 +44,11 @@ template <>
 struct Counts<false> {
   static constexpr int bytes = 2;
   static constexpr uint32_t count = 0x7fffu, biased = 0x8000u;
-  static __device__ __forceinline__ bool add(uint32_t* w, int i) {
-    return (atomicAdd(w + (i >> 1), 1u << (16 * (i & 1))) >> (16 * (i & 1)) & 0xffffu) == 0;
+  static __device__ __forceinline__ uint32_t add(uint32_t* w, int i) {
+    return atomicAdd(w + (i >> 1), 1u << (16 * (i & 1))) >> (16 * (i & 1)) & 0xffffu;
   }
-  static __device__ __forceinline__ bool mark(uint32_t* w, int i) {
-    return (atomicOr(w + (i >> 1), biased << (16 * (i & 1))) >> (16 * (i & 1)) & 0xffffu) == 0;
+  static __device__ __forceinline__ uint32_t mark(uint32_t* w, int i) {
+    return atomicOr(w + (i >> 1), biased << (16 * (i & 1))) >> (16 * (i & 1)) & 0xffffu;
   }
   static __device__ __forceinline__ uint32_t word(const uint32_t* w, int i) { return ((const uint16_t*)w)[i]; }
   // bit k: whether word i + k is not 0 (i a multiple of 4)
@@ -61,30 +62,31 @@ template <>
 struct Counts<true> {
   static constexpr int bytes = 4;
   static constexpr uint32_t count = 0x7fffffffu, biased = 0x80000000u;
-  static __device__ __forceinline__ bool add(uint32_t* w, int i) { return atomicAdd(w + i, 1u) == 0; }
-  static __device__ __forceinline__ bool mark(uint32_t* w, int i) { return atomicOr(w + i, biased) == 0; }
+  static __device__ __forceinline__ uint32_t add(uint32_t* w, int i) { return atomicAdd(w + i, 1u); }
+  static __device__ __forceinline__ uint32_t mark(uint32_t* w, int i) { return atomicOr(w + i, biased); }
   static __device__ __forceinline__ uint32_t word(const uint32_t* w, int i) { return w[i]; }
   static __device__ __forceinline__ uint32_t any4(const uint32_t* w, int i) {
     const uint4 v = *(const uint4*)(w + i);
     return (v.x ? 1u : 0u) | (v.y ? 2u : 0u) | (v.z ? 4u : 0u) | (v.w ? 8u : 0u);
   }
 };
-constexpr int kLgSlice = 20480;  // tokens counted at a time (a multiple of 32)
+constexpr int kLgSlice = 40960;  // tokens counted at a time (a multiple of 32)
 
 struct LgSmem {
-  float cv[kLgMaxCluster], wv[kLgMaxNT / 32];
-  int32_t ci[kLgMaxCluster], wi[kLgMaxNT / 32];
-  int32_t bias_of[kLgMaxNT / 32];
+  float cv[kLgMaxCluster], wv[kLgNT / 32];
+  int32_t ci[kLgMaxCluster], wi[kLgNT / 32];
+  int32_t bias_of[kLgNT / 32];
   int32_t n_list;
   int32_t list[kLgList];
   int32_t bias_id[kLgBias];
   float bias[kLgBias];
 };
 
-// VEC: rows are 16-byte aligned, so four tokens a thread at a time. NT threads.
-template <int NT, bool WIDE, bool VEC>
-__global__ void __launch_bounds__(NT) logits_process_kernel(const LogitsParams p, const int cluster, const int slice) {
+// VEC: rows are 16-byte aligned, so four tokens a thread at a time.
+template <bool WIDE, bool VEC>
+__global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParams p, const int cluster, const int slice) {
   using C = Counts<WIDE>;
+  constexpr int NT = kLgNT;
   extern __shared__ __align__(16) uint32_t cnt[];
   __shared__ LgSmem sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -107,22 +109,29 @@ __global__ void __launch_bounds__(NT) logits_process_kernel(const LogitsParams p
     const int np = n / W;  // (VEC: V is a multiple of 4, and so is n)
     float f[kLgAhead][W];
     uint32_t a[kLgAhead];
+    // (loads only, from a place that is always there: a use or a branch between them
+    // made each wait for the one before it, 6 of 19 us for 64 rows with masks)
     auto load = [&](int i0) {
 #pragma unroll
       for (int u = 0; u < kLgAhead; u++) {
-        const int i = i0 + u * NT;
-        if (i >= np) continue;
+        const int i = min(i0 + u * NT, np - 1);
         if (VEC) {
           const float4 v = *(const float4*)(x + s0 + 4 * i);
           f[u][0] = v.x, f[u][W > 1 ? 1 : 0] = v.y, f[u][W > 2 ? 2 : 0] = v.z, f[u][W > 3 ? 3 : 0] = v.w;
         } else {
           f[u][0] = x[s0 + i];
         }
-        a[u] = allowed ? allowed[(s0 + W * i) >> 5] >> ((W * i) & 31) : 15u;
+        a[u] = allowed ? allowed[(s0 + W * i) >> 5] : ~0u;
       }
     };
     load(tid);
     if (special) {
+      int32_t h[8];
+      auto history = [&](int64_t i0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[e] = i0 + e * NT < p.n_hist ? hist[i0 + e * NT] : -1;
+      };
+      history(tid);
       for (int i = tid; i < (n * C::bytes + 15) / 16; i += NT) ((uint4*)cnt)[i] = make_uint4(0, 0, 0, 0);
       if (tid == 0) sm.n_list = 0;
       __syncthreads();
@@ -131,14 +140,16 @@ __global__ void __launch_bounds__(NT) logits_process_kernel(const LogitsParams p
         if (at < kLgList) sm.list[at] = u;
       };
       for (int64_t i0 = tid; i0 < p.n_hist; i0 += 8 * NT) {
-        int32_t h[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) h[e] = i0 + e * NT < p.n_hist ? hist[i0 + e * NT] : -1;
+        if (i0 != tid) history(i0);
+        uint32_t old[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const int64_t u = (int64_t)h[e] - s0;
-          if (u >= 0 && u < n && C::add(cnt, (int)u)) met((int)u);
+          old[e] = u >= 0 && u < n ? C::add(cnt, (int)u) : 1u;
         }
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (old[e] == 0) met((int)(h[e] - s0));
       }
       // the part's biases in the list's order; above kLgBias of them the caller's list is read
       int n_bias = 0;
@@ -155,7 +166,7 @@ __global__ void __launch_bounds__(NT) logits_process_kernel(const LogitsParams p
           all += sm.bias_of[w];
         }
         if (in) {
-          if (C::mark(cnt, (int)u)) met((int)u);
+          if (C::mark(cnt, (int)u) == 0) met((int)u);
           if (at < kLgBias) {
             sm.bias_id[at] = (int32_t)u;
             sm.bias[at] = p.bias[i];
@@ -206,7 +217,7 @@ __global__ void __launch_bounds__(NT) logits_process_kernel(const LogitsParams p
         if (special) skip = VEC ? C::any4(cnt, 4 * i) : (C::word(cnt, i) ? 1u : 0u);
 #pragma unroll
         for (int k = 0; k < W; k++) {
-          if (!((a[u] >> k) & 1u)) f[u][k] = -INFINITY;
+          if (!((a[u] >> ((j + k) & 31)) & 1u)) f[u][k] = -INFINITY;
           if (f[u][k] > best && !((skip >> k) & 1u)) best = f[u][k], best_i = j + k;
         }
         if (VEC && skip == 0) {
@@ -255,11 +266,11 @@ __global__ void __launch_bounds__(NT) logits_process_kernel(const LogitsParams p
   }
 }
 
-template <int NT, bool WIDE, bool VEC>
+template <bool WIDE, bool VEC>
 cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, int cluster, int slice, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_rows * cluster));
-  cfg.blockDim = dim3(NT);
+  cfg.blockDim = dim3(kLgNT);
   cfg.dynamicSmemBytes = p.n_hist || p.n_bias ? (size_t)slice * Counts<WIDE>::bytes : 0;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -268,51 +279,41 @@ cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, int cluster, in
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, logits_process_kernel<NT, WIDE, VEC>, p, cluster, slice);
+  return cudaLaunchKernelEx(&cfg, logits_process_kernel<WIDE, VEC>, p, cluster, slice);
 }
 
-template <int NT, bool WIDE, bool VEC>
+template <bool WIDE, bool VEC>
 cudaError_t prepare_logits() {
-  cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<NT, WIDE, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        kLgSlice * Counts<WIDE>::bytes);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(logits_process_kernel<NT, WIDE, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   return e;
-}
-
-template <int NT>
-cudaError_t prepare_nt() {
-  cudaError_t e = prepare_logits<NT, false, false>();
-  if (e == cudaSuccess) e = prepare_logits<NT, false, true>();
-  if (e == cudaSuccess) e = prepare_logits<NT, true, false>();
-  if (e == cudaSuccess) e = prepare_logits<NT, true, true>();
-  return e;
-}
-
-template <int NT>
-cudaError_t launch_nt(const LogitsParams& p, int64_t n_rows, int cluster, cudaStream_t s) {
-  const int64_t per = ((p.n_vocab + cluster - 1) / cluster + 31) / 32 * 32;
-  const int slice = (int)std::min<int64_t>(per, kLgSlice);
-  const bool vec = ((uintptr_t)p.logits | (uintptr_t)p.out) % 16 == 0 && p.stride % 4 == 0 && p.n_vocab % 4 == 0;
-  if (p.n_hist <= kLgNarrow)
-    return vec ? launch_logits<NT, false, true>(p, n_rows, cluster, slice, s) : launch_logits<NT, false, false>(p, n_rows, cluster, slice, s);
-  return vec ? launch_logits<NT, true, true>(p, n_rows, cluster, slice, s) : launch_logits<NT, true, false>(p, n_rows, cluster, slice, s);
 }
 
 }  // namespace
 
-// (clusters of 16 CTAs need an attribute; per device, at init)
+// (the counts' shared memory and clusters of 16 CTAs need attributes; per device, at init)
 cudaError_t prepare_logits_kernels() {
-  const cudaError_t e = prepare_nt<256>();
-  return e == cudaSuccess ? prepare_nt<512>() : e;
+  cudaError_t e = prepare_logits<false, false>();
+  if (e == cudaSuccess) e = prepare_logits<false, true>();
+  if (e == cudaSuccess) e = prepare_logits<true, false>();
+  return e == cudaSuccess ? prepare_logits<true, true>() : e;
 }
 
-// Few rows: 16 CTAs of 512 threads a row (one row of 151936: 7.3 us). As soon as
-// those do not all run at once (64 rows: two waves, 39 us), 8 CTAs of 256, of which
-// an SM holds four.
+// CTAs of a row: 16 while the rows are few, 8, and 4 where all of them still run at
+// once (us for 4 / 13 / 24 / 64 rows of 152000: 7.5 / 10.0 / 18.2 / 50.1 with 16,
+// 9.0 / 9.1 / 12.4 / 29.4 with 8, 11.6 / 11.9 / 12.0 / 22.7 with 4; every CTA of a row
+// reads all of its history).
 cudaError_t launch_logits_process(const LogitsParams& p, int64_t n_rows, cudaStream_t s) {
   if (n_rows == 0) return cudaSuccess;
-  return n_rows * 16 <= 148 ? launch_nt<512>(p, n_rows, 16, s) : launch_nt<256>(p, n_rows, 8, s);
+  const int cluster = n_rows <= 6 ? 16 : n_rows <= 20 ? 8 : 4;
+  const int64_t per = ((p.n_vocab + cluster - 1) / cluster + 31) / 32 * 32;
+  const int slice = (int)std::min<int64_t>(per, kLgSlice);
+  const bool vec = ((uintptr_t)p.logits | (uintptr_t)p.out) % 16 == 0 && p.stride % 4 == 0 && p.n_vocab % 4 == 0;
+  if (p.n_hist <= kLgNarrow)
+    return vec ? launch_logits<false, true>(p, n_rows, cluster, slice, s) : launch_logits<false, false>(p, n_rows, cluster, slice, s);
+  return vec ? launch_logits<true, true>(p, n_rows, cluster, slice, s) : launch_logits<true, false>(p, n_rows, cluster, slice, s);
 }
 
 }  // namespace mi
