@@ -267,11 +267,14 @@ int mi_cuda_kv_read_q8_0(const void* d_cache_k, const void* d_cache_v, int64_t h
  * [n_head][head_dim], rotated. Token i attends to rows [0, n_past) and to row
  * n_past + j where bit j (bit j % 32 of word j / 32) of its mask row is set; d_mask
  * is [n_tokens][ceil(n_tokens / 32)] words, NULL for causal (j <= i). A token that
- * attends to nothing gives zeros; what masked rows and rows from n_past + n_tokens
- * on hold is never used. n_tokens = 1 is the single-token form. head_dim 32, 64, 96
- * or 128, n_head a multiple of n_head_kv, at most 4096. d_scratch holds mi_cuda_attention_tree_scratch_bytes() bytes
- * (those for a larger n_kv = n_past + n_tokens or n_tokens are enough too) and belongs to this call until it has run;
- * caches and scratch 16-byte aligned. dst [n_tokens][n_head][head_dim].
+ * attends to nothing gives zeros; one that attends to a row with an infinity or a
+ * NaN gives NaN there (in some or all values of that head). What masked rows and rows
+ * from n_past + n_tokens on hold is never used. n_tokens = 1 is the single-token form.
+ * head_dim 32, 64, 96 or 128, n_head a multiple of n_head_kv, at most 4096. d_scratch
+ * holds mi_cuda_attention_tree_scratch_bytes() bytes (those for a larger n_kv = n_past
+ * + n_tokens or n_tokens are enough too) and belongs to this call until it has run
+ * (two captured graphs that may run at once need one each); caches and scratch 16-byte
+ * aligned. dst [n_tokens][n_head][head_dim].
  * mi_cuda_attention_tree reads F32 caches [n_ctx][n_head_kv][head_dim],
  * mi_cuda_attention_tree_q8_0 caches of mi_cuda_kv_append_q8_0. */
 size_t mi_cuda_attention_tree_scratch_bytes(int64_t n_head, int64_t n_head_kv, int64_t n_kv, int64_t n_tokens,

@@ -554,6 +554,59 @@ def test_attention_tree_same_from_call_to_call_and_over_batches(torch):
     assert torch.equal(first, tree(torch, True, q, caches, HKV, n_ctx, past, 0.125))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("H,HKV,D,T,past,bad", [(14, 2, 64, 2, 70, math.inf), (28, 4, 128, 1, 200, -math.inf), (6, 2, 96, 9, 30, math.nan),
+                                                (14, 2, 64, 40, 300, math.inf), (17, 1, 32, 20, 129, math.nan)])
+def test_attention_tree_values_that_are_not_finite(torch, q8, H, HKV, D, T, past, bad):
+    """An infinity or a NaN in a value row: NaN for the tokens that attend to it, nothing for the others."""
+    q, caches, _, n_ctx = attn_inputs(torch, T, H, HKV, D, past, T, False)
+    k, v = (x.clone() for x in caches)
+    v[past + T - 1, HKV - 1, 1] = bad  # (the last token's own row)
+    if q8:
+        caches = [mi_cuda.kv_q8_0_cache(n_ctx, HKV, D) for _ in range(2)]
+        mi_cuda.kv_append_q8_0(k, v, *caches, n_ctx)
+        rows = mi_cuda.kv_read_q8_0(*caches, HKV, D, n_ctx, 0, past + T)
+    else:
+        caches, rows = (k, v), (k[: past + T], v[: past + T])
+    got = tree(torch, q8, q, caches, HKV, n_ctx, past, 0.125).unflatten(1, (HKV, -1))
+    assert torch.isnan(got[-1, -1]).any(-1).all()
+    clean = torch.where(torch.isfinite(rows[1]), rows[1], 0.0)
+    want, tol = attn_f64(torch, q, rows[0], clean, seen_of(torch, None, T, past), 0.125)
+    want = want.unflatten(1, (HKV, -1))
+    assert T == 1 or float((got[:-1].double() - want[:-1]).abs().max()) <= tol
+    assert HKV == 1 or float((got[:, :-1].double() - want[:, :-1]).abs().max()) <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,HKV,D,T,past", [(14, 2, 64, 40, 3000), (28, 4, 128, 20, 900), (40, 1, 32, 9, 2000)])
+def test_attention_tree_two_at_once(torch, H, HKV, D, T, past):
+    """Calls on two streams, each with its own scratch, and a replayed graph beside an eager call."""
+    sets = [attn_inputs(torch, T, H, HKV, D, past, seed, True) for seed in (1, 2)]
+    scratch = [mi_cuda.attention_tree_scratch(H, HKV, past + T, T, D) for _ in sets]
+    call = lambda i: tree(torch, True, sets[i][0], sets[i][1], HKV, sets[i][3], past, 0.125, scratch=scratch[i])  # noqa: E731
+    want = [call(0).clone(), call(1).clone()]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        out = call(0)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        graph.replay()
+        with torch.cuda.stream(streams[1]):
+            other = call(1)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[0]) and torch.equal(other, want[1])
+
+
 def check_logits(torch, x, out, tokens, hist, repeat, freq, pres, ids, bias, allowed):
     for i in range(x.shape[0]):
         h = hist[i] if hist.ndim == 2 else hist
@@ -597,6 +650,20 @@ def test_logits_process(torch, n, V, nh, nb, mask, form):
         Y = X.clone()
         o2, t2 = mi_cuda.logits_process(Y, hist=H, out=Y, **kw)
         assert o2 is Y and torch.equal(o2.view(torch.int32), out.view(torch.int32)) and torch.equal(t2, tok)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [6, 7, 20, 21, 40])
+@pytest.mark.parametrize("V", [3001, 40004, 200000])
+def test_logits_process_numbers_of_rows(torch, n, V):
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal((n, V)) * 4).astype(np.float32)
+    hist = rng.integers(0, V, (n, 700)).astype(np.int32)
+    hist[:, ::3] = hist[:, :1]
+    allowed = rng.integers(0, 2**32, (n, (V + 31) // 32), dtype=np.uint64).astype(np.uint32)
+    out, tok = mi_cuda.logits_process(torch.from_numpy(x).cuda(), hist=torch.from_numpy(hist).cuda(), repeat=1.15, frequency=0.3,
+                                      presence=-0.2, allowed=torch.from_numpy(allowed.view(np.int32)).cuda())
+    check_logits(torch, x, out, tok, hist, 1.15, 0.3, -0.2, None, None, allowed)
 
 
 @pytest.mark.gpu
