@@ -71,6 +71,7 @@ constexpr int kTrParts = 4;      // softmax threads per row: 32 positions each, 
 constexpr int kTrRows = 128;     // rows per CTA (MMA M)
 constexpr int kTrWarpK = 16, kTrWarpV = 20, kTrWarpMma = 24;
 constexpr int kTrThreads = 28 * 32;  // (the last three warps complete the MMA warp's group for setmaxnreg)
+constexpr int kTrChunk = 16;     // F32: rows of a cache that are copied at a time
 constexpr int kTrSlots = 8;      // steps whose exponents are kept (see the roles' waits)
 constexpr uint32_t kTrCols = 512;  // all of TMEM: its base is 0
 constexpr uint32_t kTmem = 0;
@@ -81,19 +82,24 @@ constexpr uint32_t kColS = 0, kColP = 128, kColO = 256, kColQ = 384;
 constexpr int kRegsSoftmax = 88, kRegsConvert = 56, kRegsMma = 40;
 
 // PAIR: two CTAs share the products' B operand.
-template <int D, bool PAIR>
+template <int D, bool Q8, bool PAIR>
 struct TrSmem {
-  static constexpr int n_k = 2, n_v = PAIR || D <= 64 ? 2 : 1;  // steps whose planes there is room for
+  // steps whose planes there is room for
+  static constexpr int n_v = PAIR || D <= 64 ? 2 : 1, n_k = Q8 ? 2 : n_v;
   static constexpr int plane = kTrTile * D * 2 / (PAIR ? 2 : 1);  // of a CTA's share of the keys or the values
   static constexpr int k = 0;                      // [step % n_k][hi, lo]; at the end float [128][D + 4], the rows' records
   static constexpr int v = k + n_k * 2 * plane;    // [step % n_v][hi, lo]; before the first step the queries
-  static constexpr int col = v + n_v * 2 * plane;  // float [kTrSlots][half][3][64]: key factor, value exponent, the same where finite
-  static constexpr int info = col + kTrSlots * 2 * 3 * kTrHalf * 4;  // float [kTrSlots][half][4]: key factor, whether the positions have
+  static constexpr int col = v + n_v * 2 * plane;  // float [kTrSlots][half][2][64]: key factor, value exponent
+  static constexpr int info = col + kTrSlots * 2 * 2 * kTrHalf * 4;  // float [kTrSlots][half][4]: key factor, whether the positions have
                                                                      // their own, value exponent, whether they have their own
   static constexpr int ends = info + kTrSlots * 2 * 16;  // int2 [keys, values][step & 1][half][4 warps]: largest and least exponent
   static constexpr int mx = ends + 2 * 2 * 2 * 4 * 8;    // float [2][part][128]: the parts' maxima (at the end their sums)
-  static constexpr int bars = mx + 2 * kTrParts * kTrRows * 4;
-  static constexpr int n_bars = 2 * n_k + 2 * n_v + 2 * kTrSlots + 8;
+  // F32: rows as they are, in chunks of 16 (8 where there is room for them)
+  static constexpr int n_rows = Q8 ? 0 : D <= 96 ? 8 : 5, pitch = D + 4;  // chunks of each cache; floats between rows (a
+                                                                         // column of eight rows in all banks)
+  static constexpr int rows = mx + 2 * kTrParts * kTrRows * 4;           // float [keys, values][n_rows][16][pitch]
+  static constexpr int bars = rows + 2 * n_rows * kTrChunk * pitch * 4;
+  static constexpr int n_bars = 2 * n_k + 2 * n_v + 2 * kTrSlots + 8 + 4 * n_rows;
   static constexpr int misc = bars + n_bars * 8;   // TMEM base, abort flag
   static constexpr int used = misc + 16;
   // above half of an SM's shared memory: two CTAs must not share its TMEM
@@ -220,25 +226,6 @@ __device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// A cached row of floats held by four lanes (lane bits 3 and 4), N values each: the
-// exponent e that brings its largest magnitude to [2^14, 2^15) as 2^(14 - e), or
-// false where the row holds an infinity or a NaN. Rows below 2^-100 keep e = -100:
-// their halves lose bits below 2^-138, nothing that a float sum of products shows.
-template <int N>
-__device__ __forceinline__ bool row_exponent(const float* x, int& e) {
-  float m = 0.0f;
-  bool fine = true;
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    m = fmaxf(m, fabsf(x[i]));
-    fine &= fabsf(x[i]) <= 3.402823466e38f;
-  }
-  if (!fine) m = INFINITY;
-  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-  e = max((int)(__float_as_uint(m) >> 23) - 127, -100);
-  return m <= 3.402823466e38f;
-}
 // A CTA's share of one cache (keys or values) of one KV head, by four warps: of a
 // step's 128 positions NK * 4 row groups of eight, of their dims CH pieces of eight
 // (all of both by itself; in a pair half the groups of the keys, half the pieces of
@@ -248,13 +235,10 @@ __device__ __forceinline__ bool row_exponent(const float* x, int& e) {
 //
 // The exponent of a row (planes = row * 2^-e brings it to fp16's range) is that of
 // its largest scale, or for F32 of its largest value.
-template <int D, bool Q8, int NK, int CH>
-struct KvRows;
-
 // Q8_0: two of a warp's rows are in registers; a row that has been converted makes
 // room for the one after the next.
 template <int D, int NK, int CH>
-struct KvRows<D, true, NK, CH> {
+struct KvRows {
   static constexpr int NC = D / 32, ND = (NC + 1) / 2, NI = (CH + 3) / 4;
   uint2 q[2][NI];
   uint32_t d[2][ND];    // two scales a word
@@ -307,7 +291,7 @@ struct KvRows<D, true, NK, CH> {
   // (least is -2000 where a row has a NaN scale); those of rows that have their own
   // go to put(half, position in it, exponent, whether it is no NaN).
   template <class Own, class Put>
-  __device__ __forceinline__ void exponents(int at, int w, int lane, int2*, int, int (&most)[2], bool (&own)[2], Own judge, Put put) {
+  __device__ __forceinline__ void exponents(int at, int w, int lane, int (&most)[2], bool (&own)[2], Own judge, Put put) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       bool bad = false;
@@ -384,115 +368,6 @@ struct KvRows<D, true, NK, CH> {
   }
 };
 
-// F32: a step's rows would take too many registers; they are read for their
-// exponents (all of them) and again for their planes.
-template <int D, int NK, int CH>
-struct KvRows<D, false, NK, CH> {
-  static constexpr int NC = D / 32, NI = (CH + 3) / 4;
-  const float* rows;  // the head's, from this CTA's first position on
-  int64_t row, left;  // floats between positions; positions
-  int row0, ch0;
-
-  // pieces g + 4 i (i < N) of a row from `first` on, up to `end`
-  template <int N>
-  __device__ __forceinline__ void load_row(int pos, int first, int end, int lane, float (&x)[N * 8]) const {
-    const int g = lane >> 3;
-    const bool in = pos < left;
-    const float* src = rows + (int64_t)pos * row + 8 * (first + g);
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const bool here = in && first + g + 4 * i < end;
-      const float4 a = here ? *(const float4*)(src + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 b = here ? *(const float4*)(src + 32 * i + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      float* o = &x[8 * i];
-      o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
-    }
-  }
-  __device__ __forceinline__ void begin(const TreeAttnParams& p, const void* cache, int kvh, int64_t pos0, int64_t n_kv, int, int,
-                                        int first_row, int first_piece) {
-    row = (int64_t)p.HKV * D;
-    rows = (const float*)cache + pos0 * row + (int64_t)kvh * D;
-    left = n_kv - pos0;
-    row0 = first_row;
-    ch0 = first_piece;
-  }
-  // (as above; `ends` [half][4]: what the four warps found, met at barrier `id`, also
-  // by warps that have given up)
-  template <class Own, class Put>
-  __device__ __forceinline__ void exponents(int at, int w, int lane, int2* ends, int id, int (&most)[2], bool (&own)[2], Own judge,
-                                            Put put) const {
-    int e[4];
-    bool fine[4];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      bool bad = false;
-      int hi = -1000, lo = 1000;
-#pragma unroll
-      for (int k = 2 * h; k < 2 * h + 2; k++) {
-        float x[NC * 8];
-        load_row<NC>(at + (w + 4 * k) * 8 + (lane & 7), 0, D / 8, lane, x);
-        fine[k] = row_exponent<NC * 8>(x, e[k]);
-        bad |= !fine[k];
-        const bool any = e[k] > -100;
-        e[k] -= 14;
-        if (fine[k] && any) {
-          hi = max(hi, e[k]);
-          lo = min(lo, e[k]);
-        }
-      }
-      hi = __reduce_max_sync(0xffffffffu, hi);
-      lo = __reduce_min_sync(0xffffffffu, lo);
-      if (__any_sync(0xffffffffu, bad)) lo = -2000;
-      if (lane == 0) ends[h * 4 + w] = make_int2(hi, lo);
-    }
-    asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      int hi = -1000, lo = 1000;
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int2 o = ends[h * 4 + k];
-        hi = max(hi, o.x);
-        lo = min(lo, o.y);
-      }
-      most[h] = hi;
-      own[h] = judge(hi, lo);
-      if (own[h] && lane < 8) {
-#pragma unroll
-        for (int k = 0; k < 2; k++) put(h, (w + 4 * k) * 8 + lane, e[2 * h + k], fine[2 * h + k]);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(int at, uint8_t* planes, int w, int lane, const int (&most)[2], const bool (&own)[2]) const {
-    const int g = lane >> 3;
-#pragma unroll 1
-    for (int k = 0; k < NK; k++) {
-      const int in_step = row0 + (w + 4 * k) * 8 + (lane & 7);
-      const bool second = row0 + 32 * k >= kTrHalf;
-      int e = second ? most[1] : most[0];
-      bool fine = true;
-      if (second ? own[1] : own[0]) {
-        float x[NC * 8];
-        load_row<NC>(at + in_step, 0, D / 8, lane, x);
-        fine = row_exponent<NC * 8>(x, e);
-        e -= 14;
-      }
-      float x[NI * 8];
-      load_row<NI>(at + in_step, ch0, ch0 + CH, lane, x);
-      uint8_t* dst = planes + (w + 4 * k) * (CH * 128) + g * 128 + (lane & 7) * 16;
-#pragma unroll
-      for (int i = 0; i < NI; i++) {
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (fine) split8(&x[8 * i], pow2f(-e), hi, lo);
-        if (CH % 4 == 0 || g + 4 * i < CH) {
-          *(uint4*)(dst + i * 512) = hi;
-          *(uint4*)(dst + NK * 4 * CH * 128 + i * 512) = lo;
-        }
-      }
-    }
-  }
-};
-
 // What a converting warp needs of its CTA.
 struct TrConvert {
   int64_t pos0, n_kv;
@@ -503,44 +378,52 @@ struct TrConvert {
   uint64_t *empty, *col_full;
   uint32_t full;    // shared::cluster address of the issuing CTA's barriers
   float *col, *info;
-  int2* ends;
   volatile int* abort_flag;
+  // F32
+  float* rows;      // [n_rows][kTrChunk][D + 4]
+  uint64_t *rows_full, *rows_empty;
+  int2* ends;       // [step & 1][half][4 warps]: largest and least exponent
 };
+
+// Where 64 positions have magnitudes too far apart for one exponent (or one that is
+// not finite).
+__device__ __forceinline__ bool too_far_apart(int hi, int lo) { return lo < 1000 && hi - lo > 10; }
+
+// One position's own exponent.
+template <bool IS_V>
+__device__ __forceinline__ void put_own(const TrConvert& r, int slot, int half, int at, int e, bool fine) {
+  float* c = r.col + (slot * 2 + half) * 2 * kTrHalf;
+  const float nan = __int_as_float(0x7fffffff);
+  if (IS_V) c[kTrHalf + at] = fine ? (float)e : nan;
+  else c[at] = fine ? pow2f(e) : nan;
+}
+template <bool IS_V>
+__device__ __forceinline__ void put_info(const TrConvert& r, int slot, int half, int most, bool own) {
+  if (r.w == 0 && r.lane == 0)
+    *(float2*)(r.info + (slot * 2 + half) * 4 + (IS_V ? 2 : 0)) = make_float2(IS_V ? (float)most : pow2f(most), own ? 1.0f : 0.0f);
+}
 
 // The keys (or values) of every step. A step's exponents go out before its planes,
 // which wait for the products that read the planes there before. Their slot is
 // written again eight steps later: after the planes of seven, for which the scores of
 // five were done, for which the softmax had read those of four, and so had long left
 // the step itself.
-template <int D, bool Q8, bool PAIR, bool IS_V>
-__device__ __forceinline__ void convert_role(const TreeAttnParams& p, const TrConvert& r, uint64_t* queries_done, bool wait_queries) {
+template <int D, bool PAIR, bool IS_V>
+__device__ __forceinline__ void convert_q8_0(const TreeAttnParams& p, const TrConvert& r, uint64_t* queries_done, bool wait_queries) {
   constexpr int NK = PAIR && !IS_V ? 2 : 4, CH = PAIR && IS_V ? D / 16 : D / 8, plane = NK * 4 * CH * 128;
-  KvRows<D, Q8, NK, CH> kv;
+  KvRows<D, NK, CH> kv;
   kv.begin(p, r.cache, r.kvh, r.pos0, r.n_kv, r.w, r.lane, PAIR && !IS_V ? r.rank * kTrHalf : 0, PAIR && IS_V ? r.rank * CH : 0);
   bool ok = true;
   for (int j = 0; j < r.n; j++) {
     const int slot = j & (kTrSlots - 1), b = j % r.buffers;
     int most[2];
     bool own[2];
-    kv.exponents(
-        j * kTrTile, r.w, r.lane, r.ends + (j & 1) * 8, IS_V ? 6 : 5, most, own, [](int hi, int lo) { return lo < 1000 && hi - lo > 10; },
-        [&](int h, int at, int e, bool fine) {
-          float* c = r.col + (slot * 2 + h) * 3 * kTrHalf;
-          const float nan = __int_as_float(0x7fffffff);
-          if (IS_V) {
-            c[kTrHalf + at] = fine ? (float)e : nan;
-            // (finite in every case: a masked position's weight is 0 whatever its row holds)
-            c[2 * kTrHalf + at] = fine ? (float)e : 0.0f;
-          } else {
-            c[at] = fine ? pow2f(e) : nan;
-          }
-        });
+    kv.exponents(j * kTrTile, r.w, r.lane, most, own, too_far_apart,
+                 [&](int h, int at, int e, bool fine) { put_own<IS_V>(r, slot, h, at, e, fine); });
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       if (most[h] < -999) most[h] = 0;  // (nothing but zeros)
-      if (r.w == 0 && r.lane == 0)
-        *(float2*)(r.info + (slot * 2 + h) * 4 + (IS_V ? 2 : 0)) =
-            make_float2(IS_V ? (float)most[h] : pow2f(most[h]), own[h] ? 1.0f : 0.0f);
+      put_info<IS_V>(r, slot, h, most[h], own[h]);
     }
     __syncwarp();
     if (r.lane < 2) mbar_arrive_one(&r.col_full[slot * 2 + r.lane]);
@@ -556,11 +439,147 @@ __device__ __forceinline__ void convert_role(const TreeAttnParams& p, const TrCo
   }
 }
 
+// The same from an F32 cache, whose rows the copying warps leave in shared memory,
+// 64 positions at a time: read there for their exponents, and again for their planes.
+// (Both times from global memory, a step took 15 us at D = 128, 5 times the softmax.)
+template <int D, bool PAIR, bool IS_V, int n_rows>
+__device__ __forceinline__ void convert_f32(const TreeAttnParams& p, const TrConvert& r, uint64_t* queries_done, bool wait_queries) {
+  constexpr int NK = PAIR && !IS_V ? 2 : 4, CH = PAIR && IS_V ? D / 16 : D / 8, plane = NK * 4 * CH * 128, pitch = D + 4;
+  const int ch0 = PAIR && IS_V ? r.rank * CH : 0, w = r.w, lane = r.lane, g = lane >> 3;
+  const int64_t left = r.n_kv - r.pos0;
+  bool ok = true;
+  for (int j = 0; j < r.n; j++) {
+    const int slot = j & (kTrSlots - 1), b = j % r.buffers;
+#pragma unroll 1
+    for (int h = 0; h < 2; h++) {
+      // row groups w + 4 k of the step, k = 2 h and 2 h + 1: half a chunk each
+      const float* src[2];
+      int e[2], hi = -1000, lo = 1000;
+      bool fine[2], in[2], bad = false;
+      uint64_t* done[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int k = 2 * h + u, c = j * (kTrTile / kTrChunk) + (w >> 1) + 2 * k, at = c % n_rows;
+        ok = ok && tc_wait_ready(&r.rows_full[at], (uint32_t)(c / n_rows) & 1u, r.abort_flag, p.err);
+        done[u] = &r.rows_empty[at];
+        src[u] = r.rows + (at * kTrChunk + (w & 1) * 8 + (lane & 7)) * pitch;
+        in[u] = (int64_t)j * kTrTile + (w + 4 * k) * 8 + (lane & 7) < left;
+        uint32_t m = 0;  // the largest magnitude's bits (those of an infinity or a NaN are above all others)
+        if (ok && in[u]) {
+#pragma unroll
+          for (int i = 0; i < D / 32; i++) {
+            const uint4* x = (const uint4*)(src[u] + (g + 4 * i) * 8);
+            const uint4 a = x[0], c4 = x[1];
+            m = max(max(max(m, a.x & 0x7fffffffu), max(a.y & 0x7fffffffu, a.z & 0x7fffffffu)), a.w & 0x7fffffffu);
+            m = max(max(max(m, c4.x & 0x7fffffffu), max(c4.y & 0x7fffffffu, c4.z & 0x7fffffffu)), c4.w & 0x7fffffffu);
+          }
+        }
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        // The row's largest magnitude becomes 2^14..2^15. Rows below 2^-100 keep -100:
+        // their halves lose bits below 2^-138, nothing that a float sum of products shows.
+        fine[u] = m < 0x7f800000u;
+        e[u] = max((int)(m >> 23) - 127, -100);
+        bad |= !fine[u];
+        const bool any = e[u] > -100;
+        e[u] -= 14;
+        if (fine[u] && any) {
+          hi = max(hi, e[u]);
+          lo = min(lo, e[u]);
+        }
+      }
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      if (__any_sync(0xffffffffu, bad)) lo = -2000;
+      int2* ends = r.ends + ((j & 1) * 2 + h) * 4;
+      if (lane == 0) ends[w] = make_int2(hi, lo);
+      // (also warps that have given up)
+      asm volatile("bar.sync %0, 128;" ::"r"(IS_V ? 6 : 5) : "memory");
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int2 o = ends[k];
+        hi = max(hi, o.x);
+        lo = min(lo, o.y);
+      }
+      const bool own = too_far_apart(hi, lo);
+      const int most = hi < -999 ? 0 : hi;
+      if (own && lane < 8) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) put_own<IS_V>(r, slot, h, (w + 4 * u) * 8 + lane, e[u], fine[u]);
+      }
+      put_info<IS_V>(r, slot, h, most, own);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&r.col_full[slot * 2 + h]);
+      const bool share = !PAIR || IS_V || h == r.rank;  // whether these rows' planes are this CTA's
+      if (share && (h == 0 || (PAIR && !IS_V))) {       // (the step's first)
+        ok = ok && (j < r.buffers || tc_wait_ready(&r.empty[b], (uint32_t)(j / r.buffers - 1) & 1u, r.abort_flag, p.err));
+        // (the first values lie where the queries were)
+        if (IS_V && j == 0 && wait_queries) ok = ok && tc_wait_ready(queries_done, 0, r.abort_flag, p.err);
+      }
+      if (ok && share) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const bool take = in[u] && (!own || fine[u]);
+          const float f = pow2f(own ? -e[u] : -most);
+          uint8_t* dst = r.planes + b * 2 * plane + (w + 4 * (NK == 2 ? u : 2 * h + u)) * (CH * 128) + g * 128 + (lane & 7) * 16;
+#pragma unroll
+          for (int i = 0; i < (CH + 3) / 4; i++) {
+            if (CH % 4 != 0 && g + 4 * i >= CH) continue;
+            uint4 up = make_uint4(0, 0, 0, 0), down = up;
+            if (take) {
+              const float4* from = (const float4*)(src[u] + (ch0 + g + 4 * i) * 8);
+              const float4 a = from[0], c4 = from[1];
+              const float x[8] = {a.x, a.y, a.z, a.w, c4.x, c4.y, c4.z, c4.w};
+              split8(x, f, up, down);
+            }
+            *(uint4*)(dst + i * 512) = up;
+            *(uint4*)(dst + plane + i * 512) = down;
+          }
+        }
+      }
+      __syncwarp();
+      if (ok && lane < 2) mbar_arrive_one(lane == 0 ? done[0] : done[1]);
+    }
+    if (ok) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive_lead(r.full + 8 * b);
+    }
+  }
+}
+
+// One warp copies the rows of an F32 cache into shared memory, as far ahead as there
+// is room. (In 16-byte pieces: a bulk copy a row took some 45 cycles each whatever its
+// size, 11 us a step.) It leaves only when its copies have arrived.
+template <int D, int n_rows>
+__device__ __forceinline__ void copy_rows(const TreeAttnParams& p, const float* cache, int kvh, int64_t pos0, int64_t n_kv, int n, int lane,
+                                          float* rows, uint64_t* full, uint64_t* empty, volatile int* abort_flag) {
+  constexpr int pitch = D + 4, pieces = D / 4;
+  const int64_t row = (int64_t)p.HKV * D;
+  const float* src = cache + pos0 * row + (int64_t)kvh * D;
+  const int64_t left = n_kv - pos0;
+  for (int c = 0; c < n * (kTrTile / kTrChunk); c++) {
+    const int at = c % n_rows;
+    if (c >= n_rows && !tc_wait_ready(&empty[at], (uint32_t)(c / n_rows - 1) & 1u, abort_flag, p.err)) break;
+    const uint32_t to = smem_addr(rows + at * kTrChunk * pitch);
+    const float* from = src + (int64_t)c * kTrChunk * row;
+    const int here = (int)max((int64_t)0, min((int64_t)kTrChunk, left - (int64_t)c * kTrChunk));
+#pragma unroll
+    for (int i = 0; i < kTrChunk * pieces / 32; i++) {
+      const int e = lane + 32 * i, r = e / pieces, k = e - r * pieces;
+      if (r < here)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (r * pitch + 4 * k) * 4), "l"(from + r * row + 4 * k) : "memory");
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_addr(&full[at])) : "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 template <int D, bool Q8, bool PAIR>
 __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_constant__ TreeAttnParams p,
                                                                   const TreeSplit sp, const int vec_q) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  using L = TrSmem<D, PAIR>;
+  using L = TrSmem<D, Q8, PAIR>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int split = blockIdx.z, kvh = blockIdx.y, r0 = blockIdx.x * kTrRows;
   const int rep = p.H / p.HKV;
@@ -588,6 +607,8 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   uint64_t* q_full = s_full + 5;  // the queries are in TMEM (of both CTAs)
   uint64_t* drain = s_full + 6;
   uint64_t* q_here = s_full + 7;  // ... of this one
+  uint64_t* rows_full = s_full + 8;               // F32: [keys, values][chunk % n_rows]
+  uint64_t* rows_empty = rows_full + 2 * L::n_rows;
   uint32_t* tmem_base = (uint32_t*)(smem + L::misc);
   volatile int* abort_flag = (volatile int*)(smem + L::misc + 4);
 
@@ -611,6 +632,10 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     mbar_init(q_full, kTrParts * nq_all + (PAIR ? 2 : 1));
     mbar_init(drain, 1);
     mbar_init(q_here, max(1, kTrParts * nq));
+    for (int i = 0; i < 2 * L::n_rows; i++) {
+      mbar_init(&rows_full[i], 32);
+      mbar_init(&rows_empty[i], 2);  // (a chunk is read by two warps)
+    }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -701,20 +726,20 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       for (uint32_t it = 0; it < kSpinLimit && !__all_sync(0xffffffffu, mbar_try_wait_sleep(drain, 0)); it++) {
       }
     } else if (warp < kTrWarpMma + 3) {
-      // Two of the other warps of the group ask for the whole range, keys and values,
-      // ahead of the converters (whose first read of a line from HBM takes 2 us).
-      const void* cache = warp == kTrWarpMma + 1 ? p.cache_k : p.cache_v;
-      const int64_t pend = min(n_kv, pos0 + (int64_t)n * kTrTile);
-      if (Q8) {
+      const int v = warp - kTrWarpMma - 1;  // keys, values
+      const void* cache = v ? p.cache_v : p.cache_k;
+      if constexpr (Q8) {
+        // Two of the other warps of the group ask for the whole range, keys and values,
+        // ahead of the converters (whose first read of a line from HBM takes 2 us).
+        const int64_t pend = min(n_kv, pos0 + (int64_t)n * kTrTile);
         const uint8_t* src = (const uint8_t*)cache + ((int64_t)kvh * p.n_ctx + pos0) * D;
         for (int64_t o = (int64_t)lane * 4096; o < (pend - pos0) * D; o += 32 * 4096)
           asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + o),
                        "r"((uint32_t)min((int64_t)4096, (pend - pos0) * D - o))
                        : "memory");
       } else {
-        const float* src = (const float*)cache + (int64_t)kvh * D;
-        for (int64_t pos = pos0 + lane; pos < pend; pos += 32)
-          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + pos * p.HKV * D), "n"(D * 4) : "memory");
+        copy_rows<D, L::n_rows>(p, (const float*)cache, kvh, pos0, n_kv, n, lane, (float*)(smem + L::rows) + v * L::n_rows * kTrChunk * L::pitch,
+                                rows_full + v * L::n_rows, rows_empty + v * L::n_rows, abort_flag);
       }
     }
   } else if (warp >= kTrWarpK) {
@@ -737,10 +762,18 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
     r.col_full = col_full;
     r.col = col;
     r.info = info;
-    r.ends = (int2*)(smem + L::ends) + (is_v ? 16 : 0);
     r.abort_flag = abort_flag;
-    if (is_v) convert_role<D, Q8, PAIR, true>(p, r, q_here, nq > 0);
-    else convert_role<D, Q8, PAIR, false>(p, r, q_here, false);
+    r.rows = (float*)(smem + L::rows) + is_v * L::n_rows * kTrChunk * L::pitch;
+    r.rows_full = rows_full + is_v * L::n_rows;
+    r.rows_empty = rows_empty + is_v * L::n_rows;
+    r.ends = (int2*)(smem + L::ends) + (is_v ? 16 : 0);
+    if constexpr (Q8) {
+      if (is_v) convert_q8_0<D, PAIR, true>(p, r, q_here, nq > 0);
+      else convert_q8_0<D, PAIR, false>(p, r, q_here, false);
+    } else {
+      if (is_v) convert_f32<D, PAIR, true, L::n_rows>(p, r, q_here, nq > 0);
+      else convert_f32<D, PAIR, false, L::n_rows>(p, r, q_here, false);
+    }
   } else {
     // ---------------- softmax: four threads per row ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -842,7 +875,9 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       for (int j = 0; j < n; j++) {
         const int slot = (j & (kTrSlots - 1)) * 2 + (part >> 1);
         const int64_t pt = pos0 + (int64_t)j * kTrTile + part * HT;
-        const float* c = col + slot * 3 * kTrHalf + (part & 1) * HT;
+        const float* c = col + slot * 2 * kTrHalf + (part & 1) * HT;
+        // (a masked position's weight is 0 whatever its row holds)
+        auto finite = [](float e) { return e == e ? e : 0.0f; };
         ok = ok && tc_wait_ready(&col_full[slot], (uint32_t)(j / kTrSlots) & 1u, abort_flag, p.err) &&
              tc_wait_ready(s_full, (uint32_t)j & 1u, abort_flag, p.err);
         if (!ok) {
@@ -907,7 +942,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
           float ms = -INFINITY;
           if (own) {
 #pragma unroll
-            for (int k = 0; k < HT; k++) ms = fmaxf(ms, __fsub_rn(x[k], in.w != 0.0f ? c[2 * kTrHalf + k] : in.z));
+            for (int k = 0; k < HT; k++) ms = fmaxf(ms, __fsub_rn(x[k], in.w != 0.0f ? finite(c[kTrHalf + k]) : in.z));
             ms = ceilf(ms);
           } else {
             ms = __fsub_rn(mx[0], in.z);
@@ -924,7 +959,7 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         if (apart) {
 #pragma unroll
           for (int k = 0; k < HT; k++) {
-            const float ve = in.w != 0.0f ? c[2 * kTrHalf + k] : in.z, g = __fsub_rn(ls, ve);
+            const float ve = in.w != 0.0f ? finite(c[kTrHalf + k]) : in.z, g = __fsub_rn(ls, ve);
             const float s = own ? x[k] : __fmaf_rn(x[k], fac, off);
             l = g > 100.0f ? __fadd_rn(l, exp2_approx(__fsub_rn(__fsub_rn(s, ve), lr0)))
                            : __fmaf_rn(exp2_approx(__fsub_rn(s, Ms)), exp2_approx(g), l);
@@ -1028,7 +1063,7 @@ cudaError_t launch_tiles(const TreeAttnParams& p, const TreeSplit& sp, cudaStrea
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(PAIR ? (sp.RG + 1) / 2 * 2 : sp.RG), (unsigned)p.HKV, (unsigned)sp.S);
   cfg.blockDim = dim3(kTrThreads);
-  cfg.dynamicSmemBytes = TrSmem<D, PAIR>::total;
+  cfg.dynamicSmemBytes = TrSmem<D, Q8, PAIR>::total;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1056,9 +1091,9 @@ cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
 template <int D, bool Q8>
 cudaError_t prepare_tiles() {
   const cudaError_t e = cudaFuncSetAttribute(attn_tree_kernel<D, Q8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             TrSmem<D, false>::total);
+                                             TrSmem<D, Q8, false>::total);
   if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(attn_tree_kernel<D, Q8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D, true>::total);
+  return cudaFuncSetAttribute(attn_tree_kernel<D, Q8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D, Q8, true>::total);
 }
 template <int D>
 cudaError_t prepare_tree() {
