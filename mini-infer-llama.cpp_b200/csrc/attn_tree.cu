@@ -57,6 +57,7 @@
 // The positions are split over CTAs to fill the GPU; a second kernel joins the
 // splits' (M, sum, O) records.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_tree.cuh"
 #include "mi_tc.cuh"
@@ -373,8 +374,7 @@ struct TrConvert {
   int64_t pos0, n_kv;
   int kvh, n, w, lane, rank;
   const void* cache;
-  uint8_t* planes;  // [buffers][hi, lo]
-  int buffers;
+  uint8_t* planes;  // [n_buf][hi, lo]
   uint64_t *empty, *col_full;
   uint32_t full;    // shared::cluster address of the issuing CTA's barriers
   float *col, *info;
@@ -408,14 +408,14 @@ __device__ __forceinline__ void put_info(const TrConvert& r, int slot, int half,
 // written again eight steps later: after the planes of seven, for which the scores of
 // five were done, for which the softmax had read those of four, and so had long left
 // the step itself.
-template <int D, bool PAIR, bool IS_V>
+template <int D, bool PAIR, bool IS_V, int n_buf>
 __device__ __forceinline__ void convert_q8_0(const TreeAttnParams& p, const TrConvert& r, uint64_t* queries_done, bool wait_queries) {
   constexpr int NK = PAIR && !IS_V ? 2 : 4, CH = PAIR && IS_V ? D / 16 : D / 8, plane = NK * 4 * CH * 128;
   KvRows<D, NK, CH> kv;
   kv.begin(p, r.cache, r.kvh, r.pos0, r.n_kv, r.w, r.lane, PAIR && !IS_V ? r.rank * kTrHalf : 0, PAIR && IS_V ? r.rank * CH : 0);
   bool ok = true;
   for (int j = 0; j < r.n; j++) {
-    const int slot = j & (kTrSlots - 1), b = j % r.buffers;
+    const int slot = j & (kTrSlots - 1), b = j % n_buf;
     int most[2];
     bool own[2];
     kv.exponents(j * kTrTile, r.w, r.lane, most, own, too_far_apart,
@@ -427,7 +427,7 @@ __device__ __forceinline__ void convert_q8_0(const TreeAttnParams& p, const TrCo
     }
     __syncwarp();
     if (r.lane < 2) mbar_arrive_one(&r.col_full[slot * 2 + r.lane]);
-    ok = ok && (j < r.buffers || tc_wait_ready(&r.empty[b], (uint32_t)(j / r.buffers - 1) & 1u, r.abort_flag, p.err));
+    ok = ok && (j < n_buf || tc_wait_ready(&r.empty[b], (uint32_t)(j / n_buf - 1) & 1u, r.abort_flag, p.err));
     // (the first values lie where the queries were)
     if (IS_V && j == 0 && wait_queries) ok = ok && tc_wait_ready(queries_done, 0, r.abort_flag, p.err);
     if (ok) {
@@ -442,14 +442,14 @@ __device__ __forceinline__ void convert_q8_0(const TreeAttnParams& p, const TrCo
 // The same from an F32 cache, whose rows the copying warps leave in shared memory,
 // 64 positions at a time: read there for their exponents, and again for their planes.
 // (Both times from global memory, a step took 15 us at D = 128, 5 times the softmax.)
-template <int D, bool PAIR, bool IS_V, int n_rows>
+template <int D, bool PAIR, bool IS_V, int n_buf, int n_rows>
 __device__ __forceinline__ void convert_f32(const TreeAttnParams& p, const TrConvert& r, uint64_t* queries_done, bool wait_queries) {
   constexpr int NK = PAIR && !IS_V ? 2 : 4, CH = PAIR && IS_V ? D / 16 : D / 8, plane = NK * 4 * CH * 128, pitch = D + 4;
   const int ch0 = PAIR && IS_V ? r.rank * CH : 0, w = r.w, lane = r.lane, g = lane >> 3;
   const int64_t left = r.n_kv - r.pos0;
   bool ok = true;
   for (int j = 0; j < r.n; j++) {
-    const int slot = j & (kTrSlots - 1), b = j % r.buffers;
+    const int slot = j & (kTrSlots - 1), b = j % n_buf;
 #pragma unroll 1
     for (int h = 0; h < 2; h++) {
       // row groups w + 4 k of the step, k = 2 h and 2 h + 1: half a chunk each
@@ -512,7 +512,7 @@ __device__ __forceinline__ void convert_f32(const TreeAttnParams& p, const TrCon
       if (lane == 0) mbar_arrive_one(&r.col_full[slot * 2 + h]);
       const bool share = !PAIR || IS_V || h == r.rank;  // whether these rows' planes are this CTA's
       if (share && (h == 0 || (PAIR && !IS_V))) {       // (the step's first)
-        ok = ok && (j < r.buffers || tc_wait_ready(&r.empty[b], (uint32_t)(j / r.buffers - 1) & 1u, r.abort_flag, p.err));
+        ok = ok && (j < n_buf || tc_wait_ready(&r.empty[b], (uint32_t)(j / n_buf - 1) & 1u, r.abort_flag, p.err));
         // (the first values lie where the queries were)
         if (IS_V && j == 0 && wait_queries) ok = ok && tc_wait_ready(queries_done, 0, r.abort_flag, p.err);
       }
@@ -745,35 +745,33 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
   } else if (warp >= kTrWarpK) {
     // ---------------- keys (warps 16-19) and values (20-23) ----------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
-    const bool is_v = warp >= kTrWarpV;
-    TrConvert r;
-    r.pos0 = pos0;
-    r.n_kv = n_kv;
-    r.kvh = kvh;
-    r.n = n;
-    r.w = warp & 3;
-    r.lane = lane;
-    r.rank = rank;
-    r.cache = is_v ? p.cache_v : p.cache_k;
-    r.planes = smem + (is_v ? L::v : L::k);
-    r.buffers = is_v ? L::n_v : L::n_k;
-    r.empty = is_v ? v_empty : k_empty;
-    r.full = lead(is_v ? v_full : k_full);
-    r.col_full = col_full;
-    r.col = col;
-    r.info = info;
-    r.abort_flag = abort_flag;
-    r.rows = (float*)(smem + L::rows) + is_v * L::n_rows * kTrChunk * L::pitch;
-    r.rows_full = rows_full + is_v * L::n_rows;
-    r.rows_empty = rows_empty + is_v * L::n_rows;
-    r.ends = (int2*)(smem + L::ends) + (is_v ? 16 : 0);
-    if constexpr (Q8) {
-      if (is_v) convert_q8_0<D, PAIR, true>(p, r, q_here, nq > 0);
-      else convert_q8_0<D, PAIR, false>(p, r, q_here, false);
-    } else {
-      if (is_v) convert_f32<D, PAIR, true, L::n_rows>(p, r, q_here, nq > 0);
-      else convert_f32<D, PAIR, false, L::n_rows>(p, r, q_here, false);
-    }
+    auto convert = [&](auto which) {
+      constexpr bool is_v = decltype(which)::value;
+      TrConvert r;
+      r.pos0 = pos0;
+      r.n_kv = n_kv;
+      r.kvh = kvh;
+      r.n = n;
+      r.w = warp & 3;
+      r.lane = lane;
+      r.rank = rank;
+      r.cache = is_v ? p.cache_v : p.cache_k;
+      r.planes = smem + (is_v ? L::v : L::k);
+      r.empty = is_v ? v_empty : k_empty;
+      r.full = lead(is_v ? v_full : k_full);
+      r.col_full = col_full;
+      r.col = col;
+      r.info = info;
+      r.abort_flag = abort_flag;
+      r.rows = (float*)(smem + L::rows) + is_v * L::n_rows * kTrChunk * L::pitch;
+      r.rows_full = rows_full + is_v * L::n_rows;
+      r.rows_empty = rows_empty + is_v * L::n_rows;
+      r.ends = (int2*)(smem + L::ends) + is_v * 16;
+      if constexpr (Q8) convert_q8_0<D, PAIR, is_v, is_v ? L::n_v : L::n_k>(p, r, q_here, is_v && nq > 0);
+      else convert_f32<D, PAIR, is_v, is_v ? L::n_v : L::n_k, L::n_rows>(p, r, q_here, is_v && nq > 0);
+    };
+    if (warp < kTrWarpV) convert(std::false_type{});
+    else convert(std::true_type{});
   } else {
     // ---------------- softmax: four threads per row ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -1131,14 +1129,15 @@ cudaError_t prepare_attn_tree_kernels() {
 // 16000 positions (16.1 / 18.3 at 8000, 46.4 / 36.7 at 32000, heads of 128) and 28
 // up to some 8000 of 64 dims (10.9 / 12.6 at 8000; heads of 128 19.7 / 19.0).
 //
-// Over an F32 cache (28 / 4 heads of 128, 14 / 2 of 64 and 6 / 2 of 96): up to 8 rows
-// always (12.5 / 21.0 at 2000 positions of 128, 78 / 98 at 32000), up to 16 until the
-// one pass over the cache takes longer than the converters (29 / 36 at 8000, 114 / 98
-// at 32000), and with more passes while the cache is small (63 rows of 64 over 2000
-// 11.9 / 14.2, 91 rows 20.2 / 14.8; 126 rows of 128 over 100 16.7 / 22.2).
+// Over an F32 cache: up to 8 rows always (14 / 2 heads of 64: 7.6 / 13.2 at 2000
+// positions, 21 / 25 at 32000), up to 16 nearly always (14 rows 12.0 / 14.3 at 8000; 12
+// of 96 dims 34 / 41 at 32000) but at 128 dims, where they no longer fit the registers
+// (14 rows 13.2 / 17.5 at 500, 19.5 / 16.1 at 2000), and with more passes of 16 rows
+// while the cache is small (63 rows of 64 over 2000 11.8 / 13.5, 91 rows 20.2 / 13.7).
 static bool few_rows(bool q8, int64_t R, int64_t n_kv, int64_t HKV, int64_t D) {
   if (q8) return R <= 8 || (R <= 16 && n_kv <= 16384) || (R <= 32 && n_kv * D <= (1 << 19));
-  return R <= 8 || (R <= 128 && (R + 15) / 16 * n_kv * HKV * D <= (R <= 16 ? 1 << 23 : R <= 64 ? 1 << 20 : 1 << 19));
+  const int64_t most = D > 96 ? 1 << 19 : R <= 16 ? 1 << 23 : R <= 64 ? 1 << 20 : 1 << 19;
+  return R <= 8 || (R <= 128 && (R + 15) / 16 * n_kv * HKV * D <= most);
 }
 
 cudaError_t launch_attn_tree(const TreeAttnParams& p, cudaStream_t s) {
