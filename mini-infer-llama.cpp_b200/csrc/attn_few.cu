@@ -183,9 +183,10 @@ struct FewCache<D, false> {
 // along the splits.
 //
 // Registers: one group over a Q8_0 cache for 4 CTAs of an SM (3 of 96 and 128 dims; 2
-// took 36 us for a token over 32000 positions of 28 / 4 heads of 128, 3 take 23).
+// took 36 us for a token over 32000 positions of 28 / 4 heads of 128, 3 take 23); over
+// an F32 cache for 3 of 32 dims (16 heads over 2000 positions: 11.5 us with 2, 7.2 with 3).
 template <int D, int NR, bool Q8>
-__global__ void __launch_bounds__(kFewNT, NR == 1 && Q8 ? (D <= 64 ? 4 : 3) : 1) attn_few_kernel(const __grid_constant__ TreeAttnParams p, const TreeSplit sp,
+__global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : D <= 32 ? 3 : 1) attn_few_kernel(const __grid_constant__ TreeAttnParams p, const TreeSplit sp,
                                                           const int cluster) {
   constexpr int NC = D / 32, PT = kFewTiles<D, Q8>, step = kFewStep<D, Q8>;
   extern __shared__ __align__(16) uint8_t few_raw[];
