@@ -138,22 +138,23 @@ __global__ void __launch_bounds__(kKvNT) kv_read_q8_kernel(const KvReadParams p,
   const __half* ds = (const __half*)(c + plane) + at * nb + b;
   float* out = (is_v ? p.v : p.k) + (int64_t)piece * 4;
   const int64_t i0 = (int64_t)blockIdx.x * g.rows * kKvAhead + r;
+  // (loads only, from a row that is there: a use or a branch between them would make
+  // each wait for the one before it)
   char4 q[kKvAhead];
-  float d[kKvAhead];
+  __half dh[kKvAhead];
 #pragma unroll
   for (int u = 0; u < kKvAhead; u++) {
-    const int64_t i = i0 + u * g.rows;
-    if (i < p.n_rows) {
-      q[u] = *(const char4*)(qs + i * p.D);
-      d[u] = __half2float(ds[i * nb]);
-    }
+    const int64_t i = min(i0 + u * g.rows, p.n_rows - 1);
+    q[u] = *(const char4*)(qs + i * p.D);
+    dh[u] = ds[i * nb];
   }
 #pragma unroll
   for (int u = 0; u < kKvAhead; u++) {
     const int64_t i = i0 + u * g.rows;
+    const float d = __half2float(dh[u]);
     if (i < p.n_rows)
-      *(float4*)(out + i * g.pieces * 4) = make_float4(__fmul_rn((float)q[u].x, d[u]), __fmul_rn((float)q[u].y, d[u]),
-                                                       __fmul_rn((float)q[u].z, d[u]), __fmul_rn((float)q[u].w, d[u]));
+      *(float4*)(out + i * g.pieces * 4) = make_float4(__fmul_rn((float)q[u].x, d), __fmul_rn((float)q[u].y, d),
+                                                       __fmul_rn((float)q[u].z, d), __fmul_rn((float)q[u].w, d));
   }
 }
 
