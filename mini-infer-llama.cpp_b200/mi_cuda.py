@@ -447,12 +447,13 @@ def kv_q8_0_cache(n_ctx: int, n_head_kv: int, head_dim: int, device="cuda"):
 
 
 def _kv_q8_0_args(cache_k, cache_v, n_ctx: int, n_head_kv: int, head_dim: int):
-    nb = lib().mi_cuda_kv_q8_0_bytes(n_ctx, n_head_kv, head_dim)
-    if nb == 0:
+    # (mi_cuda_kv_q8_0_bytes, without the call: 34 bytes per 32 values)
+    if head_dim % 32 or not 0 < head_dim <= 256 or n_ctx < 1 or n_head_kv < 1:
         raise ValueError(f"no Q8_0 cache of {n_ctx} rows of {n_head_kv} heads of {head_dim}")
+    size = (n_ctx * n_head_kv * (head_dim // 32) * 34,)
     u8 = _torch().uint8
-    _dense(cache_k, "cache_k", u8, (nb,))
-    _dense(cache_v, "cache_v", u8, (nb,))
+    _dense(cache_k, "cache_k", u8, size)
+    _dense(cache_v, "cache_v", u8, size)
 
 
 def kv_append_q8_0(k, v, cache_k, cache_v, n_ctx: int, n_past: int = 0, slots=None):
