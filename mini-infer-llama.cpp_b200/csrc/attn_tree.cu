@@ -27,7 +27,8 @@
 //
 // One CTA: 128 rows (a TMEM lane each) over one range of positions, 128 a step.
 // Warps 0-15 softmax: four threads per row, 32 positions each; 16-19 convert keys
-// and 20-23 values into the MMAs' layout in shared memory; 24 issues the MMAs. The
+// and 20-23 values into the MMAs' layout in shared memory; 24 issues the MMAs; 25 and
+// 26 ask for the cache ahead (Q8_0: into L2; F32: its rows into shared memory). The
 // queries' planes are copied into TMEM: as a shared-memory operand they are 4 KB a
 // product beside the keys' 4, and shared memory, not the tensor core, set the pace.
 // S, P's planes, O and the queries' planes fill TMEM's 512 columns at D = 128. The
@@ -71,7 +72,7 @@ constexpr int kTrHalf = 64;      // ... that share their exponents
 constexpr int kTrParts = 4;      // softmax threads per row: 32 positions each, and a quarter of O's dims
 constexpr int kTrRows = 128;     // rows per CTA (MMA M)
 constexpr int kTrWarpK = 16, kTrWarpV = 20, kTrWarpMma = 24;
-constexpr int kTrThreads = 28 * 32;  // (the last three warps complete the MMA warp's group for setmaxnreg)
+constexpr int kTrThreads = 28 * 32;  // (the last warp completes the MMA warp's group for setmaxnreg)
 constexpr int kTrChunk = 16;     // F32: rows of a cache that are copied at a time
 constexpr int kTrSlots = 8;      // steps whose exponents are kept (see the roles' waits)
 constexpr uint32_t kTrCols = 512;  // all of TMEM: its base is 0
@@ -1086,17 +1087,22 @@ cudaError_t launch_tree(const TreeAttnParams& p, cudaStream_t s) {
   return launch_tree_join<D>(p, sp, s);
 }
 
-template <int D, bool Q8>
+template <int D, bool Q8, bool PAIR>
 cudaError_t prepare_tiles() {
-  const cudaError_t e = cudaFuncSetAttribute(attn_tree_kernel<D, Q8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             TrSmem<D, Q8, false>::total);
+  // A build that gave the kernel fewer registers than its roles share out would wait
+  // for them for good.
+  cudaFuncAttributes a;
+  const cudaError_t e = cudaFuncGetAttributes(&a, attn_tree_kernel<D, Q8, PAIR>);
   if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(attn_tree_kernel<D, Q8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D, Q8, true>::total);
+  if (a.numRegs * kTrThreads < kRegsSoftmax * 512 + kRegsConvert * 256 + kRegsMma * 128) return cudaErrorInvalidConfiguration;
+  return cudaFuncSetAttribute(attn_tree_kernel<D, Q8, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TrSmem<D, Q8, PAIR>::total);
 }
 template <int D>
 cudaError_t prepare_tree() {
-  const cudaError_t e = prepare_tiles<D, false>();
-  return e == cudaSuccess ? prepare_tiles<D, true>() : e;
+  cudaError_t e = prepare_tiles<D, false, false>();
+  if (e == cudaSuccess) e = prepare_tiles<D, false, true>();
+  if (e == cudaSuccess) e = prepare_tiles<D, true, false>();
+  return e == cudaSuccess ? prepare_tiles<D, true, true>() : e;
 }
 
 }  // namespace
