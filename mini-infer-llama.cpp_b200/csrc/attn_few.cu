@@ -12,8 +12,12 @@
 //     k-steps of V^T's.
 // int8 is exact in fp16, so S needs two MMAs (hi, lo) per step and block, the block's
 // scale multiplies its sum in float, and P carries the values' scales: P d_v 2^(13 -
-// E), E the largest scale's exponent of the step, again as hi + lo, turned from S's
-// layout into the operand's by an 8 x 8 transpose.
+// E), again as hi + lo, turned from S's layout into the operand's by an 8 x 8
+// transpose. E is the exponent of the row's largest P d_v in the step, so that hi + lo
+// holds 22 bits of what counts for this row: a masked position has P = 0 and a scale
+// that is NaN is left out, so neither moves E, and a large scale moves it only by
+// what its weight leaves of it. (One E a warp, from all scales that it holds, cost
+// values of 0.01 beside a masked NaN 2.7e-3.)
 //
 // From an F32 cache the same tiles as m16n8k8 of tf32, every operand as hi + lo (11
 // bits each: 2^-21 of a value is left out) and three MMAs a product; tf32 has float's
@@ -260,9 +264,10 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
   if (!Q8) __syncthreads();
 
   float M[NR][2], l[NR][2], acc[NR][NC][2][4];
-  int E = 13;  // O is in units of 2^(E - 13)
+  int E[NR][2];  // O is in units of 2^(E - 13) (F32: of 1)
 #pragma unroll
   for (int n = 0; n < NR; n++) {
+    E[n][0] = E[n][1] = 13;
     M[n][0] = M[n][1] = -INFINITY;
     l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
@@ -337,16 +342,19 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
     // ---- masks, maxima
     uint32_t seen[PT][NR];  // bit k: x[..][k] is attended to
     float fac[NR][2];
-    int En = 13;
+    float dmax[Q8 ? PT : 1][2];  // the values' largest scale of positions g, g + 8 that is no NaN
     if constexpr (Q8) {
-      uint32_t top = 0;  // the values' largest scale
 #pragma unroll
       for (int q = 0; q < PT; q++)
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int h = 0; h < 2; h++) {
+          dmax[q][h] = 0.0f;
 #pragma unroll
-          for (int i = 0; i < FewCache<D, Q8>::ND; i++) top = max(top, max(kv.dv[q][h][i] & 0x7fffu, (kv.dv[q][h][i] >> 16) & 0x7fffu));
-      En = max((int)(__reduce_max_sync(0xffffffffu, top) >> 10), 1) - 15;
+          for (int i = 0; i < FewCache<D, Q8>::ND; i++) {
+            const float2 d = __half22float2(__habs2(*reinterpret_cast<const __half2*>(&kv.dv[q][h][i])));
+            dmax[q][h] = fmaxf(dmax[q][h], fmaxf(d.x, d.y));
+          }
+        }
     }
 #pragma unroll
     for (int n = 0; n < NR; n++) {
@@ -373,7 +381,7 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
         for (int s = 4; s < 32; s *= 2) mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], s));
         const float Mn = fmaxf(M[n][u], mx[u]), Mr = Mn == -INFINITY ? 0.0f : Mn;
         const float f = exp2_approx(__fsub_rn(M[n][u], Mr));
-        fac[n][u] = Q8 ? __fmul_rn(f, pow2f(E - En)) : f;
+        fac[n][u] = f;
         l[n][u] = __fmul_rn(l[n][u], f);
         M[n][u] = Mn;
         // weights
@@ -386,11 +394,33 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
             l[n][u] = __fadd_rn(l[n][u], y);
           }
       }
+      if constexpr (Q8) {
+        // both rows' E in one word (not below -40, so that O, which moves to the new unit,
+        // stays in a float's range)
+        float top[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < PT; q++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) top[k & 1] = fmaxf(top[k & 1], __fmul_rn(x[q][n][k], dmax[q][k >> 1]));
+        uint32_t both = __float_as_uint(top[0]) >> 23 | __float_as_uint(top[1]) >> 23 << 16;
+#pragma unroll
+        for (int s = 4; s < 32; s *= 2) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, s));
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int En = min(max((int)(both >> (16 * u) & 0xffffu) - 127, -40), 16);
+          fac[n][u] = __fmul_rn(fac[n][u], pow2f(E[n][u] - En));
+          E[n][u] = En;
+        }
+      }
     }
-    E = En;
     // ---- O = O fac + P V
     if constexpr (Q8) {
-      const float unit = pow2f(13 - En);
+#pragma unroll
+      for (int n = 0; n < NR; n++)
+#pragma unroll
+        for (int q = 0; q < PT; q++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) x[q][n][k] = __fmul_rn(x[q][n][k], pow2f(13 - E[n][k & 1]));
 #pragma unroll
       for (int q = 0; q < PT; q++)
 #pragma unroll
@@ -406,8 +436,8 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
             v[h][2] = bytes_to_h2(hi, 0x4140);
             v[h][3] = bytes_to_h2(hi, 0x4342);
           }
-          const float s0 = __fmul_rn(__half2float(__ushort_as_half((uint16_t)(c & 1 ? kv.dv[q][0][c / 2] >> 16 : kv.dv[q][0][c / 2]))), unit);
-          const float s1 = __fmul_rn(__half2float(__ushort_as_half((uint16_t)(c & 1 ? kv.dv[q][1][c / 2] >> 16 : kv.dv[q][1][c / 2]))), unit);
+          const float s0 = __half2float(__ushort_as_half((uint16_t)(c & 1 ? kv.dv[q][0][c / 2] >> 16 : kv.dv[q][0][c / 2])));
+          const float s1 = __half2float(__ushort_as_half((uint16_t)(c & 1 ? kv.dv[q][1][c / 2] >> 16 : kv.dv[q][1][c / 2])));
 #pragma unroll
           for (int n = 0; n < NR; n++) {
             float w[4];
@@ -505,7 +535,7 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
       if (g == 0) {
         sm.m[warp][8 * n + 2 * t + u] = M[n][u];
         sm.l[warp][8 * n + 2 * t + u] = l[n][u];
-        sm.scale[warp][8 * n + 2 * t + u] = pow2f(E - 13);
+        sm.scale[warp][8 * n + 2 * t + u] = pow2f(E[n][u] - 13);
       }
     }
 #pragma unroll

@@ -607,6 +607,70 @@ def test_attention_tree_two_at_once(torch, H, HKV, D, T, past):
     assert torch.equal(out, want[0]) and torch.equal(other, want[1])
 
 
+def attn_componentwise(torch, got, q, k, v, seen, scale, rows=None):
+    """Holds got [T, H, D] (or its tokens `rows`) to a bound of its own per value, from the rows that the
+    token attends to alone, so that nothing a masked row holds may cost precision. Weight j is off by
+    d_j + eps of itself and the sum of the weights by what that comes to: d_j is the score's error,
+    (D + 8) u scale max|q| sum|k_j| as in check_attn plus 4 u |s_j| for its scaling and the difference to
+    the maximum; eps 2 * 2^-22 for exp2 in numerator and sum, 2^-20 for operands held as halves (11 + 11
+    bits) and 256 u for the sums. A weight's lower half stops 2^-37 below the largest weight times value:
+    n of those are added. Rows with a NaN may be passed where no checked token attends to them."""
+    T, H, D = q.shape
+    rep, n = H // k.shape[1], k.shape[0]
+    for i in range(T) if rows is None else rows:
+        at = torch.nonzero(seen[i])[:, 0]
+        kk, vv = (x[at].double().repeat_interleave(rep, 1).transpose(0, 1) for x in (k, v))  # [H, m, D]
+        s = (kk @ q[i].double()[:, :, None]).squeeze(-1) * scale  # [H, m]
+        p = torch.softmax(s, -1)
+        d = (D + 8) * U * abs(scale) * q[i].double().abs().amax(-1)[:, None] * kk.abs().sum(-1) + 4 * U * s.abs()
+        eps = 2.0**-21 + 2.0**-20 + 256 * U + (p * d).sum(-1, keepdim=True)
+        want = (p[:, None] @ vv).squeeze(1)
+        tol = ((p * (d + eps))[:, None] @ vv.abs()).squeeze(1) + n * 2.0**-37 * (p * vv.abs().amax(-1)).amax(-1)[:, None]
+        diff = (got[i].double() - want).abs()
+        assert (diff <= tol).all(), (i, float((diff / tol).max()), float(diff.norm() / want.norm()))
+
+
+def set_row(torch, caches, kv, n_ctx, d, at, what):
+    """Row `at` of both Q8_0 caches: quants 127 with a scale of NaN, of 65504, or of 1000 times the row's own."""
+    for c in caches:
+        q, s = planes(c, kv, n_ctx, d)
+        q[:, at] = 127
+        s[:, at] = {"nan": math.nan, "max": 65504.0}[what] if what != "1000" else s[:, at] * 1000
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["nan", "max", "1000"])
+@pytest.mark.parametrize("H,HKV,D,T,past", [(14, 2, 64, 1, 20), (14, 2, 64, 2, 18), (14, 2, 64, 4, 30), (28, 4, 128, 2, 40), (28, 4, 128, 1, 7),
+                                            (6, 2, 96, 2, 300), (6, 2, 96, 5, 20), (16, 16, 32, 4, 20), (16, 16, 32, 20, 11), (14, 2, 64, 2, 3000),
+                                            (28, 4, 128, 24, 150)])
+def test_attention_tree_q8_0_beside_masked_rows(torch, H, HKV, D, T, past, what):
+    """A masked row of a large scale (or a NaN, as in a row that was never written) takes nothing from the
+    precision of the others, however small their values; nor does an attended row whose weight is negligible."""
+    g = torch.Generator(device="cuda").manual_seed(T + past + D)
+    uniform = lambda *s: torch.rand(s, generator=g, device="cuda") * 2 - 1  # noqa: E731
+    n_ctx, n = past + T + 3, past + T
+    for size in (1.0, 0.01, 0.001):
+        q, k, v = uniform(T, H, D) * 0.3, uniform(n_ctx, HKV, D), uniform(n_ctx, HKV, D) * size
+        caches = [mi_cuda.kv_q8_0_cache(n_ctx, HKV, D) for _ in range(2)]
+        mi_cuda.kv_append_q8_0(k, v, *caches, n_ctx)
+        # the last token's row: no one's, or (causal) its own alone
+        set_row(torch, caches, HKV, n_ctx, D, n - 1, what)
+        mask = mi_cuda.tree_mask(list(range(-1, T - 1)))
+        mask[T - 1, (T - 1) // 32] &= ~np.int32(1 << (T - 1) % 32) if (T - 1) % 32 < 31 else np.int32(2**31 - 1)
+        rows = mi_cuda.kv_read_q8_0(*caches, HKV, D, n_ctx, 0, n)
+        attn_componentwise(torch, tree(torch, True, q, caches, HKV, n_ctx, past, 0.125, mask), q, *rows, seen_of(torch, mask, T, past), 0.125)
+        if T > 1:
+            attn_componentwise(torch, tree(torch, True, q, caches, HKV, n_ctx, past, 0.125), q, *rows, seen_of(torch, None, T, past), 0.125,
+                               range(T - 1))
+    # attended, but at a score of -60 below the others': a value of 8e6 counts 1e-19
+    q, k, v = uniform(T, H, D) * 0.1 + 0.5, uniform(n_ctx, HKV, D), uniform(n_ctx, HKV, D) * 0.01
+    k[past - 1], v[past - 1] = -2.0 * 60 / (0.125 * D), 8e6
+    caches = [mi_cuda.kv_q8_0_cache(n_ctx, HKV, D) for _ in range(2)]
+    mi_cuda.kv_append_q8_0(k, v, *caches, n_ctx)
+    rows = mi_cuda.kv_read_q8_0(*caches, HKV, D, n_ctx, 0, n)
+    attn_componentwise(torch, tree(torch, True, q, caches, HKV, n_ctx, past, 0.125), q, *rows, seen_of(torch, None, T, past), 0.125)
+
+
 def check_logits(torch, x, out, tokens, hist, repeat, freq, pres, ids, bias, allowed):
     for i in range(x.shape[0]):
         h = hist[i] if hist.ndim == 2 else hist
