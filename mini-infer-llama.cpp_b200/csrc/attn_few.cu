@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
 
   // the queries: row 8n + g, the dims that this lane's key bytes stand for
   uint32_t qh[Q8 ? NR : 1][NC][4], ql[Q8 ? NR : 1][NC][4];  // (F32: in shared memory)
-  float rf[NR][2];  // |scale| * log2(e) * the factor of rows 8n + 2t, 8n + 2t + 1
+  float rf[NR][2];  // |scale| * log2(e) * the factor of rows 8n + 2t, 8n + 2t + 1 (F32: 2^-16 of it)
   int tok[NR][2];
 #pragma unroll
   for (int n = 0; n < NR; n++) {
@@ -225,9 +225,10 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     fine = m <= 3.402823466e38f;
     // The row's largest value becomes 2^14..2^15; with an F32 cache 2^-9..2^-8, so that
-    // no score leaves a float's range. A row with an infinity or a NaN: NaN.
-    constexpr int up = Q8 ? 14 : -9;
-    const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), Q8 ? 127 : 117);
+    // no score leaves a float's range before its factor. (Both in two steps there, for
+    // their powers of two pass a float's range.) A row with an infinity or a NaN: NaN.
+    constexpr int up = Q8 ? 14 : 23;
+    const int ex = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127);
     const float f = p.scale < 0.0f ? -pow2f(up - ex) : pow2f(up - ex);
 #pragma unroll
     for (int c = 0; c < NC; c++) {
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
         uint32_t h[8], l[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          split_tf32(__fmul_rn(x[c][e], f), h[e], l[e]);
+          split_tf32(__fmul_rn(__fmul_rn(x[c][e], f), pow2f(-32)), h[e], l[e]);
           if (!fine) h[e] = 0x7fc00000u;
         }
         sm.q[n][c][0][lane] = make_uint4(h[0], h[1], h[2], h[3]);
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
         sm.q[n][c][3][lane] = make_uint4(l[4], l[5], l[6], l[7]);
       }
     }
-    const float own = __fmul_rn(__fmul_rn(fabsf(p.scale), 1.4426950408889634f), pow2f(ex - up));
+    const float own = __fmul_rn(__fmul_rn(fabsf(p.scale), 1.4426950408889634f), pow2f(Q8 ? ex - up : ex - up + 16));
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       rf[n][u] = __shfl_sync(0xffffffffu, own, 4 * (2 * t + u));
@@ -336,7 +337,12 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
 #pragma unroll
         for (int n = 0; n < NR; n++)
 #pragma unroll
-          for (int k = 0; k < 4; k++) x[q][n][k] = __fadd_rn(s[n][2][k], __fadd_rn(s[n][0][k], s[n][1][k]));
+          for (int k = 0; k < 4; k++) {
+            // (a finite key's score is finite: one that is not comes from an infinity or a NaN in
+            // the key or the query, whatever the halves made of it, and becomes NaN)
+            const float y = __fadd_rn(s[n][2][k], __fadd_rn(s[n][0][k], s[n][1][k]));
+            x[q][n][k] = __fmaf_rn(y, 0.0f, y);
+          }
       }
     }
     // ---- masks, maxima
@@ -372,6 +378,7 @@ __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : 
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           x[q][n][k] = (seen[q][n] >> k) & 1u ? __fmul_rn(x[q][n][k], rf[n][k & 1]) : -INFINITY;
+          if (!Q8) x[q][n][k] = __fmul_rn(x[q][n][k], 65536.0f);
           mx[k & 1] = fmaxf(mx[k & 1], x[q][n][k]);
         }
       }

@@ -671,6 +671,49 @@ def test_attention_tree_q8_0_beside_masked_rows(torch, H, HKV, D, T, past, what)
     attn_componentwise(torch, tree(torch, True, q, caches, HKV, n_ctx, past, 0.125), q, *rows, seen_of(torch, None, T, past), 0.125)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("word", [0x7f800000, 0xff800000, 0x7f800001, 0x7fc00000])
+@pytest.mark.parametrize("H,HKV,D,T,past", [(14, 2, 64, 1, 40), (28, 4, 128, 1, 200), (6, 2, 96, 2, 30), (14, 2, 64, 2, 70), (16, 16, 32, 9, 500),
+                                            (14, 2, 64, 24, 300)])
+def test_attention_tree_f32_keys_that_are_not_finite(torch, H, HKV, D, T, past, word):
+    """An infinity of either sign or a NaN (of any payload) in an F32 key: NaN for the tokens that attend to
+    it, whatever their queries' signs, nothing for the others."""
+    q, caches, rows, n_ctx = attn_inputs(torch, T, H, HKV, D, past, T + past, False)
+    bad = past + T - 1  # the last token's own row
+    at = (bad, HKV - 1, D // 2 + 3)
+    k = caches[0].clone()
+    k.view(torch.int32)[at] = word - (word >> 31 << 32)
+    clean = rows[0].clone()
+    clean[at] = 0.0
+    for sign in (1.0, -1.0, 0.0):
+        x = q.clone()
+        x[..., at[2]] = x[..., at[2]].abs() * sign
+        got = tree(torch, False, x, (k, caches[1]), HKV, n_ctx, past, 0.125).unflatten(1, (HKV, -1))
+        assert torch.isnan(got[-1, -1]).any(-1).all(), sign
+        want, tol = attn_f64(torch, x, clean, rows[1], seen_of(torch, None, T, past), 0.125)
+        want = want.unflatten(1, (HKV, -1))
+        assert T == 1 or float((got[:-1].double() - want[:-1]).norm()) <= 2e-5 * float(want[:-1].norm())
+        assert HKV == 1 or float((got[-1, :-1].double() - want[-1, :-1]).norm()) <= 2e-5 * float(want[-1, :-1].norm())
+
+
+def check_scores_past_a_floats_range(torch, H, HKV, D, T, past):
+    """Finite F32 keys with a score below a float's range: weight 0, and 1 each for the others' scores of 0."""
+    q, caches, rows, n_ctx = attn_inputs(torch, T, H, HKV, D, past, 5, False)
+    k = torch.zeros_like(caches[0])
+    k[1] = -3e38
+    got = tree(torch, False, torch.full_like(q, 3e38), (k, caches[1]), HKV, n_ctx, past, 0.125)
+    for i in range(T):
+        v = rows[1][: past + i + 1].double()
+        want = ((v.sum(0) - v[1]) / (past + i)).repeat_interleave(H // HKV, 0)
+        assert float((got[i].double() - want).norm()) <= 2e-5 * float(want.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,HKV,D,T,past", [(14, 2, 64, 1, 40), (6, 2, 96, 3, 30)])
+def test_attention_tree_scores_past_a_floats_range(torch, H, HKV, D, T, past):
+    check_scores_past_a_floats_range(torch, H, HKV, D, T, past)
+
+
 def check_logits(torch, x, out, tokens, hist, repeat, freq, pres, ids, bias, allowed):
     for i in range(x.shape[0]):
         h = hist[i] if hist.ndim == 2 else hist
