@@ -894,14 +894,16 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
         float2* x2 = (float2*)x;
         const float4 in = *(const float4*)(info + slot * 4);
         const bool own = in.y != 0.0f || in.w != 0.0f;  // the positions have exponents of their own
-        // score + exponent = x * fac + off; the factor stays above 0, so that a masked -inf does
-        float fac = fmaxf(__fmul_rn(in.x, rf), 1e-37f), off = in.z;
+        // score + exponent = x * fac + off; the factor stays above 0, so that a masked -inf does, and
+        // finite, so that a product of 0 stays 0
+        auto factor = [](float f) { return fminf(fmaxf(f, 1e-37f), 3.4e38f); };
+        float fac = factor(__fmul_rn(in.x, rf)), off = in.z;
         if (own) {
           const float kc = in.y != 0.0f ? 0.0f : in.x, vc = in.z;
 #pragma unroll
           for (int k = 0; k < HT; k++) {
             const float kf = in.y != 0.0f ? c[k] : kc, ve = in.w != 0.0f ? c[kTrHalf + k] : vc;
-            x[k] = __fmaf_rn(x[k], fmaxf(__fmul_rn(kf, rf), kf == kf ? 1e-37f : kf), ve);
+            x[k] = __fmaf_rn(x[k], kf == kf ? factor(__fmul_rn(kf, rf)) : kf, ve);
           }
           fac = 1.0f;
           off = 0.0f;

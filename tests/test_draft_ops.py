@@ -714,6 +714,12 @@ def test_attention_tree_scores_past_a_floats_range(torch, H, HKV, D, T, past):
     check_scores_past_a_floats_range(torch, H, HKV, D, T, past)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,HKV,D,T,past", [(14, 2, 64, 24, 300), (14, 2, 64, 10, 30), (16, 16, 32, 140, 5)])
+def test_attention_tree_many_rows_with_scores_past_a_floats_range(torch, H, HKV, D, T, past):
+    check_scores_past_a_floats_range(torch, H, HKV, D, T, past)
+
+
 def check_logits(torch, x, out, tokens, hist, repeat, freq, pres, ids, bias, allowed):
     for i in range(x.shape[0]):
         h = hist[i] if hist.ndim == 2 else hist
