@@ -482,7 +482,7 @@ __device__ __forceinline__ void convert_f32(const TreeAttnParams& p, const TrCon
         fine[u] = m < 0x7f800000u;
         e[u] = max((int)(m >> 23) - 127, -100);
         bad |= !fine[u];
-        const bool any = e[u] > -100;
+        const bool any = m != 0;
         e[u] -= 14;
         if (fine[u] && any) {
           hi = max(hi, e[u]);
@@ -1013,14 +1013,19 @@ __global__ void __launch_bounds__(kTrThreads, 1) attn_tree_kernel(const __grid_c
       // attends to nothing has l = 0.
       const float Ms = M == -INFINITY ? -INFINITY : __fsub_ru(M, 14.0f);
       float* rec = (float*)(smem + L::k) + lr * (D + 4);
-      float inv = 1.0f;
-      if (sp.S == 1) inv = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), Ms == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(Ms, m)));
+      if (sp.S == 1) {
+        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l), down = Ms == -INFINITY ? 0.0f : __fsub_rn(Ms, m);
+#pragma unroll
+        for (int k = 0; k < NA; k++) {
+          acc[k] = __fmul_rn(acc[k], inv);
+          if (!Q8) acc[k] = times_pow2(acc[k], down);  // (Q8_0: 0)
+        }
+      }
       if (ok) {
         if (part == 0) *(float4*)rec = make_float4(Ms, m, l, 0.0f);
 #pragma unroll
         for (int k = 0; k < NA; k += 4)
-          *(float4*)(rec + 4 + NA * part + k) =
-              make_float4(__fmul_rn(acc[k], inv), __fmul_rn(acc[k + 1], inv), __fmul_rn(acc[k + 2], inv), __fmul_rn(acc[k + 3], inv));
+          *(float4*)(rec + 4 + NA * part + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
       }
     }
   }

@@ -22,6 +22,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// x 2^k for a whole k, where 2^k alone may lie outside of a float's normal range
+// (ex2.approx.ftz gives 0 below 2^-126).
+__device__ __forceinline__ float times_pow2(float x, float k) {
+  const float h = truncf(__fmul_rn(0.5f, k));
+  return __fmul_rn(__fmul_rn(x, exp2_approx(h)), exp2_approx(__fsub_rn(k, h)));
+}
+
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
@@ -92,10 +99,9 @@ __global__ void __launch_bounds__(kTrJoinNT) attn_tree_join_kernel(const TreeAtt
   const int rep = p.H / p.HKV, i = r / rep;
   float* out = p.out + ((int64_t)i * p.H + kvh * rep + (r - i * rep)) * D;
   if constexpr (W == 1) {
-    const float down = exp2_approx(__fsub_rn(Mr, mr));
 #pragma unroll
     for (int k = 0; k < D / 32; k++)
-      out[(lane + 32 * (k / V)) * V + k % V] = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(acc[k], l), down);
+      out[(lane + 32 * (k / V)) * V + k % V] = l == 0.0f ? 0.0f : times_pow2(__fdiv_rn(acc[k], l), __fsub_rn(Mr, mr));
   } else {
     __shared__ float red[W][D + 1];
 #pragma unroll
@@ -110,7 +116,7 @@ __global__ void __launch_bounds__(kTrJoinNT) attn_tree_join_kernel(const TreeAtt
         o = __fadd_rn(o, red[w][tid]);
         l = __fadd_rn(l, red[w][D]);
       }
-      out[tid] = l == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(o, l), exp2_approx(__fsub_rn(Mr, mr)));
+      out[tid] = l == 0.0f ? 0.0f : times_pow2(__fdiv_rn(o, l), __fsub_rn(Mr, mr));
     }
   }
 }

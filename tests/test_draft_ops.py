@@ -720,6 +720,25 @@ def test_attention_tree_many_rows_with_scores_past_a_floats_range(torch, H, HKV,
     check_scores_past_a_floats_range(torch, H, HKV, D, T, past)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("H,HKV,D,T,past", [(14, 2, 64, 1, 100), (14, 2, 64, 30, 100), (28, 4, 128, 64, 3000), (14, 14, 32, 200, 70), (6, 2, 96, 80, 500)])
+def test_attention_tree_values_of_any_size(torch, q8, H, HKV, D, T, past):
+    """All values of one size, tiny to huge (Q8_0: its scales' range)."""
+    for size in (6e-5, 1.0, 60000.0) if q8 else (2.0**-105, 2.0**-101, 2.0**-99, 2.0**-60, 2.0**100, 2.0**110):
+        q, caches, _, n_ctx = attn_inputs(torch, T, H, HKV, D, past, 7, False)
+        k, v = caches[0], caches[1].clamp(-7, 7) * size
+        rows = (k[: past + T], v[: past + T])
+        caches = (k, v)
+        if q8:
+            caches = [mi_cuda.kv_q8_0_cache(n_ctx, HKV, D) for _ in range(2)]
+            mi_cuda.kv_append_q8_0(k, v, *caches, n_ctx)
+            rows = mi_cuda.kv_read_q8_0(*caches, HKV, D, n_ctx, 0, past + T)
+        got = tree(torch, q8, q, caches, HKV, n_ctx, past, 0.125)
+        want, _ = attn_f64(torch, q, *rows, seen_of(torch, None, T, past), 0.125)
+        assert float((got.double() - want).norm()) <= 2e-5 * float(want.norm()), size
+
+
 def check_logits(torch, x, out, tokens, hist, repeat, freq, pres, ids, bias, allowed):
     for i in range(x.shape[0]):
         h = hist[i] if hist.ndim == 2 else hist
