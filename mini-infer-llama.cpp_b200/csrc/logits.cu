@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kLgNT = 512;
 constexpr int kLgMaxCluster = 16;
-constexpr int kLgBias = 512;     // biases of a CTA's part that are kept in shared memory
+constexpr int kLgBias = 2048;    // biases of a CTA's part that are kept in shared memory
 constexpr int kLgList = 2048;    // tokens of a part with a count or a bias that are listed
 constexpr int kLgAhead = 4;      // 16-byte pieces that a thread has under way
 
@@ -70,7 +70,14 @@ struct Counts<true> {
     return (v.x ? 1u : 0u) | (v.y ? 2u : 0u) | (v.z ? 4u : 0u) | (v.w ? 8u : 0u);
   }
 };
-constexpr int kLgSlice = 40960;  // tokens counted at a time (a multiple of 32)
+// tokens counted at a time (a multiple of 32), at most; where their biases have sums, what
+// lets two CTAs share an SM (64 rows, 4093 ids of history, 5000 biases: 140 us, 160 with
+// one CTA; 40000 ids: 265 and 343)
+constexpr int kLgSlice = 40960;
+template <bool WIDE, bool MANY>
+constexpr int kLgPer = MANY ? (WIDE ? 9600 : 12800) : kLgSlice;
+template <bool WIDE, bool MANY>
+constexpr int kLgBytes = Counts<WIDE>::bytes + (MANY ? 4 : 0);  // shared memory of a token
 
 struct LgSmem {
   float cv[kLgMaxCluster], wv[kLgNT / 32];
@@ -78,16 +85,24 @@ struct LgSmem {
   int32_t bias_of[kLgNT / 32];
   int32_t n_list;
   int32_t list[kLgList];
-  int32_t bias_id[kLgBias];
-  float bias[kLgBias];
 };
 
-// VEC: rows are 16-byte aligned, so four tokens a thread at a time.
-template <bool WIDE, bool VEC>
+// VEC: rows are 16-byte aligned, so four tokens a thread at a time. MANY: there are more
+// than kLgBias biases, so that a part's may not fit; each token then has a sum beside its
+// count, and when the list is full its biases are added there, a token's by one thread
+// (in order). Otherwise each biased token goes through the part's list by itself: 64 rows
+// with 2048 biases take 66 us so, 81 with 2049 and sums. (Tokens that went through the
+// caller's list in global memory took 290 us there, 10 ms with 5000.)
+template <bool WIDE, bool VEC, bool MANY>
 __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParams p, const int cluster, const int slice) {
   using C = Counts<WIDE>;
   constexpr int NT = kLgNT;
   extern __shared__ __align__(16) uint32_t cnt[];
+  // behind the counts: MANY, the tokens' sums; the part's biases, token (less s0) and value
+  float* sums = (float*)((uint8_t*)cnt + slice * C::bytes);
+  const int room = (int)min((int64_t)kLgBias, (p.n_bias + 3) / 4 * 4);
+  int32_t* bias_id = (int32_t*)(sums + (MANY ? slice : 0));
+  float* bias = (float*)(bias_id + room);
   __shared__ LgSmem sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_ctarank();
@@ -151,14 +166,33 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
         for (int e = 0; e < 8; e++)
           if (old[e] == 0) met((int)(h[e] - s0));
       }
-      // the part's biases in the list's order; above kLgBias of them the caller's list is read
+      // the part's biases in the list's order
       int n_bias = 0;
+      bool summed = false;
+      auto sum = [&]() {
+        for (int e = 0; e < n_bias; e += 4) {
+          const int4 id = *(const int4*)(bias_id + e);
+          auto add = [&](int k, int32_t u) {
+            if (e + k < n_bias && (u & (NT - 1)) == tid) sums[u] = __fadd_rn(sums[u], bias[e + k]);
+          };
+          add(0, id.x);
+          add(1, id.y);
+          add(2, id.z);
+          add(3, id.w);
+        }
+        summed = true;
+      };
+      int64_t u = tid < p.n_bias ? (int64_t)p.bias_ids[tid] - s0 : -1;
       for (int64_t b0 = 0; b0 < p.n_bias; b0 += NT) {
-        const int64_t i = b0 + tid;
-        const int64_t u = i < p.n_bias ? (int64_t)p.bias_ids[i] - s0 : -1;
         const bool in = u >= 0 && u < n;
+        const float v = in ? p.bias[b0 + tid] : 0.0f;
+        const int64_t next = b0 + NT + tid < p.n_bias ? (int64_t)p.bias_ids[b0 + NT + tid] - s0 : -1;
         const uint32_t m = __ballot_sync(0xffffffffu, in);
         if (lane == 0) sm.bias_of[warp] = __popc(m);
+        if (MANY && n_bias > kLgBias - NT) {
+          sum();
+          n_bias = 0;
+        }
         __syncthreads();
         int at = n_bias + __popc(m & ((1u << lane) - 1)), all = 0;
         for (int w = 0; w < NT / 32; w++) {
@@ -166,16 +200,23 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
           all += sm.bias_of[w];
         }
         if (in) {
-          if (C::mark(cnt, (int)u) == 0) met((int)u);
-          if (at < kLgBias) {
-            sm.bias_id[at] = (int32_t)u;
-            sm.bias[at] = p.bias[i];
-          }
+          const uint32_t old = C::mark(cnt, (int)u);
+          if (old == 0) met((int)u);
+          if (MANY && !(old & C::biased)) sums[u] = 0.0f;
+          bias_id[at] = (int32_t)u;
+          bias[at] = v;
         }
+        u = next;
         n_bias += all;
         __syncthreads();
       }
       __syncthreads();
+      const int n_list = sm.n_list;
+      // (one thread's tokens after one another go through the list as often)
+      if (MANY && n_bias > 0 && (summed || n_list > NT)) {
+        sum();
+        __syncthreads();
+      }
       auto one = [&](int u) {  // token s0 + u
         const uint32_t c = C::word(cnt, u);
         const int64_t j = s0 + u;
@@ -185,12 +226,16 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
                         __fadd_rn(__fmul_rn((float)(c & C::count), p.frequency), p.presence));
         if (c & C::biased) {
           float b = 0.0f;
-          if (n_bias <= kLgBias) {
-            for (int e = 0; e < n_bias; e++)
-              if (sm.bias_id[e] == u) b = __fadd_rn(b, sm.bias[e]);
+          if (MANY && summed) {
+            b = sums[u];
           } else {
-            for (int64_t e = 0; e < p.n_bias; e++)
-              if ((int64_t)p.bias_ids[e] - s0 == u) b = __fadd_rn(b, p.bias[e]);
+            for (int e = 0; e < n_bias; e += 4) {
+              const int4 id = *(const int4*)(bias_id + e);
+              if (id.x == u) b = __fadd_rn(b, bias[e]);
+              if (id.y == u && e + 1 < n_bias) b = __fadd_rn(b, bias[e + 1]);
+              if (id.z == u && e + 2 < n_bias) b = __fadd_rn(b, bias[e + 2]);
+              if (id.w == u && e + 3 < n_bias) b = __fadd_rn(b, bias[e + 3]);
+            }
           }
           v = __fadd_rn(v, b);
         }
@@ -198,7 +243,6 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
         y[j] = v;
         if (v > best_s || (v == best_s && (int32_t)j < best_si)) best_s = v, best_si = (int32_t)j;
       };
-      const int n_list = sm.n_list;
       if (n_list <= kLgList) {
         for (int i = tid; i < n_list; i += NT) one(sm.list[i]);
       } else {  // more than the list holds: every word is looked at
@@ -266,12 +310,20 @@ __global__ void __launch_bounds__(kLgNT) logits_process_kernel(const LogitsParam
   }
 }
 
-template <bool WIDE, bool VEC>
-cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, int cluster, int slice, cudaStream_t s) {
+template <bool WIDE, bool VEC, bool MANY>
+cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, cudaStream_t s) {
+  // CTAs of a row: 16 while the rows are few, 8, and 4 where all of them still run at
+  // once (us for 4 / 13 / 24 / 64 rows of 152000: 7.5 / 10.0 / 18.2 / 50.1 with 16,
+  // 9.0 / 9.1 / 12.4 / 29.4 with 8, 11.6 / 11.9 / 12.0 / 22.7 with 4; every CTA of a row
+  // reads all of its history).
+  const int cluster = n_rows <= 6 ? 16 : n_rows <= 20 ? 8 : 4;
+  const int64_t per = ((p.n_vocab + cluster - 1) / cluster + 31) / 32 * 32;
+  const int64_t slices = (per + kLgPer<WIDE, MANY> - 1) / kLgPer<WIDE, MANY>;
+  const int slice = (int)((per + slices - 1) / slices + 31) / 32 * 32;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_rows * cluster));
   cfg.blockDim = dim3(kLgNT);
-  cfg.dynamicSmemBytes = p.n_hist || p.n_bias ? (size_t)slice * Counts<WIDE>::bytes : 0;
+  cfg.dynamicSmemBytes = p.n_hist || p.n_bias ? (size_t)slice * kLgBytes<WIDE, MANY> + (std::min<int64_t>(p.n_bias, kLgBias) + 3) / 4 * 4 * 8 : 0;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -279,41 +331,42 @@ cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, int cluster, in
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, logits_process_kernel<WIDE, VEC>, p, cluster, slice);
+  return cudaLaunchKernelEx(&cfg, logits_process_kernel<WIDE, VEC, MANY>, p, cluster, slice);
+}
+template <bool WIDE, bool VEC>
+cudaError_t launch_logits(const LogitsParams& p, int64_t n_rows, cudaStream_t s) {
+  return p.n_bias > kLgBias ? launch_logits<WIDE, VEC, true>(p, n_rows, s) : launch_logits<WIDE, VEC, false>(p, n_rows, s);
 }
 
-template <bool WIDE, bool VEC>
+template <bool WIDE, bool VEC, bool MANY>
 cudaError_t prepare_logits() {
-  cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kLgSlice * Counts<WIDE>::bytes);
+  cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kLgPer<WIDE, MANY> * kLgBytes<WIDE, MANY> + kLgBias * 8);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(logits_process_kernel<WIDE, VEC, MANY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   return e;
+}
+template <bool WIDE>
+cudaError_t prepare_logits_of() {
+  cudaError_t e = prepare_logits<WIDE, false, false>();
+  if (e == cudaSuccess) e = prepare_logits<WIDE, true, false>();
+  if (e == cudaSuccess) e = prepare_logits<WIDE, false, true>();
+  return e == cudaSuccess ? prepare_logits<WIDE, true, true>() : e;
 }
 
 }  // namespace
 
 // (the counts' shared memory and clusters of 16 CTAs need attributes; per device, at init)
 cudaError_t prepare_logits_kernels() {
-  cudaError_t e = prepare_logits<false, false>();
-  if (e == cudaSuccess) e = prepare_logits<false, true>();
-  if (e == cudaSuccess) e = prepare_logits<true, false>();
-  return e == cudaSuccess ? prepare_logits<true, true>() : e;
+  const cudaError_t e = prepare_logits_of<false>();
+  return e == cudaSuccess ? prepare_logits_of<true>() : e;
 }
 
-// CTAs of a row: 16 while the rows are few, 8, and 4 where all of them still run at
-// once (us for 4 / 13 / 24 / 64 rows of 152000: 7.5 / 10.0 / 18.2 / 50.1 with 16,
-// 9.0 / 9.1 / 12.4 / 29.4 with 8, 11.6 / 11.9 / 12.0 / 22.7 with 4; every CTA of a row
-// reads all of its history).
 cudaError_t launch_logits_process(const LogitsParams& p, int64_t n_rows, cudaStream_t s) {
   if (n_rows == 0) return cudaSuccess;
-  const int cluster = n_rows <= 6 ? 16 : n_rows <= 20 ? 8 : 4;
-  const int64_t per = ((p.n_vocab + cluster - 1) / cluster + 31) / 32 * 32;
-  const int slice = (int)std::min<int64_t>(per, kLgSlice);
   const bool vec = ((uintptr_t)p.logits | (uintptr_t)p.out) % 16 == 0 && p.stride % 4 == 0 && p.n_vocab % 4 == 0;
-  if (p.n_hist <= kLgNarrow)
-    return vec ? launch_logits<false, true>(p, n_rows, cluster, slice, s) : launch_logits<false, false>(p, n_rows, cluster, slice, s);
-  return vec ? launch_logits<true, true>(p, n_rows, cluster, slice, s) : launch_logits<true, false>(p, n_rows, cluster, slice, s);
+  if (p.n_hist <= kLgNarrow) return vec ? launch_logits<false, true>(p, n_rows, s) : launch_logits<false, false>(p, n_rows, s);
+  return vec ? launch_logits<true, true>(p, n_rows, s) : launch_logits<true, false>(p, n_rows, s);
 }
 
 }  // namespace mi

@@ -833,6 +833,49 @@ def test_logits_process_values(torch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,V,nb", [(1, 152064, 30000), (2, 5000, 9000), (13, 40004, 513), (24, 151936, 6000), (1, 700001, 100000)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_logits_process_many_biases(torch, n, V, nb, wide):
+    """More biases than a part keeps at hand, most of their tokens distinct, some named many times."""
+    rng = np.random.default_rng(nb)
+    x = (rng.standard_normal((n, V)) * 4).astype(np.float32)
+    ids = rng.integers(-1, V + 1, nb).astype(np.int32)
+    ids[::7] = ids[0]
+    ids[1::5] = V - 1 - rng.integers(0, 20, ids[1::5].size)
+    bias = (rng.standard_normal(nb) * 3).astype(np.float32)
+    hist = rng.integers(0, V, 33000 if wide else 700).astype(np.int32)
+    allowed = rng.integers(0, 2**32, (n, (V + 31) // 32), dtype=np.uint64).astype(np.uint32)
+    X = torch.from_numpy(x).cuda()
+    kw = dict(hist=torch.from_numpy(hist).cuda(), repeat=1.15, frequency=0.3, presence=-0.2, bias_ids=torch.from_numpy(ids).cuda(),
+              bias=torch.from_numpy(bias).cuda(), allowed=torch.from_numpy(allowed.view(np.int32)).cuda())
+    out, tok = mi_cuda.logits_process(X, **kw)
+    check_logits(torch, x, out, tok, hist, 1.15, 0.3, -0.2, ids, bias, allowed)
+    o2, t2 = mi_cuda.logits_process(X, out=X, **kw)
+    assert torch.equal(o2.view(torch.int32), out.view(torch.int32)) and torch.equal(t2, tok)
+
+
+@pytest.mark.gpu
+def test_logits_process_time_grows_with_the_biases(torch):
+    """Four times the biases take some four times as long at most (not sixteen)."""
+    V, rng = 151936, np.random.default_rng(0)
+    X = torch.zeros((4, V), device="cuda")
+    took = []
+    for nb in (20000, 80000):
+        ids = torch.from_numpy(rng.permutation(V)[:nb].astype(np.int32)).cuda()
+        bias = torch.ones(nb, device="cuda")
+        best = math.inf
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            mi_cuda.logits_process(X, bias_ids=ids, bias=bias)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        took.append(best)
+    assert took[1] <= 8 * took[0], took
+
+
+@pytest.mark.gpu
 def test_calls_with_no_tokens(torch):
     e = torch.empty((0, 2, 64), device="cuda")
     q, k = mi_cuda.qk_norm_rope(e, e, None, None, 1e-6, 0, 64, 1e6)
