@@ -718,9 +718,6 @@ cudaError_t prepare_kernels() {
   if (e == cudaSuccess) e = prepare_qkv_attn_kernel(optin);
   if (e == cudaSuccess) e = prepare_persist_kernel(optin);
   if (e == cudaSuccess) e = prepare_attn_split_kernels();
-  if (e == cudaSuccess) e = prepare_attn_few_kernels();
-  if (e == cudaSuccess) e = prepare_attn_tree_kernels();
-  if (e == cudaSuccess) e = prepare_logits_kernels();
   if (e == cudaSuccess) e = prepare_attn_long_kernels(optin);
   return e;
 }

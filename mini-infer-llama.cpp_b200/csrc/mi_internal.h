@@ -507,6 +507,9 @@ struct DeviceCtx {
   float2* rope = nullptr;
   int32_t rope_n_pos = 0, rope_n_dims = 0;
   float rope_base = 0.0f;
+  // What preparing the kernels of tree attention and of logits processing gave: where it
+  // is an error these calls alone are refused.
+  cudaError_t attn_tree = cudaSuccess, logits = cudaSuccess;
 };
 
 // Per-device context, initialized on first use (loads the expf table).

@@ -106,6 +106,10 @@ DeviceCtx* device_ctx(int device, std::string* err) {
     delete c;
     return nullptr;
   }
+  c->attn_tree = prepare_attn_few_kernels();
+  if (c->attn_tree == cudaSuccess) c->attn_tree = prepare_attn_tree_kernels();
+  c->logits = prepare_logits_kernels();
+  cudaGetLastError();  // (kept above)
   if (cudaMalloc(&c->err, 4) != cudaSuccess || cudaMemset(c->err, 0, 4) != cudaSuccess ||
       cudaMalloc(&c->am_val, 1024 * 4) != cudaSuccess ||
       cudaMalloc(&c->am_idx, 1024 * 4) != cudaSuccess ||
@@ -155,6 +159,12 @@ int cuda_status(cudaError_t e, const char* what) {
   std::string _err;                                        \
   DeviceCtx* c = current_ctx(&_err);                       \
   if (!c) return fail(MI_CUDA_ERR_CUDA, _err)
+
+// Refuses a call whose kernels this build or device has no room for (found at init).
+#define MI_PREPARED(e, name)                                                                          \
+  if ((e) != cudaSuccess)                                                                             \
+  return fail(MI_CUDA_ERR_CUDA, std::string(name) + ": its kernels could not be prepared on this device (" + \
+                                    cudaGetErrorString(e) + ")")
 
 #define MI_REQUIRE(cond, msg) \
   if (!(cond)) return fail(MI_CUDA_ERR_ARG, msg)
@@ -572,6 +582,7 @@ static int attention_tree_common(const char* name, const float* d_q, int64_t q_s
   MI_REQUIRE(q_stride >= n_head * head_dim, std::string(name) + ": q_stride below a row");
   MI_REQUIRE(n_past <= n_ctx - n_tokens, std::string(name) + ": rows behind the cache's last");
   MI_CTX(c);
+  MI_PREPARED(c->attn_tree, name);
   TreeAttnParams p{};
   p.q = d_q;
   p.q_stride = q_stride;
@@ -627,6 +638,7 @@ int mi_cuda_logits_process(const float* d_logits, int64_t stride, int64_t n_voca
                  (d_dst == d_logits && (stride == n_vocab || n_rows == 1)),
              "mi_cuda_logits_process: d_dst overlaps the logits (only dense rows can be processed in place)");
   MI_CTX(c);
+  MI_PREPARED(c->logits, "mi_cuda_logits_process");
   LogitsParams p{};
   p.logits = d_logits;
   p.stride = stride;

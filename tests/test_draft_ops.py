@@ -18,11 +18,15 @@ Tolerances (u = 2^-24, half a step of a float relative to the value):
 """
 import ctypes as C
 import math
+import shutil
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 
 import mi_cuda
+from conftest import PKG
 
 U = 2.0 ** -24
 F = 256  # a fake, 16-byte aligned pointer: the arguments are refused before it is used
@@ -886,6 +890,39 @@ def test_calls_with_no_tokens(torch):
     assert mi_cuda.attention_tree_q8_0(e, *caches, 2, 4, 4, 0.1).shape == (0, 2, 64)
     out, tok = mi_cuda.logits_process(torch.empty((0, 100), device="cuda"))
     assert out.shape == (0, 100) and tok.shape == (0,)
+
+
+NOT_PREPARED = """
+import ctypes, sys
+ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)  # (found before the library's own)
+sys.path.insert(0, sys.argv[2])
+import torch, mi_cuda
+mi_cuda.init(0)
+x = torch.arange(64, device="cuda", dtype=torch.float32)
+assert int(mi_cuda.argmax(x)) == 63
+q, c = torch.ones((1, 2, 64), device="cuda"), torch.zeros((4, 2, 64), device="cuda")
+for sign, call in zip(sys.argv[3], (lambda: mi_cuda.attention_tree(q, c, c, 2, 2, 0.1), lambda: mi_cuda.logits_process(x[None]))):
+    try:
+        call()
+        assert sign == "1"
+    except mi_cuda.MiCudaError as e:
+        assert sign == "0" and e.code == mi_cuda.ERR_CUDA and "could not be prepared" in str(e), e
+torch.cuda.synchronize()
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("symbol,works", [("_ZN2mi25prepare_attn_tree_kernelsEv", "01"), ("_ZN2mi24prepare_attn_few_kernelsEv", "01"),
+                                          ("_ZN2mi22prepare_logits_kernelsEv", "10")])
+def test_kernels_that_cannot_be_prepared_refuse_their_own_calls_alone(torch, tmp_path, symbol, works):
+    """As in a build that gives a kernel too few registers: a stand-in for the host function that finds out."""
+    if shutil.which("gcc") is None:
+        pytest.skip("no C compiler")
+    (tmp_path / "f.c").write_text(f"int {symbol}(void) {{ return 9; }}  /* cudaErrorInvalidConfiguration */\n")
+    fake = str(tmp_path / "f.so")
+    subprocess.run(["gcc", "-shared", "-fPIC", str(tmp_path / "f.c"), "-o", fake], check=True)
+    r = subprocess.run([sys.executable, "-c", NOT_PREPARED, fake, PKG, works], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 class Step:
