@@ -68,10 +68,35 @@ __device__ __forceinline__ void quantise_block(const float (&x)[4], bool store, 
   }
 }
 
+// Where a later token names the same slot, an earlier one must leave the row alone. Few
+// tokens are compared in pairs. Many leave tags instead: the first word of what a CTA
+// writes of a row becomes 0x80 << 24 | t for the last token t that names the row. No
+// quants are such a word (none is -128), so a token that finds its own tag is the last
+// one, also while others' rows are being written over their tags. (Pairs cost the square
+// of the tokens, tags two launches: 512 slots of 2 heads of 64 7.2 us with pairs, 513 7.0
+// with tags; 2048 17.6 and 7.2, 65536 2 ms and 36 us, of which 27 without slots.)
+constexpr uint32_t kKvTag = 0x80000000u;
+constexpr int64_t kKvTags = 1 << 24;    // tokens that tags can tell apart
+constexpr int64_t kKvPairs = 16384;     // tokens times those of a CTA that are compared in pairs, at most
+__device__ __forceinline__ uint32_t* kv_tag(const KvAppendParams& p, bool is_v, int first_piece, int32_t slot) {
+  const int nb = p.D / 32, blk = first_piece >> 3, h = blk / nb, b = blk - h * nb;
+  return (uint32_t*)((is_v ? p.cache_v : p.cache_k) + ((int64_t)h * p.n_ctx + slot) * p.D + b * 32);
+}
+// Grid (tokens, pieces of a row, keys / values) as below: the tags' words as 0, then the tags.
+template <bool SET>
+__global__ void __launch_bounds__(kKvNT) kv_tag_kernel(const KvAppendParams p, const KvTiling g) {
+  const int64_t t = (int64_t)blockIdx.x * kKvNT + threadIdx.x;
+  const int32_t s = t < p.n_tokens ? p.slots[t] : -1;
+  if (s < 0 || s >= p.n_ctx) return;
+  uint32_t* tag = kv_tag(p, blockIdx.z, blockIdx.y * g.width, s);
+  if (SET) atomicMax(tag, kKvTag | (uint32_t)t);
+  else *tag = 0;
+}
+
 // VEC: rows are 16-byte aligned (float4 loads). Grid (rows, pieces of a row, keys /
-// values); eight threads hold a block of 32.
+// values); eight threads hold a block of 32. tagged: see above.
 template <bool VEC>
-__global__ void __launch_bounds__(kKvNT) kv_append_q8_kernel(const KvAppendParams p, const KvTiling g) {
+__global__ void __launch_bounds__(kKvNT) kv_append_q8_kernel(const KvAppendParams p, const KvTiling g, const bool tagged) {
   extern __shared__ int32_t row[];  // cache row of each of the CTA's tokens, -1: none
   const int nt_cta = g.rows * kKvAhead;
   const int64_t t0 = (int64_t)blockIdx.x * nt_cta;
@@ -103,10 +128,11 @@ __global__ void __launch_bounds__(kKvNT) kv_append_q8_kernel(const KvAppendParam
       atomicExch(p.err, 1 /* MI_CUDA_ERR_ARG */);
       s = -1;
     }
+    if (tagged && s >= 0 && *(volatile uint32_t*)kv_tag(p, is_v, blockIdx.y * g.width, s) != (kKvTag | (uint32_t)(t0 + i))) s = -1;
     row[i] = s;
   }
   __syncthreads();
-  if (p.slots) {  // a later token with the same slot wins
+  if (p.slots && !tagged) {  // a later token with the same slot wins
     for (int64_t j = t0 + 1 + tid; j < p.n_tokens; j += kKvNT) {
       const int32_t s = p.slots[j];
       if (s >= 0)
@@ -177,8 +203,22 @@ cudaError_t launch_kv_append_q8(const KvAppendParams& p, cudaStream_t s) {
   const KvTiling g = kv_tiling(p.HKV, p.D);
   const size_t smem = (size_t)g.rows * kKvAhead * 4;
   const bool vec = ((uintptr_t)p.k | (uintptr_t)p.v) % 16 == 0 && p.k_stride % 4 == 0 && p.v_stride % 4 == 0;
-  if (vec) kv_append_q8_kernel<true><<<kv_grid(g, p.n_tokens), kKvNT, smem, s>>>(p, g);
-  else kv_append_q8_kernel<false><<<kv_grid(g, p.n_tokens), kKvNT, smem, s>>>(p, g);
+  const bool tagged = p.slots && p.n_tokens * (g.rows * kKvAhead) > kKvPairs;
+  const int64_t n = tagged ? kKvTags : p.n_tokens;
+  for (int64_t t = 0; t < p.n_tokens; t += n) {  // (later tokens write last)
+    KvAppendParams c = p;
+    c.n_tokens = std::min(n, p.n_tokens - t);
+    c.k += t * p.k_stride;
+    c.v += t * p.v_stride;
+    if (tagged) {
+      c.slots += t;
+      const dim3 grid((unsigned)((c.n_tokens + kKvNT - 1) / kKvNT), kv_grid(g, 1).y, 2);
+      kv_tag_kernel<false><<<grid, kKvNT, 0, s>>>(c, g);
+      kv_tag_kernel<true><<<grid, kKvNT, 0, s>>>(c, g);
+    }
+    if (vec) kv_append_q8_kernel<true><<<kv_grid(g, c.n_tokens), kKvNT, smem, s>>>(c, g, tagged);
+    else kv_append_q8_kernel<false><<<kv_grid(g, c.n_tokens), kKvNT, smem, s>>>(c, g, tagged);
+  }
   return cudaGetLastError();
 }
 

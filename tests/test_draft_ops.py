@@ -361,6 +361,57 @@ def test_kv_append_slots(torch, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("HKV,D", [(2, 64), (16, 128), (3, 96)])
+@pytest.mark.parametrize("T,span", [(2049, 5000), (3001, 40), (9000, 4000), (5000, 5000)])
+def test_kv_append_many_slots(torch, HKV, D, T, span):
+    """A prompt's rows into slots: some skipped, some outside the cache, many named again and again."""
+    rng = np.random.default_rng(T)
+    n_ctx = 5000
+    slots = rng.integers(-1, span, T).astype(np.int32) if T != span else rng.permutation(T).astype(np.int32)
+    outside = T == 9000
+    if outside:
+        slots[[5, 8000]] = n_ctx, 2**31 - 1
+    k, v = (torch.randn((T, HKV, D), device="cuda") for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(T)
+    caches = [torch.randint(0, 256, (mi_cuda.lib().mi_cuda_kv_q8_0_bytes(n_ctx, HKV, D),), generator=g, device="cuda", dtype=torch.uint8)
+              for _ in range(2)]
+    last = {int(s): t for t, s in enumerate(slots) if 0 <= s < n_ctx}
+    at, src = (torch.tensor(x, device="cuda") for x in (list(last), list(last.values())))
+    want = []
+    for c, x in zip(caches, (k, v)):
+        q, s = (p.clone() for p in planes(c, HKV, n_ctx, D))
+        q[:, at], s[:, at] = (p[:, src] for p in quantise_f64(torch, x))
+        want.append((q, s))
+    mi_cuda.kv_append_q8_0(k, v, *caches, n_ctx, slots=torch.from_numpy(slots).cuda())
+    for c, (q, s) in zip(caches, want):
+        gq, gs = planes(c, HKV, n_ctx, D)
+        assert torch.equal(gq, q) and torch.equal(gs.view(torch.int16), s.view(torch.int16))
+    code = C.c_int32(-1)
+    assert mi_cuda.lib().mi_cuda_device_error(0, C.byref(code)) == 0
+    assert code.value == (mi_cuda.ERR_ARG if outside else 0)
+
+
+@pytest.mark.gpu
+def test_kv_append_time_grows_with_the_slots(torch):
+    """Four times the tokens take some four times as long at most (not sixteen)."""
+    took = []
+    for T in (30000, 120000):
+        k, v = (torch.randn((T, 2, 64), device="cuda") for _ in range(2))
+        caches = [mi_cuda.kv_q8_0_cache(T, 2, 64) for _ in range(2)]
+        slots = torch.randperm(T, device="cuda").to(torch.int32)
+        best = math.inf
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            mi_cuda.kv_append_q8_0(k, v, *caches, T, slots=slots)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        took.append(best)
+    assert took[1] <= 8 * took[0], took
+
+
+@pytest.mark.gpu
 def test_kv_append_values(torch):
     """Zeros, subnormal scales, borders between two integers, saturated scales, infinities and NaN."""
     rows = torch.zeros((12, 1, 32), device="cuda")
