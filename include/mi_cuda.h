@@ -215,10 +215,14 @@ int mi_cuda_expf_verify(uint64_t first, uint64_t count, uint64_t* n_mismatch);
  * they stay (slots; the rejected ones' are negative).
  *
  * Sums, norms and softmax statistics are held in 32 bits, in an order of the
- * library's own: results agree with the formulas to float rounding and are the
- * same from call to call. Pointers are of the calling thread's current device;
- * nothing is allocated, so every call can be captured into a CUDA graph once
- * mi_cuda_init has run.
+ * library's own, and are the same from call to call. Attention's operands (queries,
+ * keys, values, weights) are held as two halves of 11 bits: 2^-22 of an operand
+ * (2^-21 for a few rows over an F32 cache) is left out, relative to the largest that
+ * the row attends to. All else agrees with the formulas to float rounding. Pointers
+ * are of the calling thread's current device; nothing is allocated, so every call can be
+ * captured into a CUDA graph once mi_cuda_init has run. Where the kernels of attention or
+ * of logits processing could not be prepared on a device, these calls alone give
+ * MI_CUDA_ERR_CUDA.
  * ------------------------------------------------------------------------- */
 
 /* Norms of queries and keys per head with the rotation (NEOX pairing, as
@@ -250,7 +254,7 @@ size_t mi_cuda_kv_q8_0_bytes(int64_t n_ctx, int64_t n_head_kv, int64_t head_dim)
  * with one slot the later is kept, and a slot >= n_ctx is skipped and sets the
  * device error word to MI_CUDA_ERR_ARG (mi_cuda_device_error). Other rows stay as
  * they are. Per 32 values d = fp16(max|x| * (1 / 127 as a float)), at most
- * 65504, and q = rint(x / d) in [-127, 127] (0 where d is 0); a block with an infinity or a
+ * 65504 (a product, where mi_cuda_quantize_q8_0_act divides), and q = rint(x / d) in [-127, 127] (0 where d is 0); a block with an infinity or a
  * NaN is stored as d = NaN. Caches 16-byte aligned. */
 int mi_cuda_kv_append_q8_0(const float* d_k, int64_t k_stride, const float* d_v, int64_t v_stride,
                            int64_t head_dim, int64_t n_head_kv, int64_t n_tokens, int64_t n_ctx,

@@ -32,8 +32,8 @@
 // leave one record per cluster for the join.
 //
 // Bound by latency: a step's loads, its two products, the two reductions and, past
-// 2048 positions, the join: one token of 14 / 2 heads of 64 takes 5.9 us at 2000
-// positions and 11.3 us at 32000 (8.7 MB of cache, 0.8 TB/s).
+// 2048 positions, the join: one token of 14 / 2 heads of 64 takes 5.8 us at 2000
+// positions and 11.5 us at 32000 (8.7 MB of cache, 0.8 TB/s).
 #include <algorithm>
 
 #include "attn_tree.cuh"
@@ -187,8 +187,10 @@ struct FewCache<D, false> {
 // along the splits.
 //
 // Registers: one group over a Q8_0 cache for 4 CTAs of an SM (3 of 96 and 128 dims; 2
-// took 36 us for a token over 32000 positions of 28 / 4 heads of 128, 3 take 23); over
+// took 36 us for a token over 32000 positions of 28 / 4 heads of 128, 3 take 24.6); over
 // an F32 cache for 3 of 32 dims (16 heads over 2000 positions: 11.5 us with 2, 7.2 with 3).
+// Over an F32 cache of 128 dims they do not hold the planes: 192 bytes are spilled with one
+// row group and 640 with two (376 of 96 dims with two).
 template <int D, int NR, bool Q8>
 __global__ void __launch_bounds__(kFewNT, NR > 1 ? 1 : Q8 ? (D <= 64 ? 4 : 3) : D <= 32 ? 3 : 1) attn_few_kernel(const __grid_constant__ TreeAttnParams p, const TreeSplit sp,
                                                           const int cluster) {
@@ -608,8 +610,10 @@ cudaError_t launch_few(const TreeAttnParams& p, cudaStream_t s) {
   sp.R = p.T * (p.H / p.HKV);
   sp.RG = (sp.R + 8 * NR - 1) / (8 * NR);
   const int64_t n_kv = (int64_t)p.n_past + p.T, steps = (n_kv + kFewStep<D, Q8> - 1) / kFewStep<D, Q8>;
-  // one cluster where it holds every step; else clusters of 8 (fewer where a KV
-  // head's share of the GPU has no room for them), as many as run at once
+  // One cluster where it holds every step; else clusters of 8 (fewer where a KV head's
+  // share of the GPU has no room for them), for 4 CTAs an SM up to 64 dims and 2 above.
+  // (That is what runs at once of Q8_0 builds of 64 dims. Their registers let 3 run of 96
+  // and 128 dims, 2 of F32 builds of 64 dims, 3 of 32, and 2 of all with two row groups.)
   int cluster = 1;
   const int64_t room = std::max<int64_t>(1, kTrSms * (D <= 64 ? 4 : 2) / ((int64_t)p.HKV * sp.RG));
   if (steps <= 16) {

@@ -1136,11 +1136,12 @@ cudaError_t prepare_attn_tree_kernels() {
 }
 
 // Whether attn_few.cu is the faster one for R rows of a KV head. Q8_0: up to 8 rows it
-// always is (one token, us here / there: 4.8 / 9.7 at 500 positions, 11.3 / 18.5 at
-// 32000 with 14 / 2 heads of 64, 22.7 / 36.6 with 28 / 4 heads of 128); each further
+// always is (one token, us there / here: 5.2 / 10.0 at 500 positions, 11.5 / 18.1 at
+// 32000 with 14 / 2 heads of 64, 24.4 / 42.5 with 28 / 4 heads of 128); each further
 // 16 rows are another pass over the cache there, which 14 rows repay up to some
-// 16000 positions (16.1 / 18.3 at 8000, 46.4 / 36.7 at 32000, heads of 128) and 28
-// up to some 8000 of 64 dims (10.9 / 12.6 at 8000; heads of 128 19.7 / 19.0).
+// 16000 positions (heads of 128 16.9 / 19.1 at 8000, 52 / 42 at 32000; of 64 11.4 / 14.4 at
+// 16000, 20.3 / 18.2 at 32000) and 28 up to some 8000 of 64 dims (11.2 / 12.2 at 8000, 19.7 /
+// 14.3 at 16000; heads of 128 10.5 / 13.3 at 500, 14.9 / 13.9 at 2000, 21.2 / 19.3 at 8000).
 //
 // Over an F32 cache: up to 8 rows always (14 / 2 heads of 64: 7.6 / 13.2 at 2000
 // positions, 21 / 25 at 32000), up to 16 nearly always (14 rows 12.0 / 14.3 at 8000; 12

@@ -121,6 +121,8 @@ __global__ void __launch_bounds__(kTrJoinNT) attn_tree_join_kernel(const TreeAtt
   }
 }
 
+// (Launched as a programmatic dependent: no kernel has an early trigger, so it starts when
+// the records are complete. With one, 64 tokens over 32764 positions took 41.5 us, not 40.1.)
 template <int D>
 cudaError_t launch_tree_join(const TreeAttnParams& p, const TreeSplit& sp, cudaStream_t s) {
   constexpr int W = kTrJoinNT / 32;

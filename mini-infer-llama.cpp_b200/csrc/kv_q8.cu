@@ -8,8 +8,8 @@
 //
 // Block of 32 values of a row:
 //   d = fp16(min(max|x| * fl(1 / 127), 65504)),  q = clamp(rint(x / d), -127, 127),  q = 0 where d = 0.
-// (The product with the float nearest 1 / 127 is off by 2^-24 of the quotient at
-// most, which picks the other neighbour of d only where both are as good.) q rounds
+// (The product with the float nearest 1 / 127 is off by 2^-23 of the quotient at
+// most, which picks the other neighbour of d only where both are as good to that.) q rounds
 // against the d that is stored, so a value is off by d / 2 at most: a d below
 // max|x| / 127 makes |x| / d pass 127 by 2^-11 of it, which rounds to 127; only
 // subnormal and saturated scales reach the clamp. An infinity or a NaN makes d NaN
@@ -20,8 +20,10 @@
 // it is at least one of its own ulps away, and that moves the quotient by more than
 // half an ulp of k + 1/2.
 //
-// Both kernels pass over their data once; HBM bounds them for many rows, launch and
-// latency for few. Each thread has four 16-byte pieces of four rows under way.
+// Both kernels pass over their data once. For many rows HBM bounds the read (16384 rows of
+// 4 heads of 128 13.9 us, 6.1 TB/s); the append, with four divisions a 16-byte piece, runs
+// at half of that (27.4 us). Few rows are launch and latency. Each thread has four 16-byte
+// pieces of four rows under way.
 #include <algorithm>
 
 #include "mi_device.cuh"
