@@ -274,7 +274,7 @@ int mi_cuda_kv_read_q8_0(const void* d_cache_k, const void* d_cache_v, int64_t h
  * attends to nothing gives zeros; one that attends to a row with an infinity or a
  * NaN gives NaN there (in some or all values of that head). What masked rows and rows
  * from n_past + n_tokens on hold is never used. n_tokens = 1 is the single-token form.
- * head_dim 32, 64, 96 or 128, n_head a multiple of n_head_kv, at most 4096. d_scratch
+ * head_dim 32, 64, 96 or 128, n_head a multiple of n_head_kv, at most 4096, scale finite. d_scratch
  * holds mi_cuda_attention_tree_scratch_bytes() bytes (those for a larger n_kv = n_past
  * + n_tokens or n_tokens are enough too) and belongs to this call until it has run
  * (two captured graphs that may run at once need one each); caches and scratch 16-byte

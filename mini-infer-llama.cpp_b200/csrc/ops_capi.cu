@@ -581,6 +581,7 @@ static int attention_tree_common(const char* name, const float* d_q, int64_t q_s
              std::string(name) + ": head_dim 32, 64, 96 or 128, n_head a multiple of n_head_kv and at most 4096, at most 1024 tokens");
   MI_REQUIRE(q_stride >= n_head * head_dim, std::string(name) + ": q_stride below a row");
   MI_REQUIRE(n_past <= n_ctx - n_tokens, std::string(name) + ": rows behind the cache's last");
+  MI_REQUIRE(scale - scale == 0.0f, std::string(name) + ": scale is finite");
   MI_CTX(c);
   MI_PREPARED(c->attn_tree, name);
   TreeAttnParams p{};

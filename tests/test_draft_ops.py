@@ -93,6 +93,13 @@ def test_attention_tree_refusals(bad, q8):
     _refused(fn(*[a[x] for x in ("q", "qs", "ck", "cv", "d", "h", "kv", "ctx", "past", "t", "mask", "scale", "scratch", "out")], None))
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+def test_attention_tree_refuses_a_scale_that_is_not_finite(scale, q8):
+    fn = mi_cuda.lib().mi_cuda_attention_tree_q8_0 if q8 else mi_cuda.lib().mi_cuda_attention_tree
+    _refused(fn(F, 896, F, F, 64, 14, 2, 100, 97, 3, None, scale, F, F, None))
+
+
 def test_attention_tree_scratch_bytes():
     fn = mi_cuda.lib().mi_cuda_attention_tree_scratch_bytes
     assert fn(14, 2, 2048, 1, 64) > 0
