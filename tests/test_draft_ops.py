@@ -399,6 +399,28 @@ def test_kv_append_many_slots(torch, HKV, D, T, span):
 
 
 @pytest.mark.gpu
+def test_kv_append_many_slots_captured(torch):
+    """Recorded once and replayed with other rows and other slots, over rows that the replay before wrote."""
+    T, HKV, D, n_ctx = 1500, 2, 64, 900
+    k, v = (torch.empty((T, HKV, D), device="cuda") for _ in range(2))
+    slots = torch.zeros(T, device="cuda", dtype=torch.int32)
+    caches, alone = ([mi_cuda.kv_q8_0_cache(n_ctx, HKV, D) for _ in range(2)] for _ in range(2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mi_cuda.kv_append_q8_0(k, v, *caches, n_ctx, slots=slots)
+    for seed in range(3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        k.normal_(generator=g)
+        v.normal_(generator=g)
+        slots.random_(-1, n_ctx, generator=g)
+        graph.replay()
+        for t, s in enumerate(slots.tolist()):  # one after another
+            if s >= 0:
+                mi_cuda.kv_append_q8_0(k[t:t + 1], v[t:t + 1], *alone, n_ctx, s)
+        assert all(torch.equal(a, b) for a, b in zip(caches, alone))
+
+
+@pytest.mark.gpu
 def test_kv_append_time_grows_with_the_slots(torch):
     """Four times the tokens take some four times as long at most (not sixteen)."""
     took = []
@@ -895,7 +917,8 @@ def test_logits_process_values(torch):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,V,nb", [(1, 152064, 30000), (2, 5000, 9000), (13, 40004, 513), (24, 151936, 6000), (1, 700001, 100000)])
+@pytest.mark.parametrize("n,V,nb", [(1, 152064, 30000), (2, 5000, 9000), (13, 40004, 513), (24, 151936, 6000), (1, 700001, 100000),
+                                    (2, 655360, 2048)])
 @pytest.mark.parametrize("wide", [False, True])
 def test_logits_process_many_biases(torch, n, V, nb, wide):
     """More biases than a part keeps at hand, most of their tokens distinct, some named many times."""
